@@ -480,6 +480,167 @@ typedef struct kore_cuda_kv_view {
 int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const float *q, const float *k,
                                   const float *v, float *out, int *dev_status, void *stream);
 
+/*
+ * Operators on a caller-owned paged cache of 32, 16 or 8 bits.
+ *
+ * No counterpart in the reference: kore keeps one fp32 cache, rotates whole
+ * heads in the half layout and attends one sequence at a time. These entry
+ * points serve a batch of sequences whose lengths live on the device: each
+ * sequence brings a chunk of new tokens (one for a generation step, many for a
+ * prompt), the chunks stand one behind the other in the rows of q, k and v,
+ * and every buffer, the workspace included, is the caller's:
+ *   kore_cuda_rope_table_dev   the (cos, sin) table of a rotation, made once
+ *   kore_cuda_rope_dev         rotates rows of heads at given positions
+ *   kore_cuda_paged_append_dev stores a batch's new keys (rotated on the way)
+ *                              and values, and rotates its queries
+ *   kore_cuda_paged_attn_dev   attention of the batch's queries over the cache
+ *
+ * All pointers are device pointers; calls are ordered on `stream` (a
+ * cudaStream_t of the device that holds the buffers; NULL for the default
+ * stream), allocate nothing, return without synchronising and can be captured
+ * into a graph. The device of the first data pointer is made current for the
+ * call. dev_status (optional, zeroed by the caller) receives the first failure
+ * that a kernel meets in the device data: 3 a page id outside the pool, 6 a
+ * position outside the rotation table, 7 a sequence whose bounds do not fit
+ * the rows, its length or its page table. Such a sequence (for 6 and for an
+ * append's 3: such a token) is left out: none of its rows are written. In the
+ * attention a bad page's keys count as zeros.
+ */
+#define KORE_CUDA_E4M3 1000   /* 8 bits, 4 of exponent and 3 of mantissa, no infinities (not a GGUF type) */
+
+/* Rows of heads: element e of head h of row t is at data + (t * token_stride +
+ * h * head_stride + e) elements. A row may be a part of a wider one (q, k and v
+ * of one product). Strides and addresses of any size are allowed; 16-byte
+ * aligned ones are faster. */
+typedef struct kore_cuda_rows {
+    void *data;
+    int type;                 /* KORE_CUDA_F32, KORE_CUDA_F16 or KORE_CUDA_BF16 */
+    int n_head;
+    int head_dim;
+    long long token_stride;   /* elements */
+    long long head_stride;    /* elements */
+} kore_cuda_rows;
+
+enum kore_cuda_rope_scaling {
+    KORE_CUDA_ROPE_NONE = 0,     /* f_i = base^(-2i/n_rot) */
+    KORE_CUDA_ROPE_LINEAR = 1,   /* f_i / factor */
+    KORE_CUDA_ROPE_YARN = 2      /* by wavelength (Peng et al., 2023): pairs that turn more than beta_fast
+                                    times over original_ctx keep f_i, those under beta_slow take f_i / factor,
+                                    a ramp between; cos and sin times amplitude */
+};
+
+typedef struct kore_cuda_rope_spec {
+    int n_rot;             /* leading values of a head that are rotated; even, 2..256 */
+    int scaling;           /* kore_cuda_rope_scaling */
+    double base;           /* > 0 (kore: 1e6) */
+    double factor;         /* > 0 (LINEAR, YARN) */
+    double original_ctx;   /* > 0 (YARN) */
+    double beta_fast;      /* 0: 32 (YARN) */
+    double beta_slow;      /* 0: 1 (YARN) */
+    double amplitude;      /* 0: 0.1 ln(factor) + 1 for YARN with factor > 1, else 1 */
+} kore_cuda_rope_spec;
+
+/* The rotation's frequencies freq [n_rot/2] (host), computed in 64 bits and
+ * rounded to 32 as kore's inv_freq (kore.cpp:1337-1339), and the factor on its
+ * cosines and sines. Needs no GPU. */
+int kore_cuda_rope_freqs(const kore_cuda_rope_spec *spec, float *freq, double *amplitude);
+
+/* table [n_pos][n_rot/2][2]: (cos, sin) of position * frequency, formed in 64
+ * bits and rounded once (as kore.cpp:1405-1410), times the amplitude. With
+ * n_rot = head_dim and no scaling it is the table of kore_cuda_kv_view. */
+int kore_cuda_rope_table_dev(const kore_cuda_rope_spec *spec, int n_pos, float *table, void *stream);
+
+typedef struct kore_cuda_rope_view {
+    const float *table;   /* device [n_pos][n_rot/2][2], 16-byte aligned */
+    int n_pos;
+    int n_rot;
+    int interleaved;      /* 0: value i is paired with i + n_rot/2 (kore's rope_neox); 1: 2i with 2i + 1 */
+} kore_cuda_rope_view;
+
+/* out[t] = x[t] with the first n_rot values of every head rotated at position
+ * pos[t] (device [n_tok]) and the others copied. A row whose position is
+ * negative is left out (padding). x and out have the same type and heads and
+ * may be the same rows; they may not overlap in another way. Each product is
+ * rounded as kore's rope_neox (kore.cpp:1379-1381), the result once to the
+ * type. */
+int kore_cuda_rope_dev(const kore_cuda_rows *x, const kore_cuda_rows *out, int n_tok, const int *pos,
+                       const kore_cuda_rope_view *rope, int *dev_status, void *stream);
+
+/* The cache of one layer: the layout of kore_cuda_kv_view in any of the types. */
+typedef struct kore_cuda_pages {
+    void *k, *v;              /* device [n_pages][n_head_kv][page_tokens][head_dim], 16-byte aligned */
+    int type;                 /* KORE_CUDA_F32 (append only), _F16, _BF16 or _E4M3 */
+    int n_pages;
+    int page_tokens;          /* a multiple of 16 */
+    int n_head_kv;
+    int head_dim;             /* a multiple of 16, at most 256; the attention takes 64 and 128 */
+    long long page_stride;    /* elements from one page to the next; 0: dense. A multiple of 16 bytes */
+    const float *k_scale, *v_scale;   /* E4M3: device [n_head_kv], value = 8 bits * scale; NULL: 1 */
+} kore_cuda_pages;
+
+/* The step's batch. Sequence s has the rows q_start[s] .. q_start[s+1]-1 of q,
+ * k and v as its new tokens (none: it is skipped) and holds kv_len[s]
+ * positions with them, so that its row i is at position
+ * kv_len[s] - (q_start[s+1] - q_start[s]) + i. Rows outside every sequence (behind
+ * the last one of a padded batch) are not touched. */
+typedef struct kore_cuda_batch {
+    int n_seq;               /* at most 4096 */
+    const int *q_start;      /* device [n_seq + 1] */
+    const int *kv_len;       /* device [n_seq] */
+    const int *page_table;   /* device [n_seq][table_stride]: physical page of each logical page */
+    int table_stride;
+    int max_q;               /* longest chunk, known on the host: chooses the attention's kernel (any value gives
+                                the same attention, the wrong one a slower call) */
+} kore_cuda_batch;
+
+/* Stores the batch's keys and values at their positions: k [n_tok] rows of
+ * n_head_kv heads, rotated by `rope` (NULL: stored as they are), v as it is.
+ * q (optional; any number of heads) is rotated into q_out, which may be q's own
+ * rows. k, v, q and q_out have one type; the cache has it too, or fewer bits
+ * (F32 to F16 or BF16; any to E4M3: x / scale rounded to nearest even, values
+ * beyond +-448 to +-448). Positions must be distinct: no two sequences may
+ * write the same slot of a page. */
+int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
+                               const kore_cuda_rows *k, const kore_cuda_rows *v, const kore_cuda_rows *q,
+                               const kore_cuda_rows *q_out, const kore_cuda_rope_view *rope, int *dev_status,
+                               void *stream);
+
+typedef struct kore_cuda_attn_opts {
+    float scale;      /* factor on q.k; 0: 1/sqrt(head_dim) */
+    int causal;       /* 1: a token sees positions up to its own; 0: every position of its sequence */
+    int window;       /* > 0: of those, the last `window` up to its own position; 0: no window */
+} kore_cuda_attn_opts;
+
+/* Bytes of workspace an attention over heads of head_dim needs: 256-byte
+ * aligned device memory whose first KORE_CUDA_PAGED_WORKSPACE_ZEROED bytes the
+ * caller sets to zero once; every call leaves them zero again. Calls (and
+ * replays of graphs that captured one) that may overlap on the GPU need
+ * workspaces of their own. Negative for a head_dim that is not supported. */
+#define KORE_CUDA_PAGED_WORKSPACE_ZEROED 1024
+long long kore_cuda_paged_attn_workspace(int head_dim);
+
+/* out[t] = softmax(scale q[t] k^T) v over the cached positions that the
+ * options let row t of its sequence see (grouped heads: n_head a multiple of
+ * n_head_kv, at most 128 per KV head). A row that sees none gets zeros (and lse
+ * -inf). Only positions that some row of the sequence sees are read; what lies
+ * in a page outside them (behind the end, before the window) may hold
+ * anything, infinities and NaN too. Positions that a row of the chunk sees must
+ * hold finite values for the chunk's other rows to be right.
+ * q, out: [n_tok] rows of n_head heads, F16 or BF16, the cache of the same type
+ * or E4M3; lse (optional) [n_tok][n_head]: natural log of the softmax's sum.
+ * Products are exact and summed in 32 bits, the softmax in 32 bits; the
+ * probabilities are rounded to the type of the cache for the second product
+ * (to F16 for E4M3). The result is a function of the inputs and the batch alone
+ * (no atomics on values): the same call gives the same bits. */
+int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
+                             const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
+                             const kore_cuda_attn_opts *opts, void *workspace, long long workspace_bytes,
+                             int *dev_status, void *stream);
+
+/* Identity of the graph capture that `stream` is in (0: none), for callers that
+ * keep one workspace per capture. */
+unsigned long long kore_cuda_capture_id(void *stream);
+
 #ifdef __cplusplus
 }
 #endif

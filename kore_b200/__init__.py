@@ -7,6 +7,8 @@ kore's per-layer attention call: ``decode`` replaces kore.cpp:1424-1455 and
 the ``*_dev`` forms take device tensors and stay on the context's stream.
 ``set_attn_weights`` + ``attn_block_decode`` run a decode step's whole
 attention block (kore.cpp:1418-1457), its Q4_K / Q6_K projections included.
+``RopeTable``, ``PagedCache`` and ``PagedBatch`` (kore_b200/paged.py) are the
+operators on a caller-owned paged cache of 32, 16 or 8 bits.
 
 There is no fallback: if the library is missing, importing this module works
 but creating a context raises, naming the build command.
@@ -21,7 +23,8 @@ import numpy as np
 
 from .build import LIB, INCLUDE
 
-__all__ = ["KoreCuda", "KoreCudaError", "KvView", "Server", "load_library", "declared_symbols", "STATUS"]
+__all__ = ["KoreCuda", "KoreCudaError", "KvView", "Server", "load_library", "declared_symbols", "STATUS",
+           "RopeTable", "PagedBatch", "PagedCache", "rope_frequencies"]
 
 STATUS = {
     0: "KORE_CUDA_OK", -1: "KORE_CUDA_EINVAL", -2: "KORE_CUDA_ERANGE", -3: "KORE_CUDA_ENOMEM",
@@ -538,3 +541,6 @@ class Server:
         buf = np.zeros(max(n, 1), np.int32)
         self._L.kore_cuda_server_history(self._h, session, buf.ctypes.data_as(_ip), n)
         return buf[:n].tolist()
+
+
+from .paged import PagedBatch, PagedCache, RopeTable, rope_frequencies  # noqa: E402  (uses the names above)

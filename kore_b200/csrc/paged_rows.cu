@@ -1,0 +1,621 @@
+// paged_rows.cu — attention of few query rows a KV head (generation steps,
+// short chunks) over a caller-owned paged cache (sm_100a).
+//
+// out = softmax(scale q K^T) V for up to 16 packed rows (tokens x the group's
+// query heads) a work unit: every key and value is read once for the whole
+// group. Bound by HBM: 2 d bytes-of-type per key and head against 4 d flops a
+// row, far below what the products need on any path, so the products are
+// warp-level mma.m16n8k16 (a tcgen05 tile has 128 rows, of which 8 to 16 would
+// be used) and everything serves the stream of keys:
+//   * one CTA of 8 warps an SM; each warp streams tiles of its own, a fixed
+//     8 KB (4 KB for 8 bits and d = 64) of K and V, through a ring of 3 (6)
+//     stages filled with 16-byte cp.async (192 KB in flight an SM). No warp
+//     waits for another, and the ring runs on over the ends of units.
+//   * work in equal shares (paged.cuh): ragged lengths, one long sequence and
+//     many short ones all end at the same time. A unit cut between CTAs is
+//     joined by the CTA that finishes last, in the CTAs' order, so the sums do not
+//     depend on who that is.
+//   * keys outside the unit's range arrive as zeros (cp.async with a source size
+//     of 0): whatever the page holds there meets neither product.
+//   * the row maximum is moved only when a score passes it by 2^8, so most tiles
+//     rescale nothing; sums and outputs are fp32.
+//   * an 8-bit cache is widened to f16 on the way into the fragments (exact: e4m3
+//     has fewer exponent and mantissa bits). The order of d in the first
+//     product's sum is free, so a thread takes 4 consecutive bytes where the
+//     fragment wants (2t, 2t+1, 2t+8, 2t+9), and q the same. bf16 queries over it
+//     are scaled by a power of two a row so that they are exact in f16 down
+//     to 2^-22 of the row's largest value.
+
+#include "paged.cuh"
+
+#include "kore_cuda.h"
+
+#include <type_traits>
+
+namespace kore {
+namespace {
+
+constexpr unsigned FULL = 0xffffffffu;
+constexpr int kWarps = 8;
+constexpr int kRowsU = 16;          // packed rows of a unit
+constexpr float kSlack = 8.0f;      // log2 slack before the reference maximum moves
+
+template <int D, int ES>   // ES: bytes of a cached value
+struct RowsCfg {
+    static constexpr int KT = (D == 128 && ES == 2) ? 16 : 32;   // keys of a warp's tile
+    static constexpr int STAGES = (D == 64 && ES == 1) ? 6 : 3;
+    static constexpr int ROWB = D * ES;                          // bytes of a key
+    static constexpr int HALF = KT * ROWB;                       // K (V) bytes of a stage
+    static constexpr int STAGE = 2 * HALF;
+    static constexpr int CT = kWarps * KT;                       // keys of a CTA's tile
+    static constexpr int CH = ROWB / 16;                         // 16-byte pieces of a key
+    static constexpr int RING = kWarps * STAGES * STAGE;
+    static constexpr int MERGE = kWarps * 8 * D * 4;             // 8 rows of every warp
+    static constexpr int CUM = (kPagedMaxSeqs + 1) * 8;          // shares MERGE's place
+    static constexpr int TOP = MERGE > CUM ? MERGE : CUM;
+    static constexpr int ML = RING + (TOP + 15) / 16 * 16;
+    static constexpr int BYTES = ML + 2 * kWarps * kRowsU * 8 + 16;
+};
+
+// Byte offset of 16-byte piece c of key r within a stage's half, permuted so
+// that the pieces c of 8 consecutive keys lie in distinct banks.
+template <int ROWB>
+__device__ __forceinline__ int piece(int r, int c) {
+    if constexpr (ROWB == 64) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    else return r * ROWB + ((c ^ (r & 7)) << 4);
+}
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(a)
+                 : "memory");
+}
+
+template <bool BF>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+                     "{%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
+// two e4m3 values (first in the low byte) as two f16
+__device__ __forceinline__ uint32_t widen2(uint32_t x) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(x));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t ld_u32(const void *p, bool aligned) {
+    if (aligned) return __ldg(static_cast<const unsigned int *>(p));
+    const unsigned short *h = static_cast<const unsigned short *>(p);
+    return (uint32_t)__ldg(h) | ((uint32_t)__ldg(h + 1) << 16);
+}
+
+// QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16).
+template <int D, bool QBF, bool E4M3>
+__global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
+    constexpr int ES = E4M3 ? 1 : 2;
+    using C = RowsCfg<D, ES>;
+    constexpr bool BF = QBF && !E4M3;   // type of the products
+    using U = Unit<kRowsU, C::CT>;
+    using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int g8 = lane >> 2, t4 = lane & 3;
+    float *merge = reinterpret_cast<float *>(smem + C::RING);
+    // [warp][row] (max, sum), in two places by turns: a warp may be writing the
+    // next unit's while another still reads this one's
+    float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
+    int ml_turn = kWarps * kRowsU;
+    int *flag = reinterpret_cast<int *>(smem + C::ML + 2 * kWarps * kRowsU * 8);
+    grid_dep_wait();
+    grid_dep_launch();
+
+    U u;
+    long long total, x0, x1;
+    int ctas;
+    if (!find_share<kRowsU, C::CT>(p, reinterpret_cast<long long *>(smem + C::RING), 2, u, total, ctas, x0, x1)) return;
+
+    const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
+    const uint8_t *kbase = static_cast<const uint8_t *>(p.k), *vbase = static_cast<const uint8_t *>(p.v);
+
+    // ---- the load side: a unit and a tile that run ahead of the products
+    U lu = u;
+    bool l_more = true;
+    int lt, lt1;   // next tile to load and the end of the share within lu, relative to lu.tile0
+    auto share_tiles = [&](const U &a, int &t0, int &t1) {   // tiles of unit a in [x0, x1)
+        const long long first = a.u0 + kUnitCost;
+        t0 = (int)max(0ll, min((long long)a.nt, x0 - first));
+        t1 = (int)max(0ll, min((long long)a.nt, x1 - first));
+    };
+    auto l_skip = [&]() {   // to the next unit that has a tile left
+        while (l_more && lt >= lt1) {
+            if (lu.u0 + kUnitCost + lu.nt >= x1 || !lu.next(p)) {
+                l_more = false;
+                return;
+            }
+            share_tiles(lu, lt, lt1);
+        }
+    };
+    share_tiles(lu, lt, lt1);
+    l_skip();
+    // pages of the 16-key groups of the next tile to load, a tile ahead
+    constexpr int NG = C::KT / 16;
+    auto page_of_next = [&]() -> int {   // lane i < NG: page of group i
+        int ph = -1;
+        if (l_more && lane < NG) {
+            const int key = (lu.tile0 + lt) * C::CT + warp * C::KT + lane * 16;
+            if (key < lu.hi && key + 16 > lu.lo) {
+                ph = __ldg(p.page_table + (long long)lu.s * p.table_stride + key / p.P);
+                if (ph < 0 || ph >= p.n_pages) {
+                    raise_error(p.status, DEV_BAD_PAGE);
+                    ph = -1;
+                }
+            }
+        }
+        return ph;
+    };
+    int pages = page_of_next();
+    int l_stage = 0;
+    auto load_tile = [&]() {   // one tile (or nothing) and its group
+        if (l_more) {
+            const int key0 = (lu.tile0 + lt) * C::CT + warp * C::KT;
+            const uint32_t dst = ring + l_stage * C::STAGE;
+            constexpr int N = C::HALF / 512;   // pieces a lane
+            long long row[NG];
+            bool ok[NG];
+#pragma unroll
+            for (int i = 0; i < NG; ++i) {
+                const int ph = __shfl_sync(FULL, pages, i);
+                ok[i] = ph >= 0;
+                row[i] = ((long long)max(ph, 0) * p.page_stride + ((long long)lu.g * p.P + (key0 + 16 * i) % p.P) * D) * ES;
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int c = i * 32 + lane;
+                const int r = c / C::CH, cc = c % C::CH;
+                const int grp = (i * 32) / (16 * C::CH);   // all lanes of a step are in one group
+                const bool in = ok[grp] && key0 + r >= lu.lo && key0 + r < lu.hi;
+                const long long off = in ? row[grp] + (r - 16 * grp) * C::ROWB + cc * 16 : 0;
+                cp16(dst + piece<C::ROWB>(r, cc), kbase + off, in);
+                cp16(dst + C::HALF + piece<C::ROWB>(r, cc), vbase + off, in);
+            }
+            ++lt;
+            l_skip();
+            pages = page_of_next();
+        }
+        l_stage = l_stage + 1 == C::STAGES ? 0 : l_stage + 1;
+        cp_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < C::STAGES - 1; ++i) load_tile();
+
+    // ---- the products
+    int stage = 0;
+    for (;;) {
+        int t0, t1;
+        share_tiles(u, t0, t1);
+        if (t0 < t1) {
+            const int r0 = u.b * kRowsU + g8, r1 = r0 + 8;   // this thread's packed rows
+            const bool in0 = g8 < u.rows, in1 = g8 + 8 < u.rows;
+            // keys [lo, hi) of the two rows
+            int lo0 = 0, hi0 = 0, lo1 = 0, hi1 = 0;
+            if (in0) key_range(p, u.q, r0, r0 + 1, lo0, hi0);
+            if (in1) key_range(p, u.q, r1, r1 + 1, lo1, hi1);
+            // keys that every valid row sees
+            int all_lo, all_hi, t;
+            key_range(p, u.q, u.b * kRowsU, u.b * kRowsU + 1, t, all_hi);
+            key_range(p, u.q, u.b * kRowsU + u.rows - 1, u.b * kRowsU + u.rows, all_lo, t);
+
+            // q fragments
+            uint32_t qf[D / 16][4];
+            float qs0 = p.scale * 1.44269504088896340736f, qs1 = qs0;
+            {
+                const int i0 = r0 / p.rep, i1 = r1 / p.rep;
+                const qt *s0 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i0) * p.q_ts +
+                               (long long)(u.g * p.rep + r0 - i0 * p.rep) * p.q_hs;
+                const qt *s1 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i1) * p.q_ts +
+                               (long long)(u.g * p.rep + r1 - i1 * p.rep) * p.q_hs;
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const int e = E4M3 ? t4 * (D / 4) + 4 * k : 16 * k + 2 * t4;
+                    const int f = E4M3 ? e + 2 : e + 8;
+                    qf[k][0] = in0 ? ld_u32(s0 + e, p.q_vec) : 0;
+                    qf[k][1] = in1 ? ld_u32(s1 + e, p.q_vec) : 0;
+                    qf[k][2] = in0 ? ld_u32(s0 + f, p.q_vec) : 0;
+                    qf[k][3] = in1 ? ld_u32(s1 + f, p.q_vec) : 0;
+                }
+                if constexpr (E4M3) {
+                    if constexpr (QBF) {
+                        // bf16 -> f16 with the row's largest value at 2^7 .. 2^8
+                        float m0 = 0.f, m1 = 0.f;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float a = __uint_as_float(qf[k][i] << 16), b = __uint_as_float(qf[k][i] & 0xffff0000u);
+                                const float x = fmaxf(fabsf(a), fabsf(b));
+                                if (i & 1) m1 = fmaxf(m1, x);
+                                else m0 = fmaxf(m0, x);
+                            }
+#pragma unroll
+                        for (int o = 1; o < 4; o <<= 1) {
+                            m0 = fmaxf(m0, __shfl_xor_sync(FULL, m0, o));
+                            m1 = fmaxf(m1, __shfl_xor_sync(FULL, m1, o));
+                        }
+                        auto shift = [](float m) {   // 2^(7 - exponent of m); 1 for 0, infinities and NaN
+                            const int e = (__float_as_int(m) >> 23) - 127;
+                            return m > 0.f && m < INFINITY ? __int_as_float((127 + min(max(7 - e, -100), 100)) << 23) : 1.f;
+                        };
+                        const float f0 = shift(m0), f1 = shift(m1);
+                        qs0 /= f0;
+                        qs1 /= f1;
+#pragma unroll
+                        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float f = (i & 1) ? f1 : f0;
+                                const float a = __uint_as_float(qf[k][i] << 16) * f;
+                                const float b = __uint_as_float(qf[k][i] & 0xffff0000u) * f;
+                                qf[k][i] = pack2<false>(a, b);
+                            }
+                    }
+                    if (p.k_scale) {
+                        const float ks = __ldg(p.k_scale + u.g);
+                        qs0 *= ks;
+                        qs1 *= ks;
+                    }
+                }
+            }
+
+            float o[D / 8][4];
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) o[i][k] = 0.f;
+            float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // l: this thread's keys only
+
+            for (int tt = t0; tt < t1; ++tt) {
+                cp_wait<C::STAGES - 2>();
+                __syncwarp();   // this tile has landed, and every lane is done with the one before
+                load_tile();    // into the stage of the one before
+                const uint32_t kt = ring + stage * C::STAGE, vt = kt + C::HALF;
+                const int key0 = (u.tile0 + tt) * C::CT + warp * C::KT;
+                if (key0 < u.hi && key0 + C::KT > u.lo) {
+                    float s[C::KT / 8][4];
+#pragma unroll
+                    for (int j = 0; j < C::KT / 8; ++j) {
+                        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+                        if constexpr (!E4M3) {
+#pragma unroll
+                            for (int k = 0; k < D / 32; ++k) {
+                                uint32_t b[4];
+                                ldsm4(b, kt + piece<C::ROWB>(8 * j + (lane & 7), 4 * k + (lane >> 3)));
+                                mma<BF>(s[j], qf[2 * k], b[0], b[1]);
+                                mma<BF>(s[j], qf[2 * k + 1], b[2], b[3]);
+                            }
+                        } else {
+                            // thread t4 takes bytes t4*D/4 .. of key g8
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h) {
+                                uint32_t w[4];
+                                const uint32_t a = kt + piece<C::ROWB>(8 * j + g8, t4 * (D / 64) + h);
+                                asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                             : "r"(a)
+                                             : "memory");
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    mma<false>(s[j], qf[4 * h + i], widen2(w[i] & 0xffffu), widen2(w[i] >> 16));
+                            }
+                        }
+                    }
+                    float x0m = -INFINITY, x1m = -INFINITY;
+                    const bool masked = key0 < all_lo || key0 + C::KT > all_hi;
+#pragma unroll
+                    for (int j = 0; j < C::KT / 8; ++j) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            s[j][i] *= qs0;
+                            s[j][2 + i] *= qs1;
+                            if (masked) {
+                                const int key = key0 + 8 * j + 2 * t4 + i;
+                                if (key < lo0 || key >= hi0) s[j][i] = -INFINITY;
+                                if (key < lo1 || key >= hi1) s[j][2 + i] = -INFINITY;
+                            }
+                            x0m = fmaxf(x0m, s[j][i]);
+                            x1m = fmaxf(x1m, s[j][2 + i]);
+                        }
+                    }
+#pragma unroll
+                    for (int f = 1; f < 4; f <<= 1) {
+                        x0m = fmaxf(x0m, __shfl_xor_sync(FULL, x0m, f));
+                        x1m = fmaxf(x1m, __shfl_xor_sync(FULL, x1m, f));
+                    }
+                    const bool need0 = x0m > m0 + kSlack, need1 = x1m > m1 + kSlack;
+                    if (__any_sync(FULL, need0 || need1)) {
+                        const float n0 = need0 ? x0m : m0, n1 = need1 ? x1m : m1;
+                        const float a0 = n0 == m0 ? 1.f : fast_exp2(m0 - n0), a1 = n1 == m1 ? 1.f : fast_exp2(m1 - n1);
+                        m0 = n0;
+                        m1 = n1;
+                        l0 *= a0;
+                        l1 *= a1;
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) {
+                            o[i][0] *= a0;
+                            o[i][1] *= a0;
+                            o[i][2] *= a1;
+                            o[i][3] *= a1;
+                        }
+                    }
+                    const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+#pragma unroll
+                    for (int j = 0; j < C::KT / 8; ++j) {
+                        s[j][0] = fast_exp2(s[j][0] - z0);
+                        s[j][1] = fast_exp2(s[j][1] - z0);
+                        s[j][2] = fast_exp2(s[j][2] - z1);
+                        s[j][3] = fast_exp2(s[j][3] - z1);
+                        l0 += s[j][0] + s[j][1];
+                        l1 += s[j][2] + s[j][3];
+                    }
+#pragma unroll
+                    for (int jj = 0; jj < C::KT / 16; ++jj) {
+                        const uint32_t a[4] = {pack2<BF>(s[2 * jj][0], s[2 * jj][1]), pack2<BF>(s[2 * jj][2], s[2 * jj][3]),
+                                               pack2<BF>(s[2 * jj + 1][0], s[2 * jj + 1][1]),
+                                               pack2<BF>(s[2 * jj + 1][2], s[2 * jj + 1][3])};
+#pragma unroll
+                        for (int c = 0; c < C::CH / 2; ++c) {
+                            uint32_t b[4];   // pieces 2c (b0, b1) and 2c + 1 (b2, b3), keys 0-7 and 8-15
+                            ldsm4t(b, vt + piece<C::ROWB>(16 * jj + (lane & 7) + (lane & 8), 2 * c + (lane >> 4)));
+                            if constexpr (!E4M3) {
+                                mma<BF>(o[2 * c], a, b[0], b[1]);
+                                mma<BF>(o[2 * c + 1], a, b[2], b[3]);
+                            } else {
+                                // b holds, for keys 2t and 2t+1, the bytes d = 2g, 2g+1 of the piece
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    const uint32_t w0 = widen2(b[2 * h] & 0xffffu), w1 = widen2(b[2 * h] >> 16);
+                                    const uint32_t y0 = widen2(b[2 * h + 1] & 0xffffu), y1 = widen2(b[2 * h + 1] >> 16);
+                                    const int i = 4 * c + 2 * h;
+                                    mma<false>(o[i], a, __byte_perm(w0, w1, 0x5410), __byte_perm(y0, y1, 0x5410));
+                                    mma<false>(o[i + 1], a, __byte_perm(w0, w1, 0x7632), __byte_perm(y0, y1, 0x7632));
+                                }
+                            }
+                        }
+                    }
+                }
+                stage = stage + 1 == C::STAGES ? 0 : stage + 1;
+            }
+
+            // ---- join the warps: rows g8 in one pass, rows g8 + 8 in another
+#pragma unroll
+            for (int f = 1; f < 4; f <<= 1) {
+                l0 += __shfl_xor_sync(FULL, l0, f);
+                l1 += __shfl_xor_sync(FULL, l1, f);
+            }
+            if (t4 == 0) {
+                ml[warp * kRowsU + g8] = make_float2(m0, l0);
+                ml[warp * kRowsU + g8 + 8] = make_float2(m1, l1);
+            }
+            const bool whole = t0 == 0 && t1 == u.nt;
+            const int c0 = whole ? 0 : share_of(u.u0 + kUnitCost, total, ctas);
+            const int c1 = whole ? 0 : share_of(u.u0 + kUnitCost + u.nt - 1, total, ctas);
+            // slot: [kRowsU][D] outputs to the row's maximum, then [kRowsU] (max, sum)
+            constexpr int SLOT = kRowsU * (D + 2);
+            float *slot = p.part + (size_t)(blockIdx.x * 2 + (t0 == 0)) * SLOT;
+            constexpr int VW = D / 32;   // values a lane
+            const float vs = E4M3 && p.v_scale ? __ldg(p.v_scale + u.g) : 1.f;
+            auto write_out = [&](int row, const float (&x)[VW], float M, float L) {   // row of the unit, this lane's values
+                const int r = u.b * kRowsU + row, i = r / p.rep, h = u.g * p.rep + r - i * p.rep;
+                const float inv = L > 0.f || L != L ? vs / L : 0.f;
+                qt *dst = static_cast<qt *>(p.out) + (long long)(u.q.q0 + i) * p.o_ts + (long long)h * p.o_hs + lane * VW;
+                uint32_t w[VW / 2];
+#pragma unroll
+                for (int k = 0; k < VW / 2; ++k) w[k] = pack2<QBF>(x[2 * k] * inv, x[2 * k + 1] * inv);
+                if (p.o_vec) {
+                    if constexpr (VW == 4) *reinterpret_cast<uint2 *>(dst) = make_uint2(w[0], w[1]);
+                    else *reinterpret_cast<uint32_t *>(dst) = w[0];
+                } else {
+                    const qt *y = reinterpret_cast<const qt *>(w);
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) dst[k] = y[k];
+                }
+                if (p.lse && lane == 0)
+                    p.lse[(long long)(u.q.q0 + i) * p.H + h] = L > 0.f || L != L ? M * 0.69314718055994530942f + logf(L) : -INFINITY;
+            };
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                if (half == 1 && u.rows <= 8) break;
+                __syncthreads();   // ml is written; merge is free
+                const int fr = g8 + 8 * half;
+                float M = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) M = fmaxf(M, ml[w * kRowsU + fr].x);
+                const float mine = half ? m1 : m0;
+                const float f = mine == -INFINITY ? 0.f : fast_exp2(mine - M);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    float *dst = merge + (warp * 8 + g8) * D;
+                    const int sw = (g8 & 3) * 8;
+                    if constexpr (!E4M3) {
+                        *reinterpret_cast<float2 *>(dst + ((8 * i + 2 * t4) ^ sw)) =
+                            make_float2(o[i][2 * half] * f, o[i][2 * half + 1] * f);
+                    } else if ((i & 1) == 0) {   // even and odd d of a piece of 16
+                        const int e = 8 * i + 4 * t4;
+                        *reinterpret_cast<float4 *>(dst + (e ^ sw)) =
+                            make_float4(o[i][2 * half] * f, o[i + 1][2 * half] * f, o[i][2 * half + 1] * f,
+                                        o[i + 1][2 * half + 1] * f);
+                    }
+                }
+                __syncthreads();
+                // warp w owns row w of these 8
+                const int row = warp + 8 * half;
+                float Mr = -INFINITY, Lr = 0.f;
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) Mr = fmaxf(Mr, ml[w * kRowsU + row].x);
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 v = ml[w * kRowsU + row];
+                    if (v.x != -INFINITY) Lr = fmaf(v.y, fast_exp2(v.x - Mr), Lr);
+                }
+                if (row < u.rows) {
+                    float x[VW];
+#pragma unroll
+                    for (int k = 0; k < VW; ++k) x[k] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWarps; ++w) {
+                        const float *src = merge + (w * 8 + warp) * D + ((lane * VW) ^ ((warp & 3) * 8));
+                        if constexpr (VW == 4) {
+                            const float4 v = *reinterpret_cast<const float4 *>(src);
+                            x[0] += v.x;
+                            x[1] += v.y;
+                            x[2] += v.z;
+                            x[3] += v.w;
+                        } else {
+                            const float2 v = *reinterpret_cast<const float2 *>(src);
+                            x[0] += v.x;
+                            x[1] += v.y;
+                        }
+                    }
+                    if (whole) {
+                        write_out(row, x, Mr, Lr);
+                    } else {
+                        float *dst = slot + row * D + lane * VW;
+                        if constexpr (VW == 4) *reinterpret_cast<float4 *>(dst) = make_float4(x[0], x[1], x[2], x[3]);
+                        else *reinterpret_cast<float2 *>(dst) = make_float2(x[0], x[1]);
+                        if (lane == 0)
+                            *reinterpret_cast<float2 *>(slot + kRowsU * D + 2 * row) = make_float2(Mr, Lr);
+                    }
+                }
+            }
+            if (!whole) {   // the last of the unit's CTAs joins the parts
+                __threadfence();
+                __syncthreads();
+                if (tid == 0) *flag = atomicAdd(p.counters + c0, 1) == c1 - c0;
+                __syncthreads();
+                if (*flag) {
+                    __threadfence();
+                    for (int row = warp; row < u.rows; row += kWarps) {
+                        // CTA c0's part is in its second slot, the others' in their first
+                        auto part_of = [&](int c) { return p.part + (size_t)(c * 2 + (c == c0)) * SLOT; };
+                        float M = -INFINITY;
+                        for (int c = c0 + lane; c <= c1; c += 32)
+                            M = fmaxf(M, __ldcg(part_of(c) + kRowsU * D + 2 * row));
+#pragma unroll
+                        for (int f = 16; f; f >>= 1) M = fmaxf(M, __shfl_xor_sync(FULL, M, f));
+                        float L = 0.f, x[VW];
+#pragma unroll
+                        for (int k = 0; k < VW; ++k) x[k] = 0.f;
+                        for (int cb = c0; cb <= c1; cb += 32) {
+                            float wgt = 0.f, lw = 0.f;   // of CTA cb + lane
+                            if (cb + lane <= c1) {
+                                const float2 v = __ldcg(reinterpret_cast<const float2 *>(part_of(cb + lane) + kRowsU * D + 2 * row));
+                                if (v.x != -INFINITY) {
+                                    wgt = fast_exp2(v.x - M);
+                                    lw = v.y * wgt;
+                                }
+                            }
+                            const int n = min(32, c1 - cb + 1);
+#pragma unroll 8
+                            for (int i = 0; i < n; ++i) {
+                                const float *src = part_of(cb + i) + row * D + lane * VW;
+                                const float w = __shfl_sync(FULL, wgt, i);
+                                L += __shfl_sync(FULL, lw, i);
+                                if constexpr (VW == 4) {
+                                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(src));
+                                    x[0] = fmaf(w, v.x, x[0]);
+                                    x[1] = fmaf(w, v.y, x[1]);
+                                    x[2] = fmaf(w, v.z, x[2]);
+                                    x[3] = fmaf(w, v.w, x[3]);
+                                } else {
+                                    const float2 v = __ldcg(reinterpret_cast<const float2 *>(src));
+                                    x[0] = fmaf(w, v.x, x[0]);
+                                    x[1] = fmaf(w, v.y, x[1]);
+                                }
+                            }
+                        }
+                        write_out(row, x, M, L);
+                    }
+                    if (tid == 0) p.counters[c0] = 0;   // as the next call wants it
+                }
+            }
+        }
+        if (t0 < t1) {
+            ml += ml_turn;
+            ml_turn = -ml_turn;
+        }
+        if (u.u0 + kUnitCost + u.nt >= x1 || !u.next(p)) break;
+    }
+    cp_wait<0>();
+}
+
+template <int D, bool QBF, bool E4M3>
+cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+    using C = RowsCfg<D, E4M3 ? 1 : 2>;
+    auto kernel = paged_rows_kernel<D, QBF, E4M3>;
+    static_assert(C::BYTES <= 232448, "shared memory of an SM");
+    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(kernel), C::BYTES)) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_ctas);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = C::BYTES;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+}  // namespace
+
+cudaError_t launch_paged_rows(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s) {
+    const bool bf = q_type == KORE_CUDA_BF16, e = cache_type == KORE_CUDA_E4M3;
+    if (d == 128) {
+        if (e) return bf ? launch_k<128, true, true>(p, n_ctas, s) : launch_k<128, false, true>(p, n_ctas, s);
+        return bf ? launch_k<128, true, false>(p, n_ctas, s) : launch_k<128, false, false>(p, n_ctas, s);
+    }
+    if (d == 64) {
+        if (e) return bf ? launch_k<64, true, true>(p, n_ctas, s) : launch_k<64, false, true>(p, n_ctas, s);
+        return bf ? launch_k<64, true, false>(p, n_ctas, s) : launch_k<64, false, false>(p, n_ctas, s);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace kore
