@@ -19,6 +19,7 @@ constexpr int kPagedMaxSeqs = 4096;      // sequences of one batch
 constexpr int kPagedMaxCtas = 160;       // CTAs (SMs) that an attention launch uses at most
 constexpr int kPagedRowsMax = 256;       // query rows of a work unit at most
 constexpr size_t kPagedZeroed = 1024;    // leading workspace bytes that are zero between calls
+constexpr size_t kPagedCutBytes = 32;    // of a cut unit's description
 
 // A tensor of rows of heads: element e of head h of row t at t*ts + h*hs + e.
 struct HeadRows {
@@ -60,6 +61,7 @@ struct PagedAttnParams {
     int q_vec, o_vec;          // q (out) rows are 16-byte aligned
     int box;                   // rows of a tensor-map box
     int *counters;             // [kPagedMaxCtas] zero between calls
+    void *cut;                 // [kPagedMaxCtas] units that were cut (many-row kernel)
     float *part;               // [kPagedMaxCtas][2] partial results
     int *status;
 };
@@ -68,6 +70,7 @@ cudaError_t launch_rope_table(const float *freq, int half, double amp, int n_pos
 cudaError_t launch_rotate(const RotateParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
 // n_ctas: SMs of the device, at most kPagedMaxCtas
 cudaError_t launch_paged_rows(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
+cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int type, int n_ctas, cudaStream_t s);
 
 // ---------------------------------------------------------------- division of the attention's work
 //

@@ -6,6 +6,8 @@
 
 #include "kore_cuda.h"
 
+#include <cuda.h>
+
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -126,6 +128,37 @@ int check_batch(const kore_cuda_batch *b, int n_tok) {
     if (b->n_seq > 0 && b->table_stride <= 0) return refuse(KORE_CUDA_EINVAL, "table_stride %d", b->table_stride);
     if (b->max_q < 0) return refuse(KORE_CUDA_EINVAL, "max_q %d", b->max_q);
     return KORE_CUDA_OK;
+}
+
+// The pool as a tensor [page][head][token][d] of 16-bit values, boxes of 64
+// values (128 bytes, swizzled as the MMA reads them) x `box` tokens.
+bool encode_pages(const void *base, const kore_cuda_pages *c, int box, TmaDesc *out) {
+    using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const encode_fn fn = []() -> encode_fn {
+        void *f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess ||
+            r != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            return nullptr;
+        }
+        return reinterpret_cast<encode_fn>(f);
+    }();
+    if (!fn) return false;
+    const cuuint64_t d = c->head_dim, P = c->page_tokens, G = c->n_head_kv;
+    const cuuint64_t dims[4] = {d, P, G, (cuuint64_t)c->n_pages};
+    const cuuint64_t strides[3] = {d * 2, P * d * 2, (cuuint64_t)page_stride(c) * 2};
+    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
+    CUtensorMap m;
+    static_assert(sizeof m == sizeof *out, "tensor map size");
+    if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, boxes, steps,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    memcpy(out, &m, sizeof m);
+    return true;
 }
 
 bool rotates_in_vectors(int d, const kore_cuda_rope_view *r) { return d % 16 == 0 && (!r || r->n_rot % 16 == 0); }
@@ -292,7 +325,8 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
 
 extern "C" long long kore_cuda_paged_attn_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return refuse(KORE_CUDA_EINVAL, "head_dim %d is not supported here", head_dim);
-    return (long long)kPagedZeroed + (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
+    return (long long)(kPagedZeroed + kPagedMaxCtas * kPagedCutBytes) +
+           (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
 }
 
 extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
@@ -359,9 +393,18 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.q_vec = aligned16(*q);
     p.o_vec = aligned16(*out);
     p.counters = static_cast<int *>(workspace);
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed);
+    p.cut = static_cast<char *>(workspace) + kPagedZeroed;
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed + kPagedMaxCtas * kPagedCutBytes);
     p.status = dev_status;
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
+    // more packed rows than a unit of the row kernel takes: the tensor cores
+    if (cache->type != KORE_CUDA_E4M3 && (long long)batch->max_q * p.rep > 16) {
+        p.box = 16;   // the largest power of two, up to a tile, that pages are made of
+        while (p.box < 128 && p.P % (2 * p.box) == 0) p.box *= 2;
+        if (!encode_pages(cache->k, cache, p.box, &p.tm_k) || !encode_pages(cache->v, cache, p.box, &p.tm_v))
+            return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
+        return launched(launch_paged_tiles(p, d, q->type, ctas, (cudaStream_t)stream), "paged_attn");
+    }
     return launched(launch_paged_rows(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
 }
 
