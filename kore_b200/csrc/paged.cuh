@@ -19,7 +19,22 @@ constexpr int kPagedMaxSeqs = 4096;      // sequences of one batch
 constexpr int kPagedMaxCtas = 160;       // CTAs (SMs) that an attention launch uses at most
 constexpr int kPagedRowsMax = 256;       // query rows of a work unit at most
 constexpr size_t kPagedZeroed = 1024;    // leading workspace bytes that are zero between calls
-constexpr size_t kPagedCutBytes = 32;    // of a cut unit's description
+
+// n / d for 0 <= n < 2^31 by a multiplication and a shift (Granlund and
+// Montgomery, 1994): the kernels divide by the group's size and the page's at
+// every unit and tile.
+struct FastDiv {
+    uint32_t mul, shift, d;
+    static FastDiv of(uint32_t d) {
+        uint32_t s = 0;
+        while ((1ull << s) < d) ++s;
+        return {(uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s, d};
+    }
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+    __device__ __forceinline__ int mod(int n, int q) const { return n - q * (int)d; }
+};
 
 // A tensor of rows of heads: element e of head h of row t at t*ts + h*hs + e.
 struct HeadRows {
@@ -51,6 +66,7 @@ struct PagedAttnParams {
     long long page_stride;     // elements
     const int *q_start, *kv_len, *page_table;
     int table_stride, n_seq, n_tok, n_pages, P, H, G, rep;
+    FastDiv by_rep, by_page;
     const void *q;
     void *out;
     long long q_ts, q_hs, o_ts, o_hs;
@@ -61,7 +77,6 @@ struct PagedAttnParams {
     int q_vec, o_vec;          // q (out) rows are 16-byte aligned
     int box;                   // rows of a tensor-map box
     int *counters;             // [kPagedMaxCtas] zero between calls
-    void *cut;                 // [kPagedMaxCtas] units that were cut (many-row kernel)
     float *part;               // [kPagedMaxCtas][2] partial results
     int *status;
 };
@@ -106,7 +121,7 @@ __device__ __forceinline__ Seq load_seq(const PagedAttnParams &p, int s, bool re
 
 // Keys [lo, hi) that some token of the packed rows [r0, r1) of the chunk sees.
 __device__ __forceinline__ void key_range(const PagedAttnParams &p, const Seq &q, int r0, int r1, int &lo, int &hi) {
-    const int first = q.kv - q.n + r0 / p.rep, last = q.kv - q.n + (r1 - 1) / p.rep;
+    const int first = q.kv - q.n + p.by_rep.div(r0), last = q.kv - q.n + p.by_rep.div(r1 - 1);
     hi = p.causal ? min(q.kv, last + 1) : q.kv;
     lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
     hi = max(hi, 0);
@@ -147,78 +162,162 @@ struct Unit {
     }
 };
 
-// Cost of one KV head of a sequence, in tiles: summed by one thread.
+// Cost (tiles and kUnitCost a unit) of blocks b0 + lane of one head of a
+// sequence; 0 behind its last block.
 template <int ROWS, int KEYS>
-__device__ __forceinline__ long long seq_cost(const PagedAttnParams &p, const Seq &q) {
+__device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q, int b, int nb) {
+    if (b >= nb) return 0;
     Unit<ROWS, KEYS> u;
     u.q = q;
-    long long c = 0;
-    const int nb = u.blocks(p);
-    for (u.b = 0; u.b < nb; ++u.b) {
-        u.range(p);
-        c += kUnitCost + u.nt;
+    u.b = b;
+    u.range(p);
+    return kUnitCost + u.nt;
+}
+
+// Asks for a tensor map ahead of its first copy.
+__device__ __forceinline__ void prefetch_map(const TmaDesc *m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
+
+// Quotient of two non-negative numbers that fit 32 bits in all but absurd cases
+// (a 64-bit division takes some hundreds of cycles).
+__device__ __forceinline__ long long quick_div(long long a, long long b) {
+    if (((a | b) >> 32) == 0) return (unsigned)a / (unsigned)b;
+    return a / b;
+}
+
+// One head's cost of the sequences s0 + lane and their blocks: a lane a sequence;
+// sequences of several blocks by the whole warp, a lane a block.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, int s0, Seq &q, int &nb) {
+    const int lane = threadIdx.x & 31;
+    q = Seq{0, 0, 0};
+    if (s0 + lane < p.n_seq) q = load_seq(p, s0 + lane, blockIdx.x == 0);
+    nb = (q.n * p.rep + ROWS - 1) / ROWS;
+    long long cost = nb == 1 ? block_cost<ROWS, KEYS>(p, q, 0, 1) : 0;
+    for (unsigned many = __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {
+        const int from = __ffs(many) - 1;
+        const Seq w{__shfl_sync(0xffffffffu, q.q0, from), __shfl_sync(0xffffffffu, q.n, from),
+                    __shfl_sync(0xffffffffu, q.kv, from)};
+        const int wnb = __shfl_sync(0xffffffffu, nb, from);
+        long long c = 0;
+        for (int b = 0; b < wnb; b += 32)
+            c += __reduce_add_sync(0xffffffffu, (unsigned)block_cost<ROWS, KEYS>(p, w, b + lane, wnb));
+        if (lane == from) cost = c;
     }
-    return c;
+    return cost;
+}
+
+// inclusive sums over the warp
+template <typename T>
+__device__ __forceinline__ T warp_scan(T v) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const T t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
 }
 
 // The CTA's share [x0, x1) of the row of tiles and the unit that x0 lies in.
-// cum: shared memory for n_seq + 1 sums; ctas: CTAs that take a share. Called
-// by every thread of the CTA; false where there is nothing for it to do.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, int min_tiles, Unit<ROWS, KEYS> &u,
+// cum: shared memory for n_seq + 2 sums (batches of more than 32 sequences; up
+// to that every warp finds its share by itself); ctas: CTAs that take a share.
+// Called by every thread of the CTA; false where there is nothing for it to do.
+// Units of no more than WHOLE tiles on average are not cut for the sake of more
+// CTAs, since joining the parts takes as long as some tiles; others may be, down to
+// MIN tiles a CTA.
+template <int ROWS, int KEYS, int WHOLE, int MIN>
+__device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, Unit<ROWS, KEYS> &u,
                                            long long &total, int &ctas, long long &x0, long long &x1) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int s = threadIdx.x; s < p.n_seq; s += blockDim.x) {
-        const Seq q = load_seq(p, s, blockIdx.x == 0);
-        cum[s + 1] = q.n ? seq_cost<ROWS, KEYS>(p, q) : 0ll;
-    }
-    __syncthreads();
-    if (warp == 0) {   // inclusive sums, 32 sequences at a time
-        long long run = 0;
-        for (int s = 0; s < p.n_seq; s += 32) {
-            long long v = s + lane < p.n_seq ? cum[s + lane + 1] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const long long t = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += t;
-            }
-            if (s + lane < p.n_seq) cum[s + lane + 1] = run + v;
-            run += __shfl_sync(0xffffffffu, v, 31);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    const bool few = p.n_seq <= 32;
+    long long units, sum = 0, cost = 0;   // few: this lane's sequence, costs up to and with it
+    Seq q;
+    if (few) {
+        int nb;
+        cost = lane_costs<ROWS, KEYS>(p, 0, q, nb);
+        sum = warp_scan(cost);
+        total = __shfl_sync(0xffffffffu, sum, 31);
+        units = __reduce_add_sync(0xffffffffu, nb);
+    } else {
+        long long &shared_units = cum[p.n_seq + 1];   // of one head of every sequence
+        if (threadIdx.x == 0) shared_units = 0;
+        __syncthreads();
+        for (int s0 = warp * 32; s0 < p.n_seq; s0 += warps * 32) {
+            int nb;
+            const long long c = lane_costs<ROWS, KEYS>(p, s0, q, nb);
+            if (s0 + lane < p.n_seq) cum[s0 + lane + 1] = c;
+            const int n = __reduce_add_sync(0xffffffffu, nb);
+            if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long *>(&shared_units), (unsigned long long)n);
         }
-        if (lane == 0) cum[0] = 0;
+        __syncthreads();
+        if (warp == 0) {   // inclusive sums, 32 sequences at a time
+            long long run = 0;
+            for (int s = 0; s < p.n_seq; s += 32) {
+                const long long v = warp_scan(s + lane < p.n_seq ? cum[s + lane + 1] : 0ll);
+                if (s + lane < p.n_seq) cum[s + lane + 1] = run + v;
+                run += __shfl_sync(0xffffffffu, v, 31);
+            }
+            if (lane == 0) cum[0] = 0;
+        }
+        __syncthreads();
+        total = cum[p.n_seq];
+        units = shared_units;
     }
-    __syncthreads();
-    total = cum[p.n_seq] * p.G;
+    total *= p.G;
     if (total == 0) return false;
-    // no more CTAs than give each a worthwhile number of tiles; never more than
-    // tiles, so that every share holds one
-    const long long most = max(1ll, total / min_tiles);
-    ctas = (int)min((long long)gridDim.x, most);
+    units *= p.G;
+    // (never more CTAs than tiles, so that every share holds one)
+    ctas = (int)min((long long)gridDim.x, total <= (WHOLE + kUnitCost) * units ? units : max(units, quick_div(total, MIN)));
     if ((int)blockIdx.x >= ctas) return false;
-    x0 = total * blockIdx.x / ctas;
-    x1 = total * (blockIdx.x + 1) / ctas;
-    int a = 0, b = p.n_seq - 1;   // the sequence with cum[a] * G <= x0 < cum[a + 1] * G
-    while (a < b) {
-        const int m = (a + b + 1) >> 1;
-        if (cum[m] * p.G <= x0) a = m;
-        else b = m - 1;
+    x0 = quick_div(total * blockIdx.x, ctas);
+    x1 = quick_div(total * (blockIdx.x + 1), ctas);
+    long long before;   // one head's cost of the sequences before u.s
+    if (few) {
+        const int a = __ffs(__ballot_sync(0xffffffffu, sum * p.G > x0)) - 1;
+        before = __shfl_sync(0xffffffffu, sum - cost, a);
+        cost = __shfl_sync(0xffffffffu, cost, a);
+        u.s = a;
+        u.q = Seq{__shfl_sync(0xffffffffu, q.q0, a), __shfl_sync(0xffffffffu, q.n, a), __shfl_sync(0xffffffffu, q.kv, a)};
+    } else {
+        int a = 0, b = p.n_seq - 1;   // the sequence with cum[a] * G <= x0 < cum[a + 1] * G
+        while (a < b) {
+            const int m = (a + b + 1) >> 1;
+            if (cum[m] * p.G <= x0) a = m;
+            else b = m - 1;
+        }
+        u.s = a;
+        u.q = load_seq(p, a, false);
+        before = cum[a];
+        cost = cum[a + 1] - before;
+        __syncthreads();   // cum may be used for something else from here
     }
-    u.s = a;
-    u.q = load_seq(p, a, false);
-    const long long cost = cum[a + 1] - cum[a];   // of one head
-    const long long rem = x0 - cum[a] * p.G;
-    u.g = (int)(rem / cost);
+    const long long rem = x0 - before * p.G;
+    u.g = (int)quick_div(rem, cost);
+    u.u0 = before * p.G + u.g * cost;
+    // the block, a lane each
     u.b = 0;
-    u.u0 = cum[a] * p.G + u.g * cost;
+    const int nb = (u.q.n * p.rep + ROWS - 1) / ROWS;
+    for (int b0 = 0; nb > 1; b0 += 32) {
+        const int c = block_cost<ROWS, KEYS>(p, u.q, b0 + lane, nb);
+        const int v = warp_scan(c);
+        const unsigned in = __ballot_sync(0xffffffffu, u.u0 + v > x0 && c > 0);
+        if (in || b0 + 32 >= nb) {
+            const int at = in ? __ffs(in) - 1 : 0;
+            u.b = b0 + at;
+            u.u0 += __shfl_sync(0xffffffffu, v - c, at);
+            break;
+        }
+        u.u0 += __shfl_sync(0xffffffffu, v, 31);
+    }
     u.range(p);
-    while (u.u0 + kUnitCost + u.nt <= x0) u.next(p);
-    __syncthreads();   // cum may be used for something else from here
     return true;
 }
 
 // The CTA whose share position x of `total` lies in.
 __device__ __forceinline__ int share_of(long long x, long long total, int ctas) {
-    return (int)(((x + 1) * ctas - 1) / total);
+    return (int)quick_div((x + 1) * ctas - 1, total);
 }
 
 }  // namespace kore

@@ -130,8 +130,8 @@ int check_batch(const kore_cuda_batch *b, int n_tok) {
     return KORE_CUDA_OK;
 }
 
-// The pool as a tensor [page][head][token][d] of 16-bit values, boxes of 64
-// values (128 bytes, swizzled as the MMA reads them) x `box` tokens.
+// The pool as a tensor [page][head][token][d], boxes of `box` tokens x 128 bytes
+// (or the 64 of a short row), swizzled within rows of that width.
 bool encode_pages(const void *base, const kore_cuda_pages *c, int box, TmaDesc *out) {
     using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
@@ -149,13 +149,14 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, TmaDesc *
     if (!fn) return false;
     const cuuint64_t d = c->head_dim, P = c->page_tokens, G = c->n_head_kv;
     const cuuint64_t dims[4] = {d, P, G, (cuuint64_t)c->n_pages};
-    const cuuint64_t strides[3] = {d * 2, P * d * 2, (cuuint64_t)page_stride(c) * 2};
-    const cuuint32_t boxes[4] = {64, (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
+    const cuuint64_t b = type_bytes(c->type), width = d * b < 128 ? d * b : 128;
+    const cuuint64_t strides[3] = {d * b, P * d * b, (cuuint64_t)page_stride(c) * b};
+    const cuuint32_t boxes[4] = {(cuuint32_t)(width / b), (cuuint32_t)box, 1, 1}, steps[4] = {1, 1, 1, 1};
     CUtensorMap m;
     static_assert(sizeof m == sizeof *out, "tensor map size");
-    if (fn(&m, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, const_cast<void *>(base), dims, strides, boxes, steps,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    if (fn(&m, b == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, boxes, steps,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     memcpy(out, &m, sizeof m);
     return true;
@@ -325,8 +326,7 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
 
 extern "C" long long kore_cuda_paged_attn_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return refuse(KORE_CUDA_EINVAL, "head_dim %d is not supported here", head_dim);
-    return (long long)(kPagedZeroed + kPagedMaxCtas * kPagedCutBytes) +
-           (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
+    return (long long)kPagedZeroed + (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
 }
 
 extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
@@ -378,6 +378,8 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.H = q->n_head;
     p.G = G;
     p.rep = q->n_head / G;
+    p.by_rep = FastDiv::of((uint32_t)p.rep);
+    p.by_page = FastDiv::of((uint32_t)p.P);
     p.q = q->data;
     p.out = out->data;
     p.q_ts = q->token_stride;
@@ -393,18 +395,18 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.q_vec = aligned16(*q);
     p.o_vec = aligned16(*out);
     p.counters = static_cast<int *>(workspace);
-    p.cut = static_cast<char *>(workspace) + kPagedZeroed;
-    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed + kPagedMaxCtas * kPagedCutBytes);
+    p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed);
     p.status = dev_status;
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
     // more packed rows than a unit of the row kernel takes: the tensor cores
-    if (cache->type != KORE_CUDA_E4M3 && (long long)batch->max_q * p.rep > 16) {
-        p.box = 16;   // the largest power of two, up to a tile, that pages are made of
-        while (p.box < 128 && p.P % (2 * p.box) == 0) p.box *= 2;
-        if (!encode_pages(cache->k, cache, p.box, &p.tm_k) || !encode_pages(cache->v, cache, p.box, &p.tm_v))
-            return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
-        return launched(launch_paged_tiles(p, d, q->type, ctas, (cudaStream_t)stream), "paged_attn");
-    }
+    const bool tiles = cache->type != KORE_CUDA_E4M3 && (long long)batch->max_q * p.rep > 16;
+    // tokens of a box: the largest power of two that divides the page, up to a tile
+    const int most = tiles ? 128 : d * type_bytes(cache->type) == 256 ? 16 : 32;
+    p.box = 16;
+    while (p.box < most && p.P % (2 * p.box) == 0) p.box *= 2;
+    if (!encode_pages(cache->k, cache, p.box, &p.tm_k) || !encode_pages(cache->v, cache, p.box, &p.tm_v))
+        return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
+    if (tiles) return launched(launch_paged_tiles(p, d, q->type, ctas, (cudaStream_t)stream), "paged_attn");
     return launched(launch_paged_rows(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
 }
 

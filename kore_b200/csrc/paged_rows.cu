@@ -9,16 +9,17 @@
 // be used) and everything serves the stream of keys:
 //   * one CTA of 8 warps an SM; each warp streams tiles of its own, a fixed
 //     8 KB (4 KB for 8 bits and d = 64) of K and V, through a ring of 3 (6)
-//     stages filled with 16-byte cp.async (192 KB in flight an SM). No warp
-//     waits for another, and the ring runs on over the ends of units.
+//     stages that TMA boxes fill straight from the pages (192 KB in flight an SM;
+//     16-byte cp.async by the lanes took as many instructions as the products). No
+//     warp waits for another, and the ring runs on over the ends of units.
 //   * work in equal shares (paged.cuh): ragged lengths, one long sequence and
 //     many short ones all end at the same time. A unit cut between CTAs is
 //     joined by the CTA that finishes last, in the CTAs' order, so the sums do not
 //     depend on who that is.
-//   * keys outside the unit's range arrive as zeros (cp.async with a source size
-//     of 0): whatever the page holds there meets neither product.
-//   * the row maximum is moved only when a score passes it by 2^8, so most tiles
-//     rescale nothing; sums and outputs are fp32.
+//   * a page's rows outside the unit's keys are masked in S and cleared in V, so
+//     that whatever the page holds there meets neither product.
+//   * the row maximum is moved only when a score passes it by 2^8 (a vote of the
+//     warp), so most tiles reduce and rescale nothing; sums and outputs are fp32.
 //   * an 8-bit cache is widened to f16 on the way into the fragments (exact: e4m3
 //     has fewer exponent and mantissa bits). The order of d in the first
 //     product's sum is free, so a thread takes 4 consecutive bytes where the
@@ -45,34 +46,36 @@ struct RowsCfg {
     static constexpr int KT = (D == 128 && ES == 2) ? 16 : 32;   // keys of a warp's tile
     static constexpr int STAGES = (D == 64 && ES == 1) ? 6 : 3;
     static constexpr int ROWB = D * ES;                          // bytes of a key
+    static constexpr int HALVES = ROWB == 256 ? 2 : 1;           // boxes are at most 128 bytes wide
+    static constexpr int BOXB = ROWB / HALVES;
     static constexpr int HALF = KT * ROWB;                       // K (V) bytes of a stage
     static constexpr int STAGE = 2 * HALF;
     static constexpr int CT = kWarps * KT;                       // keys of a CTA's tile
     static constexpr int CH = ROWB / 16;                         // 16-byte pieces of a key
     static constexpr int RING = kWarps * STAGES * STAGE;
     static constexpr int MERGE = kWarps * 8 * D * 4;             // 8 rows of every warp
-    static constexpr int CUM = (kPagedMaxSeqs + 1) * 8;          // shares MERGE's place
+    static constexpr int CUM = (kPagedMaxSeqs + 2) * 8;          // shares MERGE's place
     static constexpr int TOP = MERGE > CUM ? MERGE : CUM;
     static constexpr int ML = RING + (TOP + 15) / 16 * 16;
-    static constexpr int BYTES = ML + 2 * kWarps * kRowsU * 8 + 16;
+    static constexpr int BARS = ML + 2 * kWarps * kRowsU * 8;
+    static constexpr int BYTES = BARS + kWarps * STAGES * 8 + 16;
 };
 
-// Byte offset of 16-byte piece c of key r within a stage's half, permuted so
-// that the pieces c of 8 consecutive keys lie in distinct banks.
-template <int ROWB>
+// Byte offset of 16-byte piece c of key r within a stage's half, as the boxes'
+// swizzle leaves it (pieces c of 8 consecutive keys lie in distinct banks).
+template <int ROWB, int KT>
 __device__ __forceinline__ int piece(int r, int c) {
     if constexpr (ROWB == 64) return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
-    else return r * ROWB + ((c ^ (r & 7)) << 4);
+    else return (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool ok) {
-    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar,
+                                        uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+        "l"(map), "r"(x), "r"(tok), "r"(g), "r"(page), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
@@ -113,17 +116,11 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// two e4m3 values (first in the low byte) as two f16
-__device__ __forceinline__ uint32_t widen2(uint32_t x) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(x));
-    return r;
-}
-
-__device__ __forceinline__ uint32_t ld_u32(const void *p, bool aligned) {
-    if (aligned) return __ldg(static_cast<const unsigned int *>(p));
-    const unsigned short *h = static_cast<const unsigned short *>(p);
-    return (uint32_t)__ldg(h) | ((uint32_t)__ldg(h + 1) << 16);
+// four e4m3 values (first in the lowest byte) as two pairs of f16
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t &a, uint32_t &b) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(x));
 }
 
 // QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16).
@@ -134,7 +131,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
     constexpr bool BF = QBF && !E4M3;   // type of the products
     using U = Unit<kRowsU, C::CT>;
     using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
-    extern __shared__ __align__(128) uint8_t smem[];
+    extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int g8 = lane >> 2, t4 = lane & 3;
     float *merge = reinterpret_cast<float *>(smem + C::RING);
@@ -142,17 +139,57 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
     // next unit's while another still reads this one's
     float2 *ml = reinterpret_cast<float2 *>(smem + C::ML);
     int ml_turn = kWarps * kRowsU;
-    int *flag = reinterpret_cast<int *>(smem + C::ML + 2 * kWarps * kRowsU * 8);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + C::BARS) + warp * C::STAGES;   // this warp's stages
+    int *flag = reinterpret_cast<int *>(smem + C::BARS + kWarps * C::STAGES * 8);
+    if (lane < C::STAGES) mbar_init(&full[lane], 1);
+    if (lane == 0) {
+        prefetch_map(&p.tm_k);
+        prefetch_map(&p.tm_v);
+    }
+    mbar_fence_init();
+    __syncwarp();
     grid_dep_wait();
     grid_dep_launch();
 
     U u;
     long long total, x0, x1;
     int ctas;
-    if (!find_share<kRowsU, C::CT>(p, reinterpret_cast<long long *>(smem + C::RING), 2, u, total, ctas, x0, x1)) return;
+    if (!find_share<kRowsU, C::CT, 5, 2>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
-    const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
-    const uint8_t *kbase = static_cast<const uint8_t *>(p.k), *vbase = static_cast<const uint8_t *>(p.v);
+    uint8_t *ring = smem + warp * C::STAGES * C::STAGE;
+
+    // q fragments of the unit's rows g8 and g8 + 8, as they are in memory
+    uint32_t qf[D / 16][4];
+    const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
+    auto load_q = [&]() {
+        const int r0 = u.b * kRowsU + g8, r1 = r0 + 8;
+        const bool in0 = g8 < u.rows, in1 = g8 + 8 < u.rows;
+        const int i0 = p.by_rep.div(r0), i1 = p.by_rep.div(r1);
+        const qt *s0 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i0) * p.q_ts +
+                       (long long)(u.g * p.rep + r0 - i0 * p.rep) * p.q_hs;
+        const qt *s1 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i1) * p.q_ts +
+                       (long long)(u.g * p.rep + r1 - i1 * p.rep) * p.q_hs;
+        auto fill = [&](auto ld) {
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {
+                const int e = E4M3 ? t4 * (D / 4) + 4 * k : 16 * k + 2 * t4;
+                const int f = E4M3 ? e + 2 : e + 8;
+                qf[k][0] = in0 ? ld(s0 + e) : 0u;
+                qf[k][1] = in1 ? ld(s1 + e) : 0u;
+                qf[k][2] = in0 ? ld(s0 + f) : 0u;
+                qf[k][3] = in1 ? ld(s1 + f) : 0u;
+            }
+        };
+        if (p.q_vec) {
+            fill([](const qt *x) { return __ldg(reinterpret_cast<const unsigned int *>(x)); });
+        } else {
+            fill([](const qt *x) {
+                const unsigned short *h = reinterpret_cast<const unsigned short *>(x);
+                return (uint32_t)__ldg(h) | ((uint32_t)__ldg(h + 1) << 16);
+            });
+        }
+    };
+    load_q();
 
     // ---- the load side: a unit and a tile that run ahead of the products
     U lu = u;
@@ -174,55 +211,46 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
     };
     share_tiles(lu, lt, lt1);
     l_skip();
-    // pages of the 16-key groups of the next tile to load, a tile ahead
-    constexpr int NG = C::KT / 16;
-    auto page_of_next = [&]() -> int {   // lane i < NG: page of group i
-        int ph = -1;
-        if (l_more && lane < NG) {
-            const int key = (lu.tile0 + lt) * C::CT + warp * C::KT + lane * 16;
-            if (key < lu.hi && key + 16 > lu.lo) {
-                ph = __ldg(p.page_table + (long long)lu.s * p.table_stride + key / p.P);
-                if (ph < 0 || ph >= p.n_pages) {
+    // a lane a box: K or V, half of d, group of p.box keys; its page a tile ahead
+    const int boxes = 2 * C::HALVES * (C::KT / p.box);
+    const int b_half = (lane >> 1) % C::HALVES, b_key = (lane >> 1) / C::HALVES * p.box;
+    const TmaDesc *map = (lane & 1) ? &p.tm_v : &p.tm_k;
+    const uint32_t b_dst = smem_u32(ring) + (lane & 1) * C::HALF + b_half * (C::KT * 128) + b_key * C::BOXB;
+    const uint64_t policy = l2_evict_first_policy();
+    int b_page, b_tok;   // page -1: the box is not needed
+    auto look_up = [&]() {
+        b_page = -1;
+        if (l_more && lane < boxes) {
+            const int key = (lu.tile0 + lt) * C::CT + warp * C::KT + b_key;
+            if (key < lu.hi && key + p.box > lu.lo) {
+                const int j = p.by_page.div(key);
+                b_tok = p.by_page.mod(key, j);
+                b_page = __ldg(p.page_table + (long long)lu.s * p.table_stride + j);
+                if (b_page < 0 || b_page >= p.n_pages) {
                     raise_error(p.status, DEV_BAD_PAGE);
-                    ph = -1;
+                    b_page = p.n_pages;   // outside the pool: arrives as zeros
                 }
             }
         }
-        return ph;
     };
-    int pages = page_of_next();
+    look_up();
+    uint32_t n_loaded = 0, n_taken = 0;   // tiles of this warp
+    bool dead = false;                    // a copy did not land in time
     int l_stage = 0;
-    auto load_tile = [&]() {   // one tile (or nothing) and its group
-        if (l_more) {
-            const int key0 = (lu.tile0 + lt) * C::CT + warp * C::KT;
-            const uint32_t dst = ring + l_stage * C::STAGE;
-            constexpr int N = C::HALF / 512;   // pieces a lane
-            long long row[NG];
-            bool ok[NG];
-#pragma unroll
-            for (int i = 0; i < NG; ++i) {
-                const int ph = __shfl_sync(FULL, pages, i);
-                ok[i] = ph >= 0;
-                row[i] = ((long long)max(ph, 0) * p.page_stride + ((long long)lu.g * p.P + (key0 + 16 * i) % p.P) * D) * ES;
-            }
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int c = i * 32 + lane;
-                const int r = c / C::CH, cc = c % C::CH;
-                const int grp = (i * 32) / (16 * C::CH);   // all lanes of a step are in one group
-                const bool in = ok[grp] && key0 + r >= lu.lo && key0 + r < lu.hi;
-                const long long off = in ? row[grp] + (r - 16 * grp) * C::ROWB + cc * 16 : 0;
-                cp16(dst + piece<C::ROWB>(r, cc), kbase + off, in);
-                cp16(dst + C::HALF + piece<C::ROWB>(r, cc), vbase + off, in);
-            }
-            ++lt;
-            l_skip();
-            pages = page_of_next();
-        }
+    auto load_tile = [&]() {
+        if (!l_more || dead) return;
+        const unsigned need = __ballot_sync(FULL, b_page >= 0);
+        if (lane == 0) mbar_arrive_expect_tx(&full[l_stage], __popc(need) * p.box * C::BOXB);
+        __syncwarp();
+        if (b_page >= 0)
+            tma_box(b_dst + l_stage * C::STAGE, map, b_half * (C::BOXB / ES), b_tok, lu.g, b_page, &full[l_stage], policy);
         l_stage = l_stage + 1 == C::STAGES ? 0 : l_stage + 1;
-        cp_commit();
+        ++n_loaded;
+        ++lt;
+        l_skip();
+        look_up();
     };
-#pragma unroll
+#pragma unroll 1
     for (int i = 0; i < C::STAGES - 1; ++i) load_tile();
 
     // ---- the products
@@ -242,23 +270,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             key_range(p, u.q, u.b * kRowsU, u.b * kRowsU + 1, t, all_hi);
             key_range(p, u.q, u.b * kRowsU + u.rows - 1, u.b * kRowsU + u.rows, all_lo, t);
 
-            // q fragments
-            uint32_t qf[D / 16][4];
-            float qs0 = p.scale * 1.44269504088896340736f, qs1 = qs0;
+            float qs0 = fabsf(p.scale) * 1.44269504088896340736f, qs1 = qs0;
             {
-                const int i0 = r0 / p.rep, i1 = r1 / p.rep;
-                const qt *s0 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i0) * p.q_ts +
-                               (long long)(u.g * p.rep + r0 - i0 * p.rep) * p.q_hs;
-                const qt *s1 = static_cast<const qt *>(p.q) + (long long)(u.q.q0 + i1) * p.q_ts +
-                               (long long)(u.g * p.rep + r1 - i1 * p.rep) * p.q_hs;
+                if (sign) {
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const int e = E4M3 ? t4 * (D / 4) + 4 * k : 16 * k + 2 * t4;
-                    const int f = E4M3 ? e + 2 : e + 8;
-                    qf[k][0] = in0 ? ld_u32(s0 + e, p.q_vec) : 0;
-                    qf[k][1] = in1 ? ld_u32(s1 + e, p.q_vec) : 0;
-                    qf[k][2] = in0 ? ld_u32(s0 + f, p.q_vec) : 0;
-                    qf[k][3] = in1 ? ld_u32(s1 + f, p.q_vec) : 0;
+                    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) qf[k][i] ^= sign;
                 }
                 if constexpr (E4M3) {
                     if constexpr (QBF) {
@@ -311,65 +329,88 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;   // l: this thread's keys only
 
             for (int tt = t0; tt < t1; ++tt) {
-                cp_wait<C::STAGES - 2>();
-                __syncwarp();   // this tile has landed, and every lane is done with the one before
-                load_tile();    // into the stage of the one before
-                const uint32_t kt = ring + stage * C::STAGE, vt = kt + C::HALF;
+                if (!dead && !__all_sync(FULL, mbar_wait(&full[stage], (n_taken / C::STAGES) & 1, p.status,
+                                                         DEV_WAIT_FULL_TIMEOUT)))
+                    dead = true;
+                if (!dead) ++n_taken;
+                __syncwarp();   // every lane is done with the tile before this one
+                load_tile();    // into its stage
+                uint8_t *st = ring + stage * C::STAGE;
+                const uint32_t kt = smem_u32(st), vt = kt + C::HALF;
                 const int key0 = (u.tile0 + tt) * C::CT + warp * C::KT;
-                if (key0 < u.hi && key0 + C::KT > u.lo) {
-                    float s[C::KT / 8][4];
+                if (!dead && key0 < u.hi && key0 + C::KT > u.lo) {
+                    if (key0 < u.lo || key0 + C::KT > u.hi) {   // rows outside the unit's keys
+                        for (int r = 0; r < C::KT; ++r)
+                            if ((key0 + r < u.lo || key0 + r >= u.hi) && lane < C::CH)
+                                *reinterpret_cast<uint4 *>(st + C::HALF + piece<C::ROWB, C::KT>(r, lane)) = make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();   // before the stage is filled again
+                        __syncwarp();
+                    }
+                    constexpr int NJ = C::KT / 8;   // groups of 8 keys
+                    float s[NJ][4];
 #pragma unroll
-                    for (int j = 0; j < C::KT / 8; ++j) {
-                        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-                        if constexpr (!E4M3) {
+                    for (int j = 0; j < NJ; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+                    // all of K's fragments, then the products with the groups by turns
+                    if constexpr (!E4M3) {
+                        uint32_t b[NJ][D / 32][4];
 #pragma unroll
-                            for (int k = 0; k < D / 32; ++k) {
-                                uint32_t b[4];
-                                ldsm4(b, kt + piece<C::ROWB>(8 * j + (lane & 7), 4 * k + (lane >> 3)));
-                                mma<BF>(s[j], qf[2 * k], b[0], b[1]);
-                                mma<BF>(s[j], qf[2 * k + 1], b[2], b[3]);
-                            }
-                        } else {
-                            // thread t4 takes bytes t4*D/4 .. of key g8
+                        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                            for (int h = 0; h < D / 64; ++h) {
-                                uint32_t w[4];
-                                const uint32_t a = kt + piece<C::ROWB>(8 * j + g8, t4 * (D / 64) + h);
+                            for (int k = 0; k < D / 32; ++k)
+                                ldsm4(b[j][k], kt + piece<C::ROWB, C::KT>(8 * j + (lane & 7), 4 * k + (lane >> 3)));
+#pragma unroll
+                        for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int j = 0; j < NJ; ++j) mma<BF>(s[j], qf[2 * k + h], b[j][k][2 * h], b[j][k][2 * h + 1]);
+                    } else {
+                        // thread t4 takes bytes t4*D/4 .. of key g8
+                        uint32_t w[NJ][D / 64][4];
+#pragma unroll
+                        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                            for (int h = 0; h < D / 64; ++h)
                                 asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
-                                             : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                             : "r"(a)
+                                             : "=r"(w[j][h][0]), "=r"(w[j][h][1]), "=r"(w[j][h][2]), "=r"(w[j][h][3])
+                                             : "r"(kt + piece<C::ROWB, C::KT>(8 * j + g8, t4 * (D / 64) + h))
                                              : "memory");
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    mma<false>(s[j], qf[4 * h + i], widen2(w[i] & 0xffffu), widen2(w[i] >> 16));
-                            }
-                        }
+                        for (int h = 0; h < D / 64; ++h)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int j = 0; j < NJ; ++j) {
+                                    uint32_t b0, b1;
+                                    widen4(w[j][h][i], b0, b1);
+                                    mma<false>(s[j], qf[4 * h + i], b0, b1);
+                                }
                     }
-                    float x0m = -INFINITY, x1m = -INFINITY;
-                    const bool masked = key0 < all_lo || key0 + C::KT > all_hi;
+                    if (key0 < all_lo || key0 + C::KT > all_hi) {
 #pragma unroll
-                    for (int j = 0; j < C::KT / 8; ++j) {
+                        for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            s[j][i] *= qs0;
-                            s[j][2 + i] *= qs1;
-                            if (masked) {
+                            for (int i = 0; i < 2; ++i) {
                                 const int key = key0 + 8 * j + 2 * t4 + i;
                                 if (key < lo0 || key >= hi0) s[j][i] = -INFINITY;
                                 if (key < lo1 || key >= hi1) s[j][2 + i] = -INFINITY;
                             }
-                            x0m = fmaxf(x0m, s[j][i]);
-                            x1m = fmaxf(x1m, s[j][2 + i]);
-                        }
                     }
+                    float x0m = fmaxf(s[0][0], s[0][1]), x1m = fmaxf(s[0][2], s[0][3]);
 #pragma unroll
-                    for (int f = 1; f < 4; f <<= 1) {
-                        x0m = fmaxf(x0m, __shfl_xor_sync(FULL, x0m, f));
-                        x1m = fmaxf(x1m, __shfl_xor_sync(FULL, x1m, f));
+                    for (int j = 1; j < NJ; ++j) {
+                        x0m = fmaxf(x0m, fmaxf(s[j][0], s[j][1]));
+                        x1m = fmaxf(x1m, fmaxf(s[j][2], s[j][3]));
                     }
-                    const bool need0 = x0m > m0 + kSlack, need1 = x1m > m1 + kSlack;
-                    if (__any_sync(FULL, need0 || need1)) {
-                        const float n0 = need0 ? x0m : m0, n1 = need1 ? x1m : m1;
+                    x0m *= qs0;
+                    x1m *= qs1;
+                    if (__any_sync(FULL, x0m > m0 + kSlack || x1m > m1 + kSlack)) {
+#pragma unroll
+                        for (int f = 1; f < 4; f <<= 1) {
+                            x0m = fmaxf(x0m, __shfl_xor_sync(FULL, x0m, f));
+                            x1m = fmaxf(x1m, __shfl_xor_sync(FULL, x1m, f));
+                        }
+                        const float n0 = x0m > m0 + kSlack ? x0m : m0, n1 = x1m > m1 + kSlack ? x1m : m1;
                         const float a0 = n0 == m0 ? 1.f : fast_exp2(m0 - n0), a1 = n1 == m1 ? 1.f : fast_exp2(m1 - n1);
                         m0 = n0;
                         m1 = n1;
@@ -383,13 +424,13 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                             o[i][3] *= a1;
                         }
                     }
-                    const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+                    const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
 #pragma unroll
-                    for (int j = 0; j < C::KT / 8; ++j) {
-                        s[j][0] = fast_exp2(s[j][0] - z0);
-                        s[j][1] = fast_exp2(s[j][1] - z0);
-                        s[j][2] = fast_exp2(s[j][2] - z1);
-                        s[j][3] = fast_exp2(s[j][3] - z1);
+                    for (int j = 0; j < NJ; ++j) {
+                        s[j][0] = fast_exp2(fmaf(s[j][0], qs0, z0));
+                        s[j][1] = fast_exp2(fmaf(s[j][1], qs0, z0));
+                        s[j][2] = fast_exp2(fmaf(s[j][2], qs1, z1));
+                        s[j][3] = fast_exp2(fmaf(s[j][3], qs1, z1));
                         l0 += s[j][0] + s[j][1];
                         l1 += s[j][2] + s[j][3];
                     }
@@ -398,19 +439,23 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                         const uint32_t a[4] = {pack2<BF>(s[2 * jj][0], s[2 * jj][1]), pack2<BF>(s[2 * jj][2], s[2 * jj][3]),
                                                pack2<BF>(s[2 * jj + 1][0], s[2 * jj + 1][1]),
                                                pack2<BF>(s[2 * jj + 1][2], s[2 * jj + 1][3])};
+                        // pieces 2c (b0, b1) and 2c + 1 (b2, b3), keys 0-7 and 8-15
+                        uint32_t b[C::CH / 2][4];
+#pragma unroll
+                        for (int c = 0; c < C::CH / 2; ++c)
+                            ldsm4t(b[c], vt + piece<C::ROWB, C::KT>(16 * jj + (lane & 15), 2 * c + (lane >> 4)));
 #pragma unroll
                         for (int c = 0; c < C::CH / 2; ++c) {
-                            uint32_t b[4];   // pieces 2c (b0, b1) and 2c + 1 (b2, b3), keys 0-7 and 8-15
-                            ldsm4t(b, vt + piece<C::ROWB>(16 * jj + (lane & 7) + (lane & 8), 2 * c + (lane >> 4)));
                             if constexpr (!E4M3) {
-                                mma<BF>(o[2 * c], a, b[0], b[1]);
-                                mma<BF>(o[2 * c + 1], a, b[2], b[3]);
+                                mma<BF>(o[2 * c], a, b[c][0], b[c][1]);
+                                mma<BF>(o[2 * c + 1], a, b[c][2], b[c][3]);
                             } else {
                                 // b holds, for keys 2t and 2t+1, the bytes d = 2g, 2g+1 of the piece
 #pragma unroll
                                 for (int h = 0; h < 2; ++h) {
-                                    const uint32_t w0 = widen2(b[2 * h] & 0xffffu), w1 = widen2(b[2 * h] >> 16);
-                                    const uint32_t y0 = widen2(b[2 * h + 1] & 0xffffu), y1 = widen2(b[2 * h + 1] >> 16);
+                                    uint32_t w0, w1, y0, y1;
+                                    widen4(b[c][2 * h], w0, w1);
+                                    widen4(b[c][2 * h + 1], y0, y1);
                                     const int i = 4 * c + 2 * h;
                                     mma<false>(o[i], a, __byte_perm(w0, w1, 0x5410), __byte_perm(y0, y1, 0x5410));
                                     mma<false>(o[i + 1], a, __byte_perm(w0, w1, 0x7632), __byte_perm(y0, y1, 0x7632));
@@ -441,7 +486,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             constexpr int VW = D / 32;   // values a lane
             const float vs = E4M3 && p.v_scale ? __ldg(p.v_scale + u.g) : 1.f;
             auto write_out = [&](int row, const float (&x)[VW], float M, float L) {   // row of the unit, this lane's values
-                const int r = u.b * kRowsU + row, i = r / p.rep, h = u.g * p.rep + r - i * p.rep;
+                const int r = u.b * kRowsU + row, i = p.by_rep.div(r), h = u.g * p.rep + r - i * p.rep;
                 const float inv = L > 0.f || L != L ? vs / L : 0.f;
                 qt *dst = static_cast<qt *>(p.out) + (long long)(u.q.q0 + i) * p.o_ts + (long long)h * p.o_hs + lane * VW;
                 uint32_t w[VW / 2];
@@ -580,8 +625,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             ml_turn = -ml_turn;
         }
         if (u.u0 + kUnitCost + u.nt >= x1 || !u.next(p)) break;
+        load_q();
     }
-    cp_wait<0>();
+    if (dead)   // copies in flight land before the CTA may end
+        for (uint32_t i = n_taken; i < n_loaded; ++i) mbar_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
 }
 
 template <int D, bool QBF, bool E4M3>

@@ -19,8 +19,10 @@
 //                   read as it lies in the page (keys x d, the MN-major operand), so
 //                   nothing is transposed. In a unit's boundary tiles this warp first clears
 //                   the rows of V outside its keys: 0 * NaN must not reach an output.
-// Work in equal shares (paged.cuh). A unit cut between CTAs leaves fp32 parts in the
-// workspace, which paged_merge_kernel joins in the CTAs' order.
+// Work in equal shares (paged.cuh). The parts of a unit cut between CTAs are joined in
+// a binary tree over the CTAs: the second of two neighbours to finish joins both, so that
+// no CTA waits and no CTA joins more than log2 of the parts; a joint is symmetric in
+// its two sides, so the bits do not depend on who is second.
 // Every wait is bounded; tensor memory is always released.
 
 #include "paged.cuh"
@@ -56,7 +58,7 @@ struct TilesCfg {
     static constexpr uint32_t BYTES = BARS + 512 + 1024;     // barriers, alignment
     static constexpr uint32_t T_S = 0, T_O = 256;            // tensor memory: S/P of tile i at 128 i, O at T_O + D i
     static_assert(BYTES <= 232448, "shared memory of an SM");
-    static_assert(STAGES * TILE >= (kPagedMaxSeqs + 1) * 8, "the sums' place");
+    static_assert(STAGES * TILE >= (kPagedMaxSeqs + 2) * 8, "the sums' place");
 };
 
 // ---------------------------------------------------------------- tcgen05
@@ -175,10 +177,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <int D>
 constexpr size_t kSlot = (size_t)kUnitRows * (D + 2);
 
-struct CutUnit {   // left by the CTA that begins the unit; rows 0: none
-    int rows, row0, q0, g, c1, pad[3];
-};
-
 template <int D, bool BF>
 __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnParams p) {
     using C = TilesCfg<D>;
@@ -197,16 +195,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     uint64_t *drained = bars + 24;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 25);
     int *abort_flag = reinterpret_cast<int *>(bars + 26);
-    CutUnit *cut = reinterpret_cast<CutUnit *>(p.cut) + blockIdx.x;
+    int *join = reinterpret_cast<int *>(bars + 27);   // [2] a tile's joint: whether it is the second
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if (threadIdx.x == 256) {
+        prefetch_map(&p.tm_k);
+        prefetch_map(&p.tm_v);
+    }
+    __syncwarp();
     grid_dep_wait();
     grid_dep_launch();
     U u;
     long long total, x0, x1;
     int ctas;
-    if (threadIdx.x == 0) cut->rows = 0;
-    if (!find_share<kUnitRows, kKeys>(p, reinterpret_cast<long long *>(smem + C::RING), 4, u, total, ctas, x0, x1)) return;
+    if (!find_share<kUnitRows, kKeys, 4, 3>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
@@ -269,13 +271,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 const bool need = key < u.hi && key + p.box > u.lo;
                 int page = p.n_pages;   // outside the pool: zeros
                 if (need) {
-                    page = __ldg(pt + key / p.P);
+                    page = __ldg(pt + p.by_page.div(key));
                     if (page < 0 || page >= p.n_pages) {
                         raise_error(p.status, DEV_BAD_PAGE);
                         page = p.n_pages;
                     }
                 }
-                const int tok = key % p.P;
+                const int tok = p.by_page.mod(key, p.by_page.div(key));
                 const unsigned mask = __ballot_sync(FULL, need && lane < boxes);
                 const uint32_t bytes = __popc(mask) * p.box * 128 * C::HALVES;
 #pragma unroll 1
@@ -397,38 +399,40 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         const uint32_t ts = tmem + C::T_S + 128 * i + lane_off, to = tmem + C::T_O + D * i + lane_off;
         uint32_t n_s = 0, n_o = 0;
         bool ok = true;
-        const float qsign = p.scale < 0.f ? -1.f : 1.f;   // a negative factor goes into q, so that maxima stay maxima
+        const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
         const float qs = fabsf(p.scale) * 1.44269504088896340736f;
         // this thread's q row of unit a into shared memory
         auto load_q = [&](const U &a) {
             if (i * kM >= a.rows) return;
             const int pr = a.b * kUnitRows + i * kM + r;   // packed row
             const bool in = i * kM + r < a.rows;
-            const int tok = pr / p.rep;
+            const int tok = p.by_rep.div(pr);
             const qt *src = static_cast<const qt *>(p.q) + (long long)(a.q.q0 + tok) * p.q_ts +
                             (long long)(a.g * p.rep + pr - tok * p.rep) * p.q_hs;
             uint8_t *dst = smem + i * C::TILE;
+            uint4 v[D / 8];   // all of the row on its way at once
+            if (p.q_vec) {
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c)
+                    v[c] = in ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0, 0, 0, 0);
+            } else {
+#pragma unroll
+                for (int c = 0; c < D / 8; ++c) {
+                    const unsigned short *h = reinterpret_cast<const unsigned short *>(src) + 8 * c;
+                    uint32_t w[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        w[k] = in ? (uint32_t)__ldg(h + 2 * k) | ((uint32_t)__ldg(h + 2 * k + 1) << 16) : 0u;
+                    v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
 #pragma unroll
             for (int c = 0; c < D / 8; ++c) {
-                uint4 v = make_uint4(0, 0, 0, 0);
-                if (in) {
-                    if (p.q_vec) {
-                        v = __ldg(reinterpret_cast<const uint4 *>(src) + c);
-                    } else {
-                        const unsigned short *h = reinterpret_cast<const unsigned short *>(src + 8 * c);
-                        uint32_t w[4];
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) w[k] = (uint32_t)__ldg(h + 2 * k) | ((uint32_t)__ldg(h + 2 * k + 1) << 16);
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    if (qsign < 0.f) {
-                        v.x ^= 0x80008000u;
-                        v.y ^= 0x80008000u;
-                        v.z ^= 0x80008000u;
-                        v.w ^= 0x80008000u;
-                    }
-                }
-                *reinterpret_cast<uint4 *>(dst + (c >> 3) * C::BLOCK + sw128(r, c & 7)) = v;
+                v[c].x ^= sign;
+                v[c].y ^= sign;
+                v[c].z ^= sign;
+                v[c].w ^= sign;
+                *reinterpret_cast<uint4 *>(dst + (c >> 3) * C::BLOCK + sw128(r, c & 7)) = v[c];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -544,9 +548,83 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
             }
             ++n_o;
             fence_after();
-            const bool whole = d0 == 0 && d1 == done.nt;
-            const int tok = pr / p.rep, h = done.g * p.rep + pr - tok * p.rep;
-            if (whole) {
+            // a part of a cut unit: up the tree of its CTAs as far as this one is the
+            // second to finish
+            bool last = d0 == 0 && d1 == done.nt;
+            if (!last) {
+                const int c0 = share_of(done.u0 + kUnitCost, total, ctas);
+                const int n = share_of(done.u0 + kUnitCost + done.nt - 1, total, ctas) - c0 + 1;   // parts
+                const int row = i * kM + r, one = 1 << (16 * i);   // the tiles count apart, in the halves of a counter
+                auto slot_of = [&](int k) { return p.part + (size_t)((c0 + k) * 2 + (k == 0)) * kSlot<D>; };
+                const int me = blockIdx.x - c0;
+                last = true;
+                for (int j = 1; (1 << (j - 1)) < n; ++j) {
+                    const int left = me >> j << j, right = left + (1 << (j - 1));   // first parts of the two sides
+                    if (right >= n) continue;                                      // no right side
+                    int *counter = p.counters + c0 + right;
+                    const bool is_left = me < right;
+                    // has the other side finished? then this one need not be written
+                    if (r == 0) join[i] = (atomicAdd(counter, 0) >> (16 * i)) & 0xffff;
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    int second = *reinterpret_cast<volatile int *>(&join[i]);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    if (!second) {
+                        float *slot = slot_of(is_left ? left : right);
+#pragma unroll 1
+                        for (int c = 0; c < D; c += 32) {
+                            float o[32];
+                            ld32(to + c, reinterpret_cast<uint32_t *>(o));
+                            wait_ld();
+#pragma unroll
+                            for (int k = 0; k < 32; k += 4)
+                                *(reinterpret_cast<float4 *>(slot) + ((c + k) / 4) * kUnitRows + row) =
+                                    make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+                        }
+                        slot[kUnitRows * D + row] = m;
+                        slot[kUnitRows * (D + 1) + row] = l;
+                        __threadfence();
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                        if (r == 0) join[i] = (atomicAdd(counter, one) >> (16 * i)) & 0xffff;
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                        second = *reinterpret_cast<volatile int *>(&join[i]);
+                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                        if (!second) {   // the other side goes on
+                            last = false;
+                            break;
+                        }
+                        if (r == 0) atomicAdd(counter, -one);   // its own count; below the other's
+                    }
+                    if (r == 0) atomicAdd(counter, -one);   // as the next call wants it
+                    __threadfence();
+                    const float *slot = slot_of(is_left ? right : left);
+                    const float m2 = __ldcg(slot + kUnitRows * D + row), l2 = __ldcg(slot + kUnitRows * (D + 1) + row);
+                    const float M = fmaxf(m, m2);
+                    const float a = m == -INFINITY ? 0.f : fast_exp2(m - M), b = m2 == -INFINITY ? 0.f : fast_exp2(m2 - M);
+                    m = M;
+                    l = __fadd_rn(__fmul_rn(a, l), __fmul_rn(b, l2));
+#pragma unroll 1
+                    for (int c = 0; c < D; c += 32) {
+                        float o[32];
+                        float4 x[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k)
+                            x[k] = __ldcg(reinterpret_cast<const float4 *>(slot) + (c / 4 + k) * kUnitRows + row);
+                        ld32(to + c, reinterpret_cast<uint32_t *>(o));
+                        wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            o[4 * k] = __fadd_rn(__fmul_rn(a, o[4 * k]), __fmul_rn(b, x[k].x));
+                            o[4 * k + 1] = __fadd_rn(__fmul_rn(a, o[4 * k + 1]), __fmul_rn(b, x[k].y));
+                            o[4 * k + 2] = __fadd_rn(__fmul_rn(a, o[4 * k + 2]), __fmul_rn(b, x[k].z));
+                            o[4 * k + 3] = __fadd_rn(__fmul_rn(a, o[4 * k + 3]), __fmul_rn(b, x[k].w));
+                        }
+                        st32(to + c, reinterpret_cast<const uint32_t *>(o));
+                    }
+                    wait_st();
+                }
+            }
+            if (last) {
+                const int tok = p.by_rep.div(pr), h = done.g * p.rep + pr - tok * p.rep;
                 const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
                 qt *dst = static_cast<qt *>(p.out) + (long long)(done.q.q0 + tok) * p.o_ts + (long long)h * p.o_hs;
 #pragma unroll 1
@@ -576,31 +654,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 }
                 if (p.lse && in)
                     p.lse[(long long)(done.q.q0 + tok) * p.H + h] = l > 0.f || l != l ? m * 0.69314718055994530942f + logf(l) : -INFINITY;
-            } else {
-                float *slot = p.part + (size_t)(blockIdx.x * 2 + (d0 == 0)) * kSlot<D>;
-                const int row = i * kM + r;
-#pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
-                    ld32(to + c, reinterpret_cast<uint32_t *>(o));
-                    wait_ld();
-#pragma unroll
-                    for (int k = 0; k < 32; k += 4)
-                        *(reinterpret_cast<float4 *>(slot) + ((c + k) / 4) * kUnitRows + row) =
-                            make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                }
-                slot[kUnitRows * D + row] = m;
-                slot[kUnitRows * (D + 1) + row] = l;
-                if (d0 == 0 && threadIdx.x == 0) {
-                    CutUnit cu;
-                    cu.rows = done.rows;
-                    cu.row0 = done.b * kUnitRows;
-                    cu.q0 = done.q.q0;
-                    cu.g = done.g;
-                    cu.c1 = share_of(done.u0 + kUnitCost + done.nt - 1, total, ctas);
-                    cu.pad[0] = cu.pad[1] = cu.pad[2] = 0;
-                    *cut = cu;
-                }
             }
             fence_before();
         }
@@ -611,59 +664,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
-}
-
-// Joins the parts of the units that were cut: CTA (32 rows, CTA that begins the
-// unit); lane = row, a warp takes D/8 columns. Bound by the parts' bytes in L2.
-template <int D, bool BF>
-__global__ void __launch_bounds__(256) paged_merge_kernel(const __grid_constant__ PagedAttnParams p) {
-    grid_dep_wait();
-    grid_dep_launch();
-    const int c0 = blockIdx.y, row = blockIdx.x * 32 + (threadIdx.x & 31), warp = threadIdx.x >> 5;
-    const CutUnit cu = reinterpret_cast<const CutUnit *>(p.cut)[c0];
-    if (row >= cu.rows) return;
-    auto part = [&](int c) { return p.part + (size_t)(c * 2 + (c == c0)) * kSlot<D>; };
-    float M = -INFINITY;
-    for (int c = c0; c <= cu.c1; ++c) M = fmaxf(M, __ldcg(part(c) + kUnitRows * D + row));
-    constexpr int N = D / 32;   // float4 a thread
-    float4 acc[N];
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-    float L = 0.f;
-#pragma unroll 4
-    for (int c = c0; c <= cu.c1; ++c) {
-        const float *s = part(c);
-        const float m = __ldcg(s + kUnitRows * D + row), l = __ldcg(s + kUnitRows * (D + 1) + row);
-        const float w = m == -INFINITY ? 0.f : fast_exp2(m - M);
-        L = fmaf(l, w, L);
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            const float4 v = __ldcg(reinterpret_cast<const float4 *>(s) + (warp * N + k) * kUnitRows + row);
-            acc[k].x = fmaf(w, v.x, acc[k].x);
-            acc[k].y = fmaf(w, v.y, acc[k].y);
-            acc[k].z = fmaf(w, v.z, acc[k].z);
-            acc[k].w = fmaf(w, v.w, acc[k].w);
-        }
-    }
-    using qt = typename std::conditional<BF, __nv_bfloat16, __half>::type;
-    const int pr = cu.row0 + row, tok = pr / p.rep, h = cu.g * p.rep + pr - tok * p.rep;
-    const float inv = L > 0.f || L != L ? 1.f / L : 0.f;
-    qt *dst = static_cast<qt *>(p.out) + (long long)(cu.q0 + tok) * p.o_ts + (long long)h * p.o_hs + warp * N * 4;
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-        const uint32_t a = pack2<BF>(acc[k].x * inv, acc[k].y * inv), b = pack2<BF>(acc[k].z * inv, acc[k].w * inv);
-        if (p.o_vec) {
-            *reinterpret_cast<uint2 *>(dst + 4 * k) = make_uint2(a, b);
-        } else {
-            unsigned short *y = reinterpret_cast<unsigned short *>(dst + 4 * k);
-            y[0] = (unsigned short)(a & 0xffffu);
-            y[1] = (unsigned short)(a >> 16);
-            y[2] = (unsigned short)(b & 0xffffu);
-            y[3] = (unsigned short)(b >> 16);
-        }
-    }
-    if (p.lse && warp == 0)
-        p.lse[(long long)(cu.q0 + tok) * p.H + h] = L > 0.f || L != L ? M * 0.69314718055994530942f + logf(L) : -INFINITY;
 }
 
 template <int D, bool BF>
@@ -680,11 +680,7 @@ cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    if (cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, BF>, p)) return e;
-    cfg.gridDim = dim3(kUnitRows / 32, n_ctas);
-    cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
-    return cudaLaunchKernelEx(&cfg, paged_merge_kernel<D, BF>, p);
+    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, BF>, p);
 }
 
 }  // namespace
