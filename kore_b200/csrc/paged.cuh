@@ -76,6 +76,7 @@ struct PagedAttnParams {
     int causal, window;
     int q_vec, o_vec;          // q (out) rows are 16-byte aligned
     int box;                   // rows of a tensor-map box
+    int small;                 // no sum of costs comes near 2^31
     int *counters;             // [kPagedMaxCtas] zero between calls
     float *part;               // [kPagedMaxCtas][2] partial results
     int *status;
@@ -231,13 +232,14 @@ template <int ROWS, int KEYS, int WHOLE, int MIN>
 __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, Unit<ROWS, KEYS> &u,
                                            long long &total, int &ctas, long long &x0, long long &x1) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const bool few = p.n_seq <= 32;
-    long long units, sum = 0, cost = 0;   // few: this lane's sequence, costs up to and with it
+    const bool few = p.n_seq <= 32 && p.small;
+    long long units, cost = 0;
+    int sum = 0;   // few: of the costs up to this lane's sequence and with it
     Seq q;
     if (few) {
         int nb;
         cost = lane_costs<ROWS, KEYS>(p, 0, q, nb);
-        sum = warp_scan(cost);
+        sum = warp_scan((int)cost);
         total = __shfl_sync(0xffffffffu, sum, 31);
         units = __reduce_add_sync(0xffffffffu, nb);
     } else {
@@ -275,9 +277,9 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     x1 = quick_div(total * (blockIdx.x + 1), ctas);
     long long before;   // one head's cost of the sequences before u.s
     if (few) {
-        const int a = __ffs(__ballot_sync(0xffffffffu, sum * p.G > x0)) - 1;
-        before = __shfl_sync(0xffffffffu, sum - cost, a);
-        cost = __shfl_sync(0xffffffffu, cost, a);
+        const int a = __ffs(__ballot_sync(0xffffffffu, (long long)sum * p.G > x0)) - 1;
+        before = __shfl_sync(0xffffffffu, sum - (int)cost, a);
+        cost = __shfl_sync(0xffffffffu, (int)cost, a);
         u.s = a;
         u.q = Seq{__shfl_sync(0xffffffffu, q.q0, a), __shfl_sync(0xffffffffu, q.n, a), __shfl_sync(0xffffffffu, q.kv, a)};
     } else {

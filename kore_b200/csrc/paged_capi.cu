@@ -398,6 +398,8 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed);
     p.status = dev_status;
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
+    // units are of 16 rows and tiles of 128 keys at least
+    p.small = ((double)n_tok * p.rep / 16 + p.n_seq) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;
     // more packed rows than a unit of the row kernel takes: the tensor cores
     const bool tiles = cache->type != KORE_CUDA_E4M3 && (long long)batch->max_q * p.rep > 16;
     // tokens of a box: the largest power of two that divides the page, up to a tile

@@ -3,22 +3,29 @@
 // (tcgen05, accumulators in tensor memory), sm_100a.
 //
 // out = softmax(scale q K^T) V for units of 256 packed rows (tokens x the group's
-// query heads), as two tiles of 128 rows that take turns: while the softmax of
-// one tile runs, the tensor cores work on the other's products. Bound by the tensor
-// cores (4 d flops a pair of row and key) and, close behind, by the exponentials.
-//   warps 0-3, 4-7  softmax of tile 0, tile 1: a thread owns a row. S from tensor
-//                   memory, mask, online softmax (the reference maximum moves only when
-//                   a score passes it by 2^8; O in tensor memory is rescaled then), P in
-//                   16 bits over S (the A operand of the second product), sums in fp32.
-//                   Prologue: its q row into shared memory, ahead of the last unit's
-//                   epilogue, so that the next unit's first products overlap it.
+// query heads), as two tiles of 128 rows that share the keys' way through shared
+// memory and are otherwise on their own. Bound by the tensor cores (4 d flops a pair
+// of row and key) and, close behind, by the exponentials.
+//   warps 0-3, 4-7  softmax of tile 0, tile 1: a thread owns a row. Per step of 64 keys:
+//                   S from tensor memory, mask, online softmax (the reference maximum
+//                   moves only when a score passes it by 2^8; O in tensor memory is
+//                   rescaled then), P in 16 bits over S (the A operand of the second
+//                   product), sums in fp32.
 //   warp 8          producer: K and V tiles of 128 keys by TMA straight from the pages
 //                   (one box of 16 to 128 tokens a page and half of d, a lane each; a
 //                   page outside the pool arrives as zeros), through a ring.
-//   warp 9          issues the MMAs: S_i = Q_i K_j^T, O_i += P_i V_j, alternating i. V is
-//                   read as it lies in the page (keys x d, the MN-major operand), so
-//                   nothing is transposed. In a unit's boundary tiles this warp first clears
-//                   the rows of V outside its keys: 0 * NaN must not reach an output.
+//   warps 9, 10     issue the MMAs of tile 0, tile 1: for each step j O += P_j V_j, then
+//                   S_{j+2} = Q K_{j+2}^T into the buffer that P_j leaves, so that the
+//                   softmax never waits for the S after its P. (With one S buffer of 128
+//                   keys a tile and one issuing warp a step of 128 keys took 2.25 us, the
+//                   chain softmax, wait, P V, S; a thread's first barrier access after a
+//                   burst of MMAs waits until the burst has left the queue, so each tile
+//                   has its own issuer.) V is read as it lies in the page (keys x d, the
+//                   MN-major operand), so nothing is transposed. In a unit's boundary
+//                   tiles the rows of V outside its keys are cleared first: 0 * NaN must not
+//                   reach an output.
+// Events: tile i's event e is on barrier ev[i][e & 1]: event j of a unit of n steps says
+// that S_j is formed and O += P_{j-2} V done; events n and n + 1 that the last two are.
 // Work in equal shares (paged.cuh). The parts of a unit cut between CTAs are joined in
 // a binary tree over the CTAs: the second of two neighbours to finish joins both, so that
 // no CTA waits and no CTA joins more than log2 of the parts; a joint is symmetric in
@@ -38,13 +45,9 @@ constexpr unsigned FULL = 0xffffffffu;
 constexpr int kM = 128;             // rows of a tile
 constexpr int kUnitRows = 2 * kM;
 constexpr int kKeys = 128;          // keys of a tile
+constexpr int kStep = 64;           // keys of a step
 constexpr float kSlack = 8.0f;      // log2 slack before the reference maximum moves
-// 12 warps: two warpgroups of softmax and one of the rest. They start with 168
-// registers a thread (64512 in all) and move 80 a thread from the last to 40 more for
-// each of the first two: a softmax thread holds a row of 128 scores.
-constexpr int kThreads = 384;
-constexpr int kRegsSoftmax = 208, kRegsRest = 88;
-static_assert((2 * kRegsSoftmax + kRegsRest) * 128 <= 168 * kThreads, "registers at launch");
+constexpr int kThreads = 384;       // 12 warps (one of them idle), 168 registers a thread
 static_assert(kUnitRows == kPagedRowsMax, "workspace slots");
 
 template <int D>
@@ -54,9 +57,10 @@ struct TilesCfg {
     static constexpr uint32_t TILE = HALVES * BLOCK;         // K or V tile
     static constexpr int STAGES = D == 128 ? 4 : 8;
     static constexpr uint32_t RING = 2 * TILE;               // behind q: [2][HALVES][kM rows][128 B]
-    static constexpr uint32_t BARS = RING + STAGES * TILE;
+    static constexpr uint32_t OUT = RING + STAGES * TILE;    // [8 warps][32 rows][128 B] on their way out
+    static constexpr uint32_t BARS = OUT + 8 * 4096;
     static constexpr uint32_t BYTES = BARS + 512 + 1024;     // barriers, alignment
-    static constexpr uint32_t T_S = 0, T_O = 256;            // tensor memory: S/P of tile i at 128 i, O at T_O + D i
+    static constexpr uint32_t T_S = 0, T_O = 256;   // tensor memory: S/P of tile i, buffer b at 128 i + 64 b, O at T_O + D i
     static_assert(BYTES <= 232448, "shared memory of an SM");
     static_assert(STAGES * TILE >= (kPagedMaxSeqs + 2) * 8, "the sums' place");
 };
@@ -66,17 +70,13 @@ struct TilesCfg {
 __device__ __forceinline__ uint32_t sw128(int r, int c) {   // 16-byte piece c of 128-byte row r
     return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
 }
-// Shared-memory matrix descriptors (128-byte swizzle, Blackwell version 1).
-// K-major: groups of 8 rows 1024 bytes apart. MN-major: blocks of 64 columns
-// `lbo` bytes apart, groups of 8 rows (keys) 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k(uint32_t a) {
-    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t a, uint32_t lbo) {
-    return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory matrix descriptors (128-byte swizzle, Blackwell version 1): the low
+// word is the address / 16, the high word and bits 16-29 are the layout's.
+// K-major: groups of 8 rows 1024 bytes apart. MN-major: blocks of 64 columns LBO
+// bytes apart, groups of 8 rows (keys) 1024 bytes apart.
+constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_k(uint32_t a) { return ((a >> 4) & 0x3FFF) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_mn(uint32_t a, uint32_t lbo) { return ((a >> 4) & 0x3FFF) | ((lbo >> 4) << 16); }
 // f16 (0) or bf16 (1) operands of one type, fp32 sums; B K-major or MN-major
 __host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int N) {
     return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
@@ -86,19 +86,32 @@ __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::be
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc)
+// The issuing thread's time is what counts here: an MMA's operands are uniform
+// registers, so the low words come from a warp-wide reduction (whose result is one) and
+// all else is constant.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+__device__ __forceinline__ bool elect() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+template <uint32_t ID, bool ACC>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(ID), "n"(ACC ? 1 : 0),
+                 "n"(kDescHi)
                  : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc)
+template <uint32_t ID>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(ID), "r"(acc),
+                 "n"(kDescHi)
                  : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t *bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 columns of this thread's row
 __device__ __forceinline__ void ld32(uint32_t a, uint32_t *r) {
@@ -157,6 +170,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
+__device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p) {
+    uint32_t v;
+    asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
+__device__ __forceinline__ void st_release(uint32_t *p, uint32_t v) {
+    asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
 template <bool BF>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
     if constexpr (BF) {
@@ -187,15 +208,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::BARS);
     uint64_t *full = bars;                  // [STAGES] a tile has landed
-    uint64_t *empty = bars + 8;             // [STAGES] its MMAs are done
+    uint64_t *empty = bars + 8;             // [STAGES] both issuers' MMAs of it are done
     uint64_t *q_full = bars + 16;           // [2] tile i's q rows are in shared memory (4 warps)
-    uint64_t *s_full = bars + 18;           // [2] S_i is formed (and every MMA before it done)
-    uint64_t *p_full = bars + 20;           // [2] P_i is written, O_i rescaled (4 warps)
-    uint64_t *o_full = bars + 22;           // [2] O_i is complete
-    uint64_t *drained = bars + 24;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 25);
-    int *abort_flag = reinterpret_cast<int *>(bars + 26);
-    int *join = reinterpret_cast<int *>(bars + 27);   // [2] a tile's joint: whether it is the second
+    uint64_t *ev = bars + 18;               // [2][2] events of tile i (above)
+    uint64_t *drained = bars + 22;          // [2]
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
+    int *abort_flag = reinterpret_cast<int *>(bars + 25);
+    // counters that the issuers poll: [8] P written (and O rescaled) by each softmax
+    // warp; [4] unused; ring tiles that have landed (V cleared outside the unit's keys)
+    uint32_t *p_seq = reinterpret_cast<uint32_t *>(bars + 26);
+    uint32_t *landed = reinterpret_cast<uint32_t *>(bars + 30);
+    int *join = reinterpret_cast<int *>(bars + 31);   // [2] a tile's joint: whether it is the second
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 256) {
@@ -213,16 +236,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::STAGES; ++i) {
             mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
+            mbar_init(&empty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
-            mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
-            mbar_init(&o_full[i], 1);
+            mbar_init(&ev[2 * i], 1);
+            mbar_init(&ev[2 * i + 1], 1);
+            mbar_init(&drained[i], 1);
         }
-        mbar_init(drained, 1);
         *abort_flag = 0;
+        for (int i = 0; i < 8; ++i) p_seq[i] = 0;
+        *landed = 0;
         mbar_fence_init();
     }
     fence_proxy_async_smem();   // the sums stood where the ring's copies will land
@@ -246,6 +270,27 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         }
         return __all_sync(FULL, got);
     };
+    // until the counters at word[lane], lane < n, have all reached `want`: bounded, by
+    // whole warps
+    auto reached = [&](const uint32_t *word, int n, uint32_t want) -> bool {
+        uint64_t since = 0;
+        for (uint32_t polls = 0;; ++polls) {
+            const uint32_t v = lane < n ? ld_acquire(word + lane) : want;
+            if (__all_sync(FULL, (int)(v - want) >= 0)) return true;
+            if ((polls & 1023) == 1023) {
+                const uint64_t now = global_ns();
+                if (!since) since = now;
+                const bool late = now - since > kWaitNs;
+                if (__any_sync(FULL, late || *reinterpret_cast<volatile int *>(abort_flag))) {
+                    if (lane == 0) {
+                        raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+                        *reinterpret_cast<volatile int *>(abort_flag) = 1;
+                    }
+                    return false;
+                }
+            }
+        }
+    };
     auto share_tiles = [&](const U &a, int &t0, int &t1) {   // tiles of unit a in [x0, x1)
         const long long first = a.u0 + kUnitCost;
         t0 = (int)max(0ll, min((long long)a.nt, x0 - first));
@@ -253,8 +298,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     };
     auto next_unit = [&](U &a) -> bool { return a.u0 + kUnitCost + a.nt < x1 && a.next(p); };
 
-    if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRest));
+    // steps [k0, k1) of 64 keys (from key 0 on) of tiles [t0, t1) of unit a; one at
+    // least (masked) where it has no keys
+    auto steps = [&](const U &a, int t0, int t1, int &k0, int &k1) {
+        k0 = max(2 * (a.tile0 + t0), a.lo / kStep);
+        k1 = max(k0 + 1, min(2 * (a.tile0 + t1), (a.hi + kStep - 1) / kStep));
+    };
+
     if (warp == 8) {
         // ------------------------------------------------------------ producer
         const int boxes = kKeys / p.box;   // token boxes of a tile; lanes (half of d, box)
@@ -302,137 +352,187 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         if (!ok)   // copies in flight land before the CTA may end
             for (uint32_t i = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; i < it; ++i)
                 mbar_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
-    } else if (warp == 9) {
-        // ------------------------------------------------------------ MMA issuer
-        constexpr uint32_t ID_S = idesc(BF, false, kKeys), ID_O = idesc(BF, true, D);
-        uint32_t it = 0;             // ring position
-        uint32_t n_q[2] = {0, 0}, n_p[2] = {0, 0};   // q and P tiles so far
+    } else if (warp == 9 || warp == 10) {
+        // ------------------------------------------------------------ MMA issuers
+        auto issuer = [&](auto tile) {
+        constexpr int i = decltype(tile)::value;
+        constexpr uint32_t ID_S = idesc(BF, false, kStep), ID_O = idesc(BF, true, D);
+        constexpr uint32_t t_s = C::T_S + 128 * i, t_o = C::T_O + D * i;   // (the CTA holds all of tensor memory, from 0 on)
+        const uint32_t q_lo = uniform(desc_k(sbase + i * C::TILE));
+        uint32_t base = 0;           // ring position of the unit's first tile (K; V follows)
+        uint32_t n_q = 0, n_p = 0, e = 0;   // q and P so far, events
         bool ok = true;
-        auto issue_s = [&](int i, uint32_t at) {   // S_i = Q_i K^T
-            if (lane == 0) {
-                const uint64_t a = desc_k(sbase + i * C::TILE), b = desc_k(sbase + C::RING + (at % C::STAGES) * C::TILE);
-#pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t o = ((k >> 2) * C::BLOCK + (k & 3) * 32) / 16;
-                    mma_ss(tmem + C::T_S + 128 * i, a + o, b + o, ID_S, k > 0);
+        auto stage_of = [&](uint32_t at) { return sbase + C::RING + (at % C::STAGES) * C::TILE; };
+        auto full_wait = [&](uint32_t at) { return reached(landed, 1, at + 1); };
+        do {
+            int t0, t1, k0, k1;
+            share_tiles(u, t0, t1);
+            if (t0 >= t1) continue;
+            steps(u, t0, t1, k0, k1);
+            const int first = u.tile0 + t0;   // the ring's first tile of this unit
+            auto k_at = [&](int k) { return base + 2 * ((k >> 1) - first); };
+            if (i * kM >= u.rows) {   // the tile has no rows: its share of the ring's releases
+                for (int t = 0; ok && t < 2 * (t1 - t0); ++t) {
+                    ok = full_wait(base + t);
+                    if (ok && lane == 0) mbar_arrive(&empty[(base + t) % C::STAGES]);
+                    __syncwarp();
                 }
-                commit(&s_full[i]);
+                base += 2 * (t1 - t0);
+                continue;
             }
-            __syncwarp();
-        };
-        auto issue_pv = [&](int i, uint32_t at, bool first) {   // O_i += P_i V
-            if (lane == 0) {
-                const uint64_t b = desc_mn(sbase + C::RING + (at % C::STAGES) * C::TILE, C::BLOCK);
+            const int n = k1 - k0;
+            // S of step k into the buffer of event `ev_no`, its commit; the K tile is
+            // released behind its last step
+            auto issue_s = [&](int k, uint32_t ev_no) {
+                const uint32_t at = k_at(k), turn = uniform(ev_no & 1);
+                const uint32_t kb = uniform(desc_k(stage_of(at) + (k & 1) * (kStep * 128)));
+                const uint32_t e_bar = uniform(smem_u32(&ev[2 * i + turn])), s_bar = uniform(smem_u32(&empty[at % C::STAGES]));
+                const bool leave = (k & 1) || k + 1 == k1;
+                if (elect()) {
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)
-                    mma_ts(tmem + C::T_O + D * i, tmem + C::T_S + 128 * i + 8 * k, b + k * (16 * 128 / 16), ID_O, !first || k > 0);
+                    for (int c = 0; c < D / 16; ++c) {
+                        const uint32_t o = ((c >> 2) * C::BLOCK + (c & 3) * 32) / 16;
+                        if (c == 0) mma_ss<ID_S, false>(t_s + 64 * turn, q_lo + o, kb + o);
+                        else mma_ss<ID_S, true>(t_s + 64 * turn, q_lo + o, kb + o);
+                    }
+                    commit(e_bar);
+                    if (leave) commit(s_bar);
+                }
+                __syncwarp();
+            };
+            ok = wait(&q_full[i], n_q & 1);
+            ++n_q;
+            for (int j = 0; ok && j < 2; ++j) {
+                if (j < n) {
+                    ok = full_wait(k_at(k0 + j));
+                    if (!ok) break;
+                    fence_after();
+                    issue_s(k0 + j, e + j);
+                } else {   // an event without an S
+                    if (lane == 0) commit(smem_u32(&ev[2 * i + ((e + j) & 1)]));
+                    __syncwarp();
+                }
             }
-            __syncwarp();
+            for (int j = 0; ok && j < n; ++j) {
+                const int k = k0 + j;
+                const uint32_t vt = k_at(k) + 1;
+                if (j == 0 || !(k & 1)) {
+                    ok = full_wait(vt);
+                    if (!ok) break;
+                }
+                if (j + 2 < n) {   // (asked before the wait for P, so that the burst below is one)
+                    ok = full_wait(k_at(k + 2));
+                    if (!ok) break;
+                }
+                ok = reached(p_seq + 4 * i, 4, ++n_p);
+                if (!ok) break;
+                fence_after();
+                const uint32_t b = uniform((e + j) & 1);
+                const uint32_t vb = uniform(desc_mn(stage_of(vt) + (k & 1) * (kStep * 128), C::BLOCK));
+                const uint32_t s_bar = uniform(smem_u32(&empty[vt % C::STAGES])), acc = uniform(j > 0);
+                const bool leave = (k & 1) || k + 1 == k1;
+                if (elect()) {   // O += P V
+#pragma unroll
+                    for (int c = 0; c < kStep / 16; ++c)
+                        mma_ts<ID_O>(t_o, t_s + 64 * b + 8 * c, vb + c * (16 * 128 / 16), c > 0 ? 1u : acc);
+                    if (leave) commit(s_bar);
+                }
+                __syncwarp();
+                if (j + 2 < n) {
+                    issue_s(k + 2, e + j + 2);
+                } else {
+                    if (lane == 0) commit(smem_u32(&ev[2 * i + b]));
+                    __syncwarp();
+                }
+            }
+            e += n + 2;
+            base += 2 * (t1 - t0);
+        } while (ok && next_unit(u));
+        // tensor memory is released below only after every MMA issued here is done
+        if (lane == 0) commit(smem_u32(&drained[i]));
+        __syncwarp();
+        mbar_wait(&drained[i], 0, p.status, DEV_WAIT_FULL_TIMEOUT);
         };
-        auto release = [&](uint32_t at) {
-            if (lane == 0) commit(&empty[at % C::STAGES]);
-            __syncwarp();
-        };
-        auto full_wait = [&](uint32_t at) { return wait(&full[at % C::STAGES], (at / C::STAGES) & 1); };
-        // clears the rows of a V tile outside the unit's keys
-        auto clear_v = [&](const U &a, int t, uint32_t at) {
-            const int key0 = (a.tile0 + t) * kKeys;
-            if (key0 >= a.lo && key0 + kKeys <= a.hi) return;
-            uint8_t *v = smem + C::RING + (at % C::STAGES) * C::TILE;
-            for (int r = lane >> 3; r < kKeys; r += 4)
-                if (key0 + r < a.lo || key0 + r >= a.hi)
-                    for (int h = 0; h < C::HALVES; ++h)
-                        *reinterpret_cast<uint4 *>(v + h * C::BLOCK + r * 128 + (lane & 7) * 16) = make_uint4(0, 0, 0, 0);
-            fence_proxy_async_smem();
-            __syncwarp();
-        };
+        if (warp == 9) issuer(std::integral_constant<int, 0>{});
+        else issuer(std::integral_constant<int, 1>{});
+    } else if (warp == 11) {
+        // ------------------------------------------------------------ watcher
+        // (an issuer's own look at a barrier after a burst of MMAs waits until the
+        // burst has left the queue; a look at a word of shared memory does not)
+        uint32_t it = 0;
+        bool ok = true;
         do {
             int t0, t1;
             share_tiles(u, t0, t1);
-            if (t0 >= t1) continue;
-            const int ni = u.rows > kM ? 2 : 1;
-            // first S of both tiles
-            for (int i = 0; ok && i < ni; ++i) {
-                ok = wait(&q_full[i], n_q[i] & 1) && full_wait(it);
-                if (!ok) break;
-                ++n_q[i];
-                fence_after();
-                issue_s(i, it);
-            }
-            if (ok) release(it);
             for (int t = t0; ok && t < t1; ++t) {
-                const uint32_t vt = it + 1, kt = it + 2;
-                for (int i = 0; i < ni; ++i) {
-                    ok = full_wait(vt);
-                    if (!ok) break;
-                    if (i == 0) clear_v(u, t, vt);
-                    ok = wait(&p_full[i], n_p[i] & 1);
-                    if (!ok) break;
-                    ++n_p[i];
-                    fence_after();
-                    issue_pv(i, vt, t == t0);
-                    if (t + 1 < t1) {
-                        ok = full_wait(kt);
-                        if (!ok) break;
-                        issue_s(i, kt);
-                    } else {
-                        if (lane == 0) commit(&o_full[i]);
-                        __syncwarp();
+                for (int kv = 0; ok && kv < 2; ++kv, ++it) {
+                    ok = wait(&full[it % C::STAGES], (it / C::STAGES) & 1);
+                    const int key0 = (u.tile0 + t) * kKeys;
+                    if (ok && kv == 1 && (key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
+                        uint8_t *v = smem + C::RING + (it % C::STAGES) * C::TILE;
+                        for (int r = lane >> 3; r < kKeys; r += 4)
+                            if (key0 + r < u.lo || key0 + r >= u.hi)
+                                for (int h = 0; h < C::HALVES; ++h)
+                                    *reinterpret_cast<uint4 *>(v + h * C::BLOCK + r * 128 + (lane & 7) * 16) =
+                                        make_uint4(0, 0, 0, 0);
+                        fence_proxy_async_smem();
                     }
+                    __syncwarp();
+                    if (ok && lane == 0) st_release(landed, it + 1);
                 }
-                if (!ok) break;
-                release(vt);
-                if (t + 1 < t1) release(kt);
-                it += 2;
             }
         } while (ok && next_unit(u));
-        // tensor memory is released below only after every MMA issued here is done
-        if (lane == 0) commit(drained);
-        __syncwarp();
-        mbar_wait(drained, 0, p.status, DEV_WAIT_FULL_TIMEOUT);
-    }
-    } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
+    } else if (warp < 8) {
         // ------------------------------------------------------------ softmax
         const int i = warp >> 2, r = threadIdx.x & 127;   // tile, row
         const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + C::T_S + 128 * i + lane_off, to = tmem + C::T_O + D * i + lane_off;
-        uint32_t n_s = 0, n_o = 0;
+        uint8_t *out_rows = smem + C::OUT + warp * 4096;
+        uint32_t e = 0, n_p = 0;   // events before this unit, P written so far
         bool ok = true;
         const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
         const float qs = fabsf(p.scale) * 1.44269504088896340736f;
-        // this thread's q row of unit a into shared memory
+        // offset of this thread's row of unit a in rows of strides ts, hs (of the unit's
+        // first row where it has none): the warp's lanes ask one another for theirs
+        auto offset_of = [&](const U &a, long long t_s, long long h_s) -> long long {
+            const int row = i * kM + r;
+            const int pr = a.b * kUnitRows + (row < a.rows ? row : 0), tok = p.by_rep.div(pr);
+            return (long long)(a.q.q0 + tok) * t_s + (long long)(a.g * p.rep + pr - tok * p.rep) * h_s;
+        };
+        // the q rows of unit a into shared memory: a warp its 32 rows, half a warp a
+        // row at d = 128 (a thread its own row would touch a cache line a lane), all of
+        // them on their way at once
         auto load_q = [&](const U &a) {
             if (i * kM >= a.rows) return;
-            const int pr = a.b * kUnitRows + i * kM + r;   // packed row
-            const bool in = i * kM + r < a.rows;
-            const int tok = p.by_rep.div(pr);
-            const qt *src = static_cast<const qt *>(p.q) + (long long)(a.q.q0 + tok) * p.q_ts +
-                            (long long)(a.g * p.rep + pr - tok * p.rep) * p.q_hs;
-            uint8_t *dst = smem + i * C::TILE;
-            uint4 v[D / 8];   // all of the row on its way at once
+            constexpr int L = D / 8, N = L;   // lanes a row, loads a lane
+            const int c = lane % L;
+            const long long off = offset_of(a, p.q_ts, p.q_hs);
+            uint8_t *dst = smem + i * C::TILE + (c >> 3) * C::BLOCK;
+            uint4 v[N];
             if (p.q_vec) {
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c)
-                    v[c] = in ? __ldg(reinterpret_cast<const uint4 *>(src) + c) : make_uint4(0, 0, 0, 0);
+                for (int k = 0; k < N; ++k)
+                    v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const qt *>(p.q) +
+                                                                 __shfl_sync(FULL, off, k * (32 / L) + lane / L) + 8 * c));
             } else {
 #pragma unroll
-                for (int c = 0; c < D / 8; ++c) {
-                    const unsigned short *h = reinterpret_cast<const unsigned short *>(src) + 8 * c;
+                for (int k = 0; k < N; ++k) {
+                    const unsigned short *h = static_cast<const unsigned short *>(p.q) + __shfl_sync(FULL, off, k * (32 / L) + lane / L) + 8 * c;
                     uint32_t w[4];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        w[k] = in ? (uint32_t)__ldg(h + 2 * k) | ((uint32_t)__ldg(h + 2 * k + 1) << 16) : 0u;
-                    v[c] = make_uint4(w[0], w[1], w[2], w[3]);
+                    for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__ldg(h + 2 * x) | ((uint32_t)__ldg(h + 2 * x + 1) << 16);
+                    v[k] = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             }
 #pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-                v[c].x ^= sign;
-                v[c].y ^= sign;
-                v[c].z ^= sign;
-                v[c].w ^= sign;
-                *reinterpret_cast<uint4 *>(dst + (c >> 3) * C::BLOCK + sw128(r, c & 7)) = v[c];
+            for (int k = 0; k < N; ++k) {
+                const int row = (warp & 3) * 32 + k * (32 / L) + lane / L;
+                v[k].x ^= sign;
+                v[k].y ^= sign;
+                v[k].z ^= sign;
+                v[k].w ^= sign;
+                if (i * kM + row >= a.rows) v[k] = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4 *>(dst + sw128(row, c & 7)) = v[k];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -462,29 +562,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 key_range(p, u.q, b1 - 1, b1, all_lo, x);
             }
             float m = -INFINITY, l = 0.f;
+            int k0, k1;
+            steps(u, t0, t1, k0, k1);
+            auto event = [&](uint32_t no) { return wait(&ev[2 * i + (no & 1)], (no >> 1) & 1); };
             if (mine) {
-                for (int t = t0; t < t1; ++t) {
-                    if (!wait(&s_full[i], n_s & 1)) {
+                for (int k = k0; k < k1; ++k) {
+                    const uint32_t no = e + (k - k0), tb = ts + 64 * (no & 1);
+                    if (!event(no)) {
                         ok = false;
                         break;
                     }
-                    ++n_s;
                     fence_after();
-                    float s[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) ld32(ts + 32 * c, reinterpret_cast<uint32_t *>(s) + 32 * c);
+                    float s[64];
+                    ld32(tb, reinterpret_cast<uint32_t *>(s));
+                    ld32(tb + 32, reinterpret_cast<uint32_t *>(s) + 32);
                     wait_ld();
-                    const int key0 = (u.tile0 + t) * kKeys;
-                    if (key0 < all_lo || key0 + kKeys > all_hi) {
+                    const int key0 = k * kStep;
+                    if (key0 < all_lo || key0 + kStep > all_hi) {
 #pragma unroll
-                        for (int k = 0; k < 128; ++k)
-                            if (key0 + k < lo || key0 + k >= hi) s[k] = -INFINITY;
+                        for (int x = 0; x < 64; ++x)
+                            if (key0 + x < lo || key0 + x >= hi) s[x] = -INFINITY;
                     }
                     float mx[8];
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) mx[k] = s[k];
+                    for (int x = 0; x < 8; ++x) mx[x] = s[x];
 #pragma unroll
-                    for (int k = 8; k < 128; k += 2) mx[(k >> 1) & 7] = max3(mx[(k >> 1) & 7], s[k], s[k + 1]);
+                    for (int x = 8; x < 64; x += 2) mx[(x >> 1) & 7] = max3(mx[(x >> 1) & 7], s[x], s[x + 1]);
                     const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], mx[4], mx[5]), fmaxf(mx[6], mx[7])) * qs;
                     const bool need = top > m + kSlack;
                     if (__any_sync(FULL, need)) {
@@ -493,7 +596,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                             m = top;
                             l *= a;
                         }
-                        if (t > t0) {
+                        if (k > k0) {   // O holds every step before this one only now
+                            if (!event(no + 1)) {
+                                ok = false;
+                                break;
+                            }
+                            fence_after();
                             const unsigned long long aa = pk2(a, a);
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
@@ -501,7 +609,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                                 ld32(to + c, reinterpret_cast<uint32_t *>(o));
                                 wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 32; k += 2) upk2(mul2(pk2(o[k], o[k + 1]), aa), o[k], o[k + 1]);
+                                for (int x = 0; x < 32; x += 2) upk2(mul2(pk2(o[x], o[x + 1]), aa), o[x], o[x + 1]);
                                 st32(to + c, reinterpret_cast<const uint32_t *>(o));
                             }
                         }
@@ -509,32 +617,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                     const float z = m == -INFINITY ? 0.f : -m;
                     const unsigned long long qq = pk2(qs, qs), zz = pk2(z, z);
                     unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
+                    uint32_t w[32];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[32];
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) {
-                            const int e = 64 * h + 2 * k;
-                            float a, b;
-                            upk2(fma2(pk2(s[e], s[e + 1]), qq, zz), a, b);
-                            a = fast_exp2(a);
-                            b = fast_exp2(b);
-                            acc[k & 3] = add2(acc[k & 3], pk2(a, b));
-                            w[k] = pack2<BF>(a, b);
-                        }
-                        st32(ts + 32 * h, w);
+                    for (int x = 0; x < 32; ++x) {
+                        float a, b;
+                        upk2(fma2(pk2(s[2 * x], s[2 * x + 1]), qq, zz), a, b);
+                        a = fast_exp2(a);
+                        b = fast_exp2(b);
+                        acc[x & 3] = add2(acc[x & 3], pk2(a, b));
+                        w[x] = pack2<BF>(a, b);
                     }
+                    st32(tb, w);
                     float x, y;
                     upk2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), x, y);
                     l += x + y;
                     wait_st();
                     fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&p_full[i]);
+                    ++n_p;
+                    if (lane == 0) st_release(p_seq + warp, n_p);
                 }
+                // the last product, before the next unit's events
+                if (ok) ok = event(e + (k1 - k0) + 1);
+                e += k1 - k0 + 2;
             }
+            fence_after();
             // the next unit's q, so that its products may start during the epilogue
-            // (every S of this unit is formed, so its q has been read)
             const U done = u;
             const int d0 = t0, d1 = t1;
             if (ok) {
@@ -542,12 +650,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 if (more) load_q(u);
             }
             if (!ok || !mine) continue;
-            if (!wait(&o_full[i], n_o & 1)) {
-                ok = false;
-                break;
-            }
-            ++n_o;
-            fence_after();
             // a part of a cut unit: up the tree of its CTAs as far as this one is the
             // second to finish
             bool last = d0 == 0 && d1 == done.nt;
@@ -563,95 +665,104 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                     if (right >= n) continue;                                      // no right side
                     int *counter = p.counters + c0 + right;
                     const bool is_left = me < right;
-                    // has the other side finished? then this one need not be written
-                    if (r == 0) join[i] = (atomicAdd(counter, 0) >> (16 * i)) & 0xffff;
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                    int second = *reinterpret_cast<volatile int *>(&join[i]);
-                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                    if (!second) {
-                        float *slot = slot_of(is_left ? left : right);
+                    float *slot = slot_of(is_left ? left : right);
 #pragma unroll 1
-                        for (int c = 0; c < D; c += 32) {
-                            float o[32];
-                            ld32(to + c, reinterpret_cast<uint32_t *>(o));
-                            wait_ld();
+                    for (int c = 0; c < D; c += 64) {
+                        float o[64];
+                        ld32(to + c, reinterpret_cast<uint32_t *>(o));
+                        ld32(to + c + 32, reinterpret_cast<uint32_t *>(o) + 32);
+                        wait_ld();
 #pragma unroll
-                            for (int k = 0; k < 32; k += 4)
-                                *(reinterpret_cast<float4 *>(slot) + ((c + k) / 4) * kUnitRows + row) =
-                                    make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-                        }
-                        slot[kUnitRows * D + row] = m;
-                        slot[kUnitRows * (D + 1) + row] = l;
-                        __threadfence();
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                        if (r == 0) join[i] = (atomicAdd(counter, one) >> (16 * i)) & 0xffff;
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                        second = *reinterpret_cast<volatile int *>(&join[i]);
-                        asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
-                        if (!second) {   // the other side goes on
-                            last = false;
-                            break;
-                        }
-                        if (r == 0) atomicAdd(counter, -one);   // its own count; below the other's
+                        for (int k = 0; k < 64; k += 4)
+                            *(reinterpret_cast<float4 *>(slot) + ((c + k) / 4) * kUnitRows + row) =
+                                make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
-                    if (r == 0) atomicAdd(counter, -one);   // as the next call wants it
+                    slot[kUnitRows * D + row] = m;
+                    slot[kUnitRows * (D + 1) + row] = l;
                     __threadfence();
-                    const float *slot = slot_of(is_left ? right : left);
-                    const float m2 = __ldcg(slot + kUnitRows * D + row), l2 = __ldcg(slot + kUnitRows * (D + 1) + row);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    if (r == 0) join[i] = (atomicAdd(counter, one) >> (16 * i)) & 0xffff;
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    const int second = *reinterpret_cast<volatile int *>(&join[i]);
+                    asm volatile("bar.sync %0, 128;" ::"r"(1 + i) : "memory");
+                    if (!second) {   // the other side goes on
+                        last = false;
+                        break;
+                    }
+                    if (r == 0) atomicAdd(counter, -2 * one);   // as the next call wants it
+                    __threadfence();
+                    const float *other = slot_of(is_left ? right : left);
+                    const float m2 = __ldcg(other + kUnitRows * D + row), l2 = __ldcg(other + kUnitRows * (D + 1) + row);
                     const float M = fmaxf(m, m2);
                     const float a = m == -INFINITY ? 0.f : fast_exp2(m - M), b = m2 == -INFINITY ? 0.f : fast_exp2(m2 - M);
                     m = M;
                     l = __fadd_rn(__fmul_rn(a, l), __fmul_rn(b, l2));
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 32) {
-                        float o[32];
-                        float4 x[8];
+                    for (int c = 0; c < D; c += 64) {
+                        float4 x[16];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k)
-                            x[k] = __ldcg(reinterpret_cast<const float4 *>(slot) + (c / 4 + k) * kUnitRows + row);
+                        for (int k = 0; k < 16; ++k)
+                            x[k] = __ldcg(reinterpret_cast<const float4 *>(other) + (c / 4 + k) * kUnitRows + row);
+                        float o[64];
                         ld32(to + c, reinterpret_cast<uint32_t *>(o));
+                        ld32(to + c + 32, reinterpret_cast<uint32_t *>(o) + 32);
                         wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) {
+                        for (int k = 0; k < 16; ++k) {
                             o[4 * k] = __fadd_rn(__fmul_rn(a, o[4 * k]), __fmul_rn(b, x[k].x));
                             o[4 * k + 1] = __fadd_rn(__fmul_rn(a, o[4 * k + 1]), __fmul_rn(b, x[k].y));
                             o[4 * k + 2] = __fadd_rn(__fmul_rn(a, o[4 * k + 2]), __fmul_rn(b, x[k].z));
                             o[4 * k + 3] = __fadd_rn(__fmul_rn(a, o[4 * k + 3]), __fmul_rn(b, x[k].w));
                         }
                         st32(to + c, reinterpret_cast<const uint32_t *>(o));
+                        st32(to + c + 32, reinterpret_cast<const uint32_t *>(o) + 32);
                     }
                     wait_st();
                 }
             }
             if (last) {
-                const int tok = p.by_rep.div(pr), h = done.g * p.rep + pr - tok * p.rep;
                 const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-                qt *dst = static_cast<qt *>(p.out) + (long long)(done.q.q0 + tok) * p.o_ts + (long long)h * p.o_hs;
+                const long long off = offset_of(done, p.o_ts, p.o_hs);
+                // 64 values of the warp's 32 rows at a time through shared memory: 8 lanes
+                // write a row's 128 bytes (a thread its own row would touch a line a lane)
 #pragma unroll 1
-                for (int c = 0; c < D; c += 32) {
-                    float o[32];
+                for (int c = 0; c < D; c += 64) {
+                    float o[64];
                     ld32(to + c, reinterpret_cast<uint32_t *>(o));
+                    ld32(to + c + 32, reinterpret_cast<uint32_t *>(o) + 32);
                     wait_ld();
-                    uint32_t w[16];
+                    // (a row without keys: O is 0 * V of cleared rows)
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        // (a row without keys: O is 0 * V of cleared rows)
-                        w[k] = pack2<BF>(o[2 * k] * inv, o[2 * k + 1] * inv);
-                    if (in) {
-                        if (p.o_vec) {
+                    for (int x = 0; x < 8; ++x)
+                        *reinterpret_cast<uint4 *>(out_rows + sw128(lane, x)) =
+                            make_uint4(pack2<BF>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<BF>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                                       pack2<BF>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                                       pack2<BF>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+                    __syncwarp();
+                    uint4 v[8];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                *(reinterpret_cast<uint4 *>(dst + c) + k) = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-                        } else {
-                            unsigned short *y = reinterpret_cast<unsigned short *>(dst + c);
+                    for (int x = 0; x < 8; ++x) v[x] = *reinterpret_cast<const uint4 *>(out_rows + sw128(4 * x + (lane >> 3), lane & 7));
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                y[2 * k] = (unsigned short)(w[k] & 0xffffu);
-                                y[2 * k + 1] = (unsigned short)(w[k] >> 16);
+                    for (int x = 0; x < 8; ++x) {
+                        const int lr = 4 * x + (lane >> 3);   // row of the warp
+                        qt *dst = static_cast<qt *>(p.out) + __shfl_sync(FULL, off, lr) + c + 8 * (lane & 7);
+                        if (i * kM + (warp & 3) * 32 + lr < done.rows) {
+                            if (p.o_vec) {
+                                *reinterpret_cast<uint4 *>(dst) = v[x];
+                            } else {
+                                unsigned short *y = reinterpret_cast<unsigned short *>(dst);
+                                const uint32_t w[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) {
+                                    y[2 * k] = (unsigned short)(w[k] & 0xffffu);
+                                    y[2 * k + 1] = (unsigned short)(w[k] >> 16);
+                                }
                             }
                         }
                     }
+                    __syncwarp();
                 }
+                const int tok = p.by_rep.div(pr), h = done.g * p.rep + pr - tok * p.rep;
                 if (p.lse && in)
                     p.lse[(long long)(done.q.q0 + tok) * p.H + h] = l > 0.f || l != l ? m * 0.69314718055994530942f + logf(l) : -INFINITY;
             }
