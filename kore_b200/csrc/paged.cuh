@@ -82,11 +82,25 @@ struct PagedAttnParams {
     int *status;
 };
 
+// four e4m3 values (first in the lowest byte) as two pairs of f16
+__device__ __forceinline__ void widen4(uint32_t x, uint32_t &a, uint32_t &b) {
+    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(a), "=r"(b)
+        : "r"(x));
+}
+
+// The power of two that takes a row's largest value m to 2^7 .. 2^8: bf16 values down
+// to 2^-22 of it are then exact in f16. 1 for 0, infinities and NaN.
+__device__ __forceinline__ float f16_shift(float m) {
+    const int e = (__float_as_int(m) >> 23) - 127;
+    return m > 0.f && m < INFINITY ? __int_as_float((127 + min(max(7 - e, -100), 100)) << 23) : 1.f;
+}
+
 cudaError_t launch_rope_table(const float *freq, int half, double amp, int n_pos, float *table, cudaStream_t s);
 cudaError_t launch_rotate(const RotateParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
 // n_ctas: SMs of the device, at most kPagedMaxCtas
 cudaError_t launch_paged_rows(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
-cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int type, int n_ctas, cudaStream_t s);
+cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
 
 // ---------------------------------------------------------------- division of the attention's work
 //

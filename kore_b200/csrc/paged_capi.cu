@@ -131,8 +131,8 @@ int check_batch(const kore_cuda_batch *b, int n_tok) {
 }
 
 // The pool as a tensor [page][head][token][d], boxes of `box` tokens x 128 bytes
-// (or the 64 of a short row), swizzled within rows of that width.
-bool encode_pages(const void *base, const kore_cuda_pages *c, int box, TmaDesc *out) {
+// (or the 64 of a short row), swizzled within rows of that width or (plain) as it is.
+bool encode_pages(const void *base, const kore_cuda_pages *c, int box, bool plain, TmaDesc *out) {
     using encode_fn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                    const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -155,7 +155,7 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, TmaDesc *
     CUtensorMap m;
     static_assert(sizeof m == sizeof *out, "tensor map size");
     if (fn(&m, b == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void *>(base), dims, strides, boxes, steps,
-           CU_TENSOR_MAP_INTERLEAVE_NONE, width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+           CU_TENSOR_MAP_INTERLEAVE_NONE, plain ? CU_TENSOR_MAP_SWIZZLE_NONE : width == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     memcpy(out, &m, sizeof m);
@@ -401,14 +401,15 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     // units are of 16 rows and tiles of 128 keys at least
     p.small = ((double)n_tok * p.rep / 16 + p.n_seq) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;
     // more packed rows than a unit of the row kernel takes: the tensor cores
-    const bool tiles = cache->type != KORE_CUDA_E4M3 && (long long)batch->max_q * p.rep > 16;
+    const bool tiles = (long long)batch->max_q * p.rep > 16;
+    const bool plain = tiles && cache->type == KORE_CUDA_E4M3;   // widened before it is read as an operand
     // tokens of a box: the largest power of two that divides the page, up to a tile
     const int most = tiles ? 128 : d * type_bytes(cache->type) == 256 ? 16 : 32;
     p.box = 16;
     while (p.box < most && p.P % (2 * p.box) == 0) p.box *= 2;
-    if (!encode_pages(cache->k, cache, p.box, &p.tm_k) || !encode_pages(cache->v, cache, p.box, &p.tm_v))
+    if (!encode_pages(cache->k, cache, p.box, plain, &p.tm_k) || !encode_pages(cache->v, cache, p.box, plain, &p.tm_v))
         return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
-    if (tiles) return launched(launch_paged_tiles(p, d, q->type, ctas, (cudaStream_t)stream), "paged_attn");
+    if (tiles) return launched(launch_paged_tiles(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
     return launched(launch_paged_rows(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
 }
 

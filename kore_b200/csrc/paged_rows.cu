@@ -116,13 +116,6 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
-// four e4m3 values (first in the lowest byte) as two pairs of f16
-__device__ __forceinline__ void widen4(uint32_t x, uint32_t &a, uint32_t &b) {
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
-        : "=r"(a), "=r"(b)
-        : "r"(x));
-}
-
 // QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16).
 template <int D, bool QBF, bool E4M3>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
@@ -296,11 +289,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                             m0 = fmaxf(m0, __shfl_xor_sync(FULL, m0, o));
                             m1 = fmaxf(m1, __shfl_xor_sync(FULL, m1, o));
                         }
-                        auto shift = [](float m) {   // 2^(7 - exponent of m); 1 for 0, infinities and NaN
-                            const int e = (__float_as_int(m) >> 23) - 127;
-                            return m > 0.f && m < INFINITY ? __int_as_float((127 + min(max(7 - e, -100), 100)) << 23) : 1.f;
-                        };
-                        const float f0 = shift(m0), f1 = shift(m1);
+                        const float f0 = f16_shift(m0), f1 = f16_shift(m1);
                         qs0 /= f0;
                         qs1 /= f1;
 #pragma unroll

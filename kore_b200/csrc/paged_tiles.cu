@@ -47,19 +47,25 @@ constexpr int kUnitRows = 2 * kM;
 constexpr int kKeys = 128;          // keys of a tile
 constexpr int kStep = 64;           // keys of a step
 constexpr float kSlack = 8.0f;      // log2 slack before the reference maximum moves
-constexpr int kThreads = 384;       // 12 warps (one of them idle), 168 registers a thread
 static_assert(kUnitRows == kPagedRowsMax, "workspace slots");
 
-template <int D>
+// E8: an 8-bit cache, whose tiles land in a ring of their own (as they are in memory) and
+// are widened into the 16-bit ring by four more warps.
+template <int D, bool E8>
 struct TilesCfg {
     static constexpr int HALVES = D / 64;                    // 128-byte wide column blocks
     static constexpr uint32_t BLOCK = kKeys * 128;           // bytes of one such block of a tile
     static constexpr uint32_t TILE = HALVES * BLOCK;         // K or V tile
-    static constexpr int STAGES = D == 128 ? 4 : 8;
+    static constexpr int STAGES = E8 ? (D == 128 ? 3 : 6) : D == 128 ? 4 : 8;
+    static constexpr int THREADS = E8 ? 512 : 384;           // 168 or 128 registers a thread
+    static constexpr uint32_t RAW_TILE = kKeys * D;          // 8-bit K or V tile
+    static constexpr int RAW_STAGES = D == 128 ? 2 : 4;
+    static constexpr int LOADS = E8 ? RAW_STAGES : STAGES;   // stages that the copies fill
     static constexpr uint32_t RING = 2 * TILE;               // behind q: [2][HALVES][kM rows][128 B]
     static constexpr uint32_t OUT = RING + STAGES * TILE;    // [8 warps][32 rows][128 B] on their way out
-    static constexpr uint32_t BARS = OUT + 8 * 4096;
-    static constexpr uint32_t BYTES = BARS + 512 + 1024;     // barriers, alignment
+    static constexpr uint32_t RAW = OUT + 8 * 4096;
+    static constexpr uint32_t BARS = RAW + (E8 ? RAW_STAGES * RAW_TILE : 0);
+    static constexpr uint32_t BYTES = BARS + 512 + (E8 ? 2 * kM * 4 : 0) + 1024;   // barriers, alignment
     static constexpr uint32_t T_S = 0, T_O = 256;   // tensor memory: S/P of tile i, buffer b at 128 i + 64 b, O at T_O + D i
     static_assert(BYTES <= 232448, "shared memory of an SM");
     static_assert(STAGES * TILE >= (kPagedMaxSeqs + 2) * 8, "the sums' place");
@@ -134,6 +140,13 @@ __device__ __forceinline__ void st32(uint32_t a, const uint32_t *r) {
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t a, const uint32_t *r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
 __device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
@@ -198,27 +211,33 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 template <int D>
 constexpr size_t kSlot = (size_t)kUnitRows * (D + 2);
 
-template <int D, bool BF>
-__global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnParams p) {
-    using C = TilesCfg<D>;
+// QBF: queries and outputs in bf16, else f16. E8: 8-bit cache, products in f16.
+template <int D, bool QBF, bool E8>
+__global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnParams p) {
+    using C = TilesCfg<D, E8>;
+    constexpr bool BF = QBF && !E8;   // type of the products
     using U = Unit<kUnitRows, kKeys>;
-    using qt = typename std::conditional<BF, __nv_bfloat16, __half>::type;
+    using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const uint32_t sbase = smem_u32(smem);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + C::BARS);
-    uint64_t *full = bars;                  // [STAGES] a tile has landed
+    uint64_t *full = bars;                  // [LOADS] a tile has landed
     uint64_t *empty = bars + 8;             // [STAGES] both issuers' MMAs of it are done
     uint64_t *q_full = bars + 16;           // [2] tile i's q rows are in shared memory (4 warps)
     uint64_t *ev = bars + 18;               // [2][2] events of tile i (above)
     uint64_t *drained = bars + 22;          // [2]
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 24);
-    int *abort_flag = reinterpret_cast<int *>(bars + 25);
+    uint64_t *raw_empty = bars + 24;        // [RAW_STAGES] a tile of 8 bits has been widened (4 warps)
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 28);
+    int *abort_flag = reinterpret_cast<int *>(bars + 29);
     // counters that the issuers poll: [8] P written (and O rescaled) by each softmax
-    // warp; [4] unused; ring tiles that have landed (V cleared outside the unit's keys)
-    uint32_t *p_seq = reinterpret_cast<uint32_t *>(bars + 26);
-    uint32_t *landed = reinterpret_cast<uint32_t *>(bars + 30);
-    int *join = reinterpret_cast<int *>(bars + 31);   // [2] a tile's joint: whether it is the second
+    // warp; ring tiles that are ready (V cleared outside the unit's keys): one by the
+    // watcher, or [4] by each widening warp
+    uint32_t *p_seq = reinterpret_cast<uint32_t *>(bars + 30);
+    uint32_t *landed = reinterpret_cast<uint32_t *>(bars + 34);
+    constexpr int kLanded = E8 ? 4 : 1;
+    int *join = reinterpret_cast<int *>(bars + 36);   // [2] a tile's joint: whether it is the second
+    float *q_shift = reinterpret_cast<float *>(bars + 38);   // [2][kM] E8: 1 / (power of two on the q row)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 256) {
@@ -234,10 +253,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     if (!find_share<kUnitRows, kKeys, 4, 3>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::STAGES; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 2);
-        }
+        for (int i = 0; i < C::LOADS; ++i) mbar_init(&full[i], 1);
+        for (int i = 0; i < C::STAGES; ++i) mbar_init(&empty[i], 2);
+        for (int i = 0; E8 && i < C::RAW_STAGES; ++i) mbar_init(&raw_empty[i], 4);
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], 4);
             mbar_init(&ev[2 * i], 1);
@@ -246,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         }
         *abort_flag = 0;
         for (int i = 0; i < 8; ++i) p_seq[i] = 0;
-        *landed = 0;
+        for (int i = 0; i < kLanded; ++i) landed[i] = 0;
         mbar_fence_init();
     }
     fence_proxy_async_smem();   // the sums stood where the ring's copies will land
@@ -329,29 +347,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 }
                 const int tok = p.by_page.mod(key, p.by_page.div(key));
                 const unsigned mask = __ballot_sync(FULL, need && lane < boxes);
-                const uint32_t bytes = __popc(mask) * p.box * 128 * C::HALVES;
+                const uint32_t bytes = __popc(mask) * p.box * (E8 ? D : 128 * C::HALVES);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; ++kv, ++it) {
-                    const int st = it % C::STAGES;
-                    if (it >= C::STAGES && !wait(&empty[st], (it / C::STAGES - 1) & 1)) {
+                    const int st = it % C::LOADS;
+                    if (it >= C::LOADS && !wait(E8 ? &raw_empty[st] : &empty[st], (it / C::LOADS - 1) & 1)) {
                         ok = false;
                         break;
                     }
                     if (lane == 0) mbar_arrive_expect_tx(&full[st], bytes);
                     __syncwarp();
-                    const uint32_t dst = sbase + C::RING + st * C::TILE;
-                    for (int i = lane; i < boxes * C::HALVES; i += 32) {   // boxes <= 8 unless box == 16 ... 32 lanes at most
-                        const int h = i / boxes;
-                        if (need)
-                            tma_box(dst + h * C::BLOCK + b * p.box * 128, kv ? &p.tm_v : &p.tm_k, h * 64, tok, u.g, page,
+                    if constexpr (E8) {
+                        if (need && lane < boxes)
+                            tma_box(sbase + C::RAW + st * C::RAW_TILE + b * p.box * D, kv ? &p.tm_v : &p.tm_k, 0, tok, u.g, page,
                                     &full[st]);
+                    } else {
+                        const int h = lane / boxes;   // boxes * HALVES <= 16
+                        if (need && h < C::HALVES)
+                            tma_box(sbase + C::RING + st * C::TILE + h * C::BLOCK + b * p.box * 128, kv ? &p.tm_v : &p.tm_k, h * 64,
+                                    tok, u.g, page, &full[st]);
                     }
                 }
             }
         } while (ok && next_unit(u));
         if (!ok)   // copies in flight land before the CTA may end
-            for (uint32_t i = it > (uint32_t)C::STAGES ? it - C::STAGES : 0; i < it; ++i)
-                mbar_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
+            for (uint32_t i = it > (uint32_t)C::LOADS ? it - C::LOADS : 0; i < it; ++i)
+                mbar_drain(&full[i % C::LOADS], (i / C::LOADS) & 1);
     } else if (warp == 9 || warp == 10) {
         // ------------------------------------------------------------ MMA issuers
         auto issuer = [&](auto tile) {
@@ -363,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         uint32_t n_q = 0, n_p = 0, e = 0;   // q and P so far, events
         bool ok = true;
         auto stage_of = [&](uint32_t at) { return sbase + C::RING + (at % C::STAGES) * C::TILE; };
-        auto full_wait = [&](uint32_t at) { return reached(landed, 1, at + 1); };
+        auto full_wait = [&](uint32_t at) { return reached(landed, kLanded, at + 1); };
         do {
             int t0, t1, k0, k1;
             share_tiles(u, t0, t1);
@@ -455,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         };
         if (warp == 9) issuer(std::integral_constant<int, 0>{});
         else issuer(std::integral_constant<int, 1>{});
-    } else if (warp == 11) {
+    } else if (!E8 && warp == 11) {
         // ------------------------------------------------------------ watcher
         // (an issuer's own look at a barrier after a burst of MMAs waits until the
         // burst has left the queue; a look at a word of shared memory does not)
@@ -482,6 +503,49 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 }
             }
         } while (ok && next_unit(u));
+    } else if (E8 && warp >= 12) {
+        // ------------------------------------------------------------ widening
+        // 32 rows a warp: 16 bytes of a row a lane become two 16-byte pieces of f16 (exact)
+        // in the layout that the MMA reads. The lanes of a row's second half (d = 128) write
+        // theirs in the other order, so that a row's 8 writes lie in distinct banks.
+        constexpr int L = D / 16;   // lanes a row
+        const int w = warp - 12, c = lane % L;
+        uint32_t it = 0;
+        bool ok = true;
+        do {
+            int t0, t1;
+            share_tiles(u, t0, t1);
+            for (int t = t0; ok && t < t1; ++t) {
+                const int key0 = (u.tile0 + t) * kKeys;
+                for (int kv = 0; ok && kv < 2; ++kv, ++it) {
+                    ok = wait(&full[it % C::RAW_STAGES], (it / C::RAW_STAGES) & 1);
+                    if (ok && it >= C::STAGES) ok = wait(&empty[it % C::STAGES], (it / C::STAGES - 1) & 1);
+                    if (!ok) break;
+                    const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 32 * D + lane * 16;
+                    uint8_t *dst = smem + C::RING + (it % C::STAGES) * C::TILE + (c >> 2) * C::BLOCK;
+#pragma unroll 4
+                    for (int x = 0; x < L; ++x) {
+                        const int row = w * 32 + x * (32 / L) + lane / L;
+                        uint4 v = *reinterpret_cast<const uint4 *>(src + x * 512);
+                        if (kv == 1 && (key0 + row < u.lo || key0 + row >= u.hi)) v = make_uint4(0, 0, 0, 0);   // of V
+                        uint4 a, b;
+                        widen4(v.x, a.x, a.y);
+                        widen4(v.y, a.z, a.w);
+                        widen4(v.z, b.x, b.y);
+                        widen4(v.w, b.z, b.w);
+                        const bool swap = (c & 4) != 0;
+                        *reinterpret_cast<uint4 *>(dst + sw128(row, 2 * (c & 3) + swap)) = swap ? b : a;
+                        *reinterpret_cast<uint4 *>(dst + sw128(row, 2 * (c & 3) + !swap)) = swap ? a : b;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        st_release(landed + w, it + 1);
+                        mbar_arrive(&raw_empty[it % C::RAW_STAGES]);
+                    }
+                }
+            }
+        } while (ok && next_unit(u));
     } else if (warp < 8) {
         // ------------------------------------------------------------ softmax
         const int i = warp >> 2, r = threadIdx.x & 127;   // tile, row
@@ -491,7 +555,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
         uint32_t e = 0, n_p = 0;   // events before this unit, P written so far
         bool ok = true;
         const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
-        const float qs = fabsf(p.scale) * 1.44269504088896340736f;
+        const float qs_all = fabsf(p.scale) * 1.44269504088896340736f;
         // offset of this thread's row of unit a in rows of strides ts, hs (of the unit's
         // first row where it has none): the warp's lanes ask one another for theirs
         auto offset_of = [&](const U &a, long long t_s, long long h_s) -> long long {
@@ -522,6 +586,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
 #pragma unroll
                     for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__ldg(h + 2 * x) | ((uint32_t)__ldg(h + 2 * x + 1) << 16);
                     v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            if constexpr (E8 && QBF) {   // to f16, each row times a power of two
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    uint32_t *x = reinterpret_cast<uint32_t *>(&v[k]);
+                    float m = 0.f;
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        m = fmaxf(m, fmaxf(fabsf(__uint_as_float(x[y] << 16)), fabsf(__uint_as_float(x[y] & 0xffff0000u))));
+#pragma unroll
+                    for (int o = 1; o < L; o <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
+                    const float f = f16_shift(m);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y)
+                        x[y] = pack2<false>(__uint_as_float(x[y] << 16) * f, __uint_as_float(x[y] & 0xffff0000u) * f);
+                    if (c == 0) q_shift[i * kM + (warp & 3) * 32 + k * (32 / L) + lane / L] = 1.f / f;
                 }
             }
 #pragma unroll
@@ -561,6 +642,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 key_range(p, u.q, b0, b0 + 1, x, all_hi);
                 key_range(p, u.q, b1 - 1, b1, all_lo, x);
             }
+            float qs = qs_all;
+            if constexpr (E8 && QBF) qs *= q_shift[i * kM + r];
+            if (E8 && p.k_scale) qs *= __ldg(p.k_scale + u.g);
             float m = -INFINITY, l = 0.f;
             int k0, k1;
             steps(u, t0, t1, k0, k1);
@@ -617,17 +701,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                     const float z = m == -INFINITY ? 0.f : -m;
                     const unsigned long long qq = pk2(qs, qs), zz = pk2(z, z);
                     unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
-                    uint32_t w[32];
 #pragma unroll
-                    for (int x = 0; x < 32; ++x) {
-                        float a, b;
-                        upk2(fma2(pk2(s[2 * x], s[2 * x + 1]), qq, zz), a, b);
-                        a = fast_exp2(a);
-                        b = fast_exp2(b);
-                        acc[x & 3] = add2(acc[x & 3], pk2(a, b));
-                        w[x] = pack2<BF>(a, b);
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t w[16];
+#pragma unroll
+                        for (int x = 0; x < 16; ++x) {
+                            float a, b;
+                            upk2(fma2(pk2(s[32 * h + 2 * x], s[32 * h + 2 * x + 1]), qq, zz), a, b);
+                            a = fast_exp2(a);
+                            b = fast_exp2(b);
+                            acc[x & 3] = add2(acc[x & 3], pk2(a, b));
+                            w[x] = pack2<BF>(a, b);
+                        }
+                        st16(tb + 16 * h, w);
                     }
-                    st32(tb, w);
                     float x, y;
                     upk2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), x, y);
                     l += x + y;
@@ -721,7 +808,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
                 }
             }
             if (last) {
-                const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+                const float vs = E8 && p.v_scale ? __ldg(p.v_scale + done.g) : 1.f;
+                const float inv = l > 0.f || l != l ? vs / l : 0.f;
                 const long long off = offset_of(done, p.o_ts, p.o_hs);
                 // 64 values of the warp's 32 rows at a time through shared memory: 8 lanes
                 // write a row's 128 bytes (a thread its own row would touch a line a lane)
@@ -735,9 +823,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
 #pragma unroll
                     for (int x = 0; x < 8; ++x)
                         *reinterpret_cast<uint4 *>(out_rows + sw128(lane, x)) =
-                            make_uint4(pack2<BF>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<BF>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
-                                       pack2<BF>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
-                                       pack2<BF>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
+                            make_uint4(pack2<QBF>(o[8 * x] * inv, o[8 * x + 1] * inv), pack2<QBF>(o[8 * x + 2] * inv, o[8 * x + 3] * inv),
+                                       pack2<QBF>(o[8 * x + 4] * inv, o[8 * x + 5] * inv),
+                                       pack2<QBF>(o[8 * x + 6] * inv, o[8 * x + 7] * inv));
                     __syncwarp();
                     uint4 v[8];
 #pragma unroll
@@ -777,29 +865,35 @@ __global__ void __launch_bounds__(kThreads, 1) paged_tiles_kernel(const __grid_c
     }
 }
 
-template <int D, bool BF>
+template <int D, bool QBF, bool E8>
 cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
-    using C = TilesCfg<D>;
-    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, BF>), C::BYTES)) return e;
+    using C = TilesCfg<D, E8>;
+    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, QBF, E8>), C::BYTES)) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(n_ctas);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(C::THREADS);
     cfg.dynamicSmemBytes = C::BYTES;
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, BF>, p);
+    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QBF, E8>, p);
 }
 
 }  // namespace
 
-cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int type, int n_ctas, cudaStream_t s) {
-    const bool bf = type == KORE_CUDA_BF16;
-    if (d == 128) return bf ? launch_k<128, true>(p, n_ctas, s) : launch_k<128, false>(p, n_ctas, s);
-    if (d == 64) return bf ? launch_k<64, true>(p, n_ctas, s) : launch_k<64, false>(p, n_ctas, s);
+cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s) {
+    const bool bf = q_type == KORE_CUDA_BF16, e8 = cache_type == KORE_CUDA_E4M3;
+    if (d == 128) {
+        if (e8) return bf ? launch_k<128, true, true>(p, n_ctas, s) : launch_k<128, false, true>(p, n_ctas, s);
+        return bf ? launch_k<128, true, false>(p, n_ctas, s) : launch_k<128, false, false>(p, n_ctas, s);
+    }
+    if (d == 64) {
+        if (e8) return bf ? launch_k<64, true, true>(p, n_ctas, s) : launch_k<64, false, true>(p, n_ctas, s);
+        return bf ? launch_k<64, true, false>(p, n_ctas, s) : launch_k<64, false, false>(p, n_ctas, s);
+    }
     return cudaErrorInvalidValue;
 }
 
