@@ -10,8 +10,8 @@
 //
 // Bound by HBM: every value is read once and written once. One CTA per token;
 // a thread keeps the (cos, sin) of its 16 values in registers and takes them
-// through every second or so head, so that the table costs one read a token
-// instead of one a head. A token's sequence is found by all threads at once
+// through several heads, so that the table costs one read a token instead of one
+// a head. A token's sequence is found by all threads at once
 // (one round of loads) while the first rows are already on the way.
 
 #include "paged.cuh"
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ Rot
         }
     }
     const int nq = p.q.heads, nk = APPEND ? nq + p.G : nq, nv = APPEND ? nk + p.G : nq;
-#pragma unroll 2
+#pragma unroll 4
     for (int h = h0; h < nv; h += lanes) {
         const bool is_q = h < nq, is_k = !is_q && h < nk;
         const HeadRows &r = !APPEND || is_q ? p.q : is_k ? p.k : p.v;
@@ -255,11 +255,14 @@ cudaError_t launch(void (*kernel)(Args...), int blocks, int threads, size_t smem
 
 template <typename T, typename C, bool APPEND>
 cudaError_t launch_tc(const RotateParams &p, bool vec, cudaStream_t s) {
-    // about two heads a thread: the table's values in its registers serve both,
-    // and a CTA stays small enough for many tokens an SM
+    // four heads a thread: the table's values in its registers serve all of them,
+    // and a CTA is small enough for many tokens an SM (12288 tokens of 28/4 heads of
+    // 128: 19.8 us; two heads 21.9, six 19.9). Two where the CTAs would not fill the SMs
+    // (48 tokens: 2.7 us; four heads 2.9)
     const int heads = p.q.heads + (APPEND ? 2 * p.G : 0);
     const int items = p.d / (vec ? 16 : 2);
-    int threads = items * ((heads + 1) / 2);
+    const int each = p.n_tok >= 4 * 148 ? 4 : 2;
+    int threads = items * ((heads + each - 1) / each);
     threads = threads < items ? items : threads;
     threads = (threads + 31) / 32 * 32;
     if (threads > 256) threads = 256;
