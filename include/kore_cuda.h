@@ -589,8 +589,9 @@ typedef struct kore_cuda_batch {
     const int *kv_len;       /* device [n_seq] */
     const int *page_table;   /* device [n_seq][table_stride]: physical page of each logical page */
     int table_stride;
-    int max_q;               /* longest chunk, known on the host: chooses the attention's kernel (any value gives
-                                the same attention, the wrong one a slower call) */
+    int max_q;               /* longest chunk and longest sequence, known on the host (max_kv 0: the page */
+    int max_kv;              /*   table's capacity): they choose the attention's kernel. A wrong value gives
+                                  the same attention, up to rounding, and a slower call */
 } kore_cuda_batch;
 
 /* Stores the batch's keys and values at their positions: k [n_tok] rows of

@@ -127,6 +127,7 @@ int check_batch(const kore_cuda_batch *b, int n_tok) {
         return refuse(KORE_CUDA_EINVAL, "q_start, kv_len or page_table is null");
     if (b->n_seq > 0 && b->table_stride <= 0) return refuse(KORE_CUDA_EINVAL, "table_stride %d", b->table_stride);
     if (b->max_q < 0) return refuse(KORE_CUDA_EINVAL, "max_q %d", b->max_q);
+    if (b->max_kv < 0) return refuse(KORE_CUDA_EINVAL, "max_kv %d", b->max_kv);
     return KORE_CUDA_OK;
 }
 
@@ -400,8 +401,17 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
     // units are of 16 rows and tiles of 128 keys at least
     p.small = ((double)n_tok * p.rep / 16 + p.n_seq) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;
-    // more packed rows than a unit of the row kernel takes: the tensor cores
-    const bool tiles = (long long)batch->max_q * p.rep > 16;
+    // The row kernel passes over the keys once for every 16 packed rows, the tile kernel
+    // once for every 256 at 2.8 times the cost and some 20 us more for its start, its
+    // outputs and the joining of cut units. So the row kernel has what fits one of its
+    // units, and chunks up to so many passes over 128 keys in the whole batch (kv counted
+    // by max_kv, a unit's own time as three passes). Measured, row against tile kernel,
+    // 28/4 heads of 128: 16-bit cache, 4488 passes 41 / 49 us, 6160 34 / 38, 6300 45 / 29,
+    // 9380 47 / 40, 10080 52 / 39; 8 bits 10080 53 / 53, 13376 74 / 86.
+    const double rows16 = (double)p.G * ((double)n_tok * p.rep / 16 + p.n_seq);
+    const double passes = (batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P) / 128 + 3;
+    const bool tiles = (long long)batch->max_q * p.rep > 16 &&
+                       rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0);
     const bool plain = tiles && cache->type == KORE_CUDA_E4M3;   // widened before it is read as an operand
     // tokens of a box: the largest power of two that divides the page, up to a tile
     const int most = tiles ? 128 : d * type_bytes(cache->type) == 256 ? 16 : 32;

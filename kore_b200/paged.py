@@ -57,7 +57,7 @@ class _Pages(ctypes.Structure):
 class _Batch(ctypes.Structure):
     """kore_cuda_batch."""
     _fields_ = [("n_seq", _i), ("q_start", _vp), ("kv_len", _vp), ("page_table", _vp), ("table_stride", _i),
-                ("max_q", _i)]
+                ("max_q", _i), ("max_kv", _i)]
 
 
 class _Opts(ctypes.Structure):
@@ -208,16 +208,17 @@ class RopeTable:
 class PagedBatch:
     """The sequences of a step: rows q_start[s] .. q_start[s+1]-1 of q, k and v are the new tokens of sequence s,
     which holds kv_len[s] positions with them, in the pages page_table[s]. All int32 on the device, read by the
-    kernels when they run, so a captured step follows what they hold at its replay. max_q: the longest chunk."""
+    kernels when they run, so a captured step follows what they hold at its replay. max_q: the longest chunk; max_kv:
+    the longest sequence (0: as much as page_table has room for). They choose a kernel and bound nothing."""
 
-    def __init__(self, q_start, kv_len, page_table, max_q: int):
+    def __init__(self, q_start, kv_len, page_table, max_q: int, max_kv: int = 0):
         _import_torch()
         if not kv_len.is_cuda:
             raise ValueError("expected CUDA tensors")
         self.device = dev = kv_len.device
         n = kv_len.shape[0]
         view = _Batch(n, _ints(q_start, "q_start", dev, 1), _ints(kv_len, "kv_len", dev, 1),
-                      _ints(page_table, "page_table", dev, 2), page_table.shape[1], max_q)
+                      _ints(page_table, "page_table", dev, 2), page_table.shape[1], max_q, max_kv)
         if q_start.shape[0] != n + 1 or page_table.shape[0] != n:
             raise ValueError(f"q_start must have {n + 1} and page_table {n} rows")
         self.q_start, self.kv_len, self.page_table, self.view = q_start, kv_len, page_table, view

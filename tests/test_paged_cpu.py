@@ -73,7 +73,7 @@ def _pages(**kw):
 
 
 def _batch(**kw):
-    a = dict(n_seq=1, q_start=A, kv_len=A, page_table=A, table_stride=4, max_q=1)
+    a = dict(n_seq=1, q_start=A, kv_len=A, page_table=A, table_stride=4, max_q=1, max_kv=0)
     a.update(kw)
     return P._Batch(*a.values())
 
@@ -103,7 +103,8 @@ BAD_PAGES = [(dict(k=None), "null"), (dict(type=99), "type"), (dict(n_pages=0), 
              (dict(page_stride=2 * 16 * 64 - 8), "page_stride"), (dict(page_stride=2 * 16 * 64 + 4), "page_stride"),
              (dict(k_scale=A), "scales")]
 BAD_BATCH = [(dict(n_seq=-1), -2), (dict(n_seq=4097), -2), (dict(q_start=None), -1), (dict(kv_len=None), -1),
-             (dict(page_table=None), -1), (dict(table_stride=0), -1), (dict(max_q=-1), -1)]
+             (dict(page_table=None), -1), (dict(table_stride=0), -1), (dict(max_q=-1), -1),
+             (dict(max_kv=-1), -1)]
 
 
 @pytest.mark.parametrize("kw,word", BAD_PAGES)

@@ -358,16 +358,20 @@ def check_attention(C, q, out, ns, scale=None, causal=True, window=0, lse=None):
         at += n
 
 
-def attend(g, C, H, ns, tq, how="dense", pad=2, max_q=None, check=True, **kw):
+# what the host says of the batch chooses the kernel: 16 rows a unit, or 256 on tcgen05
+HINTS = {"rows": dict(max_q=1), "tiles": dict(max_q=1 << 20, max_kv=1 << 30)}
+BOTH = pytest.mark.parametrize("kernel", list(HINTS))
+
+
+def attend(g, C, H, ns, tq, kernel, how="dense", pad=2, **kw):
     n = sum(ns) + pad
     q = strided(rand(g, n, H, C.d).to(DT[tq]), how)
     out = strided(torch.full((n, H, C.d), GUARD, dtype=DT[tq], device=dev()), how)
     lse = torch.full((n, H), GUARD, device=dev())
-    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, max(ns + [0]) if max_q is None else max_q)
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
     C.cache.attend(batch, q, out, lse=lse, **kw)
     C.cache.check()
-    if check:
-        check_attention(C, q, out, ns, lse=lse, **kw)
+    check_attention(C, q, out, ns, lse=lse, **kw)
     assert (out[sum(ns):] == GUARD).all() and (lse[sum(ns):] == GUARD).all()   # rows behind the last sequence
     return q, out, batch
 
@@ -389,52 +393,59 @@ BATCHES = {
 @pytest.mark.parametrize("tq,tc", KINDS)
 @pytest.mark.parametrize("H,G,d,P", [(28, 4, 128, 64), (14, 2, 64, 16), (8, 8, 128, 48), (40, 2, 64, 256), (3, 1, 128, 16)])
 @pytest.mark.parametrize("which", list(BATCHES))
-def test_attention(tq, tc, H, G, d, P, which):
+@BOTH
+def test_attention(kernel, tq, tc, H, G, d, P, which):
     g = gen(H + P)
     ns, kvs = map(list, zip(*BATCHES[which]))
     C = Cache(g, tc, G, d, P, kvs)
     for s in range(len(kvs)):
         C.fill(g, s)
-    attend(g, C, H, ns, tq)
+    attend(g, C, H, ns, tq, kernel)
 
 
+@BOTH
 @pytest.mark.parametrize("tq,tc", [("bf16", "bf16"), ("f16", "e4m3")])
 @pytest.mark.parametrize("kw", [dict(window=1), dict(window=100), dict(causal=False), dict(causal=False, window=33),
                                 dict(scale=0.5), dict(scale=-0.2), dict(window=100000)])
-def test_attention_masks_and_scales(tq, tc, kw):
+def test_attention_masks_and_scales(kernel, tq, tc, kw):
     g = gen(5)
     ns, kvs = [1, 37, 200, 1, 6], [400, 37, 900, 1, 129]
     C = Cache(g, tc, 2, 128, 64, kvs)
     for s in range(len(kvs)):
         C.fill(g, s)
-    attend(g, C, 16, ns, tq, **kw)
+    attend(g, C, 16, ns, tq, kernel, **kw)
 
 
+@BOTH
 @pytest.mark.parametrize("how", ["fused", "heads_first", "odd"])
 @pytest.mark.parametrize("ns,kvs", [([1, 1], [300, 77]), ([150, 3], [300, 77])])
-def test_attention_of_strided_rows(how, ns, kvs):
+def test_attention_of_strided_rows(kernel, how, ns, kvs):
     g = gen(6)
     for t, d in (("bf16", 128), ("f16", 64)):
         C = Cache(g, t, 2, d, 32, kvs, alternate=True)
         for s in range(2):
             C.fill(g, s)
-        attend(g, C, 14, ns, t, how=how)
+        attend(g, C, 14, ns, t, kernel, how=how)
 
 
 @pytest.mark.parametrize("max_q", [0, 1, 17, 100000])
-def test_attention_whatever_the_hint(max_q):
-    """max_q chooses the kernel and nothing else."""
+@pytest.mark.parametrize("max_kv", [0, 1, 1 << 30])
+def test_attention_whatever_the_hints(max_q, max_kv):
+    """max_q and max_kv choose the kernel and bound nothing."""
     g = gen(7)
     ns, kvs = [1, 90, 0, 30], [500, 200, 3, 31]
-    for tq, tc in KINDS:
-        C = Cache(g, tc, 2, 64, 64, kvs)
-        for s in range(4):
-            C.fill(g, s)
-        attend(g, C, 14, ns, tq, max_q=max_q)
+    C = Cache(g, "bf16", 2, 64, 64, kvs)
+    for s in range(4):
+        C.fill(g, s)
+    q = rand(g, sum(ns), 14, 64).to(torch.bfloat16)
+    out = C.cache.attend(K.PagedBatch(starts(ns), ints(kvs), C.table, max_q, max_kv), q)
+    C.cache.check()
+    check_attention(C, q, out, ns)
 
 
+@BOTH
 @pytest.mark.parametrize("tq,tc", KINDS)
-def test_attention_of_large_scores(tq, tc):
+def test_attention_of_large_scores(kernel, tq, tc):
     """Sharp softmaxes and reference maxima that move: keys that grow along the sequence."""
     g = gen(8)
     ns, kvs = [1, 140], [3000, 600]
@@ -444,35 +455,37 @@ def test_attention_of_large_scores(tq, tc):
         pg, sl = C.places(s, torch.arange(kv, device=dev()))
         k = C.kp[pg, :, sl].float() * torch.linspace(0.01, 1.0 if tc == "e4m3" else 8.0, kv, device=dev())[:, None, None]
         C.kp[pg, :, sl] = k.to(DT[tc])
-    attend(g, C, 14, ns, tq)
+    attend(g, C, 14, ns, tq, kernel)
 
 
-def test_attention_of_many_short_sequences():
+@BOTH
+def test_attention_of_many_short_sequences(kernel):
     g = gen(9)
     kvs = torch.randint(1, 90, (300,), generator=torch.Generator().manual_seed(1)).tolist()
     C = Cache(g, "bf16", 2, 64, 16, kvs)
     for s in range(len(kvs)):
         C.fill(g, s)
-    attend(g, C, 4, [1] * 300, "bf16")
+    attend(g, C, 4, [1] * 300, "bf16", kernel)
 
 
 @pytest.mark.parametrize("tq,tc", [("bf16", "bf16"), ("f16", "e4m3")])
 @pytest.mark.parametrize("n", [1, 40])
-def test_attention_of_a_long_context_is_split_and_the_same_each_time(tq, tc, n):
+@BOTH
+def test_attention_of_a_long_context_is_split_and_the_same_each_time(kernel, tq, tc, n):
     g = gen(10)
     C = Cache(g, tc, 1, 128, 256, [70001])
     C.fill(g, 0)
-    q, out, batch = attend(g, C, 8, [n], tq)
+    q, out, batch = attend(g, C, 8, [n], tq, kernel)
     again = torch.zeros_like(out)
     for _ in range(3):
         C.cache.attend(batch, q, again)
         assert torch.equal(again[:n], out[:n])
 
 
-@pytest.mark.parametrize("n", [1, 60])
-def test_attention_offsets_beyond_32_bits(n):
+@BOTH
+def test_attention_offsets_beyond_32_bits(kernel):
     """A pool of more than 2^32 elements: pages at both ends of it."""
-    G, d, P = 4, 128, 1024
+    G, d, P, n = 4, 128, 1024, 60
     pages = 2 ** 32 // (G * P * d) + 3
     kp = torch.empty(pages, G, P, d, dtype=torch.bfloat16, device=dev())
     vp = torch.empty_like(kp)
@@ -482,7 +495,7 @@ def test_attention_offsets_beyond_32_bits(n):
     C.cache = K.PagedCache(kp, vp)
     C.table = ints([[pages - 1, 0, pages - 2, -1]])
     C.fill(g, 0)
-    attend(g, C, 28, [n], "bf16")
+    attend(g, C, 28, [n], "bf16", kernel)
     k = rand(g, n, G, d).to(torch.bfloat16)
     C.table = ints([[0, 1, pages - 1, -1]])
     C.cache.append(K.PagedBatch(ints([0, n]), ints([2500]), C.table, n), k, k)
@@ -492,26 +505,27 @@ def test_attention_offsets_beyond_32_bits(n):
 
 @pytest.mark.parametrize("tq,tc", [("bf16", "bf16"), ("bf16", "e4m3")])
 @pytest.mark.parametrize("n", [1, 30])
-def test_attention_reads_nothing_before_the_window(tq, tc, n):
+@BOTH
+def test_attention_reads_nothing_before_the_window(kernel, tq, tc, n):
     """Pages wholly before every row's window may be gone from the table."""
     g = gen(12)
     C = Cache(g, tc, 2, 64, 32, [1000])
     C.fill(g, 0)
-    want, kp = C.rows(0), C.table.clone()
+    kp = C.table.clone()
     first = (1000 - n) - 200 + 1
-    q, out, batch = attend(g, C, 14, [n], tq, window=200)
+    q, out, batch = attend(g, C, 14, [n], tq, kernel, window=200)
     C.table[0, :first // 32] = -1
     pg = kp[0, first // 32].long()
     C.kp[pg, :, :first % 32] = float("nan")   # before the window, in its first page
     C.vp[pg, :, :first % 32] = float("nan")
     again = torch.zeros_like(out)
-    C.cache.attend(K.PagedBatch(starts([n]), ints([1000]), C.table, n), q, again, window=200)
+    C.cache.attend(batch, q, again, window=200)
     C.cache.check()
     assert torch.equal(again[:n], out[:n])
-    del want
 
 
-def test_attention_passes_nan_and_infinity_on_to_their_rows():
+@BOTH
+def test_attention_passes_nan_and_infinity_on_to_their_rows(kernel):
     g = gen(13)
     for tq, tc in KINDS:
         C = Cache(g, tc, 1, 64, 32, [80, 80])
@@ -520,14 +534,15 @@ def test_attention_passes_nan_and_infinity_on_to_their_rows():
         q[0, 1, 3] = math.nan
         pg, sl = C.places(1, torch.tensor([11], device=dev()))
         C.vp[pg, 0, sl, 5] = float("nan")
-        out = C.cache.attend(K.PagedBatch(ints([0, 1, 2]), ints([80, 80]), C.table, 1), q)
+        out = C.cache.attend(K.PagedBatch(ints([0, 1, 2]), ints([80, 80]), C.table, **HINTS[kernel]), q)
         assert torch.isfinite(out[0, 0]).all() and out[0, 1].isnan().all()
         assert out[1, :, 5].isnan().all() and torch.isfinite(out[1, :, :5]).all() and torch.isfinite(out[1, :, 6:]).all()
 
 
 @pytest.mark.parametrize("n", [1, 50])
+@BOTH
 @pytest.mark.parametrize("bad,word", [("page", "page id"), ("rows", "bounds"), ("long", "bounds"), ("negative", "bounds")])
-def test_attention_reports_bad_device_data(n, bad, word):
+def test_attention_reports_bad_device_data(kernel, n, bad, word):
     g = gen(14)
     ns, kvs = [n, n], [150, 150]
     C = Cache(g, "bf16", 2, 64, 16, kvs)
@@ -543,7 +558,7 @@ def test_attention_reports_bad_device_data(n, bad, word):
         kv[1] = 16 * table.shape[1] + 1
     else:
         kv[1] = -1
-    C.cache.attend(K.PagedBatch(ints(q_start), ints(kv), table, n), q, out)
+    C.cache.attend(K.PagedBatch(ints(q_start), ints(kv), table, **HINTS[kernel]), q, out)
     with pytest.raises(K.KoreCudaError, match=word):
         C.cache.check()
     C.kvs = [150]
@@ -551,7 +566,7 @@ def test_attention_reports_bad_device_data(n, bad, word):
     if bad != "page":
         assert (out[n:] == GUARD).all()
     out2 = torch.full_like(q, GUARD)   # the workspace is as it was: the next call is right
-    C.cache.attend(K.PagedBatch(ints([0, n]), ints([150]), C.table[:1].contiguous(), n), q, out2)
+    C.cache.attend(K.PagedBatch(ints([0, n]), ints([150]), C.table[:1].contiguous(), **HINTS[kernel]), q, out2)
     C.cache.check()
     assert torch.equal(out2[:n], out[:n]) or bad == "page"
 
@@ -582,12 +597,13 @@ def test_attention_refuses_tensors_that_do_not_fit():
 
 # ---------------------------------------------------------------- streams, graphs, the operators together
 
-def test_calls_on_two_streams_at_once():
+@BOTH
+def test_calls_on_two_streams_at_once(kernel):
     """Default workspaces are a stream's own."""
     g = gen(16)
     C = Cache(g, "bf16", 1, 128, 256, [30000])
     C.fill(g, 0)
-    batch = K.PagedBatch(ints([0, 1]), ints([30000]), C.table, 1)
+    batch = K.PagedBatch(ints([0, 1]), ints([30000]), C.table, **HINTS[kernel])
     qs = [rand(g, 1, 8, 128).to(torch.bfloat16) for _ in range(2)]
     want = [C.cache.attend(batch, q).clone() for q in qs]
     caches = [C.cache, K.PagedCache(C.kp, C.vp)]
@@ -605,7 +621,8 @@ def test_calls_on_two_streams_at_once():
 
 @pytest.mark.parametrize("tc", ["bf16", "e4m3"])
 @pytest.mark.parametrize("n", [1, 24])
-def test_captured_step_follows_the_lengths_on_the_device(tc, n):
+@BOTH
+def test_captured_step_follows_the_lengths_on_the_device(kernel, tc, n):
     """A step (rotate and append, attend) captured once and replayed as the sequences grow; and two graphs, captured
     one after the other on one stream, replayed on two streams at once."""
     g = gen(17)
@@ -615,7 +632,7 @@ def test_captured_step_follows_the_lengths_on_the_device(tc, n):
     C.fill(g, 0), C.fill(g, 1)
     rope = K.RopeTable(max(full), d)
     kv = ints([400 + n, 9000 + n])
-    batch = K.PagedBatch(ints([0, n, 2 * n]), kv, C.table, n)
+    batch = K.PagedBatch(ints([0, n, 2 * n]), kv, C.table, **HINTS[kernel])
     q, k, v = (rand(g, 2 * n, h, d).to(torch.bfloat16) for h in (H, G, G))
     qr, out = torch.zeros_like(q), torch.zeros_like(q)
 
@@ -655,7 +672,8 @@ def test_captured_step_follows_the_lengths_on_the_device(tc, n):
 
 
 @pytest.mark.parametrize("tq,tc,H,G,d,P", [("bf16", "bf16", 28, 4, 128, 64), ("f16", "e4m3", 14, 2, 64, 16)])
-def test_prompts_and_steps_together(tq, tc, H, G, d, P):
+@BOTH
+def test_prompts_and_steps_together(kernel, tq, tc, H, G, d, P):
     """Prompts in two chunks, then tokens, of three conversations of different lengths, as a server would run them:
     every step's attention against the formula over what the cache holds, and the cache against the keys and values
     that went in."""
@@ -674,7 +692,7 @@ def test_prompts_and_steps_together(tq, tc, H, G, d, P):
         k = torch.cat([x[a:a + n] for x, a, n in zip(keys, at, ns)])
         v = torch.cat([x[a:a + n] for x, a, n in zip(vals, at, ns)])
         q = rand(g, sum(ns), H, d).to(DT[tq])
-        batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, max(ns))
+        batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
         C.cache.append(batch, k, v, rope=rope, q=q, q_out=q)
         out = C.cache.attend(batch, q)
         C.cache.check()
