@@ -504,7 +504,9 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
  * position outside the rotation table, 7 a sequence whose bounds do not fit
  * the rows, its length or its page table. Such a sequence (for 6 and for an
  * append's 3: such a token) is left out: none of its rows are written. In the
- * attention a bad page's keys count as zeros.
+ * attention a bad page's keys count as zeros. 1 is a tile copy or a product that
+ * did not come within 2 s: the attention's outputs are void then, and the
+ * workspace has to be zeroed again.
  */
 #define KORE_CUDA_E4M3 1000   /* 8 bits, 4 of exponent and 3 of mantissa, no infinities (not a GGUF type) */
 
@@ -628,7 +630,7 @@ long long kore_cuda_paged_attn_workspace(int head_dim);
  * anything, infinities and NaN too. Positions that a row of the chunk sees must
  * hold finite values for the chunk's other rows to be right.
  * q, out: [n_tok] rows of n_head heads, F16 or BF16, the cache of the same type
- * or E4M3; lse (optional) [n_tok][n_head]: natural log of the softmax's sum.
+ * or E4M3; out may not overlap q; lse (optional) [n_tok][n_head]: natural log of the softmax's sum.
  * Products are exact and summed in 32 bits, the softmax in 32 bits; the
  * probabilities are rounded to the type of the cache for the second product
  * (to F16 for E4M3). The result is a function of the inputs and the batch alone

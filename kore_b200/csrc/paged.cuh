@@ -134,11 +134,24 @@ __device__ __forceinline__ Seq load_seq(const PagedAttnParams &p, int s, bool re
     return q;
 }
 
+// Probabilities in f16 stand 2^7 higher than exp2(score - reference): f16 ends at
+// 2^-24, and many keys of small probability each may weigh as much as one of a large
+// one. (With the references' slack of 2^8 they stay below 2^15.) Sums stand as much
+// higher, so that outputs need nothing; bf16 has fp32's range.
+template <bool BF>
+constexpr float kBias = BF ? 0.f : 7.f;
+
+// Natural log of a softmax's sum from its reference (log2) and the sum over it.
+template <bool BF>
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l > 0.f || l != l ? (m - kBias<BF>)*0.69314718055994530942f + logf(l) : -INFINITY;
+}
+
 // Keys [lo, hi) that some token of the packed rows [r0, r1) of the chunk sees.
 __device__ __forceinline__ void key_range(const PagedAttnParams &p, const Seq &q, int r0, int r1, int &lo, int &hi) {
     const int first = q.kv - q.n + p.by_rep.div(r0), last = q.kv - q.n + p.by_rep.div(r1 - 1);
     hi = p.causal ? min(q.kv, last + 1) : q.kv;
-    lo = p.window > 0 ? max(0, first - p.window + 1) : 0;
+    lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0;
     hi = max(hi, 0);
     lo = min(lo, hi);
 }

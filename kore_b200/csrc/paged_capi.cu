@@ -343,6 +343,7 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     if (int rc = check_rows(out, "out", d)) return rc;
     if (q->type == KORE_CUDA_F32 || out->type != q->type || out->n_head != q->n_head)
         return refuse(KORE_CUDA_EINVAL, "q and out must be F16 or BF16, of one type and number of heads");
+    if (out->data == q->data) return refuse(KORE_CUDA_EINVAL, "out must not be q's own rows");
     if (cache->type != q->type && cache->type != KORE_CUDA_E4M3)
         return refuse(KORE_CUDA_EINVAL, "a cache of type %d does not go with queries of type %d", cache->type, q->type);
     const int G = cache->n_head_kv;

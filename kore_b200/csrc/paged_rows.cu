@@ -116,6 +116,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+__device__ __forceinline__ uint64_t l2_evict_normal_policy() {
+    uint64_t pol;
+    asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+    return pol;
+}
+
 // QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16).
 template <int D, bool QBF, bool E4M3>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
@@ -209,7 +215,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
     const int b_half = (lane >> 1) % C::HALVES, b_key = (lane >> 1) / C::HALVES * p.box;
     const TmaDesc *map = (lane & 1) ? &p.tm_v : &p.tm_k;
     const uint32_t b_dst = smem_u32(ring) + (lane & 1) * C::HALF + b_half * (C::KT * 128) + b_key * C::BOXB;
-    const uint64_t policy = l2_evict_first_policy();
+    // a generation step reads every key once; chunks of several units come back to them
+    const uint64_t policy = (long long)p.n_tok * p.rep <= (long long)kRowsU * p.n_seq ? l2_evict_first_policy() : l2_evict_normal_policy();
     int b_page, b_tok;   // page -1: the box is not needed
     auto look_up = [&]() {
         b_page = -1;
@@ -413,7 +420,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                             o[i][3] *= a1;
                         }
                     }
-                    const float z0 = m0 == -INFINITY ? 0.f : -m0, z1 = m1 == -INFINITY ? 0.f : -m1;
+                    const float z0 = m0 == -INFINITY ? 0.f : kBias<BF> - m0, z1 = m1 == -INFINITY ? 0.f : kBias<BF> - m1;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
                         s[j][0] = fast_exp2(fmaf(s[j][0], qs0, z0));
@@ -490,7 +497,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                     for (int k = 0; k < VW; ++k) dst[k] = y[k];
                 }
                 if (p.lse && lane == 0)
-                    p.lse[(long long)(u.q.q0 + i) * p.H + h] = L > 0.f || L != L ? M * 0.69314718055994530942f + logf(L) : -INFINITY;
+                    p.lse[(long long)(u.q.q0 + i) * p.H + h] = log_sum<BF>(M, L);
             };
 #pragma unroll
             for (int half = 0; half < 2; ++half) {

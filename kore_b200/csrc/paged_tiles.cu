@@ -648,6 +648,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             float m = -INFINITY, l = 0.f;
             int k0, k1;
             steps(u, t0, t1, k0, k1);
+            int all_ok;
             auto event = [&](uint32_t no) { return wait(&ev[2 * i + (no & 1)], (no >> 1) & 1); };
             if (mine) {
                 for (int k = k0; k < k1; ++k) {
@@ -698,7 +699,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                             }
                         }
                     }
-                    const float z = m == -INFINITY ? 0.f : -m;
+                    const float z = m == -INFINITY ? 0.f : kBias<BF> - m;
                     const unsigned long long qq = pk2(qs, qs), zz = pk2(z, z);
                     unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
@@ -727,6 +728,13 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 // the last product, before the next unit's events
                 if (ok) ok = event(e + (k1 - k0) + 1);
                 e += k1 - k0 + 2;
+                // the tile's four warps go on together or not at all (they meet below)
+                asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred q, %2, 128, p;\n\t"
+                             "selp.b32 %0, 1, 0, q;\n\t}"
+                             : "=r"(all_ok)
+                             : "r"((int)ok), "r"(1 + i)
+                             : "memory");
+                ok = all_ok != 0;
             }
             fence_after();
             // the next unit's q, so that its products may start during the epilogue
@@ -852,7 +860,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 }
                 const int tok = p.by_rep.div(pr), h = done.g * p.rep + pr - tok * p.rep;
                 if (p.lse && in)
-                    p.lse[(long long)(done.q.q0 + tok) * p.H + h] = l > 0.f || l != l ? m * 0.69314718055994530942f + logf(l) : -INFINITY;
+                    p.lse[(long long)(done.q.q0 + tok) * p.H + h] = log_sum<BF>(m, l);
             }
             fence_before();
         }

@@ -10,7 +10,7 @@ A step of a batch, on the current stream of the tensors' device::
     cache.append(batch, k, v, rope=rope, q=q, q_out=q)    # a layer: store k and v, rotate k and q
     cache.attend(batch, q, out)
 
-Nothing is copied or synchronised: a failure that a kernel meets in the device
+An object is for one host thread at a time, as a context is. Nothing is copied or synchronised: a failure that a kernel meets in the device
 data (a page outside the pool, a sequence that does not fit its page table)
 is left in ``status`` and raised by ``check()``.
 """
@@ -25,7 +25,7 @@ __all__ = ["RopeTable", "PagedCache", "PagedBatch", "rope_frequencies"]
 F32, F16, BF16, E4M3 = 0, 1, 30, 1000
 WORKSPACE_ZEROED = 1024
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
-DEVICE_FAILURES = {3: "page id outside the pool", 6: "position outside the rotation table",
+DEVICE_FAILURES = {1: "a tile copy or product did not come in time", 3: "page id outside the pool", 6: "position outside the rotation table",
                    7: "a sequence's bounds do not fit the rows, its length or its page table"}
 
 _vp, _i, _ll, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
@@ -136,6 +136,8 @@ def _check_status(status) -> None:
     code = int(status.item())
     if code:
         status.zero_()
+        if code == 1:   # workspaces are not as a call leaves them
+            _workspaces.clear()
         raise KoreCudaError(-6, DEVICE_FAILURES.get(code, f"device failure {code}"))
 
 
@@ -282,7 +284,8 @@ class PagedCache:
 
     def attend(self, batch: PagedBatch, q, out=None, *, scale: float = 0.0, causal: bool = True, window: int = 0,
                lse=None, workspace=None):
-        """Attention of q [tokens][n_head][head_dim] (fp16 or bf16) over the batch's cached positions, into out.
+        """Attention of q [tokens][n_head][head_dim] (fp16 or bf16) over the batch's cached positions, into out (a new
+        tensor if None; never q's own memory). Rows outside every sequence keep what out holds.
 
         scale 0: 1/sqrt(head_dim). window: how many positions back a token sees, itself among them (0: all). lse: an
         optional float32 [tokens][n_head] for the log of the softmax's sums. workspace: a tensor of new_workspace();

@@ -9,7 +9,7 @@ import pytest
 import kore_b200 as K
 from kore_b200 import paged as P
 
-A = 0x10000   # a placeholder for an aligned device address
+A, B = 0x10000, 0x20000   # placeholders for aligned device addresses
 
 
 def _f32(x: float) -> float:
@@ -91,7 +91,7 @@ def _append(cache=None, batch=None, n=1, k=..., v=..., q=None, q_out=None, rope=
 
 def _attend(cache=None, batch=None, n=1, q=..., out=..., opts=..., ws=A, ws_bytes=1 << 40):
     L = P._library()
-    q, out = _rows(4) if q is ... else q, _rows(4) if out is ... else out
+    q, out = _rows(4) if q is ... else q, _rows(4, data=B) if out is ... else out
     opts = P._Opts(0.0, 1, 0) if opts is ... else opts
     return L.kore_cuda_paged_attn_dev(_ref(cache or _pages()), _ref(batch or _batch()), n, _ref(q), _ref(out), None,
                                       _ref(opts), ws, ws_bytes, None, None), L.kore_cuda_last_error(None).decode()
@@ -136,9 +136,9 @@ def test_append_refused(kw, word):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(q=None), "q is null"), (dict(q=_rows(4, type=P.F32), out=_rows(4, type=P.F32)), "F16 or BF16"),
-    (dict(out=_rows(4, type=P.F16)), "one type"), (dict(out=_rows(2)), "number of heads"),
-    (dict(q=_rows(4, type=P.F16), out=_rows(4, type=P.F16)), "does not go"), (dict(cache=_pages(type=P.F32)), "type"),
-    (dict(q=_rows(5), out=_rows(5)), "geometry"), (dict(q=_rows(258), out=_rows(258)), "geometry"),
+    (dict(out=_rows(4)), "own rows"), (dict(out=_rows(4, type=P.F16)), "one type"), (dict(out=_rows(2)), "number of heads"),
+    (dict(q=_rows(4, type=P.F16), out=_rows(4, type=P.F16, data=B)), "does not go"), (dict(cache=_pages(type=P.F32)), "type"),
+    (dict(q=_rows(5), out=_rows(5, data=B)), "geometry"), (dict(q=_rows(258), out=_rows(258, data=B)), "geometry"),
     (dict(cache=_pages(head_dim=96), q=_rows(4, 96), out=_rows(4, 96)), "head_dim"), (dict(opts=None), "opts"),
     (dict(opts=P._Opts(0.0, 1, -1)), "window"), (dict(opts=P._Opts(math.nan, 1, 0)), "scale"),
     (dict(ws=None), "workspace"), (dict(ws=A + 16), "workspace"), (dict(ws_bytes=1 << 20), "workspace")])

@@ -406,7 +406,8 @@ def test_attention(kernel, tq, tc, H, G, d, P, which):
 @BOTH
 @pytest.mark.parametrize("tq,tc", [("bf16", "bf16"), ("f16", "e4m3")])
 @pytest.mark.parametrize("kw", [dict(window=1), dict(window=100), dict(causal=False), dict(causal=False, window=33),
-                                dict(scale=0.5), dict(scale=-0.2), dict(window=100000)])
+                                dict(scale=0.5), dict(scale=-0.2), dict(window=100000),
+                                dict(window=2 ** 31 - 1)])
 def test_attention_masks_and_scales(kernel, tq, tc, kw):
     g = gen(5)
     ns, kvs = [1, 37, 200, 1, 6], [400, 37, 900, 1, 129]
@@ -456,6 +457,75 @@ def test_attention_of_large_scores(kernel, tq, tc):
         k = C.kp[pg, :, sl].float() * torch.linspace(0.01, 1.0 if tc == "e4m3" else 8.0, kv, device=dev())[:, None, None]
         C.kp[pg, :, sl] = k.to(DT[tc])
     attend(g, C, 14, ns, tq, kernel)
+
+
+@BOTH
+@pytest.mark.parametrize("tq,tc", KINDS)
+def test_attention_of_one_loud_key_among_many_faint_ones(kernel, tq, tc):
+    """20000 keys that each have 2^-20 of one key's weight, and together 2 % of it: probabilities far below the smallest
+    normal f16."""
+    g = gen(20)
+    kv, n = 20000, 3
+    C = Cache(g, tc, 1, 64, 64, [kv])
+    C.fill(g, 0)
+    pg, sl = C.places(0, torch.arange(kv, device=dev()))
+    scale = C.ks if tc == "e4m3" else torch.ones(1, device=dev())
+    one = torch.ones(1, 64, device=dev()) / scale[:, None]   # k: 1 at every value (the loud key: 2)
+    C.kp[pg, :, sl] = one.to(DT[tc]).expand(kv, 1, 64)
+    C.kp[pg[777], :, sl[777]] = (2 * one).to(DT[tc])
+    v = C.vp[pg, :, sl].float().abs()   # of one sign, so that what the faint keys add does not cancel
+    C.vp[pg, :, sl] = v.to(DT[tc])
+    C.vp[pg[777], :, sl[777]] = 0
+    q = torch.full((n, 2, 64), 20 * math.log(2) * 8 / 64, device=dev()).to(DT[tq])
+    out = torch.zeros_like(q)
+    C.cache.attend(K.PagedBatch(starts([n]), ints([kv]), C.table, **HINTS[kernel]), q, out)
+    C.cache.check()
+    check_attention(C, q, out, [n])
+
+
+@BOTH
+@pytest.mark.parametrize("H,G,d", [(128, 1, 64), (16, 16, 128)])
+def test_attention_of_wide_and_of_single_groups(kernel, H, G, d):
+    g = gen(21)
+    ns, kvs = [3, 1, 20], [200, 333, 20]
+    C = Cache(g, "bf16", G, d, 32, kvs)
+    for s in range(3):
+        C.fill(g, s)
+    attend(g, C, H, ns, "bf16", kernel)
+
+
+@BOTH
+def test_attention_of_a_whole_batch_of_sequences(kernel):
+    """4096 sequences, some of them empty."""
+    g = gen(22)
+    kvs = torch.randint(0, 20, (4096,), generator=torch.Generator().manual_seed(2)).tolist()
+    ns = [min(1, k) for k in kvs]
+    C = Cache(g, "f16", 1, 64, 16, kvs)
+    k = rand(g, *C.kp.shape).to(torch.float16)
+    C.kp.copy_(k), C.vp.copy_(k.flip(0))
+    n = sum(ns)
+    q = rand(g, n, 2, 64).to(torch.float16)
+    out = torch.zeros_like(q)
+    C.cache.attend(K.PagedBatch(starts(ns), ints(kvs), C.table, **HINTS[kernel]), q, out)
+    C.cache.check()
+    at = [i for i, m in enumerate(ns) if m]
+    for j in list(range(0, n, 97)) + [n - 1]:
+        D = Cache.__new__(Cache)
+        D.__dict__.update(C.__dict__, kvs=[kvs[at[j]]], table=C.table[at[j]:at[j] + 1])
+        check_attention(D, q[j:j + 1], out[j:j + 1], [1])
+
+
+@BOTH
+def test_attention_with_a_page_table_of_a_large_capacity(kernel):
+    """So wide a table that sums of work are formed in 64 bits."""
+    g = gen(23)
+    ns, kvs = [700, 600], [700, 1100]
+    C = Cache(g, "bf16", 1, 64, 256, kvs)
+    C.fill(g, 0), C.fill(g, 1)
+    wide = torch.full((2, 1500000), -1, dtype=torch.int32, device=dev())
+    wide[:, :C.table.shape[1]] = C.table
+    C.table = wide
+    attend(g, C, 7, ns, "bf16", kernel)
 
 
 @BOTH
@@ -580,7 +650,7 @@ def test_attention_refuses_tensors_that_do_not_fit():
     for bad in (q.half(), q.float(), q[:, :3], q[:, :, :32], q.cpu(), q[0], rand(g, 1, 64, 4).to(torch.bfloat16).transpose(1, 2)):
         with pytest.raises((ValueError, K.KoreCudaError)):
             C.cache.attend(batch, bad)
-    for kw in (dict(out=q[:, :2]), dict(lse=torch.zeros(1, 3, device=dev())), dict(window=-1),
+    for kw in (dict(out=q), dict(out=q[:, :2]), dict(lse=torch.zeros(1, 3, device=dev())), dict(window=-1),
                dict(workspace=torch.zeros(64, dtype=torch.uint8, device=dev()))):
         with pytest.raises((ValueError, K.KoreCudaError)):
             C.cache.attend(batch, q, **kw)
