@@ -568,52 +568,88 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         // them on their way at once
         auto load_q = [&](const U &a) {
             if (i * kM >= a.rows) return;
-            constexpr int L = D / 8, N = L;   // lanes a row, loads a lane
+            constexpr int L = D / 8, N = E8 ? 8 : L;   // lanes a row, loads a lane at a time
             const int c = lane % L;
             const long long off = offset_of(a, p.q_ts, p.q_hs);
             uint8_t *dst = smem + i * C::TILE + (c >> 3) * C::BLOCK;
-            uint4 v[N];
-            if (p.q_vec) {
 #pragma unroll
-                for (int k = 0; k < N; ++k)
-                    v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const qt *>(p.q) +
-                                                                 __shfl_sync(FULL, off, k * (32 / L) + lane / L) + 8 * c));
-            } else {
+            for (int k0 = 0; k0 < L; k0 += N) {
+                uint4 v[N];
+                if (p.q_vec) {
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        v[k] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const qt *>(p.q) +
+                                                                     __shfl_sync(FULL, off, (k0 + k) * (32 / L) + lane / L) + 8 * c));
+                } else {
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const unsigned short *h = static_cast<const unsigned short *>(p.q) +
+                                                  __shfl_sync(FULL, off, (k0 + k) * (32 / L) + lane / L) + 8 * c;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__ldg(h + 2 * x) | ((uint32_t)__ldg(h + 2 * x + 1) << 16);
+                        v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                // rows whose largest value is between 2^-4 and 2^15 go to f16 as they are (what
+                // is below its range is then below 2^-21 of the largest): all of the warp's, or
+                // each row is looked at by itself
+                bool as_is = true;
+                auto largest = [](const uint4 &x) {
+                    const __nv_bfloat162 *y = reinterpret_cast<const __nv_bfloat162 *>(&x);
+                    return __hmax2(__hmax2(__habs2(y[0]), __habs2(y[1])), __hmax2(__habs2(y[2]), __habs2(y[3])));
+                };
+                if constexpr (E8 && QBF) {
+                    constexpr unsigned GROUP = L == 32 ? FULL : (1u << (L & 31)) - 1;
+                    bool fine = true;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const __nv_bfloat162 t = largest(v[k]);
+                        const float m = fmaxf(__low2float(t), __high2float(t));
+                        const unsigned some = __ballot_sync(FULL, m >= 0.0625f) >> (lane & ~(L - 1));
+                        fine &= (some & GROUP) != 0 && m < 32768.f;
+                    }
+                    as_is = __all_sync(FULL, fine);
+                }
+                if constexpr (E8 && QBF) {
+                    if (!as_is) {   // each row times its power of two
+#pragma unroll 1
+                        for (int k = 0; k < N; ++k) {
+                            uint4 x = v[0];   // (by turns in v[0]: an index would put v into memory)
+#pragma unroll
+                            for (int y = 0; y + 1 < N; ++y) v[y] = v[y + 1];
+                            __nv_bfloat162 t = largest(x);
+#pragma unroll
+                            for (int o = 1; o < L; o <<= 1) t = __hmax2(t, __shfl_xor_sync(FULL, t, o));
+                            const float f = f16_shift(fmaxf(__low2float(t), __high2float(t)));
+                            if (c == 0) q_shift[i * kM + (warp & 3) * 32 + (k0 + k) * (32 / L) + lane / L] = 1.f / f;
+                            uint32_t *w = reinterpret_cast<uint32_t *>(&x);
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                w[y] = pack2<false>(__uint_as_float(w[y] << 16) * f, __uint_as_float(w[y] & 0xffff0000u) * f);
+                            v[N - 1] = x;
+                        }
+                    } else {
+                        if ((lane * L >> 5) / N * N == k0) q_shift[i * kM + r] = 1.f;   // (this lane's row is among these)
+#pragma unroll
+                        for (int k = 0; k < N; ++k) {
+                            uint32_t *w = reinterpret_cast<uint32_t *>(&v[k]);
+#pragma unroll
+                            for (int y = 0; y < 4; ++y)
+                                w[y] = pack2<false>(__uint_as_float(w[y] << 16), __uint_as_float(w[y] & 0xffff0000u));
+                        }
+                    }
+                }
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
-                    const unsigned short *h = static_cast<const unsigned short *>(p.q) + __shfl_sync(FULL, off, k * (32 / L) + lane / L) + 8 * c;
-                    uint32_t w[4];
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) w[x] = (uint32_t)__ldg(h + 2 * x) | ((uint32_t)__ldg(h + 2 * x + 1) << 16);
-                    v[k] = make_uint4(w[0], w[1], w[2], w[3]);
+                    const int row = (warp & 3) * 32 + (k0 + k) * (32 / L) + lane / L;
+                    v[k].x ^= sign;
+                    v[k].y ^= sign;
+                    v[k].z ^= sign;
+                    v[k].w ^= sign;
+                    if (i * kM + row >= a.rows) v[k] = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(dst + sw128(row, c & 7)) = v[k];
                 }
-            }
-            if constexpr (E8 && QBF) {   // to f16, each row times a power of two
-#pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    uint32_t *x = reinterpret_cast<uint32_t *>(&v[k]);
-                    float m = 0.f;
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        m = fmaxf(m, fmaxf(fabsf(__uint_as_float(x[y] << 16)), fabsf(__uint_as_float(x[y] & 0xffff0000u))));
-#pragma unroll
-                    for (int o = 1; o < L; o <<= 1) m = fmaxf(m, __shfl_xor_sync(FULL, m, o));
-                    const float f = f16_shift(m);
-#pragma unroll
-                    for (int y = 0; y < 4; ++y)
-                        x[y] = pack2<false>(__uint_as_float(x[y] << 16) * f, __uint_as_float(x[y] & 0xffff0000u) * f);
-                    if (c == 0) q_shift[i * kM + (warp & 3) * 32 + k * (32 / L) + lane / L] = 1.f / f;
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < N; ++k) {
-                const int row = (warp & 3) * 32 + k * (32 / L) + lane / L;
-                v[k].x ^= sign;
-                v[k].y ^= sign;
-                v[k].z ^= sign;
-                v[k].w ^= sign;
-                if (i * kM + row >= a.rows) v[k] = make_uint4(0, 0, 0, 0);
-                *reinterpret_cast<uint4 *>(dst + sw128(row, c & 7)) = v[k];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -751,6 +787,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             if (!last) {
                 const int c0 = share_of(done.u0 + kUnitCost, total, ctas);
                 const int n = share_of(done.u0 + kUnitCost + done.nt - 1, total, ctas) - c0 + 1;   // parts
+                constexpr int J = E8 ? 32 : 64;   // columns at a time, as the registers allow
                 const int row = i * kM + r, one = 1 << (16 * i);   // the tiles count apart, in the halves of a counter
                 auto slot_of = [&](int k) { return p.part + (size_t)((c0 + k) * 2 + (k == 0)) * kSlot<D>; };
                 const int me = blockIdx.x - c0;
@@ -762,13 +799,13 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     const bool is_left = me < right;
                     float *slot = slot_of(is_left ? left : right);
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 64) {
-                        float o[64];
-                        ld32(to + c, reinterpret_cast<uint32_t *>(o));
-                        ld32(to + c + 32, reinterpret_cast<uint32_t *>(o) + 32);
+                    for (int c = 0; c < D; c += J) {
+                        float o[J];
+#pragma unroll
+                        for (int x = 0; x < J; x += 32) ld32(to + c + x, reinterpret_cast<uint32_t *>(o) + x);
                         wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 64; k += 4)
+                        for (int k = 0; k < J; k += 4)
                             *(reinterpret_cast<float4 *>(slot) + ((c + k) / 4) * kUnitRows + row) =
                                 make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
@@ -793,24 +830,24 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     m = M;
                     l = __fadd_rn(__fmul_rn(a, l), __fmul_rn(b, l2));
 #pragma unroll 1
-                    for (int c = 0; c < D; c += 64) {
-                        float4 x[16];
+                    for (int c = 0; c < D; c += J) {
+                        float4 x[J / 4];
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
+                        for (int k = 0; k < J / 4; ++k)
                             x[k] = __ldcg(reinterpret_cast<const float4 *>(other) + (c / 4 + k) * kUnitRows + row);
-                        float o[64];
-                        ld32(to + c, reinterpret_cast<uint32_t *>(o));
-                        ld32(to + c + 32, reinterpret_cast<uint32_t *>(o) + 32);
+                        float o[J];
+#pragma unroll
+                        for (int k = 0; k < J; k += 32) ld32(to + c + k, reinterpret_cast<uint32_t *>(o) + k);
                         wait_ld();
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) {
+                        for (int k = 0; k < J / 4; ++k) {
                             o[4 * k] = __fadd_rn(__fmul_rn(a, o[4 * k]), __fmul_rn(b, x[k].x));
                             o[4 * k + 1] = __fadd_rn(__fmul_rn(a, o[4 * k + 1]), __fmul_rn(b, x[k].y));
                             o[4 * k + 2] = __fadd_rn(__fmul_rn(a, o[4 * k + 2]), __fmul_rn(b, x[k].z));
                             o[4 * k + 3] = __fadd_rn(__fmul_rn(a, o[4 * k + 3]), __fmul_rn(b, x[k].w));
                         }
-                        st32(to + c, reinterpret_cast<const uint32_t *>(o));
-                        st32(to + c + 32, reinterpret_cast<const uint32_t *>(o) + 32);
+#pragma unroll
+                        for (int k = 0; k < J; k += 32) st32(to + c + k, reinterpret_cast<const uint32_t *>(o) + k);
                     }
                     wait_st();
                 }

@@ -484,6 +484,26 @@ def test_attention_of_one_loud_key_among_many_faint_ones(kernel, tq, tc):
 
 
 @BOTH
+@pytest.mark.parametrize("tq,tc,top", [("bf16", "e4m3", 60), ("bf16", "bf16", 60), ("f16", "e4m3", 10)])
+def test_attention_of_queries_of_any_size(kernel, tq, tc, top):
+    """Rows of q that are all zeros, tiny or huge, and a row with one large value (bf16 queries over an 8-bit cache are
+    brought to f16 a row at a time)."""
+    g = gen(24)
+    n = 40
+    C = Cache(g, tc, 1, 128, 32, [300])
+    C.fill(g, 0)
+    q = rand(g, n, 7, 128)
+    q[::5] = 0
+    q[1::5] *= 2.0 ** -top if tq == "bf16" else 2.0 ** -6
+    q[2::5] *= 2.0 ** top
+    q[3::5, :, 17] = 1000.0
+    q = q.to(DT[tq])
+    out = torch.zeros_like(q)
+    C.cache.attend(K.PagedBatch(starts([n]), ints([300]), C.table, **HINTS[kernel]), q, out)
+    check_attention(C, q, out, [n])
+
+
+@BOTH
 @pytest.mark.parametrize("H,G,d", [(128, 1, 64), (16, 16, 128)])
 def test_attention_of_wide_and_of_single_groups(kernel, H, G, d):
     g = gen(21)
