@@ -420,13 +420,15 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                             o[i][3] *= a1;
                         }
                     }
+                    // (the product is rounded as the maximum's was: fused, a score of 2^40 would be
+                    // off its own reference by more than exp2 can take)
                     const float z0 = m0 == -INFINITY ? 0.f : kBias<BF> - m0, z1 = m1 == -INFINITY ? 0.f : kBias<BF> - m1;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) {
-                        s[j][0] = fast_exp2(fmaf(s[j][0], qs0, z0));
-                        s[j][1] = fast_exp2(fmaf(s[j][1], qs0, z0));
-                        s[j][2] = fast_exp2(fmaf(s[j][2], qs1, z1));
-                        s[j][3] = fast_exp2(fmaf(s[j][3], qs1, z1));
+                        s[j][0] = fast_exp2(__fadd_rn(__fmul_rn(s[j][0], qs0), z0));
+                        s[j][1] = fast_exp2(__fadd_rn(__fmul_rn(s[j][1], qs0), z0));
+                        s[j][2] = fast_exp2(__fadd_rn(__fmul_rn(s[j][2], qs1), z1));
+                        s[j][3] = fast_exp2(__fadd_rn(__fmul_rn(s[j][3], qs1), z1));
                         l0 += s[j][0] + s[j][1];
                         l1 += s[j][2] + s[j][3];
                     }

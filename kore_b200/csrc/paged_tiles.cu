@@ -168,11 +168,6 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
-    unsigned long long r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
 __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -736,17 +731,17 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                         }
                     }
                     const float z = m == -INFINITY ? 0.f : kBias<BF> - m;
-                    const unsigned long long qq = pk2(qs, qs), zz = pk2(z, z);
+                    // (the product is rounded as the maximum's was: fused, a score of 2^40 would be
+                    // off its own reference by more than exp2 can take; two packed instructions
+                    // are fused by the compiler)
                     unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t w[16];
 #pragma unroll
                         for (int x = 0; x < 16; ++x) {
-                            float a, b;
-                            upk2(fma2(pk2(s[32 * h + 2 * x], s[32 * h + 2 * x + 1]), qq, zz), a, b);
-                            a = fast_exp2(a);
-                            b = fast_exp2(b);
+                            const float a = fast_exp2(__fadd_rn(__fmul_rn(s[32 * h + 2 * x], qs), z));
+                            const float b = fast_exp2(__fadd_rn(__fmul_rn(s[32 * h + 2 * x + 1], qs), z));
                             acc[x & 3] = add2(acc[x & 3], pk2(a, b));
                             w[x] = pack2<BF>(a, b);
                         }
