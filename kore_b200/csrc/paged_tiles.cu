@@ -168,6 +168,11 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
     unsigned long long r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -731,22 +736,34 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                         }
                     }
                     const float z = m == -INFINITY ? 0.f : kBias<BF> - m;
-                    // (the product is rounded as the maximum's was: fused, a score of 2^40 would be
-                    // off its own reference by more than exp2 can take; two packed instructions
-                    // are fused by the compiler)
                     unsigned long long acc[4] = {0ull, 0ull, 0ull, 0ull};
+                    const unsigned long long qq = pk2(qs, qs), zz = pk2(z, z);
+                    auto probs = [&](auto huge) {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t w[16];
+                        for (int h = 0; h < 2; ++h) {
+                            uint32_t w[16];
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            const float a = fast_exp2(__fadd_rn(__fmul_rn(s[32 * h + 2 * x], qs), z));
-                            const float b = fast_exp2(__fadd_rn(__fmul_rn(s[32 * h + 2 * x + 1], qs), z));
-                            acc[x & 3] = add2(acc[x & 3], pk2(a, b));
-                            w[x] = pack2<BF>(a, b);
+                            for (int x = 0; x < 16; ++x) {
+                                float a, b;
+                                if constexpr (decltype(huge)::value) {
+                                    a = __fadd_rn(__fmul_rn(s[32 * h + 2 * x], qs), z);
+                                    b = __fadd_rn(__fmul_rn(s[32 * h + 2 * x + 1], qs), z);
+                                } else {
+                                    upk2(fma2(pk2(s[32 * h + 2 * x], s[32 * h + 2 * x + 1]), qq, zz), a, b);
+                                }
+                                a = fast_exp2(a);
+                                b = fast_exp2(b);
+                                acc[x & 3] = add2(acc[x & 3], pk2(a, b));
+                                w[x] = pack2<BF>(a, b);
+                            }
+                            st16(tb + 16 * h, w);
                         }
-                        st16(tb + 16 * h, w);
-                    }
+                    };
+                    // one fused instruction for the factor and the reference, unless a score is so
+                    // large that its product's rounding alone (2^-24 of it), which the reference has
+                    // and a fused one has not, is more than exp2 can take
+                    if (__any_sync(FULL, fabsf(m) > 4194304.f)) probs(std::true_type{});
+                    else probs(std::false_type{});
                     float x, y;
                     upk2(add2(add2(acc[0], acc[1]), add2(acc[2], acc[3])), x, y);
                     l += x + y;
