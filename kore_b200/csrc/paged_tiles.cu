@@ -1,5 +1,5 @@
 // paged_tiles.cu — attention of many query rows a KV head (prompt chunks) over a
-// caller-owned paged cache of 16 bits, on the 5th-generation tensor cores
+// caller-owned paged cache of 16 or 8 bits, on the 5th-generation tensor cores
 // (tcgen05, accumulators in tensor memory), sm_100a.
 //
 // out = softmax(scale q K^T) V for units of 256 packed rows (tokens x the group's
@@ -10,26 +10,34 @@
 //                   S from tensor memory, mask, online softmax (the reference maximum
 //                   moves only when a score passes it by 2^8; O in tensor memory is
 //                   rescaled then), P in 16 bits over S (the A operand of the second
-//                   product), sums in fp32.
+//                   product), sums in fp32. Between units: the next unit's q into shared
+//                   memory, then this one's outputs, so that the next products overlap them.
 //   warp 8          producer: K and V tiles of 128 keys by TMA straight from the pages
 //                   (one box of 16 to 128 tokens a page and half of d, a lane each; a
 //                   page outside the pool arrives as zeros), through a ring.
 //   warps 9, 10     issue the MMAs of tile 0, tile 1: for each step j O += P_j V_j, then
 //                   S_{j+2} = Q K_{j+2}^T into the buffer that P_j leaves, so that the
-//                   softmax never waits for the S after its P. (With one S buffer of 128
-//                   keys a tile and one issuing warp a step of 128 keys took 2.25 us, the
-//                   chain softmax, wait, P V, S; a thread's first barrier access after a
-//                   burst of MMAs waits until the burst has left the queue, so each tile
-//                   has its own issuer.) V is read as it lies in the page (keys x d, the
-//                   MN-major operand), so nothing is transposed. In a unit's boundary
-//                   tiles the rows of V outside its keys are cleared first: 0 * NaN must not
-//                   reach an output.
+//                   softmax never waits for the S after its P. V is read as it lies in the
+//                   page (keys x d, the MN-major operand), so nothing is transposed.
+//   warp 11         watches the ring for the issuers, and clears the rows of V outside the
+//                   unit's keys in its boundary tiles: 0 * NaN must not reach an output.
+//   warps 12-15     (8-bit caches, in warp 11's place) widen the tiles to f16 (exact) from a
+//                   ring of their own into the one that the MMAs read.
+// Measured (2048 tokens on 30720, 28/4 heads of 128, bf16): 887 us, 1050 TFLOP/s, 62 % of
+// the measured bf16 peak; a step takes 1.15 us, of which the MMAs themselves are 0.72 (S: 16
+// of N = 64, 29 ns each, both operands from shared memory; P V: 8 of N = 128, 31 ns), their
+// commits (29 ns each) and the changes of accumulator 0.35. Taken out again: one S buffer of
+// 128 keys a tile with P in two halves (844 us here with bursts by turns, but 72 us for a
+// mixed batch of 500-token chunks at d = 64 where this form takes 58: its chain softmax, P V,
+// S is as long as its step); a quarter of the exponentials by polynomial (10 % slower: the
+// exponentials are hidden already).
 // Events: tile i's event e is on barrier ev[i][e & 1]: event j of a unit of n steps says
 // that S_j is formed and O += P_{j-2} V done; events n and n + 1 that the last two are.
 // Work in equal shares (paged.cuh). The parts of a unit cut between CTAs are joined in
 // a binary tree over the CTAs: the second of two neighbours to finish joins both, so that
 // no CTA waits and no CTA joins more than log2 of the parts; a joint is symmetric in
-// its two sides, so the bits do not depend on who is second.
+// its two sides, so the bits do not depend on who is second. (It takes about 4 us; a
+// second launch for the joints took 10 to 18.)
 // Every wait is bounded; tensor memory is always released.
 
 #include "paged.cuh"
@@ -237,7 +245,8 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     uint32_t *landed = reinterpret_cast<uint32_t *>(bars + 34);
     constexpr int kLanded = E8 ? 4 : 1;
     int *join = reinterpret_cast<int *>(bars + 36);   // [2] a tile's joint: whether it is the second
-    float *q_shift = reinterpret_cast<float *>(bars + 38);   // [2][kM] E8: 1 / (power of two on the q row)
+    uint64_t *pv_done = bars + 38;          // [2] tile i's last O += P V is done
+    float *q_shift = reinterpret_cast<float *>(bars + 40);   // [2][kM] E8: 1 / (power of two on the q row)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     if (threadIdx.x == 256) {
@@ -261,6 +270,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             mbar_init(&ev[2 * i], 1);
             mbar_init(&ev[2 * i + 1], 1);
             mbar_init(&drained[i], 1);
+            mbar_init(&pv_done[i], 1);
         }
         *abort_flag = 0;
         for (int i = 0; i < 8; ++i) p_seq[i] = 0;
@@ -381,7 +391,8 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         constexpr uint32_t t_s = C::T_S + 128 * i, t_o = C::T_O + D * i;   // (the CTA holds all of tensor memory, from 0 on)
         const uint32_t q_lo = uniform(desc_k(sbase + i * C::TILE));
         uint32_t base = 0;           // ring position of the unit's first tile (K; V follows)
-        uint32_t n_q = 0, n_p = 0, e = 0;   // q and P so far, events
+        uint32_t n_q = 0, n_p = 0, e = 0, n_pv = 0;   // q and P so far, events, waits for P V
+        const uint32_t pv_bar = uniform(smem_u32(&pv_done[i]));
         bool ok = true;
         auto stage_of = [&](uint32_t at) { return sbase + C::RING + (at % C::STAGES) * C::TILE; };
         auto full_wait = [&](uint32_t at) { return reached(landed, kLanded, at + 1); };
@@ -456,10 +467,19 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
 #pragma unroll
                     for (int c = 0; c < kStep / 16; ++c)
                         mma_ts<ID_O>(t_o, t_s + 64 * b + 8 * c, vb + c * (16 * 128 / 16), c > 0 ? 1u : acc);
-                    if (leave) commit(s_bar);
+                    if (j + 2 < n) commit(pv_bar);
+                    else if (leave) commit(s_bar);
                 }
                 __syncwarp();
                 if (j + 2 < n) {
+                    // S goes over P: only MMAs of one accumulator and shape are sure to run in
+                    // the order of their issue
+                    ok = wait(&pv_done[i], n_pv & 1);
+                    if (!ok) break;
+                    ++n_pv;
+                    fence_after();
+                    if (leave && lane == 0) mbar_arrive(&empty[vt % C::STAGES]);
+                    __syncwarp();
                     issue_s(k + 2, e + j + 2);
                 } else {
                     if (lane == 0) commit(smem_u32(&ev[2 * i + b]));
