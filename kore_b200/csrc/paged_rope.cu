@@ -256,7 +256,7 @@ cudaError_t launch(void (*kernel)(Args...), int blocks, int threads, size_t smem
 template <typename T, typename C, bool APPEND>
 cudaError_t launch_tc(const RotateParams &p, bool vec, cudaStream_t s) {
     // four heads a thread: the table's values in its registers serve all of them,
-    // and a CTA is small enough for many tokens an SM (12288 tokens of 28/4 heads of
+    // and a CTA is small enough for many tokens an SM (5303 tokens of 28/4 heads of
     // 128: 19.8 us; two heads 21.9, six 19.9). Two where the CTAs would not fill the SMs
     // (48 tokens: 2.7 us; four heads 2.9)
     const int heads = p.q.heads + (APPEND ? 2 * p.G : 0);

@@ -10,7 +10,7 @@ A step of a batch, on the current stream of the tensors' device::
     cache.append(batch, k, v, rope=rope, q=q, q_out=q)    # a layer: store k and v, rotate k and q
     cache.attend(batch, q, out)
 
-An object is for one host thread at a time, as a context is. Nothing is copied or synchronised: a failure that a kernel meets in the device
+An object is for one host thread at a time, as a context is; nothing here is recorded for gradients. Nothing is copied or synchronised: a failure that a kernel meets in the device
 data (a page outside the pool, a sequence that does not fit its page table)
 is left in ``status`` and raised by ``check()``.
 """
@@ -197,6 +197,8 @@ class RopeTable:
         pp = _ints(pos, "pos", self.device, 1)
         if pos.shape[0] != n:
             raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
+        if n == 0:
+            return out
         rc = self._L.kore_cuda_rope_dev(self._px, self._pout, n, pp, self._view, self._status, _stream(self.device))
         if rc:
             _ck(self._L, rc)
@@ -269,14 +271,16 @@ class PagedCache:
         if _fill(r[1], v, "v", dev) != n:
             raise ValueError("k and v have different numbers of tokens")
         pq = pqo = None
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out come together")
         if q is not None:
-            if q_out is None:
-                raise ValueError("q comes with q_out")
             if _fill(r[2], q, "q", dev) != n or _fill(r[3], q_out, "q_out", dev) != n:
                 raise ValueError("q, q_out and k have different numbers of tokens")
             pq, pqo = self._p[2], self._p[3]
         if batch.device != dev or (rope is not None and rope.device != dev):
             raise ValueError(f"the batch or the table is not on {dev}")
+        if n == 0:
+            return
         rc = self._L.kore_cuda_paged_append_dev(self._view, batch._view, n, self._p[0], self._p[1], pq, pqo,
                                                 rope._view if rope is not None else None, self._status, _stream(dev))
         if rc:
@@ -304,6 +308,8 @@ class PagedCache:
             plse = lse.data_ptr()
         if batch.device != dev:
             raise ValueError(f"the batch is not on {dev}")
+        if n == 0:
+            return out
         s = _stream(dev)
         ws = workspace if workspace is not None else _workspace(self._L, dev, s, self.view.head_dim)
         o = self._opts

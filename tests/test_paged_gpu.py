@@ -800,6 +800,35 @@ def test_prompts_and_steps_together(kernel, tq, tc, H, G, d, P):
             assert torch.equal(got_v.float(), vals[s].float())
 
 
+def test_no_tokens_and_no_sequences():
+    g = gen(25)
+    C = Cache(g, "bf16", 2, 64, 16, [20])
+    none = torch.empty(0, 2, 64, dtype=torch.bfloat16, device=dev())
+    batch = K.PagedBatch(ints([0, 0]), ints([20]), C.table, 1)
+    C.cache.append(batch, none, none)
+    assert C.cache.attend(batch, none).shape == none.shape
+    assert K.RopeTable(4, 64).rotate(none, ints([])).shape == none.shape
+    x = torch.full((3, 2, 64), GUARD, dtype=torch.bfloat16, device=dev())
+    out = x.clone()
+    nobody = K.PagedBatch(ints([0]), ints([]), ints([]).reshape(0, 1), 1)
+    C.cache.append(nobody, x, x)
+    C.cache.attend(nobody, x + 1, out)
+    assert torch.equal(out, x)
+    C.cache.check()
+    with pytest.raises(ValueError, match="together"):
+        C.cache.append(batch, x, x, q_out=x)
+
+
+def test_sequences_may_share_pages():
+    """A common beginning in one set of pages, attended by two sequences."""
+    g = gen(26)
+    for kernel in HINTS:
+        C = Cache(g, "bf16", 2, 64, 16, [64, 100])
+        C.fill(g, 0), C.fill(g, 1)
+        C.table[0, :4] = C.table[1, :4]
+        attend(g, C, 14, [3, 40], "bf16", kernel)
+
+
 def test_tensors_on_another_device_than_the_current_one():
     if torch.cuda.device_count() < 2:
         pytest.skip("one GPU")
