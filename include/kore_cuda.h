@@ -498,7 +498,8 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
  * All pointers are device pointers; calls are ordered on `stream` (a
  * cudaStream_t of the device that holds the buffers; NULL for the default
  * stream), allocate nothing, return without synchronising and can be captured
- * into a graph. The device of the first data pointer is made current for the
+ * into a graph. What they read, the batch's arrays among it, must not change
+ * while they run. The device of the first data pointer is made current for the
  * call. dev_status (optional, zeroed by the caller) receives the first failure
  * that a kernel meets in the device data: 3 a page id outside the pool, 6 a
  * position outside the rotation table, 7 a sequence whose bounds do not fit
