@@ -17,6 +17,7 @@ is left in ``status`` and raised by ``check()``.
 from __future__ import annotations
 
 import ctypes
+import struct
 
 from . import KoreCudaError, load_library
 
@@ -72,16 +73,14 @@ def _library():
     global _fns
     if _fns is None:
         L = load_library()
-        p = ctypes.POINTER
-        L.kore_cuda_rope_freqs.argtypes = [p(_RopeSpec), p(ctypes.c_float), p(_d)]
-        L.kore_cuda_rope_table_dev.argtypes = [p(_RopeSpec), _i, _vp, _vp]
-        L.kore_cuda_rope_dev.argtypes = [p(_Rows), p(_Rows), _i, _vp, p(_RopeView), _vp, _vp]
-        L.kore_cuda_paged_append_dev.argtypes = ([p(_Pages), p(_Batch), _i] + [p(_Rows)] * 4
-                                                 + [p(_RopeView), _vp, _vp])
+        # structures go by their address: a c_void_p costs less a call than a POINTER
+        L.kore_cuda_rope_freqs.argtypes = [_vp, _vp, _vp]
+        L.kore_cuda_rope_table_dev.argtypes = [_vp, _i, _vp, _vp]
+        L.kore_cuda_rope_dev.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp]
+        L.kore_cuda_paged_append_dev.argtypes = [_vp, _vp, _i] + [_vp] * 7
         L.kore_cuda_paged_attn_workspace.argtypes = [_i]
         L.kore_cuda_paged_attn_workspace.restype = _ll
-        L.kore_cuda_paged_attn_dev.argtypes = [p(_Pages), p(_Batch), _i, p(_Rows), p(_Rows), _vp, p(_Opts), _vp, _ll,
-                                               _vp, _vp]
+        L.kore_cuda_paged_attn_dev.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp]
         L.kore_cuda_capture_id.argtypes = [_vp]
         L.kore_cuda_capture_id.restype = ctypes.c_ulonglong
         _fns = L
@@ -106,19 +105,21 @@ def _import_torch():
     return _torch
 
 
+_pack_rows = struct.Struct("@Piiiqq").pack_into   # _Rows, in one step
+
+
 def _fill(r: _Rows, t, what: str, device) -> int:
     """Describes a [tokens][heads][head_dim] tensor in r; returns its tokens."""
-    if t.dim() != 3:
-        raise ValueError(f"{what}: expected [tokens][heads][head_dim], got {tuple(t.shape)}")
-    n, h, d = t.shape
+    shape = t.shape
+    if len(shape) != 3:
+        raise ValueError(f"{what}: expected [tokens][heads][head_dim], got {tuple(shape)}")
+    n, h, d = shape
     ts, hs, es = t.stride()
     if es != 1 and d > 1:
         raise ValueError(f"{what}: the values of a head must be contiguous")
-    if t.device != device:
+    if t.get_device() != device.index:
         raise ValueError(f"{what} is on {t.device}, expected {device}")
-    r.data = t.data_ptr()
-    r.type = _types.get(t.dtype, -1)
-    r.n_head, r.head_dim, r.token_stride, r.head_stride = h, d, ts, hs
+    _pack_rows(r, 0, t.data_ptr(), _types.get(t.dtype, -1), h, d, ts, hs)
     return n
 
 
@@ -182,9 +183,9 @@ class RopeTable:
         _ck(self._L, self._L.kore_cuda_rope_table_dev(ctypes.byref(spec), n_pos, self.table.data_ptr(),
                                                       _stream(self.device)))
         self.view = _RopeView(self.table.data_ptr(), n_pos, n_rot, int(bool(interleaved)))
-        self._view = ctypes.byref(self.view)
+        self._view = ctypes.addressof(self.view)
         self._x, self._out = _Rows(), _Rows()
-        self._px, self._pout = ctypes.byref(self._x), ctypes.byref(self._out)
+        self._px, self._pout = ctypes.addressof(self._x), ctypes.addressof(self._out)
 
     def rotate(self, x, pos, out=None):
         """Rotates x [tokens][heads][head_dim] (fp32, fp16 or bf16) at the int32 positions pos [tokens] into out
@@ -226,7 +227,7 @@ class PagedBatch:
         if q_start.shape[0] != n + 1 or page_table.shape[0] != n:
             raise ValueError(f"q_start must have {n + 1} and page_table {n} rows")
         self.q_start, self.kv_len, self.page_table, self.view = q_start, kv_len, page_table, view
-        self._view = ctypes.byref(view)
+        self._view = ctypes.addressof(view)
 
 
 class PagedCache:
@@ -254,14 +255,13 @@ class PagedCache:
             scales.append(s.data_ptr() if s is not None else None)
         self.view = _Pages(k_pages.data_ptr(), v_pages.data_ptr(), _types.get(k_pages.dtype, -1), n, p, g, d,
                            k_pages.stride(0) if n > 1 else 0, *scales)
-        self._view = ctypes.byref(self.view)
+        self._view = ctypes.addressof(self.view)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._status = self.status.data_ptr()
         self._r = [_Rows() for _ in range(4)]
-        self._p = [ctypes.byref(r) for r in self._r]
+        self._p = [ctypes.addressof(r) for r in self._r]
         self._opts = _Opts()
-        self._popts = ctypes.byref(self._opts)
-        self._ws_bytes = 0
+        self._popts = ctypes.addressof(self._opts)
 
     def append(self, batch: PagedBatch, k, v, *, rope: RopeTable | None = None, q=None, q_out=None) -> None:
         """Stores k (rotated by rope at each token's position) and v [tokens][n_head_kv][head_dim] in the pages; with
@@ -345,7 +345,9 @@ _WORKSPACES_KEPT = 16
 
 
 def _workspace(L, device, stream: int, head_dim: int):
-    key = (device.index, stream, L.kore_cuda_capture_id(stream))
+    # (torch's answer is the current device's, and quicker)
+    may = _torch._C._cuda_getDevice() != device.index or _torch._C._cuda_isCurrentStreamCapturing()
+    key = (device.index, stream, L.kore_cuda_capture_id(stream) if may else 0)
     ws = _workspaces.get(key)
     if ws is None:
         # the larger of the two head sizes serves both. In a capture it is the
