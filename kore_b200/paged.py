@@ -244,9 +244,11 @@ class PagedCache:
         if (k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype or k_pages.device != v_pages.device
                 or k_pages.stride(0) != v_pages.stride(0)):
             raise ValueError("k_pages and v_pages differ in shape, type, device or page stride")
+        n, g, p, d = k_pages.shape
+        if n > 1 and k_pages.stride(0) < g * p * d:   # (an expanded page; the C side takes a stride of 0 as dense)
+            raise ValueError(f"k_pages and v_pages: the pages overlap (page stride {k_pages.stride(0)})")
         self.k, self.v, self.k_scale, self.v_scale = k_pages, v_pages, k_scale, v_scale
         self.device = k_pages.device
-        n, g, p, d = k_pages.shape
         scales = []
         for s, what in ((k_scale, "k_scale"), (v_scale, "v_scale")):
             if s is not None and (s.dtype != torch.float32 or tuple(s.shape) != (g,) or not s.is_contiguous()
