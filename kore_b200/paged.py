@@ -310,6 +310,9 @@ class PagedCache:
             plse = lse.data_ptr()
         if batch.device != dev:
             raise ValueError(f"the batch is not on {dev}")
+        if workspace is not None and (workspace.dtype != _torch.uint8 or workspace.device != dev
+                                      or not workspace.is_contiguous()):
+            raise ValueError(f"workspace: expected a contiguous uint8 tensor on {dev}, as new_workspace() makes it")
         if n == 0:
             return out
         s = _stream(dev)

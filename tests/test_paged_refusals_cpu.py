@@ -31,3 +31,19 @@ def test_pages_that_overlap_are_refused(fake):
         K.PagedCache(near, near)
     for ok in (one, cuda(4, 2, 16, 64), cuda(4, 2, 2, 16, 64)[:, 0], one.expand(1, 2, 16, 64)):
         K.PagedCache(ok, ok)
+
+
+def step(n=1, device="cuda:0"):
+    """A cache, a batch of one sequence and its queries."""
+    pages = cuda(4, 2, 16, 64, device=device)
+    ints = [cuda(*s, dtype=torch.int32, device=device) for s in ((2,), (1,), (1, 4))]
+    return K.PagedCache(pages, pages), K.PagedBatch(*ints, max_q=1), cuda(n, 4, 64, device=device)
+
+
+@pytest.mark.parametrize("workspace", [dict(device="cpu"), dict(device="cuda:1"), dict(dtype=torch.float32), dict(step=2)])
+def test_workspaces_that_the_kernels_cannot_use_are_refused(fake, workspace):
+    cache, batch, q = step()
+    skip = workspace.pop("step", 1)
+    ws = cuda(1 << 27, **{"dtype": torch.uint8, **workspace})[::skip]
+    with pytest.raises(ValueError, match="workspace"):
+        cache.attend(batch, q, cuda(1, 4, 64), workspace=ws)
