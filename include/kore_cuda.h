@@ -506,8 +506,8 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
  * the rows, its length or its page table. Such a sequence (for 6 and for an
  * append's 3: such a token) is left out: none of its rows are written. In the
  * attention a bad page's keys count as zeros. 1 is a tile copy or a product that
- * did not come within 2 s: the attention's outputs are void then, and the
- * workspace has to be zeroed again.
+ * did not come within 2 s (kore_cuda_paged_set_wait_limit): the attention's
+ * outputs are void then, and the workspace has to be zeroed again.
  */
 #define KORE_CUDA_E4M3 1000   /* 8 bits, 4 of exponent and 3 of mantissa, no infinities (not a GGUF type) */
 
@@ -640,6 +640,11 @@ int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch
                              const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
                              const kore_cuda_attn_opts *opts, void *workspace, long long workspace_bytes,
                              int *dev_status, void *stream);
+
+/* How long a wait inside an attention that is launched (or captured) from now
+ * on may take before the kernel gives up, in the whole process; 0: 2 s. A host
+ * that wants to hear of a failure sooner sets less. */
+int kore_cuda_paged_set_wait_limit(unsigned long long nanoseconds);
 
 /* Identity of the graph capture that `stream` is in (0: none), for callers that
  * keep one workspace per capture. */

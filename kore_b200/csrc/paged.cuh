@@ -80,6 +80,7 @@ struct PagedAttnParams {
     int *counters;             // [kPagedMaxCtas] zero between calls
     float *part;               // [kPagedMaxCtas][2] partial results
     int *status;
+    unsigned long long wait_ns;   // a wait gives up after so long
 };
 
 // four e4m3 values (first in the lowest byte) as two pairs of f16
@@ -200,6 +201,25 @@ __device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q
     u.b = b;
     u.range(p);
     return kUnitCost + u.nt;
+}
+
+// A wait that did not end at its first look: until the phase is done, or false when
+// `limit_ns` (or kWaitPolls looks) are over. (Inline, and without mbar_wait's timing of the
+// first look: out of line it cost the chunk kernel 1 %, with that timing 4 %.)
+__device__ __forceinline__ bool late_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
+    const uint64_t since = global_ns();
+    for (uint32_t looks = 1; looks < kWaitPolls; ++looks) {
+        // (a look may itself last until the phase is done: then it counts as well)
+        if (mbar_try_wait(bar, parity)) return global_ns() - since <= limit_ns;
+        if ((looks & 7) == 0 && global_ns() - since > limit_ns) break;
+    }
+    return false;
+}
+
+// The wait for a tile copy. Under a limit shorter than the default the first look is timed too.
+__device__ __forceinline__ bool copy_wait(uint64_t *bar, uint32_t parity, uint64_t limit_ns) {
+    if (limit_ns >= kWaitNs && mbar_try_wait(bar, parity)) return true;
+    return late_wait(bar, parity, limit_ns);
 }
 
 // Asks for a tensor map ahead of its first copy.

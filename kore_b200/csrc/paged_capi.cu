@@ -8,6 +8,7 @@
 
 #include <cuda.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
@@ -25,6 +26,8 @@ int refuse(int code, const char *fmt, ...) {
     set_ctxless_error(buf);
     return code;
 }
+
+std::atomic<unsigned long long> g_wait_ns{kWaitNs};   // of launches from now on
 
 int type_bytes(int type) {
     switch (type) {
@@ -325,6 +328,11 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
     return launched(launch_rotate(p, k->type, cache->type, vec, (cudaStream_t)stream), "paged_append");
 }
 
+extern "C" int kore_cuda_paged_set_wait_limit(unsigned long long nanoseconds) {
+    g_wait_ns = nanoseconds ? nanoseconds : kWaitNs;
+    return KORE_CUDA_OK;
+}
+
 extern "C" long long kore_cuda_paged_attn_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return refuse(KORE_CUDA_EINVAL, "head_dim %d is not supported here", head_dim);
     return (long long)kPagedZeroed + (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
@@ -399,6 +407,7 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.counters = static_cast<int *>(workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed);
     p.status = dev_status;
+    p.wait_ns = g_wait_ns;
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
     // units are of 16 rows and tiles of 128 keys at least
     p.small = ((double)n_tok * p.rep / 16 + p.n_seq) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;

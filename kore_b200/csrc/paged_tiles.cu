@@ -289,12 +289,15 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     const uint32_t tmem = *tmem_slot;
 
     // bounded, by whole warps, with one answer for the warp
-    auto wait = [&](uint64_t *bar, uint32_t parity) -> bool {
-        bool got = mbar_try_wait(bar, parity);
+    auto wait = [&](uint64_t *bar, uint32_t parity, bool copy = false) -> bool {
+        bool got = (!copy || p.wait_ns >= kWaitNs) && mbar_try_wait(bar, parity);
         if (__all_sync(FULL, got)) return true;
         if (!got && !*reinterpret_cast<volatile int *>(abort_flag)) {
-            got = mbar_wait(bar, parity, p.status, DEV_WAIT_FULL_TIMEOUT);
-            if (!got) *reinterpret_cast<volatile int *>(abort_flag) = 1;
+            got = late_wait(bar, parity, p.wait_ns);
+            if (!got) {
+                raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+                *reinterpret_cast<volatile int *>(abort_flag) = 1;
+            }
         }
         return __all_sync(FULL, got);
     };
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             if ((polls & 1023) == 1023) {
                 const uint64_t now = global_ns();
                 if (!since) since = now;
-                const bool late = now - since > kWaitNs;
+                const bool late = now - since > p.wait_ns;
                 if (__any_sync(FULL, late || *reinterpret_cast<volatile int *>(abort_flag))) {
                     if (lane == 0) {
                         raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
@@ -380,9 +383,10 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 }
             }
         } while (ok && next_unit(u));
-        if (!ok)   // copies in flight land before the CTA may end
-            for (uint32_t i = it > (uint32_t)C::LOADS ? it - C::LOADS : 0; i < it; ++i)
-                mbar_drain(&full[i % C::LOADS], (i / C::LOADS) & 1);
+        // copies in flight land before the CTA may end, also where this warp issued its last
+        // one before another gave up on it (else they have landed, or do while the others work)
+        for (uint32_t i = it > (uint32_t)C::LOADS ? it - C::LOADS : 0; i < it; ++i)
+            mbar_drain(&full[i % C::LOADS], (i / C::LOADS) & 1);
     } else if (warp == 9 || warp == 10) {
         // ------------------------------------------------------------ MMA issuers
         auto issuer = [&](auto tile) {
@@ -492,7 +496,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         // tensor memory is released below only after every MMA issued here is done
         if (lane == 0) commit(smem_u32(&drained[i]));
         __syncwarp();
-        mbar_wait(&drained[i], 0, p.status, DEV_WAIT_FULL_TIMEOUT);
+        if (!mbar_drain(&drained[i], 0)) raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
         };
         if (warp == 9) issuer(std::integral_constant<int, 0>{});
         else issuer(std::integral_constant<int, 1>{});
@@ -507,7 +511,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             share_tiles(u, t0, t1);
             for (int t = t0; ok && t < t1; ++t) {
                 for (int kv = 0; ok && kv < 2; ++kv, ++it) {
-                    ok = wait(&full[it % C::STAGES], (it / C::STAGES) & 1);
+                    ok = wait(&full[it % C::STAGES], (it / C::STAGES) & 1, true);
                     const int key0 = (u.tile0 + t) * kKeys;
                     if (ok && kv == 1 && (key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
                         uint8_t *v = smem + C::RING + (it % C::STAGES) * C::TILE;
@@ -538,7 +542,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             for (int t = t0; ok && t < t1; ++t) {
                 const int key0 = (u.tile0 + t) * kKeys;
                 for (int kv = 0; ok && kv < 2; ++kv, ++it) {
-                    ok = wait(&full[it % C::RAW_STAGES], (it / C::RAW_STAGES) & 1);
+                    ok = wait(&full[it % C::RAW_STAGES], (it / C::RAW_STAGES) & 1, true);
                     if (ok && it >= C::STAGES) ok = wait(&empty[it % C::STAGES], (it / C::STAGES - 1) & 1);
                     if (!ok) break;
                     const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 32 * D + lane * 16;

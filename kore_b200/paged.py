@@ -21,7 +21,7 @@ import struct
 
 from . import KoreCudaError, load_library
 
-__all__ = ["RopeTable", "PagedCache", "PagedBatch", "rope_frequencies"]
+__all__ = ["RopeTable", "PagedCache", "PagedBatch", "rope_frequencies", "set_wait_limit"]
 
 F32, F16, BF16, E4M3 = 0, 1, 30, 1000
 WORKSPACE_ZEROED = 1024
@@ -81,6 +81,7 @@ def _library():
         L.kore_cuda_paged_attn_workspace.argtypes = [_i]
         L.kore_cuda_paged_attn_workspace.restype = _ll
         L.kore_cuda_paged_attn_dev.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp]
+        L.kore_cuda_paged_set_wait_limit.argtypes = [ctypes.c_ulonglong]
         L.kore_cuda_capture_id.argtypes = [_vp]
         L.kore_cuda_capture_id.restype = ctypes.c_ulonglong
         _fns = L
@@ -156,6 +157,15 @@ def rope_frequencies(n_rot: int, *, base: float = 1e6, scaling: str = "none", fa
     spec = _spec(n_rot, base, scaling, factor, original_ctx, beta_fast, beta_slow, amplitude)
     _ck(L, L.kore_cuda_rope_freqs(ctypes.byref(spec), f, ctypes.byref(a)))
     return list(f[:n_rot // 2]), a.value
+
+
+def set_wait_limit(seconds: float) -> None:
+    """How long a wait inside an attention launched from now on may take before it is reported (0: 2 s), in the whole
+    process (kore_cuda_paged_set_wait_limit)."""
+    if not 0 <= seconds <= 1e9:
+        raise ValueError(f"seconds = {seconds}")
+    L = _library()
+    _ck(L, L.kore_cuda_paged_set_wait_limit(int(seconds * 1e9)))
 
 
 class RopeTable:

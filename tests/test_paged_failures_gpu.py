@@ -1,0 +1,94 @@
+"""Waits inside the attention over a paged cache that run out, without a GPU fault: under a limit far below a copy's
+latency (kore_cuda_paged_set_wait_limit) real copies land "too late". The kernel reports it, waits for its own copies and
+products still in flight, frees its tensor memory and returns; the next call is right."""
+import pytest
+
+import kore_b200 as K
+from kore_b200.paged import set_wait_limit
+from tests.test_paged_gpu import BOTH, Cache, HINTS, check_attention, dev, gen, ints, rand, starts
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+# one short unit, whose copies are all issued before the first is missed; and many, of several CTAs each
+BATCHES = {"short": [(3, 90)], "long": [(2, 9000), (40, 700), (1, 3000)]}
+
+
+@pytest.fixture
+def impatient():
+    set_wait_limit(1e-9)
+    yield
+    set_wait_limit(0)
+
+
+def ready(tc, which, seed=1):
+    g = gen(seed)
+    ns, kvs = map(list, zip(*BATCHES[which]))
+    C = Cache(g, tc, 2, 128, 64, kvs)
+    for s in range(len(kvs)):
+        C.fill(g, s)
+    return C, ns, rand(g, sum(ns), 14, 128).to(torch.bfloat16)
+
+
+def run_out(C, batch, q, **kw):
+    """Calls until a wait has run out (a copy may have landed before the kernel looks)."""
+    for _ in range(20):
+        C.cache.attend(batch, q, torch.zeros_like(q), **kw)
+        try:
+            C.cache.check()
+        except K.KoreCudaError as e:
+            return e
+    pytest.fail("no wait ran out with a limit of 1 ns")
+
+
+@BOTH
+@pytest.mark.parametrize("tc", ["bf16", "e4m3"])
+@pytest.mark.parametrize("which", list(BATCHES))
+def test_a_wait_that_runs_out_is_reported_and_the_next_call_is_right(impatient, kernel, tc, which):
+    C, ns, q = ready(tc, which)
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
+    e = run_out(C, batch, q)
+    assert e.code == -6 and "in time" in str(e)
+    set_wait_limit(0)
+    for _ in range(3):
+        out = C.cache.attend(batch, q)
+        C.cache.check()
+        check_attention(C, q, out, ns)
+
+
+@BOTH
+def test_a_workspace_of_the_callers_is_zeroed_again_after_a_failure(impatient, kernel):
+    C, ns, q = ready("bf16", "long")
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
+    ws = C.cache.new_workspace()
+    run_out(C, batch, q, workspace=ws)
+    set_wait_limit(0)
+    ws[:K.paged.WORKSPACE_ZEROED].zero_()
+    out = C.cache.attend(batch, q, workspace=ws)
+    C.cache.check()
+    check_attention(C, q, out, ns)
+
+
+@BOTH
+def test_a_captured_call_keeps_the_limit_of_its_capture(kernel):
+    C, ns, q = ready("bf16", "long")
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
+    out = torch.zeros_like(q)
+    C.cache.attend(batch, q, out)
+    torch.cuda.synchronize(dev())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        C.cache.attend(batch, q, out)
+    set_wait_limit(1e-9)
+    try:
+        graph.replay()
+        C.cache.check()
+    finally:
+        set_wait_limit(0)
+    check_attention(C, q, out, ns)
+
+
+def test_a_limit_that_is_no_time_is_refused():
+    for bad in (-1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            set_wait_limit(bad)
