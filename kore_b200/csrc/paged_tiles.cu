@@ -104,6 +104,8 @@ __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.
 // registers, so the low words come from a warp-wide reduction (whose result is one) and
 // all else is constant.
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
+// The lane that issues the products also commits them: a commit follows its own thread's
+// operations only, and which lane is elected is not said (for one mask it is always the same).
 __device__ __forceinline__ bool elect() {
     uint32_t ok;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
@@ -445,7 +447,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     fence_after();
                     issue_s(k0 + j, e + j);
                 } else {   // an event without an S
-                    if (lane == 0) commit(smem_u32(&ev[2 * i + ((e + j) & 1)]));
+                    if (elect()) commit(smem_u32(&ev[2 * i + ((e + j) & 1)]));
                     __syncwarp();
                 }
             }
@@ -486,7 +488,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     __syncwarp();
                     issue_s(k + 2, e + j + 2);
                 } else {
-                    if (lane == 0) commit(smem_u32(&ev[2 * i + b]));
+                    if (elect()) commit(smem_u32(&ev[2 * i + b]));
                     __syncwarp();
                 }
             }
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             base += 2 * (t1 - t0);
         } while (ok && next_unit(u));
         // tensor memory is released below only after every MMA issued here is done
-        if (lane == 0) commit(smem_u32(&drained[i]));
+        if (elect()) commit(smem_u32(&drained[i]));
         __syncwarp();
         if (!mbar_drain(&drained[i], 0)) raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
         };
