@@ -507,7 +507,8 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
  * append's 3: such a token) is left out: none of its rows are written. In the
  * attention a bad page's keys count as zeros. 1 is a tile copy or a product that
  * did not come within 2 s (kore_cuda_paged_set_wait_limit): the attention's
- * outputs are void then, and the workspace has to be zeroed again.
+ * outputs are void then, and the workspace has to be zeroed again. It takes the
+ * place of any other code.
  */
 #define KORE_CUDA_E4M3 1000   /* 8 bits, 4 of exponent and 3 of mantissa, no infinities (not a GGUF type) */
 

@@ -203,6 +203,11 @@ __device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q
     return kUnitCost + u.nt;
 }
 
+// A wait ran out: in place of any other code, since it is what makes the workspace unusable.
+__device__ __forceinline__ void raise_late(int *status) {
+    if (status) atomicExch(status, DEV_WAIT_FULL_TIMEOUT);
+}
+
 // A wait that did not end at its first look: until the phase is done, or false when
 // `limit_ns` (or kWaitPolls looks) are over. (Inline, and without mbar_wait's timing of the
 // first look: out of line it cost the chunk kernel 1 %, with that timing 4 %.)

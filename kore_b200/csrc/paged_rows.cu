@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             for (int tt = t0; tt < t1; ++tt) {
                 if (!dead && !__all_sync(FULL, copy_wait(&full[stage], (n_taken / C::STAGES) & 1, p.wait_ns))) {
                     dead = true;
-                    if (lane == 0) raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+                    if (lane == 0) raise_late(p.status);
                 }
                 if (!dead) ++n_taken;
                 __syncwarp();   // every lane is done with the tile before this one

@@ -297,7 +297,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         if (!got && !*reinterpret_cast<volatile int *>(abort_flag)) {
             got = late_wait(bar, parity, p.wait_ns);
             if (!got) {
-                raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+                raise_late(p.status);
                 *reinterpret_cast<volatile int *>(abort_flag) = 1;
             }
         }
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 const bool late = now - since > p.wait_ns;
                 if (__any_sync(FULL, late || *reinterpret_cast<volatile int *>(abort_flag))) {
                     if (lane == 0) {
-                        raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+                        raise_late(p.status);
                         *reinterpret_cast<volatile int *>(abort_flag) = 1;
                     }
                     return false;
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         // tensor memory is released below only after every MMA issued here is done
         if (elect()) commit(smem_u32(&drained[i]));
         __syncwarp();
-        if (!mbar_drain(&drained[i], 0)) raise_error(p.status, DEV_WAIT_FULL_TIMEOUT);
+        if (!mbar_drain(&drained[i], 0)) raise_late(p.status);
         };
         if (warp == 9) issuer(std::integral_constant<int, 0>{});
         else issuer(std::integral_constant<int, 1>{});

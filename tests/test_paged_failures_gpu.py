@@ -92,3 +92,19 @@ def test_a_limit_that_is_no_time_is_refused():
     for bad in (-1.0, float("nan"), float("inf")):
         with pytest.raises(ValueError):
             set_wait_limit(bad)
+
+
+@BOTH
+def test_a_run_out_wait_is_reported_before_bad_device_data(impatient, kernel):
+    """It is what makes the workspaces unusable: a bad page that was met before must not hide it."""
+    C, ns, q = ready("bf16", "long")
+    table = C.table.clone()
+    table[:, 0] = 10 ** 6
+    e = run_out(C, K.PagedBatch(starts(ns), ints(C.kvs), table, **HINTS[kernel]), q)
+    assert "in time" in str(e)
+    set_wait_limit(0)
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
+    for _ in range(2):
+        out = C.cache.attend(batch, q)
+        C.cache.check()
+        check_attention(C, q, out, ns)
