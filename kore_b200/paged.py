@@ -135,9 +135,11 @@ def _stream(device) -> int:
 
 
 def _check_status(status) -> None:
+    _torch.cuda.synchronize(status.device)   # the calls may be on any stream
     code = int(status.item())
     if code:
         status.zero_()
+        _torch.cuda.synchronize(status.device)   # what is launched from now on, on any stream, is kept
         if code == 1:   # workspaces are not as a call leaves them
             _workspaces.clear()
         raise KoreCudaError(-6, DEVICE_FAILURES.get(code, f"device failure {code}"))
@@ -340,7 +342,8 @@ class PagedCache:
         return _new_workspace(self._L, self.device, self.view.head_dim)
 
     def check(self) -> None:
-        """Waits for the device; raises if a kernel met a failure in the device data since the last check."""
+        """Waits for the device, all of its streams; raises if a kernel met a failure in the device data since the
+        last check."""
         _check_status(self.status)
 
 

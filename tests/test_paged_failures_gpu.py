@@ -108,3 +108,32 @@ def test_a_run_out_wait_is_reported_before_bad_device_data(impatient, kernel):
         out = C.cache.attend(batch, q)
         C.cache.check()
         check_attention(C, q, out, ns)
+
+
+@BOTH
+def test_check_waits_for_every_stream_of_the_device(kernel):
+    """A failure of a call on another stream than check()'s own, still on its way when check() is called."""
+    C, ns, q = ready("bf16", "short")
+    table = C.table.clone()
+    table[0, 0] = 10 ** 6
+    bad = K.PagedBatch(starts(ns), ints(C.kvs), table, **HINTS[kernel])
+    out = torch.zeros_like(q)
+    side = torch.cuda.Stream(dev())
+    with torch.cuda.stream(side):
+        C.cache.attend(K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel]), q, out)   # makes the workspace
+    torch.cuda.synchronize(dev())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)   # some 50 ms
+        C.cache.attend(bad, q, out)
+    other = torch.cuda.Stream(dev())
+    with torch.cuda.stream(other), pytest.raises(K.KoreCudaError, match="page id"):
+        C.cache.check()
+    C.cache.check()
+    table = K.RopeTable(8, 64)
+    pos, x = ints([9] * q.shape[0]), q[..., :64].contiguous()
+    torch.cuda.synchronize(dev())
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+        table.rotate(x, pos, out=x)
+    with torch.cuda.stream(other), pytest.raises(K.KoreCudaError, match="rotation table"):
+        table.check()
