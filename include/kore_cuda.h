@@ -579,7 +579,8 @@ typedef struct kore_cuda_pages {
     int n_head_kv;
     int head_dim;             /* a multiple of 16, at most 256; the attention takes 64 and 128 */
     long long page_stride;    /* elements from one page to the next; 0: dense. A multiple of 16 bytes */
-    const float *k_scale, *v_scale;   /* E4M3: device [n_head_kv], value = 8 bits * scale; NULL: 1 */
+    const float *k_scale, *v_scale;   /* E4M3: device [n_head_kv], value = 8 bits * scale (of any
+                                         sign, or 0); NULL: 1 */
 } kore_cuda_pages;
 
 /* The step's batch. Sequence s has the rows q_start[s] .. q_start[s+1]-1 of q,

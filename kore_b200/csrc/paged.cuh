@@ -97,6 +97,11 @@ __device__ __forceinline__ float f16_shift(float m) {
     return m > 0.f && m < INFINITY ? __int_as_float((127 + min(max(7 - e, -100), 100)) << 23) : 1.f;
 }
 
+// The factor on a unit's products with an 8-bit cache (its sign goes into q, so that the largest
+// product has the largest score): not 0, since -inf of a masked key times 0 is no mask. A
+// product is below 2^40, so that with the least normal value every score is 0 all the same.
+__device__ __forceinline__ float at_least_normal(float factor) { return factor < 0x1p-126f ? 0x1p-126f : factor; }
+
 cudaError_t launch_rope_table(const float *freq, int half, double amp, int n_pos, float *table, cudaStream_t s);
 cudaError_t launch_rotate(const RotateParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
 // n_ctas: SMs of the device, at most kPagedMaxCtas
@@ -204,8 +209,11 @@ __device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q
 }
 
 // A wait ran out: in place of any other code, since it is what makes the workspace unusable.
+// (The store is enough; without raise_error beside it the compiler's choice of registers made
+// the 8-bit chunk kernel 2 to 4 % slower.)
 __device__ __forceinline__ void raise_late(int *status) {
-    if (status) atomicExch(status, DEV_WAIT_FULL_TIMEOUT);
+    raise_error(status, DEV_WAIT_FULL_TIMEOUT);
+    if (status) *reinterpret_cast<volatile int *>(status) = DEV_WAIT_FULL_TIMEOUT;
 }
 
 // A wait that did not end at its first look: until the phase is done, or false when

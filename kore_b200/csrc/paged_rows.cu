@@ -317,9 +317,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                     }
                     if (p.k_scale) {
                         const float ks = __ldg(p.k_scale + u.g);
-                        qs0 *= ks;
-                        qs1 *= ks;
+                        if (ks < 0.f) {
+#pragma unroll
+                            for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) qf[k][i] ^= 0x80008000u;
+                        }
+                        qs0 *= fabsf(ks);
+                        qs1 *= fabsf(ks);
                     }
+                    qs0 = at_least_normal(qs0);
+                    qs1 = at_least_normal(qs1);
                 }
             }
 

@@ -580,7 +580,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         uint8_t *out_rows = smem + C::OUT + warp * 4096;
         uint32_t e = 0, n_p = 0;   // events before this unit, P written so far
         bool ok = true;
-        const uint32_t sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
+        const uint32_t scale_sign = p.scale < 0.f ? 0x80008000u : 0u;   // goes into q, so that maxima stay maxima
         const float qs_all = fabsf(p.scale) * 1.44269504088896340736f;
         // offset of this thread's row of unit a in rows of strides ts, hs (of the unit's
         // first row where it has none): the warp's lanes ask one another for theirs
@@ -594,6 +594,8 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
         // them on their way at once
         auto load_q = [&](const U &a) {
             if (i * kM >= a.rows) return;
+            uint32_t sign = scale_sign;
+            if (E8 && p.k_scale && __ldg(p.k_scale + a.g) < 0.f) sign ^= 0x80008000u;
             constexpr int L = D / 8, N = E8 ? 8 : L;   // lanes a row, loads a lane at a time
             const int c = lane % L;
             const long long off = offset_of(a, p.q_ts, p.q_hs);
@@ -706,7 +708,8 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             }
             float qs = qs_all;
             if constexpr (E8 && QBF) qs *= q_shift[i * kM + r];
-            if (E8 && p.k_scale) qs *= __ldg(p.k_scale + u.g);
+            if (E8 && p.k_scale) qs *= fabsf(__ldg(p.k_scale + u.g));
+            if constexpr (E8) qs = at_least_normal(qs);
             float m = -INFINITY, l = 0.f;
             int k0, k1;
             steps(u, t0, t1, k0, k1);
