@@ -604,7 +604,7 @@ typedef struct kore_cuda_batch {
  * q (optional; any number of heads) is rotated into q_out, which may be q's own
  * rows. k, v, q and q_out have one type; the cache has it too, or fewer bits
  * (F32 to F16 or BF16; any to E4M3: x / scale rounded to nearest even, values
- * beyond +-448 to +-448). Positions must be distinct: no two sequences may
+ * beyond +-448 to +-448; 0 where the scale is 0). Positions must be distinct: no two sequences may
  * write the same slot of a page. */
 int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
                                const kore_cuda_rows *k, const kore_cuda_rows *v, const kore_cuda_rows *q,

@@ -208,7 +208,15 @@ __global__ void __launch_bounds__(256) rotate_kernel(const __grid_constant__ Rot
             }
         } else {
             const float *scales = is_k ? p.k_scale : p.v_scale;
-            const float sc = sizeof(C) == 1 && scales ? __ldg(scales + hh) : 1.f;
+            float sc = sizeof(C) == 1 && scales ? __ldg(scales + hh) : 1.f;
+            if (sizeof(C) == 1 && sc == 0.f) {   // all that the head can hold is 0, and 0 / 0 would not be
+                sc = 1.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) {
+                    a.v[i] *= 0.f;
+                    b.v[i] *= 0.f;
+                }
+            }
             C *dst = static_cast<C *>(is_k ? p.kc : p.vc) + pl.page * p.page_stride +
                      ((long long)hh * p.P + pl.slot) * p.d;
             if constexpr (VEC) {

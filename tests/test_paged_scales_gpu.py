@@ -47,3 +47,27 @@ def test_a_factor_too_small_for_32_bits_is_as_good_as_zero(kernel, tq):
     C.cache.attend(K.PagedBatch(starts(ns), ints(kvs), C.table, **HINTS[kernel]), q, out, scale=2.0 ** -60)
     C.cache.check()
     check_attention(C, q, out, ns, scale=2.0 ** -60)
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 48])   # by vectors, and (with rows off their alignment below) one at a time
+def test_append_into_a_head_whose_scale_is_zero(t, d):
+    """All that such a head can hold is 0: what is stored must not be 0 / 0."""
+    g = gen(33)
+    C = Cache(g, "e4m3", 3, d, 16, [20], junk=7.0)
+    C.ks[0] = C.vs[1] = 0
+    x = rand(g, 20, 3, d).to({"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[t])
+    x[:, 0, ::2] = 0
+    x[:, 1, 1::2] = 0
+    rows = torch.zeros(20, 3, d + 3, dtype=x.dtype, device=dev())[:, :, 1:d + 1] if d == 48 else torch.empty_like(x)
+    rows.copy_(x)
+    C.cache.append(K.PagedBatch(ints([0, 20]), ints([20]), C.table, 20), rows, rows)
+    C.cache.check()
+    k, v = C.rows(0)
+    assert (k[:, 0] == 0).all() and (v[:, 1] == 0).all()
+    for got, scale, heads in ((k, C.ks, (1, 2)), (v, C.vs, (0, 2))):
+        for h in heads:
+            sc = scale[h].item()
+            want = x[:, h].double()
+            tol = u("e4m3") * want.abs() * (1 + 2 ** -20) + 2.0 ** -10 * sc * (1 + 2 ** -20)
+            assert ((got[:, h] - want).abs() <= tol).all()
