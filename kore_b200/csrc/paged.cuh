@@ -91,10 +91,11 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t &a, uint32_t &b) {
 }
 
 // The power of two that takes a row's largest value m to 2^7 .. 2^8: bf16 values down
-// to 2^-22 of it are then exact in f16. 1 for 0, infinities and NaN.
+// to 2^-22 of it are then exact in f16. 1 for 0, infinities and NaN; at most 2^100 (a row
+// whose largest is below 2^-93 stands lower by as much).
 __device__ __forceinline__ float f16_shift(float m) {
     const int e = (__float_as_int(m) >> 23) - 127;
-    return m > 0.f && m < INFINITY ? __int_as_float((127 + min(max(7 - e, -100), 100)) << 23) : 1.f;
+    return m > 0.f && m < INFINITY ? __int_as_float((127 + min(7 - e, 100)) << 23) : 1.f;   // (7 - e >= -120)
 }
 
 // The factor on a unit's products with an 8-bit cache (its sign goes into q, so that the largest

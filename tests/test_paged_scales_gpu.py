@@ -71,3 +71,24 @@ def test_append_into_a_head_whose_scale_is_zero(t, d):
             want = x[:, h].double()
             tol = u("e4m3") * want.abs() * (1 + 2 ** -20) + 2.0 ** -10 * sc * (1 + 2 ** -20)
             assert ((got[:, h] - want).abs() <= tol).all()
+
+
+@BOTH
+@pytest.mark.parametrize("top", [60, 112, 120])
+def test_rows_of_large_bf16_queries_over_8_bits(kernel, top):
+    """Scores of ordinary size from queries of 2^top and keys of 2^-top."""
+    g = gen(34)
+    ns, kvs = [1, 60], [200, 300]
+    C = Cache(g, "e4m3", 2, 128, 32, kvs)
+    C.fill(g, 0), C.fill(g, 1)
+    C.ks *= 2.0 ** -top
+    n = sum(ns)
+    q = rand(g, n, 14, 128)
+    q[::3] *= 0.25
+    q[1::7, :, 5] = 100.0   # one large value: 2^6.6 times the others
+    q = (q * 2.0 ** top).to(torch.bfloat16)
+    assert torch.isfinite(q).all()
+    out = torch.zeros_like(q)
+    C.cache.attend(K.PagedBatch(starts(ns), ints(kvs), C.table, **HINTS[kernel]), q, out)
+    C.cache.check()
+    check_attention(C, q, out, ns)
