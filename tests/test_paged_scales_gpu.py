@@ -92,3 +92,64 @@ def test_rows_of_large_bf16_queries_over_8_bits(kernel, top):
     C.cache.attend(K.PagedBatch(starts(ns), ints(kvs), C.table, **HINTS[kernel]), q, out)
     C.cache.check()
     check_attention(C, q, out, ns)
+
+
+@BOTH
+@pytest.mark.parametrize("tc", ["bf16", "e4m3"])
+def test_huge_queries_take_one_keys_value(kernel, tc):
+    """Scores of 2^60 and more, whose softmax is a 1 at the largest: the output is that key's value, rounded once. (Rows
+    whose two largest scores are closer than four times what a score may be off are left out: 2 d u32 sum|q k| each.)"""
+    g = gen(35)
+    n, kv, d = 40, 300, 128
+    C = Cache(g, tc, 1, d, 32, [kv])
+    C.fill(g, 0)
+    q = (rand(g, n, 7, d) * 2.0 ** 60).to(torch.bfloat16)
+    out = torch.zeros_like(q)
+    C.cache.attend(K.PagedBatch(starts([n]), ints([kv]), C.table, **HINTS[kernel]), q, out)
+    k, v = C.rows(0)
+    s = torch.einsum("nhd,td->nht", q.double(), k[:, 0]) * d ** -0.5
+    off = torch.einsum("nhd,td->nht", q.double().abs(), k[:, 0].abs()).amax(-1) * d ** -0.5 * 2 * d * 2.0 ** -24
+    pos = kv - n + torch.arange(n, device=dev())
+    s.masked_fill_(torch.arange(kv, device=dev()) > pos[:, None, None], -math.inf)
+    two, at = s.topk(2, -1)
+    clear = two[..., 0] - two[..., 1] > 4 * off
+    assert clear.double().mean() > 0.9
+    want = v[at[..., 0], 0]
+    # the value's scale, the sum's reciprocal and the product: three roundings of 32 bits, then the output's
+    tol = want.abs() * (u("bf16") + 4 * 2.0 ** -24) * (1 + 2.0 ** -7) + 2.0 ** -134
+    assert ((out.double() - want).abs() <= tol)[clear].all()
+
+
+@BOTH
+@pytest.mark.parametrize("tq,tc", KINDS)
+@pytest.mark.parametrize("window", [0, 1000])
+def test_nan_in_a_value_stays_with_the_rows_of_its_block(kernel, tq, tc, window):
+    """NaN in V reaches every row that sees it and no row whose block (256 packed rows at most) sees none: those have the
+    bits that they have without it. A window's lost positions and a chunk's later ones are such."""
+    g = gen(36)
+    n, kv, rep, d = 500, 3000, 8, 128
+    C = Cache(g, tc, 2, d, 64, [kv])
+    C.fill(g, 0)
+    q = rand(g, n, 2 * rep, d).to(getattr(torch, {"f16": "float16", "bf16": "bfloat16"}[tq]))
+    batch = K.PagedBatch(starts([n]), ints([kv]), C.table, **HINTS[kernel])
+    clean = C.cache.attend(batch, q, window=window)
+    check_attention(C, q, clean, [n], window=window)
+    spots = [(1600, 0, 3), (2504, 1, 100), (2999, 0, 64), (10, 1, 7)]   # (position, head, d)
+    for t, h, e in spots:
+        pg, sl = C.places(0, torch.tensor([t], device=dev()))
+        C.vp[pg, h, sl, e] = float("nan")
+    got = C.cache.attend(batch, q, window=window)
+    C.cache.check()
+    pos = kv - n + torch.arange(n, device=dev())
+    sees = torch.zeros(n, 2, rep, d, dtype=torch.bool, device=dev())
+    block = sees.clone()
+    tokens = 256 // rep
+    for t, h, e in spots:
+        s = (t <= pos) & ((t > pos - window) if window else torch.ones_like(pos, dtype=torch.bool))
+        sees[s, h, :, e] = True
+        near = torch.nn.functional.pad(s, (0, -n % tokens)).view(-1, tokens).any(1).repeat_interleave(tokens)[:n]
+        block[near, h, :, e] = True
+    sees, block = sees.flatten(1, 2), block.flatten(1, 2)
+    assert got[sees].isnan().all()
+    assert torch.equal(got[~block], clean[~block])
+    assert sees.any() and (~block).any()
