@@ -106,6 +106,16 @@ def _import_torch():
     return _torch
 
 
+_INT_MAX = 2 ** 31 - 1
+
+
+def _int(x, what: str) -> int:
+    """x as a C int (ctypes would cut it to 32 bits)."""
+    if not -_INT_MAX <= x <= _INT_MAX:
+        raise ValueError(f"{what} = {x} does not fit 32 bits")
+    return x
+
+
 _pack_rows = struct.Struct("@Piiiqq").pack_into   # _Rows, in one step
 
 
@@ -115,6 +125,8 @@ def _fill(r: _Rows, t, what: str, device) -> int:
     if len(shape) != 3:
         raise ValueError(f"{what}: expected [tokens][heads][head_dim], got {tuple(shape)}")
     n, h, d = shape
+    if n > _INT_MAX:
+        raise ValueError(f"{what}: {n} tokens are too many for one call")
     ts, hs, es = t.stride()
     if es != 1 and d > 1:
         raise ValueError(f"{what}: the values of a head must be contiguous")
@@ -148,7 +160,7 @@ def _check_status(status) -> None:
 def _spec(n_rot, base, scaling, factor, original_ctx, beta_fast, beta_slow, amplitude) -> _RopeSpec:
     if scaling not in SCALINGS:
         raise ValueError(f"scaling {scaling!r} is none of {sorted(SCALINGS)}")
-    return _RopeSpec(n_rot, SCALINGS[scaling], base, factor, original_ctx, beta_fast, beta_slow, amplitude)
+    return _RopeSpec(_int(n_rot, "n_rot"), SCALINGS[scaling], base, factor, original_ctx, beta_fast, beta_slow, amplitude)
 
 
 def rope_frequencies(n_rot: int, *, base: float = 1e6, scaling: str = "none", factor: float = 1.0,
@@ -183,7 +195,7 @@ class RopeTable:
         torch = _import_torch()
         self._L = _library()
         spec = _spec(n_rot, base, scaling, factor, original_ctx, beta_fast, beta_slow, amplitude)
-        if n_pos <= 0:
+        if _int(n_pos, "n_pos") <= 0:
             raise ValueError(f"n_pos = {n_pos} must be positive")
         rope_frequencies(n_rot, base=base, scaling=scaling, factor=factor, original_ctx=original_ctx,
                          beta_fast=beta_fast, beta_slow=beta_slow, amplitude=amplitude)   # refuses before it allocates
@@ -235,7 +247,8 @@ class PagedBatch:
         self.device = dev = kv_len.device
         n = kv_len.shape[0]
         view = _Batch(n, _ints(q_start, "q_start", dev, 1), _ints(kv_len, "kv_len", dev, 1),
-                      _ints(page_table, "page_table", dev, 2), page_table.shape[1], max_q, max_kv)
+                      _ints(page_table, "page_table", dev, 2), _int(page_table.shape[1], "page_table's width"),
+                      _int(max_q, "max_q"), _int(max_kv, "max_kv"))
         if q_start.shape[0] != n + 1 or page_table.shape[0] != n:
             raise ValueError(f"q_start must have {n + 1} and page_table {n} rows")
         self.q_start, self.kv_len, self.page_table, self.view = q_start, kv_len, page_table, view
@@ -322,6 +335,10 @@ class PagedCache:
             plse = lse.data_ptr()
         if batch.device != dev:
             raise ValueError(f"the batch is not on {dev}")
+        o = self._opts
+        o.scale, o.causal, o.window = scale, causal, window
+        if o.window != window or (scale and not o.scale):   # (cut to 32 bits, or to 0: the default)
+            raise ValueError(f"window = {window} or scale = {scale} is outside the range of 32 bits")
         if workspace is not None and (workspace.dtype != _torch.uint8 or workspace.device != dev
                                       or not workspace.is_contiguous()):
             raise ValueError(f"workspace: expected a contiguous uint8 tensor on {dev}, as new_workspace() makes it")
@@ -329,8 +346,6 @@ class PagedCache:
             return out
         s = _stream(dev)
         ws = workspace if workspace is not None else _workspace(self._L, dev, s, self.view.head_dim)
-        o = self._opts
-        o.scale, o.causal, o.window = scale, causal, window
         rc = self._L.kore_cuda_paged_attn_dev(self._view, batch._view, n, self._p[0], self._p[1], plse, self._popts,
                                               ws.data_ptr(), ws.numel(), self._status, s)
         if rc:

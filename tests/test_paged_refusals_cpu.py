@@ -47,3 +47,33 @@ def test_workspaces_that_the_kernels_cannot_use_are_refused(fake, workspace):
     ws = cuda(1 << 27, **{"dtype": torch.uint8, **workspace})[::skip]
     with pytest.raises(ValueError, match="workspace"):
         cache.attend(batch, q, cuda(1, 4, 64), workspace=ws)
+
+
+@pytest.mark.parametrize("kw", [dict(window=2 ** 32), dict(window=2 ** 32 + 5), dict(window=2 ** 31), dict(scale=1e-50),
+                                dict(scale=-1e-46)])
+def test_options_outside_32_bits_are_refused(fake, kw):
+    """Cut to 32 bits they would be other options: a window of 5, or none, or the default scale."""
+    cache, batch, q = step()
+    with pytest.raises(ValueError, match="32 bits"):
+        cache.attend(batch, q, cuda(1, 4, 64), **kw)
+
+
+@pytest.mark.parametrize("kw", [dict(max_q=2 ** 32 + 1), dict(max_q=1, max_kv=2 ** 31), dict(max_q=-2 ** 32)])
+def test_hints_outside_32_bits_are_refused(fake, kw):
+    with pytest.raises(ValueError, match="32 bits"):
+        K.PagedBatch(cuda(2, dtype=torch.int32), cuda(1, dtype=torch.int32), cuda(1, 4, dtype=torch.int32), **kw)
+
+
+def test_tables_outside_32_bits_are_refused(fake):
+    for n_pos, n_rot in ((2 ** 32 + 4, 8), (2 ** 31, 8), (16, 2 ** 32 + 8)):
+        with pytest.raises(ValueError, match="32 bits"):
+            K.RopeTable(n_pos, n_rot, device="cuda:0")
+    with pytest.raises(ValueError, match="32 bits"):
+        K.rope_frequencies(2 ** 32 + 8)
+
+
+def test_more_tokens_than_a_call_can_count_are_refused(fake):
+    cache, batch, _ = step()
+    rows = cuda(1, 2, 64).expand(2 ** 32 + 1, 2, 64)
+    with pytest.raises(ValueError, match="too many"):
+        cache.append(batch, rows, rows)
