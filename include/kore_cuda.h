@@ -514,8 +514,8 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
 
 /* Rows of heads: element e of head h of row t is at data + (t * token_stride +
  * h * head_stride + e) elements. A row may be a part of a wider one (q, k and v
- * of one product). Strides and addresses of any size are allowed; 16-byte
- * aligned ones are faster. */
+ * of one product). Strides and addresses of any size are allowed (for rows
+ * that are written, none of 0); 16-byte aligned ones are faster. */
 typedef struct kore_cuda_rows {
     void *data;
     int type;                 /* KORE_CUDA_F32, KORE_CUDA_F16 or KORE_CUDA_BF16 */

@@ -85,6 +85,13 @@ int check_rows(const kore_cuda_rows *r, const char *name, int head_dim) {
     return KORE_CUDA_OK;
 }
 
+// Rows that are written: several in one place would leave whichever came last.
+int check_written(const kore_cuda_rows *r, const char *name, int n_tok) {
+    if ((n_tok > 1 && r->token_stride == 0) || (r->n_head > 1 && r->head_stride == 0))
+        return refuse(KORE_CUDA_EINVAL, "%s: the rows overlap (a stride of 0)", name);
+    return KORE_CUDA_OK;
+}
+
 int check_rope(const kore_cuda_rope_view *r, int head_dim) {
     if (!r->table) return refuse(KORE_CUDA_EINVAL, "the rotation table is null");
     if (reinterpret_cast<uintptr_t>(r->table) & 15)
@@ -251,6 +258,7 @@ extern "C" int kore_cuda_rope_dev(const kore_cuda_rows *x, const kore_cuda_rows 
     if (out->type != x->type || out->n_head != x->n_head)
         return refuse(KORE_CUDA_EINVAL, "out has another type or number of heads than x");
     if (n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", n_tok);
+    if (int rc = check_written(out, "out", n_tok)) return rc;
     if (n_tok == 0) return KORE_CUDA_OK;
     OnDeviceOf on(x->data);
     if (on.rc) return on.rc;
@@ -287,6 +295,7 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
         if (int rc = check_rows(q_out, "q_out", d)) return rc;
         if (q->type != k->type || q_out->type != k->type || q_out->n_head != q->n_head)
             return refuse(KORE_CUDA_EINVAL, "q and q_out must have k's type and the same heads");
+        if (int rc = check_written(q_out, "q_out", n_tok)) return rc;
     }
     if (rope)
         if (int rc = check_rope(rope, d)) return rc;
@@ -351,6 +360,7 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     if (int rc = check_rows(out, "out", d)) return rc;
     if (q->type == KORE_CUDA_F32 || out->type != q->type || out->n_head != q->n_head)
         return refuse(KORE_CUDA_EINVAL, "q and out must be F16 or BF16, of one type and number of heads");
+    if (int rc = check_written(out, "out", n_tok)) return rc;
     if (out->data == q->data) return refuse(KORE_CUDA_EINVAL, "out must not be q's own rows");
     if (cache->type != q->type && cache->type != KORE_CUDA_E4M3)
         return refuse(KORE_CUDA_EINVAL, "a cache of type %d does not go with queries of type %d", cache->type, q->type);

@@ -1,12 +1,16 @@
 """Calls of the operators on a caller-owned paged cache that are refused before anything reaches a GPU, on tensors
 that have a device, shape and strides and no memory (torch's fake tensors). CPU only."""
+import ctypes
+
 import pytest
 
 import kore_b200 as K
+from kore_b200 import paged as P
 
 torch = pytest.importorskip("torch")
 from torch._subclasses.fake_tensor import FakeTensorMode  # noqa: E402
 
+A, B = 0x10000, 0x20000   # placeholders for aligned device addresses
 pytestmark = pytest.mark.filterwarnings("ignore:Accessing the data pointer")
 
 
@@ -77,3 +81,40 @@ def test_more_tokens_than_a_call_can_count_are_refused(fake):
     rows = cuda(1, 2, 64).expand(2 ** 32 + 1, 2, 64)
     with pytest.raises(ValueError, match="too many"):
         cache.append(batch, rows, rows)
+
+
+def test_written_rows_that_overlap_are_refused(fake):
+    """An expanded tensor may be read, not written: which of its rows stays would be chance."""
+    cache, batch, q = step(3)
+    k = cuda(3, 2, 64)
+    for out in (cuda(1, 4, 64).expand(3, 4, 64), cuda(3, 1, 64).expand(3, 4, 64)):
+        for call in (lambda: P._library().kore_cuda_paged_attn_dev(*attention(cache, batch, q, out)),
+                     lambda: P._library().kore_cuda_rope_dev(*rotation(q, out)),
+                     lambda: P._library().kore_cuda_paged_append_dev(*appended(cache, batch, k, q, out))):
+            assert call() == -1
+            assert "overlap" in P._library().kore_cuda_last_error(None).decode()
+
+
+def rows(t, address):
+    h, d = t.shape[1:]
+    return ctypes.byref(P._Rows(address, P.BF16, h, d, *t.stride()[:2]))
+
+
+def view(struct, **places):
+    """A copy of a structure with addresses in place of the fake tensors'."""
+    new = type(struct)(*[places.get(name, getattr(struct, name)) for name, _ in struct._fields_])
+    return ctypes.byref(new)
+
+
+def attention(cache, batch, q, out):
+    return (view(cache.view, k=A, v=A), view(batch.view, q_start=A, kv_len=A, page_table=A), q.shape[0], rows(q, A),
+            rows(out, B), None, ctypes.byref(P._Opts(0.0, 1, 0)), A, 1 << 40, None, None)
+
+
+def rotation(q, out):
+    return rows(q, A), rows(out, B), q.shape[0], A, ctypes.byref(P._RopeView(A, 8, 8, 0)), None, None
+
+
+def appended(cache, batch, k, q, out):
+    return (view(cache.view, k=A, v=A), view(batch.view, q_start=A, kv_len=A, page_table=A), q.shape[0], rows(k, A),
+            rows(k, A), rows(q, A), rows(out, B), None, None, None)
