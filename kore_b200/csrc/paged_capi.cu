@@ -419,8 +419,10 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.status = dev_status;
     p.wait_ns = g_wait_ns;
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
-    // units are of 16 rows and tiles of 128 keys at least
-    p.small = ((double)n_tok * p.rep / 16 + p.n_seq) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;
+    // units are of 16 rows and tiles of 128 keys at least; every sequence may have all rows (a
+    // q_start that goes back is reported, and those that fit on their own are still worked on:
+    // 16 of 31 sequences with all rows each would bring 16 times what the rows alone allow)
+    p.small = p.n_seq * ((double)n_tok * p.rep / 16 + 1) * ((double)p.table_stride * p.P / 128 + 3) < 1e9;
     // The row kernel passes over the keys once for every 16 packed rows, the tile kernel
     // once for every 256 at 2.8 times the cost and some 20 us more for its start, its
     // outputs and the joining of cut units. So the row kernel has what fits one of its

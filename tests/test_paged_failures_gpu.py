@@ -137,3 +137,20 @@ def test_check_waits_for_every_stream_of_the_device(kernel):
         table.rotate(x, pos, out=x)
     with torch.cuda.stream(other), pytest.raises(K.KoreCudaError, match="rotation table"):
         table.check()
+
+
+@BOTH
+@pytest.mark.parametrize("n", [3, 300])
+def test_starts_that_go_back_are_reported_and_the_sequences_that_fit_are_right(kernel, n):
+    """31 sequences over the same rows: the 16 whose bounds fit are worked on (here all with one cache, so that it does
+    not matter which of them writes last), the others are left out."""
+    g = gen(41)
+    C = Cache(g, "bf16", 2, 64, 32, [400])
+    C.fill(g, 0)
+    q = rand(g, n, 14, 64).to(torch.bfloat16)
+    table = C.table.expand(31, -1).contiguous()
+    batch = K.PagedBatch(ints([0, n] * 16), ints([400] * 31), table, **HINTS[kernel])
+    out = C.cache.attend(batch, q)
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        C.cache.check()
+    check_attention(C, q, out, [n])
