@@ -154,3 +154,31 @@ def test_starts_that_go_back_are_reported_and_the_sequences_that_fit_are_right(k
     with pytest.raises(K.KoreCudaError, match="bounds"):
         C.cache.check()
     check_attention(C, q, out, [n])
+
+
+@BOTH
+def test_workspaces_of_captures_that_are_over_are_given_back(kernel):
+    """They are the graphs' memory: no more than the last one is held here, and the graphs go on replaying."""
+    C, ns, q = ready("bf16", "long")
+    batch = K.PagedBatch(starts(ns), ints(C.kvs), C.table, **HINTS[kernel])
+    stream = torch.cuda.Stream(dev())
+    outs, graphs = [torch.zeros_like(q) for _ in range(4)], []
+    torch.cuda.synchronize(dev())
+    with torch.cuda.stream(stream):
+        C.cache.attend(batch, q, outs[0])
+        for out in outs:
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=stream):
+                C.cache.attend(batch, q, out)
+                C.cache.attend(batch, q, out)
+    here = [k for k in K.paged._workspaces if k[1] == stream.cuda_stream]
+    assert sum(k[2] != 0 for k in here) == 1 and sum(k[2] == 0 for k in here) == 1
+    side = [torch.cuda.Stream(dev()) for _ in graphs]
+    torch.cuda.synchronize(dev())
+    for _ in range(3):
+        for graph, s in zip(graphs, side):
+            with torch.cuda.stream(s):
+                graph.replay()
+    C.cache.check()
+    for out in outs:
+        check_attention(C, q, out, ns)
