@@ -42,7 +42,6 @@ struct HeadRows {
     void *out;
     long long in_ts, in_hs, out_ts, out_hs;
     int heads;
-    int rotate;
 };
 
 struct RotateParams {
@@ -88,6 +87,35 @@ __device__ __forceinline__ void widen4(uint32_t x, uint32_t &a, uint32_t &b) {
     asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
         : "=r"(a), "=r"(b)
         : "r"(x));
+}
+
+// two values as a pair of bf16 or of f16
+template <bool BF>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (BF) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    } else {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t *>(&v);
+    }
+}
+
+// A box of a page (tokens from tok on, values from x on) into shared memory; with an L2 policy or
+// without.
+__device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(tok), "r"(g), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar,
+                                        uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
+        "l"(map), "r"(x), "r"(tok), "r"(g), "r"(page), "r"(smem_u32(bar)), "l"(policy)
+        : "memory");
 }
 
 // The power of two that takes a row's largest value m to 2^7 .. 2^8: bf16 values down

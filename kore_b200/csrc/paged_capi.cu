@@ -427,9 +427,15 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     // once for every 256 at 2.8 times the cost and some 20 us more for its start, its
     // outputs and the joining of cut units. So the row kernel has what fits one of its
     // units, and chunks up to so many passes over 128 keys in the whole batch (kv counted
-    // by max_kv, a unit's own time as three passes). Measured, row against tile kernel,
-    // 28/4 heads of 128: 16-bit cache, 4488 passes 41 / 49 us, 6160 34 / 38, 6300 45 / 29,
-    // 9380 47 / 40, 10080 52 / 39; 8 bits 10080 53 / 53, 13376 74 / 86.
+    // by max_kv, a unit's own time as three passes). Passes are a rough measure: chunks of few
+    // tokens on long contexts favour the rows, many short ones the tiles. Measured, row
+    // against tile kernel, us, 28/4 heads of 128, 16 bits: 1179 passes (8 tokens on 8000)
+    // 23 / 34; 2465 (128 on 1000) 30 / 26; 3930 (32 on 8000) 39 / 47; 4554 (8 on 32000) 43 /
+    // 46; 4768 (8 x 16 on 2000) 43 / 32; 9864 (16 x 8 on 4000) 78 / 50. 8 bits: 2465 34 / 31;
+    // 3930 38 / 54; 4554 40 / 52; 4768 44 / 39; 9864 67 / 59; 13376 74 / 86. 14/2 heads of 64, 16
+    // bits: 2277 (8 on 32000) 23 / 31; 2595 (8 x 32 on 1000) 23 / 20; 4932 30 / 28. Either
+    // kernel is up to 1.6 times the other on the wrong side of the border. A window is not
+    // counted: 32 tokens that look back 512 of 30000 positions take the tiles' 19 where the rows take 11.
     const double rows16 = (double)p.G * ((double)n_tok * p.rep / 16 + p.n_seq);
     const double passes = (batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P) / 128 + 3;
     const bool tiles = (long long)batch->max_q * p.rep > 16 &&

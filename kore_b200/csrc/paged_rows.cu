@@ -9,7 +9,8 @@
 // be used) and everything serves the stream of keys:
 //   * one CTA of 8 warps an SM; each warp streams tiles of its own, a fixed
 //     8 KB (4 KB for 8 bits and d = 64) of K and V, through a ring of 3 (6)
-//     stages that TMA boxes fill straight from the pages (192 KB in flight an SM;
+//     stages that TMA boxes fill straight from the pages (one stage is read while the
+//     others land: 128 KB in flight an SM, 160 KB for 8 bits and d = 64;
 //     16-byte cp.async by the lanes took as many instructions as the products). No
 //     warp waits for another, and the ring runs on over the ends of units.
 //   * work in equal shares (paged.cuh): ragged lengths, one long sequence and
@@ -25,7 +26,7 @@
 //     product's sum is free, so a thread takes 4 consecutive bytes where the
 //     fragment wants (2t, 2t+1, 2t+8, 2t+9), and q the same. bf16 queries over it
 //     are scaled by a power of two a row so that they are exact in f16 down
-//     to 2^-22 of the row's largest value.
+//     to 2^-22 of the row's largest value (smaller ones lose digits: what f16 operands cost).
 // Measured: 64 sequences of up to 8192 positions, 16/2 heads of 128, bf16: 55.4 us, 5.47
 // TB/s (83 % of the measured copy rate); 12 of up to 32768, 28/4 heads, 8 bits: 48.7 us, 4.83
 // TB/s (issue: 36 % of the slots with two warps a scheduler, half of them widening);
@@ -75,15 +76,6 @@ __device__ __forceinline__ int piece(int r, int c) {
     else return (c >> 3) * (KT * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-__device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar,
-                                        uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
-        "[%0], [%1, {%2, %3, %4, %5}], [%6], %7;" ::"r"(dst),
-        "l"(map), "r"(x), "r"(tok), "r"(g), "r"(page), "r"(smem_u32(bar)), "l"(policy)
-        : "memory");
-}
-
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -109,17 +101,6 @@ __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint3
                      "{%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (BF) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __half2 v = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
 }
 
 __device__ __forceinline__ uint64_t l2_evict_normal_policy() {

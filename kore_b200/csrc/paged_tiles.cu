@@ -157,13 +157,6 @@ __device__ __forceinline__ void st16(uint32_t a, const uint32_t *r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
-__device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(map), "r"(x), "r"(tok), "r"(g), "r"(page), "r"(smem_u32(bar))
-        : "memory");
-}
-
 // two fp32 at once
 __device__ __forceinline__ unsigned long long pk2(float a, float b) {
     unsigned long long u;
@@ -201,17 +194,6 @@ __device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p) {
 __device__ __forceinline__ void st_release(uint32_t *p, uint32_t v) {
     asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
 }
-template <bool BF>
-__device__ __forceinline__ uint32_t pack2(float a, float b) {
-    if constexpr (BF) {
-        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    } else {
-        const __half2 v = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t *>(&v);
-    }
-}
-
 // ---------------------------------------------------------------- parts of a cut unit
 //
 // CTA c has two slots: slot 0 for the unit it goes on with, slot 1 for the one
