@@ -634,9 +634,11 @@ long long kore_cuda_paged_attn_workspace(int head_dim);
  * hold finite values for the chunk's other rows to be right.
  * q, out: [n_tok] rows of n_head heads, F16 or BF16, the cache of the same type
  * or E4M3; out may not overlap q; lse (optional) [n_tok][n_head]: natural log of the softmax's sum.
- * Products are exact and summed in 32 bits, the softmax in 32 bits; the
- * probabilities are rounded to the type of the cache for the second product
- * (to F16 for E4M3). The result is a function of the inputs and the batch alone
+ * Products are exact and summed in 32 bits (BF16 queries over an E4M3 cache are
+ * brought to F16 a row at a time: values below 2^-21 of the row's largest lose
+ * digits), the softmax in 32 bits; the probabilities are rounded to the type of
+ * the cache for the second product (to F16 for E4M3), their sum is of the
+ * unrounded ones. The result is a function of the inputs and the batch alone
  * (no atomics on values): the same call gives the same bits. */
 int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
                              const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,

@@ -27,9 +27,9 @@
 //     fragment wants (2t, 2t+1, 2t+8, 2t+9), and q the same. bf16 queries over it
 //     are scaled by a power of two a row so that they are exact in f16 down
 //     to 2^-22 of the row's largest value (smaller ones lose digits: what f16 operands cost).
-// Measured: 64 sequences of up to 8192 positions, 16/2 heads of 128, bf16: 55.4 us, 5.47
-// TB/s (83 % of the measured copy rate); 12 of up to 32768, 28/4 heads, 8 bits: 48.7 us, 4.83
-// TB/s (issue: 36 % of the slots with two warps a scheduler, half of them widening);
+// Measured: 64 sequences of up to 8192 positions, 16/2 heads of 128, bf16: 55.5 us, 5.46
+// TB/s (83 % of the measured copy rate); 12 of up to 32768, 28/4 heads, 8 bits: 49.3 us, 4.77
+// TB/s (latency: two warps a scheduler use 36 % of the issue slots, half of them widening);
 // one of 513, 28/4 heads: 9.0 us, of which a call on one position takes 5.1. The streaming
 // itself runs at HBM's rate; 3.5 us before it (lengths, page table, first copies) and 2
 // to 4 us behind it (joining warps and CTAs) are the rest.

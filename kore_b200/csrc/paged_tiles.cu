@@ -23,7 +23,7 @@
 //                   unit's keys in its boundary tiles: 0 * NaN must not reach an output.
 //   warps 12-15     (8-bit caches, in warp 11's place) widen the tiles to f16 (exact) from a
 //                   ring of their own into the one that the MMAs read.
-// Measured (2048 tokens at the end of 32768, 28/4 heads of 128, bf16): 887 us, 1050 TFLOP/s, 62 % of
+// Measured (2048 tokens at the end of 32768, 28/4 heads of 128, bf16): 872 to 902 us, 1030 to 1070 TFLOP/s, 61 to 63 % of
 // the measured bf16 peak; a step takes 1.15 us, of which the MMAs themselves are 0.72 (S: 16
 // of N = 64, 29 ns each, both operands from shared memory; P V: 8 of N = 128, 31 ns), their
 // commits (29 ns each) and the changes of accumulator 0.35. Taken out again: one S buffer of

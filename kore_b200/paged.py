@@ -213,7 +213,8 @@ class RopeTable:
 
     def rotate(self, x, pos, out=None):
         """Rotates x [tokens][heads][head_dim] (fp32, fp16 or bf16) at the int32 positions pos [tokens] into out
-        (a new tensor if None; x itself to rotate in place). A row with a negative position is left as it is in out."""
+        (a new tensor if None; x itself to rotate in place). A row with a negative position is left as it is in out (in
+        a new tensor: whatever the memory holds)."""
         if out is None:
             out = _torch.empty_like(x)
         n = _fill(self._x, x, "x", self.device)
@@ -316,7 +317,8 @@ class PagedCache:
     def attend(self, batch: PagedBatch, q, out=None, *, scale: float = 0.0, causal: bool = True, window: int = 0,
                lse=None, workspace=None):
         """Attention of q [tokens][n_head][head_dim] (fp16 or bf16) over the batch's cached positions, into out (a new
-        tensor if None; never q's own memory). Rows outside every sequence keep what out holds.
+        tensor if None; never q's own memory). Rows outside every sequence keep what out holds (a new tensor: whatever
+        the memory holds).
 
         scale 0: 1/sqrt(head_dim). window: how many positions back a token sees, itself among them (0: all). lse: an
         optional float32 [tokens][n_head] for the log of the softmax's sums. workspace: a tensor of new_workspace();
