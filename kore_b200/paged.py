@@ -388,10 +388,12 @@ def _workspace(L, device, stream: int, head_dim: int):
         # the larger of the two head sizes serves both. In a capture it is the
         # graph's own memory and its zeroing a node of the graph: the graph keeps it, so
         # that those of earlier captures on the stream, which are over, need no place here
-        for old in [k for k in _workspaces if k[:2] == key[:2] and k[2] not in (0, key[2])]:
-            del _workspaces[old]
+        # (other threads may change the table meanwhile: list() of it is one step)
+        for old in list(_workspaces):
+            if old[:2] == key[:2] and old[2] not in (0, key[2]):
+                _workspaces.pop(old, None)
         ws = _new_workspace(L, device, 128)
-        while len(_workspaces) >= _WORKSPACES_KEPT:
-            _workspaces.pop(next(iter(_workspaces)))
+        for old in list(_workspaces)[:1 - _WORKSPACES_KEPT]:   # the oldest beyond so many
+            _workspaces.pop(old, None)
         _workspaces[key] = ws
     return ws

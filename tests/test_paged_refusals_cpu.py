@@ -1,6 +1,9 @@
 """Calls of the operators on a caller-owned paged cache that are refused before anything reaches a GPU, on tensors
 that have a device, shape and strides and no memory (torch's fake tensors). CPU only."""
 import ctypes
+import random
+import sys
+import threading
 
 import pytest
 
@@ -118,3 +121,31 @@ def rotation(q, out):
 def appended(cache, batch, k, q, out):
     return (view(cache.view, k=A, v=A), view(batch.view, q_start=A, kv_len=A, page_table=A), q.shape[0], rows(k, A),
             rows(k, A), rows(q, A), rows(out, B), None, None, None)
+
+
+def test_default_workspaces_of_several_threads(monkeypatch):
+    """Threads with objects and streams of their own share the table of default workspaces."""
+    from types import SimpleNamespace as N
+    monkeypatch.setattr(P, "_workspaces", {})
+    monkeypatch.setattr(P, "_new_workspace", lambda L, device, d: object())
+    monkeypatch.setattr(P, "_torch", N(_C=N(_cuda_getDevice=lambda: 0, _cuda_isCurrentStreamCapturing=lambda: True)))
+    before = sys.getswitchinterval()
+    sys.setswitchinterval(1e-6)
+    failed = []
+
+    def work(seed):
+        r = random.Random(seed)
+        L = N(kore_cuda_capture_id=lambda stream: r.randrange(50))
+        try:
+            for _ in range(4000):
+                assert P._workspace(L, N(index=0), r.randrange(20), 64) is not None
+        except Exception as e:   # noqa: BLE001
+            failed.append(repr(e))
+    try:
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+        [t.start() for t in threads]
+        [t.join() for t in threads]
+    finally:
+        sys.setswitchinterval(before)
+    assert not failed
+    assert len(P._workspaces) <= P._WORKSPACES_KEPT + 8
