@@ -645,6 +645,142 @@ int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch
                              const kore_cuda_attn_opts *opts, void *workspace, long long workspace_bytes,
                              int *dev_status, void *stream);
 
+/*
+ * A step with drafted tokens over the paged cache.
+ *
+ * No counterpart in the reference. A server that drafts several tokens ahead
+ * (speculative decoding) brings, for each sequence, a small tree: token 0 is the
+ * last one accepted, every other one a draft of what may follow its parent. One
+ * pass of the model judges all branches at once:
+ *   kore_cuda_paged_plan_dev    pages, slots and positions for the step, from the
+ *                               requests' lengths
+ *   kore_cuda_tree_masks_dev    each token's ancestors and position, from its parent
+ *   kore_cuda_paged_store_dev   a layer: keys and values to their slots, with norms
+ *                               of queries and keys for each head and the rotation
+ *   kore_cuda_paged_tree_attn_dev  a layer: the tokens' attention over the context
+ *                               and their own branches
+ *   kore_cuda_tree_accept_dev   the branch that the model's choices follow
+ *   kore_cuda_paged_commit_dev  its keys and values moved together, in all layers
+ *   kore_cuda_paged_trim_dev    the pages of the refused drafts given back
+ * Plan, store and trim serve steps without trees as well. Pointers, streams, device
+ * and dev_status are as for the operators above; 8 in dev_status: the pool has too
+ * few free pages for a sequence (it is left out, and what it holds stays).
+ */
+
+/* A pool's pages and who holds them, all in device memory that these calls alone
+ * change. Request r holds length[r] positions in the first ceil(length[r] /
+ * page_tokens) pages of its row of `table`. */
+typedef struct kore_cuda_page_pool {
+    int *free_pages;      /* [n_pages]: the first n_free are free; pages are taken from the end of these */
+    int *n_free;          /* [1] */
+    int *table;           /* [n_requests][table_stride] */
+    int *length;          /* [n_requests] */
+    int n_pages;
+    int page_tokens;      /* as kore_cuda_pages */
+    int n_requests;       /* at most 65536 */
+    int table_stride;
+} kore_cuda_page_pool;
+
+/* What a plan writes: the arrays of a kore_cuda_batch, and for each of n_tok rows
+ * its slot (page * page_tokens + place in the page) and position. */
+typedef struct kore_cuda_step {
+    int *q_start;         /* [n_seq + 1] */
+    int *kv_len;          /* [n_seq] */
+    int *page_table;      /* [n_seq][table_stride] */
+    int table_stride;     /* at least the pool's */
+    int n_tok;
+    long long *slots;     /* [n_tok]; -1: the row is of no sequence, or of one that is left out */
+    int *pos;             /* [n_tok]; -1 as well */
+} kore_cuda_step;
+
+/* Plans n_new[s] >= 0 more positions for request[s] (device [n_seq], each request
+ * once; a negative one is padding: a sequence of no tokens, whatever n_new says).
+ * New pages are taken in the order of s, so that the result is a function of the
+ * inputs alone; the first sequence that the free pages do not suffice for, and all
+ * behind it that want some, are left out: their rows count in q_start, their
+ * kv_len is 0, their slots are -1 and their requests stay as they are. So are
+ * sequences of a request named twice or outside the pool, and those that pass
+ * table_stride pages or n_tok rows (7). Entries of page_table behind a sequence's
+ * pages are not written. The others' lengths become kv_len. */
+int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *n_new,
+                             const kore_cuda_step *step, int *dev_status, void *stream);
+
+/* Keeps the first keep[s] positions of request[s] and gives the pages behind them
+ * back, so that a plan would take the same ones in the same order; their entries in
+ * the pool's table become -1. A keep that is not less than the length changes
+ * nothing; 0 ends a request. A request that is negative is padding; one that is
+ * named twice or has a negative keep is left out (7). */
+int kore_cuda_paged_trim_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *keep,
+                             int *dev_status, void *stream);
+
+/* Norms of queries and keys: each head x becomes x / sqrt(mean(x^2) + eps) * weight. */
+typedef struct kore_cuda_head_norm {
+    const void *q_weight, *k_weight;   /* device, head_dim values (a head); NULL: those heads have no norm */
+    int type;                          /* KORE_CUDA_F32, _F16 or _BF16 */
+    long long q_head_stride, k_head_stride;   /* elements from one head's weights to the next; 0: one weight for all */
+    float eps;                         /* > 0 */
+} kore_cuda_head_norm;
+
+/* Stores k and v (as kore_cuda_paged_append_dev, types alike) at slots [n_tok] and
+ * rotates q into q_out; k and q are normed by `norm` (NULL: not) before the rotation at
+ * pos [n_tok] (`rope` and pos may both be NULL: no rotation). Norm and rotation are formed
+ * in 32 bits and rounded once. A row whose slot or position is negative is left out
+ * (padding: neither its key nor its query is written); 3: a slot outside the cache,
+ * 6: a position outside the table, such a row is left out. Slots must be distinct. */
+int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok, const long long *slots, const int *pos,
+                              const kore_cuda_rows *k, const kore_cuda_rows *v, const kore_cuda_rows *q,
+                              const kore_cuda_rows *q_out, const kore_cuda_rope_view *rope,
+                              const kore_cuda_head_norm *norm, int *dev_status, void *stream);
+
+/* What the tokens of a batch's chunks see of each other: bit j (from the lowest) of
+ * the `words` 32-bit words of row t is set where token t sees token j of its chunk.
+ * Any mask is allowed (bits behind the chunk count as 0); all of them see the whole
+ * context before the chunk. */
+typedef struct kore_cuda_tree {
+    const unsigned *mask;     /* device [n_tok][words] */
+    int words;                /* 1 .. 32: chunks of up to 32 * words tokens */
+} kore_cuda_tree;
+
+/* Masks and positions from parents: parent[t] is the index in the chunk of token
+ * t's parent, less than its own, or -1. mask receives the token's ancestors and
+ * itself, pos its sequence's context length and its depth. A token with a parent
+ * that is not before it above it is left out (7; mask 0, position -1); so is a sequence
+ * whose chunk is longer than its kv_len or than the mask's words (its rows are not
+ * written). Rows outside every sequence are not touched. */
+int kore_cuda_tree_masks_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, unsigned *mask, int words,
+                             int *pos, int *dev_status, void *stream);
+
+/* kore_cuda_paged_attn_dev over trees: a token sees every position before its
+ * chunk and those of its chunk that its mask names (opts: causal 1 and no window). A
+ * token that sees nothing gets zeros (and lse -inf). Tokens of the chunk that no token
+ * sees may hold anything in the cache, infinities and NaN too. kv_len counts the whole chunk. */
+int kore_cuda_paged_tree_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
+                                  const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
+                                  const kore_cuda_attn_opts *opts, const kore_cuda_tree *tree, void *workspace,
+                                  long long workspace_bytes, int *dev_status, void *stream);
+
+/* What the acceptance writes, for each sequence. */
+typedef struct kore_cuda_accepted {
+    int *path;                /* device [n_seq][path_stride]: indexes in the chunk of the accepted tokens, -1 behind them */
+    int path_stride;          /* 1 .. 1024: tokens accepted at most */
+    int *count;               /* [n_seq]: accepted tokens, token 0 among them; 0: a sequence without tokens */
+    int *next_token;          /* [n_seq]: the model's choice behind the last of them; -1 without tokens */
+    int *kept;                /* [n_seq]: positions that the sequence holds with them; -1: it is left out */
+} kore_cuda_accepted;
+
+/* The branch that the model follows: from token 0 of each chunk on, the first child
+ * (by index) whose token[t] is choice of its parent (the model's token behind it; all
+ * device [n_tok]), and so on. */
+int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
+                              const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream);
+
+/* Moves the accepted tokens' keys and values together: row path[s][j] of sequence
+ * s's chunk to row j of it, in every one of n_layers caches (of one type and geometry,
+ * with pools of their own). batch: as the step ran with it, drafts counted. A path that does
+ * not ascend, or leaves the chunk, is left out (7). */
+int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_layers, const kore_cuda_batch *batch,
+                               const int *path, int path_stride, const int *count, int *dev_status, void *stream);
+
 /* How long a wait inside an attention that is launched (or captured) from now
  * on may take before the kernel gives up, in the whole process; 0: 2 s. A host
  * that wants to hear of a failure sooner sets less. */

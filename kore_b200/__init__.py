@@ -8,7 +8,9 @@ the ``*_dev`` forms take device tensors and stay on the context's stream.
 ``set_attn_weights`` + ``attn_block_decode`` run a decode step's whole
 attention block (kore.cpp:1418-1457), its Q4_K / Q6_K projections included.
 ``RopeTable``, ``PagedCache`` and ``PagedBatch`` (kore_b200/paged.py) are the
-operators on a caller-owned paged cache of 32, 16 or 8 bits.
+operators on a caller-owned paged cache of 32, 16 or 8 bits; ``PagePool``,
+``TokenTree``, ``AcceptedPath``, ``PagedLayers`` and ``HeadNorm``
+(kore_b200/drafts.py) are what a step with drafted tokens needs beside them.
 
 There is no fallback: if the library is missing, importing this module works
 but creating a context raises, naming the build command.
@@ -24,7 +26,8 @@ import numpy as np
 from .build import LIB, INCLUDE
 
 __all__ = ["KoreCuda", "KoreCudaError", "KvView", "Server", "load_library", "declared_symbols", "STATUS",
-           "RopeTable", "PagedBatch", "PagedCache", "rope_frequencies"]
+           "RopeTable", "PagedBatch", "PagedCache", "rope_frequencies", "PagePool", "PagedStep", "TokenTree",
+           "AcceptedPath", "PagedLayers", "HeadNorm"]
 
 STATUS = {
     0: "KORE_CUDA_OK", -1: "KORE_CUDA_EINVAL", -2: "KORE_CUDA_ERANGE", -3: "KORE_CUDA_ENOMEM",
@@ -544,3 +547,4 @@ class Server:
 
 
 from .paged import PagedBatch, PagedCache, RopeTable, rope_frequencies  # noqa: E402  (uses the names above)
+from .drafts import AcceptedPath, HeadNorm, PagedLayers, PagedStep, PagePool, TokenTree  # noqa: E402

@@ -14,8 +14,12 @@ namespace kore {
 // Device status codes of these operators, beside common.cuh's (DEV_BAD_PAGE).
 constexpr int DEV_BAD_POSITION = 6;   // a position outside the rotation table
 constexpr int DEV_BAD_SEQUENCE = 7;   // a sequence's bounds, length or page table do not fit
+constexpr int DEV_NO_PAGES = 8;       // the pool has too few free pages
 
 constexpr int kPagedMaxSeqs = 4096;      // sequences of one batch
+constexpr int kPagedMaxRequests = 65536; // requests of one pool
+constexpr int kPagedMaxTree = 1024;      // tokens of a tree
+constexpr int kPagedMaxLayers = 128;     // layers of one launch
 constexpr int kPagedMaxCtas = 160;       // CTAs (SMs) that an attention launch uses at most
 constexpr int kPagedRowsMax = 256;       // query rows of a work unit at most
 constexpr size_t kPagedZeroed = 1024;    // leading workspace bytes that are zero between calls
@@ -59,6 +63,53 @@ struct RotateParams {
     int *status;
 };
 
+// A page pool and a step (paged_plan.cu); amount: new tokens (plan) or positions kept (trim).
+struct PlanParams {
+    int *free_pages, *n_free, *table, *length;
+    int n_pages, n_requests, stride, P;
+    FastDiv by_page;
+    int n_seq, n_tok, out_stride;
+    const int *request, *amount;
+    int *q_start, *kv_len, *page_table, *pos;
+    long long *slots;
+    int *status;
+};
+
+struct StoreParams {
+    HeadRows q, k, v;          // q: heads 0: none; k, v: out, strides unused
+    const long long *slots;
+    const int *pos;            // null: nothing is rotated
+    const float *table;
+    int n_tok, n_pos, rot, interleaved, d, P, G;
+    FastDiv by_page;
+    long long n_slots, page_stride;
+    void *kc, *vc;
+    const float *k_scale, *v_scale;
+    const void *q_weight, *k_weight;   // null: those heads have no norm
+    int weight_type;
+    long long q_weight_hs, k_weight_hs;
+    float eps;
+    int *status;
+};
+
+struct TreeParams {
+    const int *q_start, *kv_len, *parent, *token, *choice;
+    int n_seq, n_tok, most, words, path_stride;   // most: tokens of a sequence at most
+    long long cap;                                // positions of a sequence at most
+    uint32_t *mask;
+    int *pos, *path, *count, *next, *kept;
+    int *status;
+};
+
+struct CommitParams {
+    const int *q_start, *kv_len, *page_table, *path, *count;
+    int n_seq, table_stride, path_stride, n_pages, n_layers, P, G, row_pieces;   // pieces: of 16 bytes
+    FastDiv by_page;
+    long long page_pieces;
+    int *status;
+    void *k[kPagedMaxLayers], *v[kPagedMaxLayers];
+};
+
 struct PagedAttnParams {
     TmaDesc tm_k, tm_v;        // K and V pools as tensor maps (many-row kernel, 16-bit caches)
     const void *k, *v;
@@ -80,6 +131,8 @@ struct PagedAttnParams {
     float *part;               // [kPagedMaxCtas][2] partial results
     int *status;
     unsigned long long wait_ns;   // a wait gives up after so long
+    const uint32_t *mask;      // trees: [n_tok][words], bit j: the token sees token j of its chunk
+    int words;
 };
 
 // four e4m3 values (first in the lowest byte) as two pairs of f16
@@ -133,7 +186,12 @@ __device__ __forceinline__ float at_least_normal(float factor) { return factor <
 
 cudaError_t launch_rope_table(const float *freq, int half, double amp, int n_pos, float *table, cudaStream_t s);
 cudaError_t launch_rotate(const RotateParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
-// n_ctas: SMs of the device, at most kPagedMaxCtas
+cudaError_t launch_plan(const PlanParams &p, bool trim, cudaStream_t s);
+cudaError_t launch_store(const StoreParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
+cudaError_t launch_tree_mask(const TreeParams &p, cudaStream_t s);
+cudaError_t launch_accept(const TreeParams &p, cudaStream_t s);
+cudaError_t launch_commit(const CommitParams &p, cudaStream_t s);
+// n_ctas: SMs of the device, at most kPagedMaxCtas; trees where p.mask is given
 cudaError_t launch_paged_rows(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
 cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
 
@@ -151,18 +209,22 @@ cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int 
 
 constexpr int kUnitCost = 1;
 
+constexpr uint32_t FULL_WORD = 0xffffffffu;
+
 struct Seq {
     int q0, n, kv;
 };
 
-// The sequence's bounds; n = 0 (it is left out) where they do not fit.
+// The sequence's bounds; n = 0 (it is left out) where they do not fit. TREE: its tokens see what
+// their masks say of each other, and all that is before them.
+template <bool TREE>
 __device__ __forceinline__ Seq load_seq(const PagedAttnParams &p, int s, bool report) {
     Seq q;
     q.q0 = __ldg(p.q_start + s);
     q.n = __ldg(p.q_start + s + 1) - q.q0;
     q.kv = __ldg(p.kv_len + s);
     if (q.n != 0 && (q.n < 0 || q.q0 < 0 || q.q0 > p.n_tok - q.n || q.kv < 0 ||
-                     q.kv > (long long)p.table_stride * p.P)) {
+                     q.kv > (long long)p.table_stride * p.P || (TREE && (q.kv < q.n || q.n > p.words * 32)))) {
         if (report) raise_error(p.status, DEV_BAD_SEQUENCE);
         q.n = 0;
     }
@@ -182,8 +244,14 @@ __device__ __forceinline__ float log_sum(float m, float l) {
     return l > 0.f || l != l ? (m - kBias<BF>)*0.69314718055994530942f + logf(l) : -INFINITY;
 }
 
-// Keys [lo, hi) that some token of the packed rows [r0, r1) of the chunk sees.
+// Keys [lo, hi) that some token of the packed rows [r0, r1) of the chunk sees (TREE: may see).
+template <bool TREE>
 __device__ __forceinline__ void key_range(const PagedAttnParams &p, const Seq &q, int r0, int r1, int &lo, int &hi) {
+    if constexpr (TREE) {
+        lo = 0;
+        hi = q.kv;
+        return;
+    }
     const int first = q.kv - q.n + p.by_rep.div(r0), last = q.kv - q.n + p.by_rep.div(r1 - 1);
     hi = p.causal ? min(q.kv, last + 1) : q.kv;
     lo = p.window > 0 && first >= p.window ? first - p.window + 1 : 0;
@@ -191,7 +259,20 @@ __device__ __forceinline__ void key_range(const PagedAttnParams &p, const Seq &q
     lo = min(lo, hi);
 }
 
-template <int ROWS, int KEYS>
+// What a token of a tree sees of the keys from x on (counted from its chunk's first token; x may lie before
+// it, in the context), 32 of them; n: tokens of the chunk.
+__device__ __forceinline__ uint32_t tree_bits(const uint32_t *mask, int words, int x, int n) {
+    auto word = [&](int w) -> uint32_t {
+        if (w < 0) return FULL_WORD;
+        const int left = n - 32 * w;
+        if (left <= 0 || w >= words) return 0u;
+        return __ldg(mask + w) & (left < 32 ? (1u << left) - 1 : FULL_WORD);
+    };
+    const int w = x >> 5;
+    return __funnelshift_r(word(w), word(w + 1), x & 31);
+}
+
+template <int ROWS, int KEYS, bool TREE = false>
 struct Unit {
     int s, g, b;           // sequence, KV head, block of rows
     Seq q;
@@ -203,7 +284,7 @@ struct Unit {
     __device__ __forceinline__ int blocks(const PagedAttnParams &p) const { return (q.n * p.rep + ROWS - 1) / ROWS; }
     __device__ __forceinline__ void range(const PagedAttnParams &p) {
         rows = min(ROWS, q.n * p.rep - b * ROWS);
-        key_range(p, q, b * ROWS, b * ROWS + rows, lo, hi);
+        key_range<TREE>(p, q, b * ROWS, b * ROWS + rows, lo, hi);
         tile0 = lo / KEYS;
         nt = max(1, (hi + KEYS - 1) / KEYS - tile0);
     }
@@ -216,7 +297,7 @@ struct Unit {
                 g = 0;
                 do {
                     if (++s >= p.n_seq) return false;
-                    q = load_seq(p, s, false);
+                    q = load_seq<TREE>(p, s, false);
                 } while (q.n == 0);
             }
         }
@@ -227,10 +308,10 @@ struct Unit {
 
 // Cost (tiles and kUnitCost a unit) of blocks b0 + lane of one head of a
 // sequence; 0 behind its last block.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, bool TREE>
 __device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q, int b, int nb) {
     if (b >= nb) return 0;
-    Unit<ROWS, KEYS> u;
+    Unit<ROWS, KEYS, TREE> u;
     u.q = q;
     u.b = b;
     u.range(p);
@@ -278,13 +359,13 @@ __device__ __forceinline__ long long quick_div(long long a, long long b) {
 
 // One head's cost of the sequences s0 + lane and their blocks: a lane a sequence;
 // sequences of several blocks by the whole warp, a lane a block.
-template <int ROWS, int KEYS>
+template <int ROWS, int KEYS, bool TREE>
 __device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, int s0, Seq &q, int &nb) {
     const int lane = threadIdx.x & 31;
     q = Seq{0, 0, 0};
-    if (s0 + lane < p.n_seq) q = load_seq(p, s0 + lane, blockIdx.x == 0);
+    if (s0 + lane < p.n_seq) q = load_seq<TREE>(p, s0 + lane, blockIdx.x == 0);
     nb = (q.n * p.rep + ROWS - 1) / ROWS;
-    long long cost = nb == 1 ? block_cost<ROWS, KEYS>(p, q, 0, 1) : 0;
+    long long cost = nb == 1 ? block_cost<ROWS, KEYS, TREE>(p, q, 0, 1) : 0;
     for (unsigned many = __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {
         const int from = __ffs(many) - 1;
         const Seq w{__shfl_sync(0xffffffffu, q.q0, from), __shfl_sync(0xffffffffu, q.n, from),
@@ -292,7 +373,7 @@ __device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, int s0
         const int wnb = __shfl_sync(0xffffffffu, nb, from);
         long long c = 0;
         for (int b = 0; b < wnb; b += 32)
-            c += __reduce_add_sync(0xffffffffu, (unsigned)block_cost<ROWS, KEYS>(p, w, b + lane, wnb));
+            c += __reduce_add_sync(0xffffffffu, (unsigned)block_cost<ROWS, KEYS, TREE>(p, w, b + lane, wnb));
         if (lane == from) cost = c;
     }
     return cost;
@@ -317,8 +398,8 @@ __device__ __forceinline__ T warp_scan(T v) {
 // Units of no more than WHOLE tiles on average are not cut for the sake of more
 // CTAs, since joining the parts takes as long as some tiles; others may be, down to
 // MIN tiles a CTA.
-template <int ROWS, int KEYS, int WHOLE, int MIN>
-__device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, Unit<ROWS, KEYS> &u,
+template <int ROWS, int KEYS, int WHOLE, int MIN, bool TREE>
+__device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, Unit<ROWS, KEYS, TREE> &u,
                                            long long &total, int &ctas, long long &x0, long long &x1) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     const bool few = p.n_seq <= 32 && p.small;
@@ -327,7 +408,7 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     Seq q;
     if (few) {
         int nb;
-        cost = lane_costs<ROWS, KEYS>(p, 0, q, nb);
+        cost = lane_costs<ROWS, KEYS, TREE>(p, 0, q, nb);
         sum = warp_scan((int)cost);
         total = __shfl_sync(0xffffffffu, sum, 31);
         units = __reduce_add_sync(0xffffffffu, nb);
@@ -337,7 +418,7 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
         __syncthreads();
         for (int s0 = warp * 32; s0 < p.n_seq; s0 += warps * 32) {
             int nb;
-            const long long c = lane_costs<ROWS, KEYS>(p, s0, q, nb);
+            const long long c = lane_costs<ROWS, KEYS, TREE>(p, s0, q, nb);
             if (s0 + lane < p.n_seq) cum[s0 + lane + 1] = c;
             const int n = __reduce_add_sync(0xffffffffu, nb);
             if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long *>(&shared_units), (unsigned long long)n);
@@ -379,7 +460,7 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
             else b = m - 1;
         }
         u.s = a;
-        u.q = load_seq(p, a, false);
+        u.q = load_seq<TREE>(p, a, false);
         before = cum[a];
         cost = cum[a + 1] - before;
         __syncthreads();   // cum may be used for something else from here
@@ -391,7 +472,7 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     u.b = 0;
     const int nb = (u.q.n * p.rep + ROWS - 1) / ROWS;
     for (int b0 = 0; nb > 1; b0 += 32) {
-        const int c = block_cost<ROWS, KEYS>(p, u.q, b0 + lane, nb);
+        const int c = block_cost<ROWS, KEYS, TREE>(p, u.q, b0 + lane, nb);
         const int v = warp_scan(c);
         const unsigned in = __ballot_sync(0xffffffffu, u.u0 + v > x0 && c > 0);
         if (in || b0 + 32 >= nb) {

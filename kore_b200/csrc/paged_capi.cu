@@ -2,144 +2,17 @@
 // cache (include/kore_cuda.h): argument checks, the buffers' device, kernel
 // choice. Nothing is allocated and nothing kept between calls.
 
-#include "paged.cuh"
-
-#include "kore_cuda.h"
+#include "paged_args.cuh"
 
 #include <cuda.h>
 
 #include <atomic>
 #include <cmath>
-#include <cstdarg>
-#include <cstdio>
-#include <cstring>
 
 namespace kore {
 namespace {
 
-int refuse(int code, const char *fmt, ...) {
-    char buf[256];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    set_ctxless_error(buf);
-    return code;
-}
-
 std::atomic<unsigned long long> g_wait_ns{kWaitNs};   // of launches from now on
-
-int type_bytes(int type) {
-    switch (type) {
-        case KORE_CUDA_F32: return 4;
-        case KORE_CUDA_F16:
-        case KORE_CUDA_BF16: return 2;
-        case KORE_CUDA_E4M3: return 1;
-    }
-    return 0;
-}
-
-// Makes the device of a buffer current for the call.
-struct OnDeviceOf {
-    int prev = -1, dev = -1, rc = KORE_CUDA_OK;
-    explicit OnDeviceOf(const void *ptr) {
-        cudaPointerAttributes a;
-        cudaError_t e = cudaPointerGetAttributes(&a, ptr);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            rc = refuse(KORE_CUDA_ECUDA, "no CUDA device: %s", cudaGetErrorString(e));
-            return;
-        }
-        if (a.type != cudaMemoryTypeDevice && a.type != cudaMemoryTypeManaged) {
-            rc = refuse(KORE_CUDA_EINVAL, "expected device memory");
-            return;
-        }
-        dev = a.device;
-        if (cudaGetDevice(&prev) != cudaSuccess) prev = -1;
-        if (prev != dev && (e = cudaSetDevice(dev)) != cudaSuccess)
-            rc = refuse(KORE_CUDA_ECUDA, "cudaSetDevice(%d): %s", dev, cudaGetErrorString(e));
-    }
-    ~OnDeviceOf() {
-        if (prev >= 0 && prev != dev) cudaSetDevice(prev);
-    }
-};
-
-int launched(cudaError_t e, const char *what) {
-    if (e == cudaSuccess) return KORE_CUDA_OK;
-    cudaGetLastError();
-    return refuse(KORE_CUDA_ECUDA, "%s: %s", what, cudaGetErrorString(e));
-}
-
-bool aligned16(const kore_cuda_rows &r) {
-    const long long b = type_bytes(r.type);
-    return ((reinterpret_cast<uintptr_t>(r.data) | (uintptr_t)(r.token_stride * b) | (uintptr_t)(r.head_stride * b)) & 15) == 0;
-}
-
-int check_rows(const kore_cuda_rows *r, const char *name, int head_dim) {
-    if (!r || !r->data) return refuse(KORE_CUDA_EINVAL, "%s is null", name);
-    const int b = type_bytes(r->type);
-    if (b < 2) return refuse(KORE_CUDA_EINVAL, "%s: type %d is none of F32, F16, BF16", name, r->type);
-    if (reinterpret_cast<uintptr_t>(r->data) % b) return refuse(KORE_CUDA_EINVAL, "%s is not aligned to its type", name);
-    if (r->n_head <= 0 || r->n_head > 65535) return refuse(KORE_CUDA_EINVAL, "%s: n_head %d", name, r->n_head);
-    if (r->head_dim != head_dim) return refuse(KORE_CUDA_EINVAL, "%s: head_dim %d, expected %d", name, r->head_dim, head_dim);
-    return KORE_CUDA_OK;
-}
-
-// Rows that are written: several in one place would leave whichever came last.
-int check_written(const kore_cuda_rows *r, const char *name, int n_tok) {
-    if ((n_tok > 1 && r->token_stride == 0) || (r->n_head > 1 && r->head_stride == 0))
-        return refuse(KORE_CUDA_EINVAL, "%s: the rows overlap (a stride of 0)", name);
-    return KORE_CUDA_OK;
-}
-
-int check_rope(const kore_cuda_rope_view *r, int head_dim) {
-    if (!r->table) return refuse(KORE_CUDA_EINVAL, "the rotation table is null");
-    if (reinterpret_cast<uintptr_t>(r->table) & 15)
-        return refuse(KORE_CUDA_EINVAL, "the rotation table must be 16-byte aligned");
-    if (r->n_pos <= 0) return refuse(KORE_CUDA_EINVAL, "the rotation table holds %d positions", r->n_pos);
-    if (r->n_rot < 2 || (r->n_rot & 1) || r->n_rot > head_dim)
-        return refuse(KORE_CUDA_EINVAL, "n_rot %d must be even and at most head_dim %d", r->n_rot, head_dim);
-    return KORE_CUDA_OK;
-}
-
-int check_pages(const kore_cuda_pages *c, bool attention) {
-    if (!c || !c->k || !c->v) return refuse(KORE_CUDA_EINVAL, "the cache is null");
-    const int b = type_bytes(c->type);
-    if (b == 0 || (attention && b == 4)) return refuse(KORE_CUDA_EINVAL, "cache type %d is not supported here", c->type);
-    if (c->n_pages <= 0) return refuse(KORE_CUDA_EINVAL, "n_pages %d must be positive", c->n_pages);
-    if (c->page_tokens <= 0 || c->page_tokens % 16)
-        return refuse(KORE_CUDA_EINVAL, "page_tokens %d must be a positive multiple of 16", c->page_tokens);
-    if (c->n_head_kv <= 0 || c->n_head_kv > 65535) return refuse(KORE_CUDA_EINVAL, "n_head_kv %d", c->n_head_kv);
-    if (c->head_dim <= 0 || c->head_dim % 16 || c->head_dim > 256 ||
-        (attention && c->head_dim != 64 && c->head_dim != 128))
-        return refuse(KORE_CUDA_EINVAL, "head_dim %d is not supported here", c->head_dim);
-    if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15)
-        return refuse(KORE_CUDA_EINVAL, "the page pools must be 16-byte aligned");
-    const long long page = (long long)c->n_head_kv * c->page_tokens * c->head_dim;
-    if (c->page_stride && (c->page_stride < page || c->page_stride * b % 16))
-        return refuse(KORE_CUDA_EINVAL, "page_stride %lld must be a multiple of 16 bytes and at least a page (%lld)",
-                      c->page_stride, page);
-    if (c->type != KORE_CUDA_E4M3 && (c->k_scale || c->v_scale))
-        return refuse(KORE_CUDA_EINVAL, "scales belong to an E4M3 cache");
-    return KORE_CUDA_OK;
-}
-
-long long page_stride(const kore_cuda_pages *c) {
-    return c->page_stride ? c->page_stride : (long long)c->n_head_kv * c->page_tokens * c->head_dim;
-}
-
-int check_batch(const kore_cuda_batch *b, int n_tok) {
-    if (!b) return refuse(KORE_CUDA_EINVAL, "the batch is null");
-    if (n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", n_tok);
-    if (b->n_seq < 0 || b->n_seq > kPagedMaxSeqs)
-        return refuse(KORE_CUDA_ERANGE, "n_seq %d outside [0, %d]", b->n_seq, kPagedMaxSeqs);
-    if (b->n_seq > 0 && (!b->q_start || !b->kv_len || !b->page_table))
-        return refuse(KORE_CUDA_EINVAL, "q_start, kv_len or page_table is null");
-    if (b->n_seq > 0 && b->table_stride <= 0) return refuse(KORE_CUDA_EINVAL, "table_stride %d", b->table_stride);
-    if (b->max_q < 0) return refuse(KORE_CUDA_EINVAL, "max_q %d", b->max_q);
-    if (b->max_kv < 0) return refuse(KORE_CUDA_EINVAL, "max_kv %d", b->max_kv);
-    return KORE_CUDA_OK;
-}
 
 // The pool as a tensor [page][head][token][d], boxes of `box` tokens x 128 bytes
 // (or the 64 of a short row), swizzled within rows of that width or (plain) as it is.
@@ -171,24 +44,6 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, bool plai
         return false;
     memcpy(out, &m, sizeof m);
     return true;
-}
-
-bool rotates_in_vectors(int d, const kore_cuda_rope_view *r) { return d % 16 == 0 && (!r || r->n_rot % 16 == 0); }
-
-HeadRows head_rows(const kore_cuda_rows *in, const kore_cuda_rows *out) {
-    HeadRows h;
-    memset(&h, 0, sizeof h);
-    if (!in) return h;
-    h.in = in->data;
-    h.in_ts = in->token_stride;
-    h.in_hs = in->head_stride;
-    h.heads = in->n_head;
-    if (out) {
-        h.out = out->data;
-        h.out_ts = out->token_stride;
-        h.out_hs = out->head_stride;
-    }
-    return h;
 }
 
 }  // namespace
@@ -284,24 +139,9 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
     if (int rc = check_pages(cache, false)) return rc;
     if (int rc = check_batch(batch, n_tok)) return rc;
     const int d = cache->head_dim;
-    if (int rc = check_rows(k, "k", d)) return rc;
-    if (int rc = check_rows(v, "v", d)) return rc;
-    if (k->n_head != cache->n_head_kv || v->n_head != cache->n_head_kv)
-        return refuse(KORE_CUDA_EINVAL, "k and v must have the cache's %d heads", cache->n_head_kv);
-    if (v->type != k->type) return refuse(KORE_CUDA_EINVAL, "k and v have different types");
-    if (!q != !q_out) return refuse(KORE_CUDA_EINVAL, "q and q_out come together");
-    if (q) {
-        if (int rc = check_rows(q, "q", d)) return rc;
-        if (int rc = check_rows(q_out, "q_out", d)) return rc;
-        if (q->type != k->type || q_out->type != k->type || q_out->n_head != q->n_head)
-            return refuse(KORE_CUDA_EINVAL, "q and q_out must have k's type and the same heads");
-        if (int rc = check_written(q_out, "q_out", n_tok)) return rc;
-    }
+    if (int rc = check_appended(cache, k, v, q, q_out, n_tok)) return rc;
     if (rope)
         if (int rc = check_rope(rope, d)) return rc;
-    if (cache->type != k->type && cache->type != KORE_CUDA_E4M3 &&
-        !(k->type == KORE_CUDA_F32 && (cache->type == KORE_CUDA_F16 || cache->type == KORE_CUDA_BF16)))
-        return refuse(KORE_CUDA_EINVAL, "rows of type %d do not go into a cache of type %d", k->type, cache->type);
     if (n_tok == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
     OnDeviceOf on(cache->k);
     if (on.rc) return on.rc;
@@ -347,10 +187,10 @@ extern "C" long long kore_cuda_paged_attn_workspace(int head_dim) {
     return (long long)kPagedZeroed + (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
 }
 
-extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
-                                        const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
-                                        const kore_cuda_attn_opts *opts, void *workspace, long long workspace_bytes,
-                                        int *dev_status, void *stream) {
+// The attention of chunks (tree null) and of trees.
+static int attend(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok, const kore_cuda_rows *q,
+                  const kore_cuda_rows *out, float *lse, const kore_cuda_attn_opts *opts, const kore_cuda_tree *tree,
+                  void *workspace, long long workspace_bytes, int *dev_status, void *stream) {
     static_assert(kPagedZeroed == KORE_CUDA_PAGED_WORKSPACE_ZEROED && kPagedMaxCtas * sizeof(int) <= kPagedZeroed,
                   "the counters' place in the workspace");
     if (int rc = check_pages(cache, true)) return rc;
@@ -372,6 +212,11 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     if (!opts) return refuse(KORE_CUDA_EINVAL, "opts is null");
     if (opts->window < 0) return refuse(KORE_CUDA_EINVAL, "window %d", opts->window);
     if (!std::isfinite(opts->scale)) return refuse(KORE_CUDA_EINVAL, "scale is not finite");
+    if (tree) {
+        if (int rc = check_tree(tree)) return rc;
+        if (!opts->causal || opts->window)
+            return refuse(KORE_CUDA_EINVAL, "a tree's tokens see what their masks say: no window, and causal as it is");
+    }
     if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 255) ||
         workspace_bytes < kore_cuda_paged_attn_workspace(d))
         return refuse(KORE_CUDA_EINVAL, "the workspace must be 256-byte aligned and hold %lld bytes",
@@ -418,6 +263,10 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
     p.part = reinterpret_cast<float *>(static_cast<char *>(workspace) + kPagedZeroed);
     p.status = dev_status;
     p.wait_ns = g_wait_ns;
+    if (tree) {
+        p.mask = reinterpret_cast<const uint32_t *>(tree->mask);
+        p.words = tree->words;
+    }
     const int ctas = sms < kPagedMaxCtas ? sms : kPagedMaxCtas;
     // units are of 16 rows and tiles of 128 keys at least; every sequence may have all rows (a
     // q_start that goes back is reported, and those that fit on their own are still worked on:
@@ -449,6 +298,21 @@ extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore
         return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
     if (tiles) return launched(launch_paged_tiles(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
     return launched(launch_paged_rows(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
+}
+
+extern "C" int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
+                                        const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
+                                        const kore_cuda_attn_opts *opts, void *workspace, long long workspace_bytes,
+                                        int *dev_status, void *stream) {
+    return attend(cache, batch, n_tok, q, out, lse, opts, nullptr, workspace, workspace_bytes, dev_status, stream);
+}
+
+extern "C" int kore_cuda_paged_tree_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
+                                             const kore_cuda_rows *q, const kore_cuda_rows *out, float *lse,
+                                             const kore_cuda_attn_opts *opts, const kore_cuda_tree *tree,
+                                             void *workspace, long long workspace_bytes, int *dev_status, void *stream) {
+    if (!tree) return refuse(KORE_CUDA_EINVAL, "the tree is null");
+    return attend(cache, batch, n_tok, q, out, lse, opts, tree, workspace, workspace_bytes, dev_status, stream);
 }
 
 extern "C" unsigned long long kore_cuda_capture_id(void *stream) {

@@ -109,13 +109,14 @@ __device__ __forceinline__ uint64_t l2_evict_normal_policy() {
     return pol;
 }
 
-// QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16).
-template <int D, bool QBF, bool E4M3>
+// QBF: queries (and output) in bf16, else f16. E4M3: 8-bit cache (products in f16). TREE: the chunks
+// are trees of drafted tokens.
+template <int D, bool QBF, bool E4M3, bool TREE>
 __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid_constant__ PagedAttnParams p) {
     constexpr int ES = E4M3 ? 1 : 2;
     using C = RowsCfg<D, ES>;
     constexpr bool BF = QBF && !E4M3;   // type of the products
-    using U = Unit<kRowsU, C::CT>;
+    using U = Unit<kRowsU, C::CT, TREE>;
     using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
     extern __shared__ __align__(1024) uint8_t smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -140,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
     U u;
     long long total, x0, x1;
     int ctas;
-    if (!find_share<kRowsU, C::CT, 5, 2>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
+    if (!find_share<kRowsU, C::CT, 5, 2, TREE>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
     uint8_t *ring = smem + warp * C::STAGES * C::STAGE;
 
@@ -250,12 +251,18 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
             const bool in0 = g8 < u.rows, in1 = g8 + 8 < u.rows;
             // keys [lo, hi) of the two rows
             int lo0 = 0, hi0 = 0, lo1 = 0, hi1 = 0;
-            if (in0) key_range(p, u.q, r0, r0 + 1, lo0, hi0);
-            if (in1) key_range(p, u.q, r1, r1 + 1, lo1, hi1);
             // keys that every valid row sees
-            int all_lo, all_hi, t;
-            key_range(p, u.q, u.b * kRowsU, u.b * kRowsU + 1, t, all_hi);
-            key_range(p, u.q, u.b * kRowsU + u.rows - 1, u.b * kRowsU + u.rows, all_lo, t);
+            int all_lo = 0, all_hi = u.q.kv - u.q.n, t;
+            const uint32_t *mask0 = nullptr, *mask1 = nullptr;   // TREE: the two rows'
+            if constexpr (TREE) {
+                mask0 = p.mask + (long long)(u.q.q0 + p.by_rep.div(in0 ? r0 : u.b * kRowsU)) * p.words;
+                mask1 = p.mask + (long long)(u.q.q0 + p.by_rep.div(in1 ? r1 : u.b * kRowsU)) * p.words;
+            } else {
+                if (in0) key_range<TREE>(p, u.q, r0, r0 + 1, lo0, hi0);
+                if (in1) key_range<TREE>(p, u.q, r1, r1 + 1, lo1, hi1);
+                key_range<TREE>(p, u.q, u.b * kRowsU, u.b * kRowsU + 1, t, all_hi);
+                key_range<TREE>(p, u.q, u.b * kRowsU + u.rows - 1, u.b * kRowsU + u.rows, all_lo, t);
+            }
 
             float qs0 = fabsf(p.scale) * 1.44269504088896340736f, qs1 = qs0;
             {
@@ -331,9 +338,16 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
                 const uint32_t kt = smem_u32(st), vt = kt + C::HALF;
                 const int key0 = (u.tile0 + tt) * C::CT + warp * C::KT;
                 if (!dead && key0 < u.hi && key0 + C::KT > u.lo) {
-                    if (key0 < u.lo || key0 + C::KT > u.hi) {   // rows outside the unit's keys
+                    uint32_t see0 = 0, see1 = 0;   // TREE: the tile's keys that the two rows see
+                    uint32_t some = ~0u;           // ... and any row of the unit
+                    if (TREE && key0 + C::KT > all_hi) {
+                        if (in0) see0 = tree_bits(mask0, p.words, key0 - all_hi, u.q.n);
+                        if (in1) see1 = tree_bits(mask1, p.words, key0 - all_hi, u.q.n);
+                        some = __reduce_or_sync(FULL, see0 | see1);
+                    }
+                    if (TREE ? (~some << (32 - C::KT)) != 0 : key0 < u.lo || key0 + C::KT > u.hi) {   // rows outside the unit's keys
                         for (int r = 0; r < C::KT; ++r)
-                            if ((key0 + r < u.lo || key0 + r >= u.hi) && lane < C::CH)
+                            if ((TREE ? !(some >> r & 1) : key0 + r < u.lo || key0 + r >= u.hi) && lane < C::CH)
                                 *reinterpret_cast<uint4 *>(st + C::HALF + piece<C::ROWB, C::KT>(r, lane)) = make_uint4(0, 0, 0, 0);
                         fence_proxy_async_smem();   // before the stage is filled again
                         __syncwarp();
@@ -384,8 +398,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 const int key = key0 + 8 * j + 2 * t4 + i;
-                                if (key < lo0 || key >= hi0) s[j][i] = -INFINITY;
-                                if (key < lo1 || key >= hi1) s[j][2 + i] = -INFINITY;
+                                if (TREE ? !(see0 >> (key - key0) & 1) : key < lo0 || key >= hi0) s[j][i] = -INFINITY;
+                                if (TREE ? !(see1 >> (key - key0) & 1) : key < lo1 || key >= hi1) s[j][2 + i] = -INFINITY;
                             }
                     }
                     float x0m = fmaxf(s[0][0], s[0][1]), x1m = fmaxf(s[0][2], s[0][3]);
@@ -625,10 +639,10 @@ __global__ void __launch_bounds__(kWarps * 32, 1) paged_rows_kernel(const __grid
         for (uint32_t i = n_taken; i < n_loaded; ++i) mbar_drain(&full[i % C::STAGES], (i / C::STAGES) & 1);
 }
 
-template <int D, bool QBF, bool E4M3>
-cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+template <int D, bool QBF, bool E4M3, bool TREE>
+cudaError_t launch_t(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     using C = RowsCfg<D, E4M3 ? 1 : 2>;
-    auto kernel = paged_rows_kernel<D, QBF, E4M3>;
+    auto kernel = paged_rows_kernel<D, QBF, E4M3, TREE>;
     static_assert(C::BYTES <= 232448, "shared memory of an SM");
     if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(kernel), C::BYTES)) return e;
     cudaLaunchConfig_t cfg = {};
@@ -642,6 +656,11 @@ cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D, bool QBF, bool E4M3>
+cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+    return p.mask ? launch_t<D, QBF, E4M3, true>(p, n_ctas, s) : launch_t<D, QBF, E4M3, false>(p, n_ctas, s);
 }
 
 }  // namespace

@@ -203,12 +203,24 @@ __device__ __forceinline__ void st_release(uint32_t *p, uint32_t v) {
 template <int D>
 constexpr size_t kSlot = (size_t)kUnitRows * (D + 2);
 
-// QBF: queries and outputs in bf16, else f16. E8: 8-bit cache, products in f16.
-template <int D, bool QBF, bool E8>
+// What some row of the unit, a block of a tree's rows, sees of the keys from x on (counted as for
+// tree_bits); by a whole warp.
+template <int ROWS, int KEYS>
+__device__ __forceinline__ uint32_t seen_by_some(const PagedAttnParams &p, const Unit<ROWS, KEYS, true> &u, int x) {
+    const int t0 = p.by_rep.div(u.b * ROWS), t1 = p.by_rep.div(u.b * ROWS + u.rows - 1);
+    uint32_t bits = 0;
+    for (int t = t0 + (threadIdx.x & 31); t <= t1; t += 32)
+        bits |= tree_bits(p.mask + (long long)(u.q.q0 + t) * p.words, p.words, x, u.q.n);
+    return __reduce_or_sync(FULL, bits);
+}
+
+// QBF: queries and outputs in bf16, else f16. E8: 8-bit cache, products in f16. TREE: the chunks
+// are trees of drafted tokens.
+template <int D, bool QBF, bool E8, bool TREE>
 __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnParams p) {
     using C = TilesCfg<D, E8>;
     constexpr bool BF = QBF && !E8;   // type of the products
-    using U = Unit<kUnitRows, kKeys>;
+    using U = Unit<kUnitRows, kKeys, TREE>;
     using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -243,7 +255,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     U u;
     long long total, x0, x1;
     int ctas;
-    if (!find_share<kUnitRows, kKeys, 4, 3>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
+    if (!find_share<kUnitRows, kKeys, 4, 3, TREE>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::LOADS; ++i) mbar_init(&full[i], 1);
@@ -497,10 +509,23 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 for (int kv = 0; ok && kv < 2; ++kv, ++it) {
                     ok = wait(&full[it % C::STAGES], (it / C::STAGES) & 1, true);
                     const int key0 = (u.tile0 + t) * kKeys;
-                    if (ok && kv == 1 && (key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
+                    const int first = u.q.kv - u.q.n;   // TREE: the chunk's first key
+                    if (ok && kv == 1 && (TREE ? key0 + kKeys > first : key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
                         uint8_t *v = smem + C::RING + (it % C::STAGES) * C::TILE;
+                        uint32_t some[kKeys / 32];
+                        if constexpr (TREE) {
+#pragma unroll
+                            for (int x = 0; x < kKeys / 32; ++x) some[x] = seen_by_some(p, u, key0 + 32 * x - first);
+                        }
+                        auto outside = [&](int r) {
+                            if constexpr (TREE) {
+                                const uint32_t a = r & 32 ? some[1] : some[0], b = r & 32 ? some[3] : some[2];
+                                return !((r & 64 ? b : a) >> (r & 31) & 1);
+                            }
+                            return key0 + r < u.lo || key0 + r >= u.hi;
+                        };
                         for (int r = lane >> 3; r < kKeys; r += 4)
-                            if (key0 + r < u.lo || key0 + r >= u.hi)
+                            if (outside(r))
                                 for (int h = 0; h < C::HALVES; ++h)
                                     *reinterpret_cast<uint4 *>(v + h * C::BLOCK + r * 128 + (lane & 7) * 16) =
                                         make_uint4(0, 0, 0, 0);
@@ -529,13 +554,19 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     ok = wait(&full[it % C::RAW_STAGES], (it / C::RAW_STAGES) & 1, true);
                     if (ok && it >= C::STAGES) ok = wait(&empty[it % C::STAGES], (it / C::STAGES - 1) & 1);
                     if (!ok) break;
+                    // TREE: which of this warp's 32 keys any row of the unit sees
+                    uint32_t some = ~0u;
+                    const int first = u.q.kv - u.q.n;
+                    if constexpr (TREE) {
+                        if (kv == 1 && key0 + kKeys > first) some = seen_by_some(p, u, key0 + 32 * w - first);
+                    }
                     const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 32 * D + lane * 16;
                     uint8_t *dst = smem + C::RING + (it % C::STAGES) * C::TILE + (c >> 2) * C::BLOCK;
 #pragma unroll 4
                     for (int x = 0; x < L; ++x) {
                         const int row = w * 32 + x * (32 / L) + lane / L;
                         uint4 v = *reinterpret_cast<const uint4 *>(src + x * 512);
-                        if (kv == 1 && (key0 + row < u.lo || key0 + row >= u.hi)) v = make_uint4(0, 0, 0, 0);   // of V
+                        if (kv == 1 && (TREE ? !(some >> (row & 31) & 1) : key0 + row < u.lo || key0 + row >= u.hi)) v = make_uint4(0, 0, 0, 0);   // of V
                         uint4 a, b;
                         widen4(v.x, a.x, a.y);
                         widen4(v.y, a.z, a.w);
@@ -681,12 +712,16 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             const bool in = i * kM + r < u.rows;
             const int pr = u.b * kUnitRows + i * kM + r;
             int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
-            if (mine) {
-                if (in) key_range(p, u.q, pr, pr + 1, lo, hi);
+            const uint32_t *mask = nullptr;   // TREE: this row's
+            if constexpr (TREE) {
+                all_hi = u.q.kv - u.q.n;
+                mask = p.mask + (long long)(u.q.q0 + p.by_rep.div(in ? pr : 0)) * p.words;
+            } else if (mine) {
+                if (in) key_range<TREE>(p, u.q, pr, pr + 1, lo, hi);
                 const int b0 = u.b * kUnitRows + i * kM, b1 = u.b * kUnitRows + min(u.rows, (i + 1) * kM);
                 int x;
-                key_range(p, u.q, b0, b0 + 1, x, all_hi);
-                key_range(p, u.q, b1 - 1, b1, all_lo, x);
+                key_range<TREE>(p, u.q, b0, b0 + 1, x, all_hi);
+                key_range<TREE>(p, u.q, b1 - 1, b1, all_lo, x);
             }
             float qs = qs_all;
             if constexpr (E8 && QBF) qs *= q_shift[i * kM + r];
@@ -710,7 +745,13 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     ld32(tb + 32, reinterpret_cast<uint32_t *>(s) + 32);
                     wait_ld();
                     const int key0 = k * kStep;
-                    if (key0 < all_lo || key0 + kStep > all_hi) {
+                    if (TREE && key0 + kStep > all_hi) {
+                        const uint32_t see[2] = {in ? tree_bits(mask, p.words, key0 - all_hi, u.q.n) : 0u,
+                                                 in ? tree_bits(mask, p.words, key0 + 32 - all_hi, u.q.n) : 0u};
+#pragma unroll
+                        for (int x = 0; x < 64; ++x)
+                            if (!(see[x >> 5] >> (x & 31) & 1)) s[x] = -INFINITY;
+                    } else if (!TREE && (key0 < all_lo || key0 + kStep > all_hi)) {
 #pragma unroll
                         for (int x = 0; x < 64; ++x)
                             if (key0 + x < lo || key0 + x >= hi) s[x] = -INFINITY;
@@ -933,10 +974,10 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     }
 }
 
-template <int D, bool QBF, bool E8>
-cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+template <int D, bool QBF, bool E8, bool TREE>
+cudaError_t launch_t(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     using C = TilesCfg<D, E8>;
-    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, QBF, E8>), C::BYTES)) return e;
+    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, QBF, E8, TREE>), C::BYTES)) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -947,7 +988,12 @@ cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QBF, E8>, p);
+    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QBF, E8, TREE>, p);
+}
+
+template <int D, bool QBF, bool E8>
+cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+    return p.mask ? launch_t<D, QBF, E8, true>(p, n_ctas, s) : launch_t<D, QBF, E8, false>(p, n_ctas, s);
 }
 
 }  // namespace

@@ -10,6 +10,9 @@ A step of a batch, on the current stream of the tensors' device::
     cache.append(batch, k, v, rope=rope, q=q, q_out=q)    # a layer: store k and v, rotate k and q
     cache.attend(batch, q, out)
 
+kore_b200/drafts.py has what a step with drafted tokens needs beside them: pages and slots planned on the GPU, trees,
+and the accepted branch.
+
 An object is for one host thread at a time, as a context is; nothing here is recorded for gradients. Nothing is copied or synchronised: a failure that a kernel meets in the device
 data (a page outside the pool, a sequence that does not fit its page table)
 is left in ``status`` and raised by ``check()``.
@@ -27,7 +30,8 @@ F32, F16, BF16, E4M3 = 0, 1, 30, 1000
 WORKSPACE_ZEROED = 1024
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
 DEVICE_FAILURES = {1: "a tile copy or product did not come in time", 3: "page id outside the pool", 6: "position outside the rotation table",
-                   7: "a sequence's bounds do not fit the rows, its length or its page table"}
+                   7: "a sequence's bounds do not fit the rows, its length or its page table",
+                   8: "too few free pages in the pool"}
 
 _vp, _i, _ll, _d = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_double
 
@@ -66,6 +70,34 @@ class _Opts(ctypes.Structure):
     _fields_ = [("scale", ctypes.c_float), ("causal", _i), ("window", _i)]
 
 
+class _Norm(ctypes.Structure):
+    """kore_cuda_head_norm."""
+    _fields_ = [("q_weight", _vp), ("k_weight", _vp), ("type", _i), ("q_head_stride", _ll), ("k_head_stride", _ll),
+                ("eps", ctypes.c_float)]
+
+
+class _Tree(ctypes.Structure):
+    """kore_cuda_tree."""
+    _fields_ = [("mask", _vp), ("words", _i)]
+
+
+class _Pool(ctypes.Structure):
+    """kore_cuda_page_pool."""
+    _fields_ = [("free_pages", _vp), ("n_free", _vp), ("table", _vp), ("length", _vp), ("n_pages", _i),
+                ("page_tokens", _i), ("n_requests", _i), ("table_stride", _i)]
+
+
+class _Step(ctypes.Structure):
+    """kore_cuda_step."""
+    _fields_ = [("q_start", _vp), ("kv_len", _vp), ("page_table", _vp), ("table_stride", _i), ("n_tok", _i),
+                ("slots", _vp), ("pos", _vp)]
+
+
+class _Accepted(ctypes.Structure):
+    """kore_cuda_accepted."""
+    _fields_ = [("path", _vp), ("path_stride", _i), ("count", _vp), ("next_token", _vp), ("kept", _vp)]
+
+
 _fns = None
 
 
@@ -81,6 +113,13 @@ def _library():
         L.kore_cuda_paged_attn_workspace.argtypes = [_i]
         L.kore_cuda_paged_attn_workspace.restype = _ll
         L.kore_cuda_paged_attn_dev.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _ll, _vp, _vp]
+        L.kore_cuda_paged_plan_dev.argtypes = [_vp, _i] + [_vp] * 5
+        L.kore_cuda_paged_trim_dev.argtypes = [_vp, _i] + [_vp] * 4
+        L.kore_cuda_paged_store_dev.argtypes = [_vp, _i] + [_vp] * 10
+        L.kore_cuda_tree_masks_dev.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp]
+        L.kore_cuda_paged_tree_attn_dev.argtypes = [_vp, _vp, _i] + [_vp] * 6 + [_ll, _vp, _vp]
+        L.kore_cuda_tree_accept_dev.argtypes = [_vp, _i] + [_vp] * 6
+        L.kore_cuda_paged_commit_dev.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp]
         L.kore_cuda_paged_set_wait_limit.argtypes = [ctypes.c_ulonglong]
         L.kore_cuda_capture_id.argtypes = [_vp]
         L.kore_cuda_capture_id.restype = ctypes.c_ulonglong
@@ -314,15 +353,53 @@ class PagedCache:
         if rc:
             _ck(self._L, rc)
 
+    def store(self, slots, pos, k, v, *, rope: RopeTable | None = None, norm=None, q=None, q_out=None) -> None:
+        """Stores k and v [tokens][n_head_kv][head_dim] at the slots [tokens] (int64: page * page_tokens + place in the
+        page; negative: the row is left out). norm (a HeadNorm of kore_b200/drafts.py) norms each head of k and q, rope
+        rotates them at the int32 positions pos [tokens] (None without rope); with q, it goes into q_out (which may be q)
+        in the same launch."""
+        dev, r = self.device, self._r
+        n = _fill(r[0], k, "k", dev)
+        if _fill(r[1], v, "v", dev) != n:
+            raise ValueError("k and v have different numbers of tokens")
+        if (slots.dtype != _torch.int64 or slots.dim() != 1 or slots.shape[0] != n or not slots.is_contiguous()
+                or slots.device != dev):
+            raise ValueError(f"slots: expected {n} contiguous int64 values on {dev}")
+        pq = pqo = pp = pr = pn = None
+        if (q is None) != (q_out is None):
+            raise ValueError("q and q_out come together")
+        if q is not None:
+            if _fill(r[2], q, "q", dev) != n or _fill(r[3], q_out, "q_out", dev) != n:
+                raise ValueError("q, q_out and k have different numbers of tokens")
+            pq, pqo = self._p[2], self._p[3]
+        if rope is not None:
+            if rope.device != dev:
+                raise ValueError(f"the table is not on {dev}")
+            if pos is None:
+                raise ValueError("a rotation needs positions")
+            pp, pr = _ints(pos, "pos", dev, 1), rope._view
+            if pos.shape[0] != n:
+                raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
+        if norm is not None:
+            pn = norm._for(dev, self.view.head_dim, r[2].n_head if q is not None else None, r[0].n_head)
+        if n == 0:
+            return
+        rc = self._L.kore_cuda_paged_store_dev(self._view, n, slots.data_ptr(), pp, self._p[0], self._p[1], pq, pqo, pr,
+                                               pn, self._status, _stream(dev))
+        if rc:
+            _ck(self._L, rc)
+
     def attend(self, batch: PagedBatch, q, out=None, *, scale: float = 0.0, causal: bool = True, window: int = 0,
-               lse=None, workspace=None):
+               lse=None, workspace=None, tree=None):
         """Attention of q [tokens][n_head][head_dim] (fp16 or bf16) over the batch's cached positions, into out (a new
         tensor if None; never q's own memory). Rows outside every sequence keep what out holds (a new tensor: whatever
         the memory holds).
 
         scale 0: 1/sqrt(head_dim). window: how many positions back a token sees, itself among them (0: all). lse: an
         optional float32 [tokens][n_head] for the log of the softmax's sums. workspace: a tensor of new_workspace();
-        by default one that this device and stream (or the capture that the stream is in) keep."""
+        by default one that this device and stream (or the capture that the stream is in) keep. tree (a TokenTree of
+        kore_b200/drafts.py): each chunk is a tree of drafted tokens, which see their context and what the tree's masks
+        name of their chunk (no window, causal as it is)."""
         dev, r = self.device, self._r
         if out is None:
             out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
@@ -344,12 +421,19 @@ class PagedCache:
         if workspace is not None and (workspace.dtype != _torch.uint8 or workspace.device != dev
                                       or not workspace.is_contiguous()):
             raise ValueError(f"workspace: expected a contiguous uint8 tensor on {dev}, as new_workspace() makes it")
+        if tree is not None and (tree.device != dev or tree.mask.shape[0] != n):
+            raise ValueError(f"tree: expected masks of {n} tokens on {dev}")
         if n == 0:
             return out
         s = _stream(dev)
         ws = workspace if workspace is not None else _workspace(self._L, dev, s, self.view.head_dim)
-        rc = self._L.kore_cuda_paged_attn_dev(self._view, batch._view, n, self._p[0], self._p[1], plse, self._popts,
-                                              ws.data_ptr(), ws.numel(), self._status, s)
+        if tree is None:
+            rc = self._L.kore_cuda_paged_attn_dev(self._view, batch._view, n, self._p[0], self._p[1], plse, self._popts,
+                                                  ws.data_ptr(), ws.numel(), self._status, s)
+        else:
+            rc = self._L.kore_cuda_paged_tree_attn_dev(self._view, batch._view, n, self._p[0], self._p[1], plse,
+                                                       self._popts, tree._view, ws.data_ptr(), ws.numel(),
+                                                       self._status, s)
         if rc:
             _ck(self._L, rc)
         return out
