@@ -718,7 +718,7 @@ typedef struct kore_cuda_head_norm {
     const void *q_weight, *k_weight;   /* device, head_dim values (a head); NULL: those heads have no norm */
     int type;                          /* KORE_CUDA_F32, _F16 or _BF16 */
     long long q_head_stride, k_head_stride;   /* elements from one head's weights to the next; 0: one weight for all */
-    float eps;                         /* > 0 */
+    float eps;                         /* > 0, a normal number */
 } kore_cuda_head_norm;
 
 /* Stores k and v (as kore_cuda_paged_append_dev, types alike) at slots [n_tok] and

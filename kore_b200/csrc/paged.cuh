@@ -154,6 +154,31 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     }
 }
 
+// two fp32 at once
+__device__ __forceinline__ unsigned long long pk2(float a, float b) {
+    unsigned long long u;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(u) : "f"(a), "f"(b));
+    return u;
+}
+__device__ __forceinline__ void upk2(unsigned long long u, float &a, float &b) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(u));
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
 // A box of a page (tokens from tok on, values from x on) into shared memory; with an L2 policy or
 // without.
 __device__ __forceinline__ void tma_box(uint32_t dst, const TmaDesc *map, int x, int tok, int g, int page, uint64_t *bar) {
@@ -187,7 +212,7 @@ __device__ __forceinline__ float at_least_normal(float factor) { return factor <
 cudaError_t launch_rope_table(const float *freq, int half, double amp, int n_pos, float *table, cudaStream_t s);
 cudaError_t launch_rotate(const RotateParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
 cudaError_t launch_plan(const PlanParams &p, bool trim, cudaStream_t s);
-cudaError_t launch_store(const StoreParams &p, int in_type, int cache_type, bool vec, cudaStream_t s);
+cudaError_t launch_store(const StoreParams &p, int in_type, int cache_type, bool vec, int sms, cudaStream_t s);
 cudaError_t launch_tree_mask(const TreeParams &p, cudaStream_t s);
 cudaError_t launch_accept(const TreeParams &p, cudaStream_t s);
 cudaError_t launch_commit(const CommitParams &p, cudaStream_t s);

@@ -4,6 +4,7 @@
 
 #include "paged_args.cuh"
 
+#include <cfloat>
 #include <cmath>
 
 namespace kore {
@@ -110,7 +111,8 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
         if (!norm->q_weight && !norm->k_weight) return refuse(KORE_CUDA_EINVAL, "norm: no weights");
         if ((reinterpret_cast<uintptr_t>(norm->q_weight) | reinterpret_cast<uintptr_t>(norm->k_weight)) % b)
             return refuse(KORE_CUDA_EINVAL, "norm: the weights are not aligned to their type");
-        if (!(norm->eps > 0) || !std::isfinite(norm->eps)) return refuse(KORE_CUDA_EINVAL, "norm: eps must be positive");
+        if (!(norm->eps >= FLT_MIN) || !std::isfinite(norm->eps))
+            return refuse(KORE_CUDA_EINVAL, "norm: eps must be a positive normal number");
         weights16 = ((reinterpret_cast<uintptr_t>(norm->q_weight) | reinterpret_cast<uintptr_t>(norm->k_weight) |
                       (uintptr_t)(norm->q_head_stride * b) | (uintptr_t)(norm->k_head_stride * b)) & 15) == 0;
     }
@@ -150,9 +152,13 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
         p.eps = norm->eps;
     }
     p.status = dev_status;
-    const bool vec = (d == 32 || d == 64 || d == 128 || d == 256) && rotates_in_vectors(d, rope) && weights16 &&
+    const bool vec = (d == 64 || d == 128 || d == 256) && rotates_in_vectors(d, rope) && weights16 &&
+                     (!norm || norm->type == KORE_CUDA_F32 || norm->type == k->type) &&
                      aligned16(*k) && aligned16(*v) && (!q || (aligned16(*q) && aligned16(*q_out)));
-    return launched(launch_store(p, k->type, cache->type, vec, (cudaStream_t)stream), "paged_store");
+    int sms = 0;
+    if (cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, on.dev))
+        return launched(e, "cudaDeviceGetAttribute");
+    return launched(launch_store(p, k->type, cache->type, vec, sms, (cudaStream_t)stream), "paged_store");
 }
 
 extern "C" int kore_cuda_tree_masks_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, unsigned *mask, int words,

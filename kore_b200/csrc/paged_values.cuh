@@ -67,9 +67,9 @@ __device__ __forceinline__ void store1(T *p, float x, float scale) {
 }
 
 template <typename... Args>
-cudaError_t launch(void (*kernel)(Args...), int blocks, int threads, size_t smem, cudaStream_t s, Args... args) {
+cudaError_t launch(void (*kernel)(Args...), dim3 blocks, int threads, size_t smem, cudaStream_t s, Args... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(blocks);
+    cfg.gridDim = blocks;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;

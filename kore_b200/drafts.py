@@ -135,8 +135,8 @@ class HeadNorm:
                     or w.device != some[0].device or w.dtype not in (torch.float32, torch.float16, torch.bfloat16)):
                 raise ValueError("weights: expected CUDA tensors [head_dim] or [heads][head_dim] of one type (fp32, fp16 "
                                  "or bf16) and device, contiguous in a head")
-        if not 0 < eps < float("inf") or not ctypes.c_float(eps).value:
-            raise ValueError(f"eps = {eps} must be positive in 32 bits")
+        if not 2.0 ** -126 <= eps < 2.0 ** 128:
+            raise ValueError(f"eps = {eps} must be a positive normal number in 32 bits")
         self.q_weight, self.k_weight, self.eps, self.device = q_weight, k_weight, eps, some[0].device
         self._shapes = [None if w is None else (tuple(w.shape)) for w in (q_weight, k_weight)]
         at = [None if w is None else w.data_ptr() for w in (q_weight, k_weight)]
