@@ -216,8 +216,9 @@ cudaError_t launch_store(const StoreParams &p, int in_type, int cache_type, bool
 cudaError_t launch_tree_mask(const TreeParams &p, cudaStream_t s);
 cudaError_t launch_accept(const TreeParams &p, cudaStream_t s);
 cudaError_t launch_commit(const CommitParams &p, cudaStream_t s);
-// n_ctas: SMs of the device, at most kPagedMaxCtas; trees where p.mask is given
+// n_ctas, n_sms: SMs of the device, at most kPagedMaxCtas. Rows: trees where p.mask is given
 cudaError_t launch_paged_rows(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
+cudaError_t launch_paged_tree_tiles(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_sms, cudaStream_t s);
 cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int cache_type, int n_ctas, cudaStream_t s);
 
 // ---------------------------------------------------------------- division of the attention's work
@@ -233,6 +234,10 @@ cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int 
 // CTA needs two slots for partial results, whatever the batch.
 
 constexpr int kUnitCost = 1;
+// Of the trees' 64-key tiles: the change from one unit to the next and the joint of its parts take about as
+// long as these (32 sequences of 16 tokens on up to 8192, 28/4 heads of 128: 73.9 us with 1, 71.4 with 8 and 15;
+// 48 of up to 33 on 3000, 14/2 heads of 64: 36.3, 34.6 and 36.8).
+constexpr int kTreeUnitCost = 8;
 
 constexpr uint32_t FULL_WORD = 0xffffffffu;
 
@@ -299,6 +304,7 @@ __device__ __forceinline__ uint32_t tree_bits(const uint32_t *mask, int words, i
 
 template <int ROWS, int KEYS, bool TREE = false>
 struct Unit {
+    static constexpr int COST = TREE && ROWS == 128 ? kTreeUnitCost : kUnitCost;
     int s, g, b;           // sequence, KV head, block of rows
     Seq q;
     int rows;              // valid rows of the block
@@ -315,7 +321,7 @@ struct Unit {
     }
     // To the next unit; false behind the last one.
     __device__ __forceinline__ bool next(const PagedAttnParams &p) {
-        u0 += kUnitCost + nt;
+        u0 += COST + nt;
         if (++b == blocks(p)) {
             b = 0;
             if (++g == p.G) {
@@ -340,7 +346,7 @@ __device__ __forceinline__ int block_cost(const PagedAttnParams &p, const Seq &q
     u.q = q;
     u.b = b;
     u.range(p);
-    return kUnitCost + u.nt;
+    return u.COST + u.nt;
 }
 
 // A wait ran out: in place of any other code, since it is what makes the workspace unusable.
@@ -391,7 +397,10 @@ __device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, int s0
     if (s0 + lane < p.n_seq) q = load_seq<TREE>(p, s0 + lane, blockIdx.x == 0);
     nb = (q.n * p.rep + ROWS - 1) / ROWS;
     long long cost = nb == 1 ? block_cost<ROWS, KEYS, TREE>(p, q, 0, 1) : 0;
-    for (unsigned many = __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {
+    if constexpr (TREE) {   // every block has the whole sequence's keys
+        if (nb > 1) cost = (long long)nb * block_cost<ROWS, KEYS, TREE>(p, q, 0, 1);
+    }
+    for (unsigned many = TREE ? 0u : __ballot_sync(0xffffffffu, nb > 1); many; many &= many - 1) {
         const int from = __ffs(many) - 1;
         const Seq w{__shfl_sync(0xffffffffu, q.q0, from), __shfl_sync(0xffffffffu, q.n, from),
                     __shfl_sync(0xffffffffu, q.kv, from)};
@@ -466,7 +475,7 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     if (total == 0) return false;
     units *= p.G;
     // (never more CTAs than tiles, so that every share holds one)
-    ctas = (int)min((long long)gridDim.x, total <= (WHOLE + kUnitCost) * units ? units : max(units, quick_div(total, MIN)));
+    ctas = (int)min((long long)gridDim.x, total <= (WHOLE + u.COST) * units ? units : max(units, quick_div(total, MIN)));
     if ((int)blockIdx.x >= ctas) return false;
     x0 = quick_div(total * blockIdx.x, ctas);
     x1 = quick_div(total * (blockIdx.x + 1), ctas);
@@ -496,7 +505,12 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     // the block, a lane each
     u.b = 0;
     const int nb = (u.q.n * p.rep + ROWS - 1) / ROWS;
-    for (int b0 = 0; nb > 1; b0 += 32) {
+    if constexpr (TREE) {
+        const int c = block_cost<ROWS, KEYS, TREE>(p, u.q, 0, 1);
+        u.b = (int)quick_div(x0 - u.u0, c);
+        u.u0 += (long long)u.b * c;
+    }
+    for (int b0 = 0; !TREE && nb > 1; b0 += 32) {
         const int c = block_cost<ROWS, KEYS, TREE>(p, u.q, b0 + lane, nb);
         const int v = warp_scan(c);
         const unsigned in = __ballot_sync(0xffffffffu, u.u0 + v > x0 && c > 0);

@@ -291,11 +291,12 @@ static int attend(const kore_cuda_pages *cache, const kore_cuda_batch *batch, in
                        rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0);
     const bool plain = tiles && cache->type == KORE_CUDA_E4M3;   // widened before it is read as an operand
     // tokens of a box: the largest power of two that divides the page, up to a tile
-    const int most = tiles ? 128 : d * type_bytes(cache->type) == 256 ? 16 : 32;
+    const int most = tiles ? (tree ? 64 : 128) : d * type_bytes(cache->type) == 256 ? 16 : 32;
     p.box = 16;
     while (p.box < most && p.P % (2 * p.box) == 0) p.box *= 2;
     if (!encode_pages(cache->k, cache, p.box, plain, &p.tm_k) || !encode_pages(cache->v, cache, p.box, plain, &p.tm_v))
         return refuse(KORE_CUDA_ECUDA, "the pages' tensor maps could not be encoded");
+    if (tiles && tree) return launched(launch_paged_tree_tiles(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_tree_attn");
     if (tiles) return launched(launch_paged_tiles(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
     return launched(launch_paged_rows(p, d, q->type, cache->type, ctas, (cudaStream_t)stream), "paged_attn");
 }

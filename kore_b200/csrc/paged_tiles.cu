@@ -40,7 +40,7 @@
 // second launch for the joints took 10 to 18.)
 // Every wait is bounded; tensor memory is always released.
 
-#include "paged.cuh"
+#include "paged_mma.cuh"
 
 #include "kore_cuda.h"
 
@@ -49,8 +49,6 @@
 namespace kore {
 namespace {
 
-constexpr unsigned FULL = 0xffffffffu;
-constexpr int kM = 128;             // rows of a tile
 constexpr int kUnitRows = 2 * kM;
 constexpr int kKeys = 128;          // keys of a tile
 constexpr int kStep = 64;           // keys of a step
@@ -79,97 +77,6 @@ struct TilesCfg {
     static_assert(STAGES * TILE >= (kPagedMaxSeqs + 2) * 8, "the sums' place");
 };
 
-// ---------------------------------------------------------------- tcgen05
-
-__device__ __forceinline__ uint32_t sw128(int r, int c) {   // 16-byte piece c of 128-byte row r
-    return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4));
-}
-// Shared-memory matrix descriptors (128-byte swizzle, Blackwell version 1): the low
-// word is the address / 16, the high word and bits 16-29 are the layout's.
-// K-major: groups of 8 rows 1024 bytes apart. MN-major: blocks of 64 columns LBO
-// bytes apart, groups of 8 rows (keys) 1024 bytes apart.
-constexpr uint32_t kDescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ uint32_t desc_k(uint32_t a) { return ((a >> 4) & 0x3FFF) | (1u << 16); }
-__device__ __forceinline__ uint32_t desc_mn(uint32_t a, uint32_t lbo) { return ((a >> 4) & 0x3FFF) | ((lbo >> 4) << 16); }
-// f16 (0) or bf16 (1) operands of one type, fp32 sums; B K-major or MN-major
-__host__ __device__ constexpr uint32_t idesc(bool bf, bool b_mn, int N) {
-    return (1u << 4) | ((bf ? 1u : 0u) << 7) | ((bf ? 1u : 0u) << 10) | ((b_mn ? 1u : 0u) << 16) |
-           ((uint32_t)(N >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
-}
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// The issuing thread's time is what counts here: an MMA's operands are uniform
-// registers, so the low words come from a warp-wide reduction (whose result is one) and
-// all else is constant.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_max_sync(0xffffffffu, v); }
-// The lane that issues the products also commits them: a commit follows its own thread's
-// operations only, and which lane is elected is not said (for one mask it is always the same).
-__device__ __forceinline__ bool elect() {
-    uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
-    return ok != 0;
-}
-template <uint32_t ID, bool ACC>
-__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(ID), "n"(ACC ? 1 : 0),
-                 "n"(kDescHi)
-                 : "memory");
-}
-template <uint32_t ID>
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t acc) {
-    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 y, {%2, %5};\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "n"(ID), "r"(acc),
-                 "n"(kDescHi)
-                 : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-// 32 columns of this thread's row
-__device__ __forceinline__ void ld32(uint32_t a, uint32_t *r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(a));
-}
-__device__ __forceinline__ void st32(uint32_t a, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(a),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void st16(uint32_t a, const uint32_t *r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(a),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-    return r;
-}
-__device__ __forceinline__ uint32_t ld_acquire(const uint32_t *p) {
-    uint32_t v;
-    asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(v) : "r"(smem_u32(p)) : "memory");
-    return v;
-}
-__device__ __forceinline__ void st_release(uint32_t *p, uint32_t v) {
-    asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(p)), "r"(v) : "memory");
-}
 // ---------------------------------------------------------------- parts of a cut unit
 //
 // CTA c has two slots: slot 0 for the unit it goes on with, slot 1 for the one
@@ -179,24 +86,12 @@ __device__ __forceinline__ void st_release(uint32_t *p, uint32_t v) {
 template <int D>
 constexpr size_t kSlot = (size_t)kUnitRows * (D + 2);
 
-// What some row of the unit, a block of a tree's rows, sees of the keys from x on (counted as for
-// tree_bits); by a whole warp.
-template <int ROWS, int KEYS>
-__device__ __forceinline__ uint32_t seen_by_some(const PagedAttnParams &p, const Unit<ROWS, KEYS, true> &u, int x) {
-    const int t0 = p.by_rep.div(u.b * ROWS), t1 = p.by_rep.div(u.b * ROWS + u.rows - 1);
-    uint32_t bits = 0;
-    for (int t = t0 + (threadIdx.x & 31); t <= t1; t += 32)
-        bits |= tree_bits(p.mask + (long long)(u.q.q0 + t) * p.words, p.words, x, u.q.n);
-    return __reduce_or_sync(FULL, bits);
-}
-
-// QBF: queries and outputs in bf16, else f16. E8: 8-bit cache, products in f16. TREE: the chunks
-// are trees of drafted tokens.
-template <int D, bool QBF, bool E8, bool TREE>
+// QBF: queries and outputs in bf16, else f16. E8: 8-bit cache, products in f16.
+template <int D, bool QBF, bool E8>
 __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kernel(const __grid_constant__ PagedAttnParams p) {
     using C = TilesCfg<D, E8>;
     constexpr bool BF = QBF && !E8;   // type of the products
-    using U = Unit<kUnitRows, kKeys, TREE>;
+    using U = Unit<kUnitRows, kKeys>;
     using qt = typename std::conditional<QBF, __nv_bfloat16, __half>::type;
     extern __shared__ uint8_t smem_raw[];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -231,7 +126,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     U u;
     long long total, x0, x1;
     int ctas;
-    if (!find_share<kUnitRows, kKeys, 4, 3, TREE>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
+    if (!find_share<kUnitRows, kKeys, 4, 3, false>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::LOADS; ++i) mbar_init(&full[i], 1);
@@ -485,23 +380,10 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                 for (int kv = 0; ok && kv < 2; ++kv, ++it) {
                     ok = wait(&full[it % C::STAGES], (it / C::STAGES) & 1, true);
                     const int key0 = (u.tile0 + t) * kKeys;
-                    const int first = u.q.kv - u.q.n;   // TREE: the chunk's first key
-                    if (ok && kv == 1 && (TREE ? key0 + kKeys > first : key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
+                    if (ok && kv == 1 && (key0 < u.lo || key0 + kKeys > u.hi)) {   // V's rows outside the unit's keys
                         uint8_t *v = smem + C::RING + (it % C::STAGES) * C::TILE;
-                        uint32_t some[kKeys / 32];
-                        if constexpr (TREE) {
-#pragma unroll
-                            for (int x = 0; x < kKeys / 32; ++x) some[x] = seen_by_some(p, u, key0 + 32 * x - first);
-                        }
-                        auto outside = [&](int r) {
-                            if constexpr (TREE) {
-                                const uint32_t a = r & 32 ? some[1] : some[0], b = r & 32 ? some[3] : some[2];
-                                return !((r & 64 ? b : a) >> (r & 31) & 1);
-                            }
-                            return key0 + r < u.lo || key0 + r >= u.hi;
-                        };
                         for (int r = lane >> 3; r < kKeys; r += 4)
-                            if (outside(r))
+                            if (key0 + r < u.lo || key0 + r >= u.hi)
                                 for (int h = 0; h < C::HALVES; ++h)
                                     *reinterpret_cast<uint4 *>(v + h * C::BLOCK + r * 128 + (lane & 7) * 16) =
                                         make_uint4(0, 0, 0, 0);
@@ -530,19 +412,13 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     ok = wait(&full[it % C::RAW_STAGES], (it / C::RAW_STAGES) & 1, true);
                     if (ok && it >= C::STAGES) ok = wait(&empty[it % C::STAGES], (it / C::STAGES - 1) & 1);
                     if (!ok) break;
-                    // TREE: which of this warp's 32 keys any row of the unit sees
-                    uint32_t some = ~0u;
-                    const int first = u.q.kv - u.q.n;
-                    if constexpr (TREE) {
-                        if (kv == 1 && key0 + kKeys > first) some = seen_by_some(p, u, key0 + 32 * w - first);
-                    }
                     const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 32 * D + lane * 16;
                     uint8_t *dst = smem + C::RING + (it % C::STAGES) * C::TILE + (c >> 2) * C::BLOCK;
 #pragma unroll 4
                     for (int x = 0; x < L; ++x) {
                         const int row = w * 32 + x * (32 / L) + lane / L;
                         uint4 v = *reinterpret_cast<const uint4 *>(src + x * 512);
-                        if (kv == 1 && (TREE ? !(some >> (row & 31) & 1) : key0 + row < u.lo || key0 + row >= u.hi)) v = make_uint4(0, 0, 0, 0);   // of V
+                        if (kv == 1 && (key0 + row < u.lo || key0 + row >= u.hi)) v = make_uint4(0, 0, 0, 0);   // of V
                         uint4 a, b;
                         widen4(v.x, a.x, a.y);
                         widen4(v.y, a.z, a.w);
@@ -688,16 +564,12 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
             const bool in = i * kM + r < u.rows;
             const int pr = u.b * kUnitRows + i * kM + r;
             int lo = 0, hi = 0, all_lo = 0, all_hi = 0;
-            const uint32_t *mask = nullptr;   // TREE: this row's
-            if constexpr (TREE) {
-                all_hi = u.q.kv - u.q.n;
-                mask = p.mask + (long long)(u.q.q0 + p.by_rep.div(in ? pr : 0)) * p.words;
-            } else if (mine) {
-                if (in) key_range<TREE>(p, u.q, pr, pr + 1, lo, hi);
+            if (mine) {
+                if (in) key_range<false>(p, u.q, pr, pr + 1, lo, hi);
                 const int b0 = u.b * kUnitRows + i * kM, b1 = u.b * kUnitRows + min(u.rows, (i + 1) * kM);
                 int x;
-                key_range<TREE>(p, u.q, b0, b0 + 1, x, all_hi);
-                key_range<TREE>(p, u.q, b1 - 1, b1, all_lo, x);
+                key_range<false>(p, u.q, b0, b0 + 1, x, all_hi);
+                key_range<false>(p, u.q, b1 - 1, b1, all_lo, x);
             }
             float qs = qs_all;
             if constexpr (E8 && QBF) qs *= q_shift[i * kM + r];
@@ -721,13 +593,7 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
                     ld32(tb + 32, reinterpret_cast<uint32_t *>(s) + 32);
                     wait_ld();
                     const int key0 = k * kStep;
-                    if (TREE && key0 + kStep > all_hi) {
-                        const uint32_t see[2] = {in ? tree_bits(mask, p.words, key0 - all_hi, u.q.n) : 0u,
-                                                 in ? tree_bits(mask, p.words, key0 + 32 - all_hi, u.q.n) : 0u};
-#pragma unroll
-                        for (int x = 0; x < 64; ++x)
-                            if (!(see[x >> 5] >> (x & 31) & 1)) s[x] = -INFINITY;
-                    } else if (!TREE && (key0 < all_lo || key0 + kStep > all_hi)) {
+                    if (key0 < all_lo || key0 + kStep > all_hi) {
 #pragma unroll
                         for (int x = 0; x < 64; ++x)
                             if (key0 + x < lo || key0 + x >= hi) s[x] = -INFINITY;
@@ -950,10 +816,10 @@ __global__ void __launch_bounds__(TilesCfg<D, E8>::THREADS, 1) paged_tiles_kerne
     }
 }
 
-template <int D, bool QBF, bool E8, bool TREE>
-cudaError_t launch_t(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
+template <int D, bool QBF, bool E8>
+cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     using C = TilesCfg<D, E8>;
-    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, QBF, E8, TREE>), C::BYTES)) return e;
+    if (cudaError_t e = ensure_smem_limit(reinterpret_cast<const void *>(paged_tiles_kernel<D, QBF, E8>), C::BYTES)) return e;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -964,12 +830,7 @@ cudaError_t launch_t(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QBF, E8, TREE>, p);
-}
-
-template <int D, bool QBF, bool E8>
-cudaError_t launch_k(const PagedAttnParams &p, int n_ctas, cudaStream_t s) {
-    return p.mask ? launch_t<D, QBF, E8, true>(p, n_ctas, s) : launch_t<D, QBF, E8, false>(p, n_ctas, s);
+    return cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QBF, E8>, p);
 }
 
 }  // namespace
