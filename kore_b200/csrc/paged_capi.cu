@@ -46,6 +46,31 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, bool plai
     return true;
 }
 
+// Whether a batch of trees goes to the 128-row kernel on the tensor cores, or to the one of 16 rows. What each
+// would take, in us, from what they were measured to take on a B200: the row kernel its start, and for each
+// unit of 16 rows an SM works on a time of its own and one for every 128 keys; the tile kernel its start, a
+// time for every 64 keys (and 8 more of them a unit) of a CTA's share, and a joint for each doubling of the CTAs that
+// share a unit. Row against tile kernel, 28/4 heads of 128, 16 bits: 8 tokens on 520 positions 11 / 16; 16
+// on 16000 41 / 43; 16 x 8 on 1008 33 / 26; 16 x 24 on 324 42 / 15; 16 x 8 on 8008 161 / 68; 48 x 2 on 1002 31 /
+// 40; 64 x 32 on 1532 415 / 94. 8 bits: 16 x 4 on 4004 41 / 50; 64 x 24 on 124 132 / 41. 14/2 heads of 64:
+// 64 on 1064 11 / 16; 64 on 30064 58 / 41. Over 144 batches of three head layouts the choice takes 0.6 % more than the
+// better kernel of each, 21 % at worst.
+bool trees_in_tiles(int d, bool e8, int G, int rep, int n_seq, int n_tok, double kv, int sms) {
+    struct Cost {
+        double unit, pass, start, tile, joint;
+    };
+    const Cost c = d == 128 ? e8 ? Cost{5.0, 0.72, 11.0, 1.6, 5.0} : Cost{3.5, 1.05, 9.5, 1.3, 5.0}
+                            : e8 ? Cost{3.6, 0.55, 9.5, 1.2, 4.5} : Cost{3.0, 0.5, 8.5, 1.05, 4.5};
+    const double packed = (double)n_tok * rep, half = 0.5 * n_seq;
+    const double units16 = G * std::fmax(n_seq, packed / 16 + half), units = G * std::fmax(n_seq, packed / 128 + half);
+    const double rows = 7 + std::fmax(4, units16 / sms * (c.unit + kv / 128 * c.pass));
+    const double tiles = kv / 64, total = units * (tiles + kTreeUnitCost), ctas = 2.0 * sms;
+    // (as find_share divides them: short units are not cut)
+    const double used = tiles <= 8 || units >= ctas ? std::fmin(units, ctas) : std::fmin(ctas, std::fmax(units, total / 6));
+    const double share = used <= units && units <= ctas ? tiles : total / used;
+    return c.start + share * c.tile + c.joint * std::log2(std::fmax(1, used / units)) < rows;
+}
+
 }  // namespace
 }  // namespace kore
 
@@ -288,7 +313,9 @@ static int attend(const kore_cuda_pages *cache, const kore_cuda_batch *batch, in
     const double rows16 = (double)p.G * ((double)n_tok * p.rep / 16 + p.n_seq);
     const double passes = (batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P) / 128 + 3;
     const bool tiles = (long long)batch->max_q * p.rep > 16 &&
-                       rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0);
+                       (tree ? trees_in_tiles(d, cache->type == KORE_CUDA_E4M3, G, p.rep, p.n_seq, n_tok,
+                                              batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P, ctas)
+                             : rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0));
     const bool plain = tiles && cache->type == KORE_CUDA_E4M3;   // widened before it is read as an operand
     // tokens of a box: the largest power of two that divides the page, up to a tile
     const int most = tiles ? (tree ? 64 : 128) : d * type_bytes(cache->type) == 256 ? 16 : 32;

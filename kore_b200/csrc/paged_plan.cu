@@ -21,27 +21,37 @@ namespace kore {
 namespace {
 
 constexpr unsigned FULL = 0xffffffffu;
+#ifndef PLT
+#define PLT 1024
+#endif
+#ifndef PLN
+#define PLN 16
+#endif
+#ifndef PLC
+#define PLC 8
+#endif
 
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Inclusive sums of a and b over the block, on top of what came before (run_a, run_b: updated).
-__device__ __forceinline__ void block_scan(long long &a, long long (&part)[33], long long &run) {
+__device__ __forceinline__ void block_scan(long long &a, long long &b, longlong2 (&part)[33], long long &run_a, long long &run_b) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     a = warp_scan(a);
-    if (lane == 31) part[warp] = a;
+    b = warp_scan(b);
+    if (lane == 31) part[warp + 1] = make_longlong2(a, b);
     __syncthreads();
-    if (warp == 0) {
-        const long long w = warp_scan(lane < warps ? part[lane] : 0ll);
-        __syncwarp();
-        part[lane + 1] = w;
-        if (lane == 0) part[0] = 0;
-    }
-    __syncthreads();
-    a += run + part[warp];
-    run += part[warps];
-    __syncthreads();   // part may be written again
+    // (every warp sums up the warps' totals for itself)
+    longlong2 w = lane < warps ? part[lane + 1] : make_longlong2(0, 0);
+    w.x = warp_scan(w.x);
+    w.y = warp_scan(w.y);
+    const int from = warp ? warp - 1 : 0;
+    const long long xa = __shfl_sync(FULL, w.x, from), xb = __shfl_sync(FULL, w.y, from);
+    a += run_a + (warp ? xa : 0);
+    b += run_b + (warp ? xb : 0);
+    run_a += __shfl_sync(FULL, w.x, 31);
+    run_b += __shfl_sync(FULL, w.y, 31);
 }
 
 // ceil(n / P) for 0 <= n
@@ -53,7 +63,7 @@ __device__ __forceinline__ int pages_of(const PlanParams &p, int n) {
 template <bool TRIM>
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanParams p) {
     extern __shared__ int smem[];
-    __shared__ long long part[33];
+    __shared__ longlong2 part[33];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int words = (p.n_requests + 31) / 32;
     // requests named by the batch, and those named twice
@@ -66,15 +76,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
     __syncthreads();
     grid_dep_wait();
     grid_dep_launch();
-    for (int s = tid; s < p.n_seq; s += blockDim.x) {
-        const int r = __ldg(p.request + s);
-        if (r >= 0 && r < p.n_requests && (atomicOr(seen + (r >> 5), 1u << (r & 31)) >> (r & 31) & 1))
-            atomicOr(twice + (r >> 5), 1u << (r & 31));
-    }
+    // the first sequences' requests, and what is known of them, are on their way before anything else
+    const long long cap = min((long long)p.stride * p.P, 0x7fffffffll);
+    auto known = [&](int r) { return r >= 0 && r < p.n_requests; };
     const int listed = *p.n_free;
+    int r = tid < p.n_seq ? __ldg(p.request + tid) : -1, a = tid < p.n_seq ? __ldg(p.amount + tid) : 0;
+    int len = known(r) ? p.length[r] : 0;
+    auto mark = [&](int x) {
+        if (known(x) && (atomicOr(seen + (x >> 5), 1u << (x & 31)) >> (x & 31) & 1)) atomicOr(twice + (x >> 5), 1u << (x & 31));
+    };
+    mark(r);
+    for (int s = tid + blockDim.x; s < p.n_seq; s += blockDim.x) mark(__ldg(p.request + s));
     const bool list_ok = listed >= 0 && listed <= p.n_pages;
     const int n_free = list_ok ? listed : 0;
-    const long long cap = min((long long)p.stride * p.P, 0x7fffffffll);
     const bool report = blockIdx.x == 0;
     if (report && tid == 0 && !list_ok) raise_error(p.status, DEV_BAD_SEQUENCE);
     __syncthreads();
@@ -82,27 +96,27 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
     long long rows_run = 0, pages_run = 0;
     for (int s0 = 0; s0 < p.n_seq; s0 += blockDim.x) {
         const int s = s0 + tid;
-        int r = s < p.n_seq ? __ldg(p.request + s) : -1, code = 0, a = 0, len = 0;
-        const bool asked = r >= 0;
-        if (asked) {
-            a = __ldg(p.amount + s);
-            if (r >= p.n_requests || (twice[r >> 5] >> (r & 31) & 1)) code = DEV_BAD_SEQUENCE;
-            else if ((len = p.length[r]) < 0 || len > cap) code = DEV_BAD_SEQUENCE;
-            if (a < 0) {
-                code = DEV_BAD_SEQUENCE;
-                a = 0;
-            }
+        if (s0 > 0) {
+            r = s < p.n_seq ? __ldg(p.request + s) : -1;
+            a = s < p.n_seq ? __ldg(p.amount + s) : 0;
+            len = known(r) ? p.length[r] : 0;
+            __syncthreads();   // part may be written again
         }
+        const bool asked = r >= 0;
+        int code = 0;
+        if (!asked) a = 0;
+        if (asked && (!known(r) || (twice[r >> 5] >> (r & 31) & 1) || len < 0 || len > cap || a < 0)) code = DEV_BAD_SEQUENCE;
+        if (a < 0) a = 0;
         if constexpr (!TRIM) {
-            long long rows = a, need = 0;
-            block_scan(rows, part, rows_run);
-            if (asked && !code && (rows > p.n_tok || (long long)len + a > cap)) code = DEV_BAD_SEQUENCE;
+            // Sums of rows and of pages at once: the pages of sequences whose rows do not fit count too, but behind the
+            // first of these no sequence has rows that do.
+            if (asked && !code && (long long)len + a > cap) code = DEV_BAD_SEQUENCE;
             const int have = code ? 0 : pages_of(p, len);
-            if (asked && !code) need = pages_of(p, len + a) - have;
-            const bool wants = need > 0;
-            const long long mine = need;
-            block_scan(need, part, pages_run);
-            if (wants && need > n_free) code = DEV_NO_PAGES;
+            const long long mine = asked && !code ? pages_of(p, len + a) - have : 0;
+            long long rows = a, need = mine;
+            block_scan(rows, need, part, rows_run, pages_run);
+            if (asked && !code && rows > p.n_tok) code = DEV_BAD_SEQUENCE;
+            if (!code && mine > 0 && need > n_free) code = DEV_NO_PAGES;
             if (s < p.n_seq) {
                 end[s] = (int)min(rows, 0x7fffffffll);
                 base[s] = len;
@@ -110,15 +124,16 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
                 who[s] = code ? -1 : r;
             }
         } else {
-            long long gone = 0;
-            if (asked && !code && a < len) gone = pages_of(p, len) - pages_of(p, a);
-            const long long mine = gone;
-            block_scan(gone, part, pages_run);
+            const bool cut = asked && !code && a < len;
+            const int stay = cut ? pages_of(p, a) : 0;
+            const long long mine = cut ? pages_of(p, len) - stay : 0;
+            long long gone = mine, unused = 0;
+            block_scan(gone, unused, part, pages_run, rows_run);
             if (s < p.n_seq) {
                 end[s] = (int)min(gone, 0x7fffffffll);
-                base[s] = asked && !code && a < len ? pages_of(p, a) : 0;
+                base[s] = stay;
                 first[s] = (int)mine;
-                who[s] = asked && !code && a < len ? r : -1;
+                who[s] = cut ? r : -1;
             }
         }
         if (code && report) raise_error(p.status, code);
@@ -126,22 +141,36 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
     __syncthreads();
 
     const int warps = gridDim.x * (blockDim.x >> 5), w = blockIdx.x * (blockDim.x >> 5) + warp;
+    // a warp some of a sequence's pages, four of them a lane on their way at once
+    const int split = p.n_seq ? max(1, min(32, warps / p.n_seq)) : 1;
+    constexpr int N = 4;
     if constexpr (TRIM) {
         const bool fits = list_ok && pages_run <= p.n_pages - n_free;   // (else a page was given back that none held)
         if (!fits && report && tid == 0) raise_error(p.status, DEV_BAD_SEQUENCE);
         if (fits) {
             const int top = n_free + (int)pages_run - 1;
-            for (int s = w; s < p.n_seq; s += warps) {
+            for (int x = w; x < p.n_seq * split; x += warps) {
+                const int s = x / split;
                 if (who[s] < 0) continue;
                 int *row = p.table + (long long)who[s] * p.stride + base[s];
                 const int n = first[s], at = end[s] - n;
-                for (int j = lane; j < n; j += 32) {
-                    p.free_pages[top - at - j] = row[j];
-                    row[j] = -1;
+                for (int j = (x - s * split) * 32 + lane; j < n; j += 32 * split * N) {
+                    int page[N];
+#pragma unroll
+                    for (int k = 0; k < N; ++k)
+                        if (j + k * 32 * split < n) page[k] = row[j + k * 32 * split];
+#pragma unroll
+                    for (int k = 0; k < N; ++k) {
+                        const int i = j + k * 32 * split;
+                        if (i >= n) continue;
+                        p.free_pages[top - at - i] = page[k];
+                        row[i] = -1;
+                    }
                 }
             }
         }
-        cluster_barrier();   // every CTA has read the state
+        if (gridDim.x > 1) cluster_barrier();   // every CTA has read the state
+        else __syncthreads();
         if (blockIdx.x != 0 || !fits) return;
         for (int s = tid; s < p.n_seq; s += blockDim.x)
             if (who[s] >= 0) p.length[who[s]] = __ldg(p.amount + s);
@@ -151,17 +180,24 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
         auto page_of = [&](int s, int have, int j) -> int {
             return j < have ? p.table[(long long)who[s] * p.stride + j] : p.free_pages[n_free - 1 - (first[s] + j)];
         };
-        // tables: a warp some of a sequence's pages
-        const int split = max(1, min(8, warps / max(1, p.n_seq)));
+        // tables
         for (int x = w; x < p.n_seq * split; x += warps) {
             const int s = x / split;
             if (who[s] < 0) continue;
             const int have = pages_of(p, base[s]), want = pages_of(p, base[s] + end[s] - (s ? end[s - 1] : 0));
             int *out = p.page_table + (long long)s * p.out_stride, *row = p.table + (long long)who[s] * p.stride;
-            for (int j = (x - s * split) * 32 + lane; j < want; j += 32 * split) {
-                const int page = page_of(s, have, j);
-                out[j] = page;
-                if (j >= have) row[j] = page;
+            for (int j = (x - s * split) * 32 + lane; j < want; j += 32 * split * N) {
+                int page[N];
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    if (j + k * 32 * split < want) page[k] = page_of(s, have, j + k * 32 * split);
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int i = j + k * 32 * split;
+                    if (i >= want) continue;
+                    out[i] = page[k];
+                    if (i >= have) row[i] = page[k];
+                }
             }
         }
         // tokens: a warp a run of them
@@ -175,25 +211,35 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
                 else b = m;
             }
             const int t1 = (int)min((long long)p.n_tok, t0 + each);
-            for (int t = (int)t0 + lane; t < t1; t += 32) {
-                while (s < p.n_seq && end[s] <= t) ++s;
-                long long slot = -1;
-                int pos = -1;
-                if (s < p.n_seq && who[s] >= 0) {
-                    pos = base[s] + t - (s ? end[s - 1] : 0);
-                    const int j = p.by_page.div(pos);
-                    slot = (long long)page_of(s, pages_of(p, base[s]), j) * p.P + p.by_page.mod(pos, j);
+            for (int t = (int)t0 + lane; t < t1; t += 32 * N) {
+                int pos[N], page[N], in[N];   // (in: place in the page)
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int x = t + 32 * k;
+                    pos[k] = -1;
+                    if (x >= t1) continue;
+                    while (s < p.n_seq && end[s] <= x) ++s;
+                    if (s >= p.n_seq || who[s] < 0) continue;
+                    pos[k] = base[s] + x - (s ? end[s - 1] : 0);
+                    const int j = p.by_page.div(pos[k]);
+                    in[k] = p.by_page.mod(pos[k], j);
+                    page[k] = page_of(s, pages_of(p, base[s]), j);
                 }
-                p.slots[t] = slot;
-                p.pos[t] = pos;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const int x = t + 32 * k;
+                    if (x >= t1) continue;
+                    p.slots[x] = pos[k] < 0 ? -1ll : (long long)page[k] * p.P + in[k];
+                    p.pos[x] = pos[k];
+                }
             }
         }
-        cluster_barrier();   // every CTA has read the state
+        if (gridDim.x > 1) cluster_barrier();   // every CTA has read the state
+        else __syncthreads();
         if (blockIdx.x != 0) return;
         long long taken = 0;
         for (int s = tid; s < p.n_seq; s += blockDim.x) {
             const int from = s ? end[s - 1] : 0;
-            if (s == 0) p.q_start[0] = 0;
             p.q_start[s + 1] = end[s];
             const int kv = base[s] + end[s] - from;
             p.kv_len[s] = who[s] >= 0 ? kv : 0;
@@ -205,10 +251,11 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
         }
         // (those that get pages are the first ones of those that want some)
         taken = __reduce_max_sync(FULL, (int)taken);
-        if (lane == 0) part[warp] = taken;
+        if (lane == 0) part[warp].x = taken;
         __syncthreads();
         if (tid == 0) {
-            for (int i = 1; i < (int)(blockDim.x >> 5); ++i) taken = max(taken, part[i]);
+            for (int i = 1; i < (int)(blockDim.x >> 5); ++i) taken = max(taken, part[i].x);
+            p.q_start[0] = 0;
             if (list_ok) *p.n_free = n_free - (int)taken;
         }
     }
@@ -239,11 +286,10 @@ cudaError_t launch_p(const PlanParams &p, int ctas, int threads, cudaStream_t s)
 }  // namespace
 
 cudaError_t launch_plan(const PlanParams &p, bool trim, cudaStream_t s) {
-    // small batches: one CTA of as many threads as sequences or tokens; else a cluster
+    // small batches: one CTA; else a cluster
     const int n = p.n_tok > p.n_seq ? p.n_tok : p.n_seq;
-    int threads = 128;
-    while (threads < 1024 && threads < n) threads *= 2;
-    const int ctas = n > 1024 ? 8 : 1;
+    const int threads = PLT;
+    const int ctas = n > PLN ? PLC : 1;
     return trim ? launch_p<true>(p, ctas, threads, s) : launch_p<false>(p, ctas, threads, s);
 }
 
