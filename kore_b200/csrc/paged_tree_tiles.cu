@@ -709,11 +709,10 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     } else if constexpr (E8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         // ------------------------------------------------------------ widening
-        // 16 rows a warp: 16 bytes of a row a lane become two 16-byte pieces of f16 (exact)
-        // in the layout that the MMA reads. The lanes of a row's second half (d = 128) write
-        // theirs in the other order, so that a row's 8 writes lie in distinct banks.
-        constexpr int L = D / 16;   // lanes a row
-        const int w = warp - 8, c = lane % L;
+        // 16 rows a warp: 8 bytes of a row a lane become one 16-byte piece of f16 (exact) in the
+        // layout that the MMA reads (8 lanes write a row's 128 bytes: no bank twice).
+        constexpr int L = D / 8, R = 32 / L;   // lanes a row, rows at a time
+        const int w = warp - 8, c = lane % L, hi = lane / L;
         uint32_t it = 0;
         bool ok = true;
         do {
@@ -726,21 +725,22 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
                 const int key0 = (u.tile0 + t) * kKeys;
                 uint32_t some = ~0u;   // which of this warp's keys any row of the unit sees
                 if (v && key0 + kKeys > first) some = seen_by_some(p, u, key0 + 16 * w - first);
-                const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 16 * D + lane * 16;
-                uint8_t *dst = smem + C::RING + (it % C::STAGES) * C::TILE + (c >> 2) * C::BLOCK;
+                const uint8_t *src = smem + C::RAW + (it % C::RAW_STAGES) * C::RAW_TILE + w * 16 * D + lane * 8;
+                uint8_t *dst = smem + C::RING + (it % C::STAGES) * C::TILE + (c >> 3) * C::BLOCK + (w * 16 + hi) * 128;
+                uint2 y[16 / R];
 #pragma unroll
-                for (int x = 0; x < L / 2; ++x) {
-                    const int r = x * (32 / L) + lane / L, row = w * 16 + r;
-                    uint4 y = *reinterpret_cast<const uint4 *>(src + x * 512);
-                    if (!(some >> r & 1)) y = make_uint4(0, 0, 0, 0);
-                    uint4 a, b;
-                    widen4(y.x, a.x, a.y);
-                    widen4(y.y, a.z, a.w);
-                    widen4(y.z, b.x, b.y);
-                    widen4(y.w, b.z, b.w);
-                    const bool swap = (c & 4) != 0;
-                    *reinterpret_cast<uint4 *>(dst + sw128(row, 2 * (c & 3) + swap)) = swap ? b : a;
-                    *reinterpret_cast<uint4 *>(dst + sw128(row, 2 * (c & 3) + !swap)) = swap ? a : b;
+                for (int x = 0; x < 16 / R; ++x) y[x] = *reinterpret_cast<const uint2 *>(src + x * 256);
+                if (some != ~0u) {
+#pragma unroll
+                    for (int x = 0; x < 16 / R; ++x)
+                        if (!(some >> (x * R + hi) & 1)) y[x] = make_uint2(0, 0);
+                }
+#pragma unroll
+                for (int x = 0; x < 16 / R; ++x) {
+                    uint4 a;
+                    widen4(y[x].x, a.x, a.y);
+                    widen4(y[x].y, a.z, a.w);
+                    *reinterpret_cast<uint4 *>(dst + x * R * 128 + (((c & 7) ^ ((x * R + hi) & 7)) << 4)) = a;
                 }
                 fence_proxy_async_smem();
                 __syncwarp();

@@ -132,15 +132,15 @@ def _ck(L, rc: int) -> None:
         raise KoreCudaError(rc, L.kore_cuda_last_error(None).decode())
 
 
-_torch = None
+_torch = _int32 = _int64 = None
 _types: dict = {}
 
 
 def _import_torch():
-    global _torch
+    global _torch, _int32, _int64
     if _torch is None:
         import torch
-        _torch = torch
+        _torch, _int32, _int64 = torch, torch.int32, torch.int64
         _types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3})
     return _torch
 
@@ -176,7 +176,7 @@ def _fill(r: _Rows, t, what: str, device) -> int:
 
 
 def _ints(t, what: str, device, shape_len: int):
-    if t.dtype != _torch.int32 or t.dim() != shape_len or not t.is_contiguous() or t.device != device:
+    if t.dtype is not _int32 or t.ndim != shape_len or not t.is_contiguous() or t.get_device() != device.index:
         raise ValueError(f"{what}: expected a contiguous {shape_len}-d int32 tensor on {device}")
     return t.data_ptr()
 
@@ -362,8 +362,8 @@ class PagedCache:
         n = _fill(r[0], k, "k", dev)
         if _fill(r[1], v, "v", dev) != n:
             raise ValueError("k and v have different numbers of tokens")
-        if (slots.dtype != _torch.int64 or slots.dim() != 1 or slots.shape[0] != n or not slots.is_contiguous()
-                or slots.device != dev):
+        if (slots.dtype is not _int64 or slots.ndim != 1 or slots.shape[0] != n or not slots.is_contiguous()
+                or slots.get_device() != dev.index):
             raise ValueError(f"slots: expected {n} contiguous int64 values on {dev}")
         pq = pqo = pp = pr = pn = None
         if (q is None) != (q_out is None):
