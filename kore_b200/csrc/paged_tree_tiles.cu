@@ -35,15 +35,18 @@ constexpr float kSlack = 8.0f;      // log2 slack before the reference maximum m
 static_assert(kCtas * kM <= kPagedRowsMax, "workspace slots");
 static_assert(kCtas * kPagedMaxCtas * sizeof(int) / 2 <= kPagedZeroed, "two CTAs' counters in a word");
 
+// Ring depths: HBM is as busy with 3 to 5 stages of 16 bits (d = 128: 70.5, 71.0 and 71.9 us for 32 sequences of 16
+// tokens on up to 8192), with 3 or 4 of 8 bits (119.8, 122.0 for 6 of up to 60 on 32768); what is more in flight
+// only waits longer, and the other loads with it.
 template <int D, bool E8>
 struct TreeCfg {
     static constexpr int HALVES = D / 64;                    // 128-byte wide column blocks
     static constexpr uint32_t BLOCK = kKeys * 128;           // bytes of one such block of a tile
     static constexpr uint32_t TILE = HALVES * BLOCK;         // K or V tile
-    static constexpr int STAGES = E8 ? (D == 128 ? 3 : 6) : D == 128 ? 5 : 8;
+    static constexpr int STAGES = E8 ? (D == 128 ? 3 : 6) : D == 128 ? 4 : 6;
     static constexpr int THREADS = E8 ? 384 : 256;           // 80 or 128 registers a thread
     static constexpr uint32_t RAW_TILE = kKeys * D;          // 8-bit K or V tile
-    static constexpr int RAW_STAGES = D == 128 ? 4 : 8;
+    static constexpr int RAW_STAGES = D == 128 ? 3 : 8;
     static constexpr int LOADS = E8 ? RAW_STAGES : STAGES;   // stages that the copies fill
     static constexpr uint32_t RING = HALVES * kM * 128;      // behind q: [HALVES][kM rows][128 B]
     static constexpr uint32_t RAW = RING + STAGES * TILE;
