@@ -219,3 +219,28 @@ def test_python_objects_refuse_what_does_not_fit(fake):  # noqa: F811
     for kw in (dict(tree=tree), dict(tree=K.TokenTree(8, 5, device="cuda:1"))):
         with pytest.raises(ValueError, match="tree"):
             cache.attend(step, q[:8], cuda(8, 4, 64), **kw)
+
+
+def test_products_and_their_commits_are_one_threads():
+    """As tests/test_paged_sources_cpu.py says of the chunks' kernel: a commit follows the operations that its own thread
+    issued, so every product and every commit of the trees' stands under elect()."""
+    import os
+    import re
+    from kore_b200.build import CSRC
+    with open(os.path.join(CSRC, "paged_tree_tiles.cu")) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    calls = [m.start() for m in re.finditer(r"\b(?:commit|mma_ss<[^>]*>|mma_ts<[^>]*>)\(", text)]
+    assert len(calls) >= 9
+    covered = []
+    for g in re.finditer(r"if \(elect\(\)\)\s*", text):
+        if text[g.end()] != "{":
+            covered.append((g.end(), text.index(";", g.end())))
+            continue
+        depth, end = 0, g.end()
+        while True:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            if depth == 0:
+                break
+            end += 1
+        covered.append((g.end(), end))
+    assert all(any(a <= c < b for a, b in covered) for c in calls)
