@@ -723,7 +723,7 @@ typedef struct kore_cuda_head_norm {
 
 /* Stores k and v (as kore_cuda_paged_append_dev, types alike) at slots [n_tok] and
  * rotates q into q_out; k and q are normed by `norm` (NULL: not) before the rotation at
- * pos [n_tok] (`rope` and pos may both be NULL: no rotation). Norm and rotation are formed
+ * pos [n_tok] (`rope` NULL: no rotation; pos too may be NULL then). Norm and rotation are formed
  * in 32 bits and rounded once. A row whose slot or position is negative is left out
  * (padding: neither its key nor its query is written); 3: a slot outside the cache,
  * 6: a position outside the table, such a row is left out. Slots must be distinct. */
@@ -770,7 +770,8 @@ typedef struct kore_cuda_accepted {
 
 /* The branch that the model follows: from token 0 of each chunk on, the first child
  * (by index) whose token[t] is choice of its parent (the model's token behind it; all
- * device [n_tok]), and so on. */
+ * device [n_tok]), and so on. A sequence that does not fit (as for the masks, or of more
+ * than 1024 tokens) is left out (7): count 0, kept -1. */
 int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
                               const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream);
 

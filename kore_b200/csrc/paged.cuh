@@ -78,7 +78,7 @@ struct PlanParams {
 struct StoreParams {
     HeadRows q, k, v;          // q: heads 0: none; k, v: out, strides unused
     const long long *slots;
-    const int *pos;            // null: nothing is rotated
+    const int *pos;            // null: no row is left out for its position
     const float *table;
     int n_tok, n_pos, rot, interleaved, d, P, G;
     FastDiv by_page;

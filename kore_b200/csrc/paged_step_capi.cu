@@ -67,6 +67,8 @@ extern "C" int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_s
     if (step->n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", step->n_tok);
     if (n_seq > 0 && (!step->kv_len || !step->page_table)) return refuse(KORE_CUDA_EINVAL, "kv_len or page_table is null");
     if (step->n_tok > 0 && (!step->slots || !step->pos)) return refuse(KORE_CUDA_EINVAL, "slots or pos is null");
+    if ((reinterpret_cast<uintptr_t>(step->slots) & 7) || (reinterpret_cast<uintptr_t>(step->pos) & 3))
+        return refuse(KORE_CUDA_EINVAL, "slots or pos is not aligned to its type");
     if (step->table_stride < pool->table_stride)
         return refuse(KORE_CUDA_EINVAL, "the step's table_stride %d is less than the pool's %d", step->table_stride, pool->table_stride);
     OnDeviceOf on(pool->table);
@@ -98,6 +100,8 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
     if (int rc = check_pages(cache, false)) return rc;
     if (n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", n_tok);
     if (n_tok > 0 && !slots) return refuse(KORE_CUDA_EINVAL, "slots is null");
+    if ((reinterpret_cast<uintptr_t>(slots) & 7) || (reinterpret_cast<uintptr_t>(pos) & 3))
+        return refuse(KORE_CUDA_EINVAL, "slots or pos is not aligned to its type");
     const int d = cache->head_dim;
     if (int rc = check_appended(cache, k, v, q, q_out, n_tok)) return rc;
     if (rope) {
@@ -125,8 +129,8 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
     p.k = head_rows(k, nullptr);
     p.v = head_rows(v, nullptr);
     p.slots = slots;
+    p.pos = pos;
     if (rope) {
-        p.pos = pos;
         p.table = rope->table;
         p.n_pos = rope->n_pos;
         p.rot = rope->n_rot;

@@ -33,11 +33,15 @@ __device__ __forceinline__ Seq tree_seq(const TreeParams &p, int s, bool report)
     return q;
 }
 
-// A CTA a sequence, a thread a token: the way up the parents goes to ever lower bits.
+// A CTA a sequence, a thread a token: the way up the parents, which stand in shared memory, goes to ever
+// lower bits.
 __global__ void __launch_bounds__(128) tree_mask_kernel(const __grid_constant__ TreeParams p) {
     grid_dep_wait();
     grid_dep_launch();
+    __shared__ int parent[kPagedMaxTree];
     const Seq q = tree_seq(p, blockIdx.x, threadIdx.x == 0);
+    for (int i = threadIdx.x; i < q.n; i += blockDim.x) parent[i] = __ldg(p.parent + q.q0 + i);
+    __syncthreads();
     for (int i = threadIdx.x; i < q.n; i += blockDim.x) {
         uint32_t *row = p.mask + (long long)(q.q0 + i) * p.words;
         int x = i, depth = 0, w = p.words - 1;
@@ -48,7 +52,7 @@ __global__ void __launch_bounds__(128) tree_mask_kernel(const __grid_constant__ 
                 bits = 0;
             }
             bits |= 1u << (x & 31);
-            const int up = __ldg(p.parent + q.q0 + x);
+            const int up = parent[x];
             if (up == -1) break;
             if (up < -1 || up >= x) {   // no tree: the token is left out
                 raise_error(p.status, DEV_BAD_SEQUENCE);
@@ -68,26 +72,40 @@ __global__ void __launch_bounds__(128) tree_mask_kernel(const __grid_constant__ 
     }
 }
 
-// A warp a sequence.
+// A warp a sequence; trees of up to kNear tokens are walked in shared memory.
+constexpr int kNear = 256;
 __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ TreeParams p) {
     grid_dep_wait();
     grid_dep_launch();
     const int lane = threadIdx.x & 31, s = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (s >= p.n_seq) return;
+    __shared__ int near[4][3][kNear];
     const Seq q = tree_seq(p, s, lane == 0);
     int *path = p.path + (long long)s * p.path_stride;
     int count = 0, now = 0, next = -1;
     if (q.n > 0) {
-        const int *parent = p.parent + q.q0, *token = p.token + q.q0;
+        const int *parent = p.parent + q.q0, *token = p.token + q.q0, *choice = p.choice + q.q0;
+        if (q.n <= kNear) {
+            int(*to)[kNear] = near[threadIdx.x >> 5];
+            for (int i = lane; i < q.n; i += 32) {
+                to[0][i] = __ldg(parent + i);
+                to[1][i] = __ldg(token + i);
+                to[2][i] = __ldg(choice + i);
+            }
+            __syncwarp();
+            parent = to[0];
+            token = to[1];
+            choice = to[2];
+        }
         for (;;) {
             if (lane == 0) path[count] = now;
             ++count;
-            next = __ldg(p.choice + q.q0 + now);
+            next = choice[now];
             if (count == p.path_stride) break;
             int child = -1;
             for (int i0 = now + 1; i0 < q.n; i0 += 32) {
                 const int i = i0 + lane;
-                const unsigned hit = __ballot_sync(FULL, i < q.n && __ldg(parent + i) == now && __ldg(token + i) == next);
+                const unsigned hit = __ballot_sync(FULL, i < q.n && parent[i] == now && token[i] == next);
                 if (hit) {
                     child = i0 + __ffs(hit) - 1;
                     break;

@@ -356,7 +356,7 @@ class PagedCache:
     def store(self, slots, pos, k, v, *, rope: RopeTable | None = None, norm=None, q=None, q_out=None) -> None:
         """Stores k and v [tokens][n_head_kv][head_dim] at the slots [tokens] (int64: page * page_tokens + place in the
         page; negative: the row is left out). norm (a HeadNorm of kore_b200/drafts.py) norms each head of k and q, rope
-        rotates them at the int32 positions pos [tokens] (None without rope); with q, it goes into q_out (which may be q)
+        rotates them at the int32 positions pos [tokens] (may be None without rope; negative: the row is left out); with q, it goes into q_out (which may be q)
         in the same launch."""
         dev, r = self.device, self._r
         n = _fill(r[0], k, "k", dev)
@@ -372,14 +372,16 @@ class PagedCache:
             if _fill(r[2], q, "q", dev) != n or _fill(r[3], q_out, "q_out", dev) != n:
                 raise ValueError("q, q_out and k have different numbers of tokens")
             pq, pqo = self._p[2], self._p[3]
+        if pos is not None:
+            pp = _ints(pos, "pos", dev, 1)
+            if pos.shape[0] != n:
+                raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
         if rope is not None:
             if rope.device != dev:
                 raise ValueError(f"the table is not on {dev}")
             if pos is None:
                 raise ValueError("a rotation needs positions")
-            pp, pr = _ints(pos, "pos", dev, 1), rope._view
-            if pos.shape[0] != n:
-                raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
+            pr = rope._view
         if norm is not None:
             pn = norm._for(dev, self.view.head_dim, r[2].n_head if q is not None else None, r[0].n_head)
         if n == 0:

@@ -55,7 +55,7 @@ def test_bad_plans_and_trims_refused():
         assert call(n=-1)[0] == -2 and call(n=4097)[0] == -2 and call(request=None)[0] == -1
     assert _plan(n_new=None)[0] == -1 and _trim(keep=None)[0] == -1 and _plan(step=None)[0] == -1
     for kw in (dict(q_start=None), dict(kv_len=None), dict(page_table=None), dict(table_stride=3), dict(n_tok=-1),
-               dict(slots=None), dict(pos=None)):
+               dict(slots=None), dict(pos=None), dict(slots=A + 4), dict(pos=A + 2)):
         assert _plan(step=_step(**kw))[0] == -1
     assert _trim(n=0)[0] == 0
 
@@ -80,7 +80,7 @@ def test_bad_pages_refused(kw, word):
 
 
 @pytest.mark.parametrize("kw,word", [
-    (dict(n=-1), "n_tok"), (dict(slots=None), "slots"), (dict(k=None), "k is null"), (dict(v=_rows(data=None)), "v is null"),
+    (dict(n=-1), "n_tok"), (dict(slots=None), "slots"), (dict(slots=A + 4), "aligned"), (dict(pos=A + 2), "aligned"), (dict(k=None), "k is null"), (dict(v=_rows(data=None)), "v is null"),
     (dict(k=_rows(3)), "heads"), (dict(v=_rows(type=P.F16)), "different types"), (dict(q=_rows(4)), "together"),
     (dict(q=_rows(4), q_out=_rows(5)), "heads"), (dict(q=_rows(4), q_out=_rows(4, ts=0), n=2), "overlap"),
     (dict(k=_rows(type=P.F16), v=_rows(type=P.F16)), "do not go"),

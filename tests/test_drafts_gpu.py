@@ -270,9 +270,7 @@ def test_store(t, c, G, H, d, rot, P, how, inter, wt, each):
     kp0, vp0 = C.kp.clone(), C.vp.clone()
     C.cache.store(slots, pos, k, v, rope=rope, norm=norm, q=q, q_out=q_out)
     C.cache.check()
-    keep = slots >= 0
-    if rot:
-        keep &= pos >= 0
+    keep = (slots >= 0) & (pos >= 0)
     freq, amp = K.rope_frequencies(rot) if rot else ([], 1.0)
     pg, sl = slots[keep] // P, slots[keep] % P
     for x, w, pages, scale in ((k, kw, C.kp, C.ks), (v, None, C.vp, C.vs)):
