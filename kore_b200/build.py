@@ -1,6 +1,7 @@
 """Builds kore_b200/libkore_cuda.so (the C-ABI library) with nvcc for sm_100a.
 
-Usage: ``python -m kore_b200.build [--force] [--verbose] [--trace]``. The
+Usage: ``python -m kore_b200.build [--force] [--verbose] [--trace]``; also
+kore_b200/_tensors.so, with which the Python operators describe torch tensors. The
 library is built in-tree so that it travels with the repository to the GPU
 machine. ``--trace`` builds kore_b200/libkore_cuda_trace.so instead: the same
 library compiled with KORE_TRACE, whose decode and merge CTAs record
@@ -13,12 +14,14 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libkore_cuda.so")
+TENSORS = os.path.join(PKG, "_tensors.so")   # the Python module that describes torch tensors for the library
 TRACE_LIB = os.path.join(PKG, "libkore_cuda_trace.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -73,6 +76,27 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, out: 
     return lib
 
 
+def build_tensors(force: bool = False) -> str | None:
+    """Compiles csrc/tensors.cpp against the torch that is installed (none: there are no tensors to describe)."""
+    try:
+        import torch
+    except ImportError:
+        return None
+    src = os.path.join(CSRC, "tensors.cpp")
+    deps = [src, os.path.join(INCLUDE, "kore_cuda.h"), torch.__file__]
+    if not force and os.path.exists(TENSORS) and all(os.path.getmtime(d) <= os.path.getmtime(TENSORS) for d in deps):
+        return TENSORS
+    home = os.path.dirname(torch.__file__)
+    cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
+    tmp = TENSORS + ".tmp"
+    subprocess.run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                    "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], "-isystem", os.path.join(home, "include"),
+                    "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                    src, "-o", tmp, "-L", os.path.join(home, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"], check=True)
+    os.replace(tmp, TENSORS)
+    return TENSORS
+
+
 if __name__ == "__main__":
     import argparse
     ap = argparse.ArgumentParser()
@@ -83,3 +107,5 @@ if __name__ == "__main__":
     ap.add_argument("-D", dest="defines", action="append", default=[], help="NAME=VALUE for a variant build")
     a = ap.parse_args()
     print(build(force=a.force, verbose=a.verbose, trace=a.trace, out=a.out, defines=tuple(a.defines)))
+    if not a.trace and not a.out:
+        print(build_tensors(force=a.force))

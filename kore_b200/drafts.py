@@ -25,7 +25,7 @@ from __future__ import annotations
 import ctypes
 
 from . import paged as P
-from .paged import PagedBatch, PagedCache, _ck, _fill, _int, _ints, _stream   # noqa: F401
+from .paged import PagedBatch, PagedCache, _ck, _int, _ints, _stream   # noqa: F401
 
 __all__ = ["PagePool", "PagedStep", "TokenTree", "AcceptedPath", "PagedLayers", "HeadNorm"]
 
@@ -91,11 +91,8 @@ class PagePool:
         return PagedStep(n_seq, _size(n_tok, "n_tok", 0), self.view.table_stride, max_q, max_kv, self.device)
 
     def _two(self, request, amount, what: str):
-        pr, pa = _ints(request, "request", self.device, 1), _ints(amount, what, self.device, 1)
-        n = request.shape[0]
-        if amount.shape[0] != n:
-            raise ValueError(f"{n} requests, but {amount.shape[0]} values of {what}")
-        return n, pr, pa
+        pr, n = _ints(request, "request", self.device, 1), request.shape[0]
+        return n, pr, _ints(amount, what, self.device, 1, n)
 
     def plan(self, step: PagedStep, request, n_new) -> None:
         """Plans n_new[s] more positions for request[s] (int32 on the device, each request once; negative: padding) into
@@ -180,9 +177,9 @@ class TokenTree:
         before the token's own; -1: none): a token sees its ancestors and itself, and stands at the context's
         length and its depth."""
         n = self.mask.shape[0]
-        pp = _ints(parent, "parent", self.device, 1)
-        if parent.shape[0] != n or batch.device != self.device:
-            raise ValueError(f"expected {n} parents and a batch on {self.device}")
+        pp = _ints(parent, "parent", self.device, 1, n)
+        if batch.device != self.device:
+            raise ValueError(f"expected a batch on {self.device}")
         if n == 0:
             return
         rc = self._L.kore_cuda_tree_masks_dev(batch._view, n, pp, self._mask, self.view.words, self._pos, self._status,
@@ -215,10 +212,8 @@ class AcceptedPath:
     def accept(self, batch: PagedBatch, parent, token, choice) -> None:
         """From token 0 of each chunk on, the first child whose token is the model's choice behind its parent, and so on
         (parent as for TokenTree.build, token and choice [n_tok]; all int32)."""
-        pp, pt, pc = (_ints(x, what, self.device, 1) for x, what in ((parent, "parent"), (token, "token"), (choice, "choice")))
-        n = parent.shape[0]
-        if token.shape[0] != n or choice.shape[0] != n:
-            raise ValueError(f"{n} parents, {token.shape[0]} tokens and {choice.shape[0]} choices")
+        pp, n = _ints(parent, "parent", self.device, 1), parent.shape[0]
+        pt, pc = _ints(token, "token", self.device, 1, n), _ints(choice, "choice", self.device, 1, n)
         if batch.device != self.device or batch.view.n_seq != self.path.shape[0]:
             raise ValueError(f"expected a batch of {self.path.shape[0]} sequences on {self.device}")
         if batch.view.n_seq == 0:

@@ -132,16 +132,17 @@ def _ck(L, rc: int) -> None:
         raise KoreCudaError(rc, L.kore_cuda_last_error(None).decode())
 
 
-_torch = _int32 = _int64 = None
+_torch = None
 _types: dict = {}
 
 
 def _import_torch():
-    global _torch, _int32, _int64
+    global _torch
     if _torch is None:
         import torch
-        _torch, _int32, _int64 = torch, torch.int32, torch.int64
+        _torch = torch
         _types.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16, torch.float8_e4m3fn: E4M3})
+        _describe_natively()
     return _torch
 
 
@@ -158,27 +159,53 @@ def _int(x, what: str) -> int:
 _pack_rows = struct.Struct("@Piiiqq").pack_into   # _Rows, in one step
 
 
-def _fill(r: _Rows, t, what: str, device) -> int:
-    """Describes a [tokens][heads][head_dim] tensor in r; returns its tokens."""
+def _rows_of(r: int, t, what: str, device: int) -> int:
+    """Describes a [tokens][heads][head_dim] tensor in the _Rows at address r; returns its tokens. (What _tensors.rows
+    does in a seventh of the time.)"""
     shape = t.shape
     if len(shape) != 3:
-        raise ValueError(f"{what}: expected [tokens][heads][head_dim], got {tuple(shape)}")
+        raise ValueError(f"{what}: expected [tokens][heads][head_dim], got {len(shape)} dimensions")
     n, h, d = shape
-    if n > _INT_MAX:
+    if max(shape) > _INT_MAX:
         raise ValueError(f"{what}: {n} tokens are too many for one call")
     ts, hs, es = t.stride()
     if es != 1 and d > 1:
         raise ValueError(f"{what}: the values of a head must be contiguous")
-    if t.get_device() != device.index:
-        raise ValueError(f"{what} is on {t.device}, expected {device}")
-    _pack_rows(r, 0, t.data_ptr(), _types.get(t.dtype, -1), h, d, ts, hs)
+    if not t.is_cuda or t.get_device() != device:
+        raise ValueError(f"{what} is on {t.device}, expected cuda:{device}")
+    _pack_rows(_Rows.from_address(r), 0, t.data_ptr(), _types.get(t.dtype, -1), h, d, ts, hs)
     return n
 
 
-def _ints(t, what: str, device, shape_len: int):
-    if t.dtype is not _int32 or t.ndim != shape_len or not t.is_contiguous() or t.get_device() != device.index:
-        raise ValueError(f"{what}: expected a contiguous {shape_len}-d int32 tensor on {device}")
+def _ints_of(t, what: str, device: int, dims: int, size: int, length: int) -> int:
+    """The address of a contiguous tensor of integers of 4 or 8 bytes, of length `length` if that is not -1
+    (_tensors.ints)."""
+    if (t.dtype is not (_torch.int64 if size == 8 else _torch.int32) or t.ndim != dims or not t.is_contiguous()
+            or not t.is_cuda or t.get_device() != device):
+        raise ValueError(f"{what}: expected a contiguous {dims}-d int{8 * size} tensor on cuda:{device}")
+    if length >= 0 and t.shape[0] != length:
+        raise ValueError(f"{what}: expected {length} values, got {t.shape[0]}")
     return t.data_ptr()
+
+
+_rows_in, _ints_in = _rows_of, _ints_of
+
+
+def _describe_natively() -> bool:
+    """Takes the built module in place of the two above, if it is there and of this torch."""
+    global _rows_in, _ints_in
+    try:
+        from . import _tensors as m
+    except ImportError:
+        return False
+    if m.torch_version != _torch.__version__.split("+")[0]:
+        return False
+    _rows_in, _ints_in = m.rows, m.ints
+    return True
+
+
+def _ints(t, what: str, device, dims: int, length: int = -1) -> int:
+    return _ints_in(t, what, device.index, dims, 4, length)
 
 
 def _stream(device) -> int:
@@ -256,12 +283,10 @@ class RopeTable:
         a new tensor: whatever the memory holds)."""
         if out is None:
             out = _torch.empty_like(x)
-        n = _fill(self._x, x, "x", self.device)
-        if _fill(self._out, out, "out", self.device) != n:
+        n = _rows_in(self._px, x, "x", self.device.index)
+        if _rows_in(self._pout, out, "out", self.device.index) != n:
             raise ValueError("x and out have different numbers of tokens")
-        pp = _ints(pos, "pos", self.device, 1)
-        if pos.shape[0] != n:
-            raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
+        pp = _ints(pos, "pos", self.device, 1, n)
         if n == 0:
             return out
         rc = self._L.kore_cuda_rope_dev(self._px, self._pout, n, pp, self._view, self._status, _stream(self.device))
@@ -333,15 +358,16 @@ class PagedCache:
     def append(self, batch: PagedBatch, k, v, *, rope: RopeTable | None = None, q=None, q_out=None) -> None:
         """Stores k (rotated by rope at each token's position) and v [tokens][n_head_kv][head_dim] in the pages; with
         q, rotates it into q_out (which may be q) in the same launch."""
-        dev, r = self.device, self._r
-        n = _fill(r[0], k, "k", dev)
-        if _fill(r[1], v, "v", dev) != n:
+        dev, p = self.device, self._p
+        i = dev.index
+        n = _rows_in(p[0], k, "k", i)
+        if _rows_in(p[1], v, "v", i) != n:
             raise ValueError("k and v have different numbers of tokens")
         pq = pqo = None
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out come together")
         if q is not None:
-            if _fill(r[2], q, "q", dev) != n or _fill(r[3], q_out, "q_out", dev) != n:
+            if _rows_in(p[2], q, "q", i) != n or _rows_in(p[3], q_out, "q_out", i) != n:
                 raise ValueError("q, q_out and k have different numbers of tokens")
             pq, pqo = self._p[2], self._p[3]
         if batch.device != dev or (rope is not None and rope.device != dev):
@@ -356,26 +382,23 @@ class PagedCache:
     def store(self, slots, pos, k, v, *, rope: RopeTable | None = None, norm=None, q=None, q_out=None) -> None:
         """Stores k and v [tokens][n_head_kv][head_dim] at the slots [tokens] (int64: page * page_tokens + place in the
         page; negative: the row is left out). norm (a HeadNorm of kore_b200/drafts.py) norms each head of k and q, rope
-        rotates them at the int32 positions pos [tokens] (may be None without rope; negative: the row is left out); with q, it goes into q_out (which may be q)
-        in the same launch."""
-        dev, r = self.device, self._r
-        n = _fill(r[0], k, "k", dev)
-        if _fill(r[1], v, "v", dev) != n:
+        rotates them at the int32 positions pos [tokens] (may be None without rope; negative: the row is left out); with
+        q, it goes into q_out (which may be q) in the same launch."""
+        dev, p = self.device, self._p
+        i = dev.index
+        n = _rows_in(p[0], k, "k", i)
+        if _rows_in(p[1], v, "v", i) != n:
             raise ValueError("k and v have different numbers of tokens")
-        if (slots.dtype is not _int64 or slots.ndim != 1 or slots.shape[0] != n or not slots.is_contiguous()
-                or slots.get_device() != dev.index):
-            raise ValueError(f"slots: expected {n} contiguous int64 values on {dev}")
+        ps = _ints_in(slots, "slots", i, 1, 8, n)
         pq = pqo = pp = pr = pn = None
         if (q is None) != (q_out is None):
             raise ValueError("q and q_out come together")
         if q is not None:
-            if _fill(r[2], q, "q", dev) != n or _fill(r[3], q_out, "q_out", dev) != n:
+            if _rows_in(p[2], q, "q", i) != n or _rows_in(p[3], q_out, "q_out", i) != n:
                 raise ValueError("q, q_out and k have different numbers of tokens")
             pq, pqo = self._p[2], self._p[3]
         if pos is not None:
-            pp = _ints(pos, "pos", dev, 1)
-            if pos.shape[0] != n:
-                raise ValueError(f"{pos.shape[0]} positions for {n} tokens")
+            pp = _ints_in(pos, "pos", i, 1, 4, n)
         if rope is not None:
             if rope.device != dev:
                 raise ValueError(f"the table is not on {dev}")
@@ -383,10 +406,11 @@ class PagedCache:
                 raise ValueError("a rotation needs positions")
             pr = rope._view
         if norm is not None:
+            r = self._r
             pn = norm._for(dev, self.view.head_dim, r[2].n_head if q is not None else None, r[0].n_head)
         if n == 0:
             return
-        rc = self._L.kore_cuda_paged_store_dev(self._view, n, slots.data_ptr(), pp, self._p[0], self._p[1], pq, pqo, pr,
+        rc = self._L.kore_cuda_paged_store_dev(self._view, n, ps, pp, self._p[0], self._p[1], pq, pqo, pr,
                                                pn, self._status, _stream(dev))
         if rc:
             _ck(self._L, rc)
@@ -402,15 +426,16 @@ class PagedCache:
         by default one that this device and stream (or the capture that the stream is in) keep. tree (a TokenTree of
         kore_b200/drafts.py): each chunk is a tree of drafted tokens, which see their context and what the tree's masks
         name of their chunk (no window, causal as it is)."""
-        dev, r = self.device, self._r
+        dev, p = self.device, self._p
+        i = dev.index
         if out is None:
             out = _torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        n = _fill(r[0], q, "q", dev)
-        if _fill(r[1], out, "out", dev) != n:
+        n = _rows_in(p[0], q, "q", i)
+        if _rows_in(p[1], out, "out", i) != n:
             raise ValueError("q and out have different numbers of tokens")
         plse = None
         if lse is not None:
-            if (lse.dtype != _torch.float32 or tuple(lse.shape) != (n, r[0].n_head) or not lse.is_contiguous()
+            if (lse.dtype != _torch.float32 or tuple(lse.shape) != (n, self._r[0].n_head) or not lse.is_contiguous()
                     or lse.device != dev):
                 raise ValueError("lse: expected a contiguous float32 tensor [tokens][n_head]")
             plse = lse.data_ptr()
