@@ -668,7 +668,7 @@ int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch
  */
 
 /* A pool's pages and who holds them, all in device memory that these calls alone
- * change. Request r holds length[r] positions in the first ceil(length[r] /
+ * change, one after the other (a stream's, or streams in order). Request r holds length[r] positions in the first ceil(length[r] /
  * page_tokens) pages of its row of `table`. */
 typedef struct kore_cuda_page_pool {
     int *free_pages;      /* [n_pages]: the first n_free are free; pages are taken from the end of these */
@@ -688,7 +688,7 @@ typedef struct kore_cuda_step {
     int *kv_len;          /* [n_seq] */
     int *page_table;      /* [n_seq][table_stride] */
     int table_stride;     /* at least the pool's */
-    int n_tok;
+    int n_tok;            /* at most 2^30 */
     long long *slots;     /* [n_tok]; -1: the row is of no sequence, or of one that is left out */
     int *pos;             /* [n_tok]; -1 as well */
 } kore_cuda_step;
@@ -726,7 +726,7 @@ typedef struct kore_cuda_head_norm {
  * pos [n_tok] (`rope` NULL: no rotation; pos too may be NULL then). Norm and rotation are formed
  * in 32 bits and rounded once. A row whose slot or position is negative is left out
  * (padding: neither its key nor its query is written); 3: a slot outside the cache,
- * 6: a position outside the table, such a row is left out. Slots must be distinct. */
+ * 6: a position outside the table, such a row is left out. Slots must be distinct, n_tok at most 2^30. */
 int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok, const long long *slots, const int *pos,
                               const kore_cuda_rows *k, const kore_cuda_rows *v, const kore_cuda_rows *q,
                               const kore_cuda_rows *q_out, const kore_cuda_rope_view *rope,
@@ -777,7 +777,7 @@ int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int
 
 /* Moves the accepted tokens' keys and values together: row path[s][j] of sequence
  * s's chunk to row j of it, in every one of n_layers caches (of one type and geometry,
- * with pools of their own). batch: as the step ran with it, drafts counted. A path that does
+ * in memory of their own). batch: as the step ran with it, drafts counted. A path that does
  * not ascend, or leaves the chunk, is left out (7). */
 int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_layers, const kore_cuda_batch *batch,
                                const int *path, int path_stride, const int *count, int *dev_status, void *stream);

@@ -19,6 +19,7 @@ constexpr int DEV_NO_PAGES = 8;       // the pool has too few free pages
 constexpr int kPagedMaxSeqs = 4096;      // sequences of one batch
 constexpr int kPagedMaxRequests = 65536; // requests of one pool
 constexpr int kPagedMaxTree = 1024;      // tokens of a tree
+constexpr int kPagedMaxTokens = 1 << 30; // rows of a plan or a store: steps beyond the last stay in 32 bits
 constexpr int kPagedMaxLayers = 128;     // layers of one launch
 constexpr int kPagedMaxCtas = 160;       // CTAs (SMs) that an attention launch uses at most
 constexpr int kPagedRowsMax = 256;       // query rows of a work unit at most

@@ -23,6 +23,12 @@ int check_pool(const kore_cuda_page_pool *p, int n_seq, const int *request, cons
     return KORE_CUDA_OK;
 }
 
+int check_tokens(int n_tok) {
+    if (n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", n_tok);
+    if (n_tok > kPagedMaxTokens) return refuse(KORE_CUDA_ERANGE, "n_tok %d is more than %d", n_tok, kPagedMaxTokens);
+    return KORE_CUDA_OK;
+}
+
 PlanParams plan_params(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *amount, int *status) {
     PlanParams p;
     memset(&p, 0, sizeof p);
@@ -64,7 +70,7 @@ extern "C" int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_s
                                         const kore_cuda_step *step, int *dev_status, void *stream) {
     if (int rc = check_pool(pool, n_seq, request, n_new)) return rc;
     if (!step || !step->q_start) return refuse(KORE_CUDA_EINVAL, "the step is null");
-    if (step->n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", step->n_tok);
+    if (int rc = check_tokens(step->n_tok)) return rc;
     if (n_seq > 0 && (!step->kv_len || !step->page_table)) return refuse(KORE_CUDA_EINVAL, "kv_len or page_table is null");
     if (step->n_tok > 0 && (!step->slots || !step->pos)) return refuse(KORE_CUDA_EINVAL, "slots or pos is null");
     if ((reinterpret_cast<uintptr_t>(step->slots) & 7) || (reinterpret_cast<uintptr_t>(step->pos) & 3))
@@ -98,7 +104,7 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
                                          const kore_cuda_rows *q_out, const kore_cuda_rope_view *rope,
                                          const kore_cuda_head_norm *norm, int *dev_status, void *stream) {
     if (int rc = check_pages(cache, false)) return rc;
-    if (n_tok < 0) return refuse(KORE_CUDA_EINVAL, "n_tok %d", n_tok);
+    if (int rc = check_tokens(n_tok)) return rc;
     if (n_tok > 0 && !slots) return refuse(KORE_CUDA_EINVAL, "slots is null");
     if ((reinterpret_cast<uintptr_t>(slots) & 7) || (reinterpret_cast<uintptr_t>(pos) & 3))
         return refuse(KORE_CUDA_EINVAL, "slots or pos is not aligned to its type");
@@ -209,12 +215,25 @@ extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_l
                                           const int *path, int path_stride, const int *count, int *dev_status, void *stream) {
     if (n_layers < 0) return refuse(KORE_CUDA_EINVAL, "n_layers %d", n_layers);
     if (n_layers > 0 && !layers) return refuse(KORE_CUDA_EINVAL, "layers is null");
+    // A layer named twice would be moved by two threads at once. Bits of the addresses so far tell most layers
+    // apart; only where one's are there already are the earlier ones looked through.
+    unsigned long long named[16] = {};
+    auto fresh = [&](const void *x) {
+        const uint64_t bit = (reinterpret_cast<uintptr_t>(x) >> 4) * 0x9e3779b97f4a7c15ull >> 54;
+        const bool was = named[bit >> 6] >> (bit & 63) & 1;
+        named[bit >> 6] |= 1ull << (bit & 63);
+        return !was;
+    };
     for (int l = 0; l < n_layers; ++l) {
         const kore_cuda_pages &c = layers[l];
         if (int rc = check_pages(&c, false)) return rc;
         if (c.type != layers->type || c.n_pages != layers->n_pages || c.page_tokens != layers->page_tokens ||
             c.n_head_kv != layers->n_head_kv || c.head_dim != layers->head_dim || page_stride(&c) != page_stride(layers))
             return refuse(KORE_CUDA_EINVAL, "layer %d has another type or geometry than layer 0", l);
+        const bool k_fresh = fresh(c.k), v_fresh = fresh(c.v);
+        for (int x = 0; (!k_fresh || !v_fresh) && x < l; ++x)
+            if (layers[x].k == c.k || layers[x].v == c.k || layers[x].k == c.v || layers[x].v == c.v)
+                return refuse(KORE_CUDA_EINVAL, "layers %d and %d have the same pages", x, l);
     }
     if (int rc = check_batch(batch, 0, true)) return rc;
     if (batch->n_seq > 0 && (!path || !count)) return refuse(KORE_CUDA_EINVAL, "path or count is null");

@@ -227,6 +227,20 @@ class AcceptedPath:
         P._check_status(self.status)
 
 
+def _check_apart(caches) -> None:
+    """Raises if two caches' pages (which may lie between one another's) share memory."""
+    v = caches[0].view
+    size = caches[0].k.element_size()
+    page = v.n_head_kv * v.page_tokens * v.head_dim * size
+    stride = v.page_stride * size or page
+    pools = [(a, i) for i, c in enumerate(caches) for a in (c.view.k, c.view.v)]
+    for x, (a, i) in enumerate(pools):
+        for b, j in pools[x + 1:]:
+            n, rest = divmod(abs((a or 0) - (b or 0)), stride)
+            if i != j and ((n < v.n_pages and rest < page) or (n + 1 < v.n_pages and stride - rest < page)):
+                raise ValueError(f"caches {i} and {j} share pages")
+
+
 class PagedLayers:
     """The caches of a model's layers, of one type and geometry, whose page tables are the same."""
 
@@ -236,6 +250,7 @@ class PagedLayers:
             raise ValueError("expected at least one cache")
         if any(c.device != caches[0].device for c in caches):
             raise ValueError("the caches are on different devices")
+        _check_apart(caches)
         self._L, self.device = P._library(), caches[0].device
         self.views = (P._Pages * len(caches))(*[c.view for c in caches])
         self._views = ctypes.addressof(self.views)

@@ -7,6 +7,7 @@ from types import SimpleNamespace
 import pytest
 
 import kore_b200 as K
+from kore_b200 import drafts
 from kore_b200 import paged as P
 from tests.test_paged_cpu import BAD_PAGES, A, B, _batch, _pages, _ref, _rows
 from tests.test_paged_refusals_cpu import cuda, fake  # noqa: F401
@@ -131,6 +132,45 @@ def test_bad_trees_refused():
         rc, msg = _commit((P._Pages * 2)(_pages(), _pages(**other)), 2)
         assert rc == -1 and "layer 1" in msg
     assert _masks(n=0)[0] == 0 and _accept(batch=_batch(n_seq=0))[0] == 0 and _commit(n=0)[0] == 0
+    assert all(c[0] == -2 for c in (_store(n=(1 << 30) + 1), _plan(step=_step(n_tok=(1 << 30) + 1))))
+
+
+def test_a_layer_named_twice_is_refused():
+    """Its rows would be moved by two threads at once, the second time from where the first has written."""
+    far = [dict(k=B + 4096 * i, v=B + 4096 * i + 2048) for i in range(300)]
+    for same in (far[7], dict(k=far[7]["v"], v=B - 4096), dict(k=B - 4096, v=far[299]["k"])):
+        layers = (P._Pages * 301)(*[_pages(**x) for x in far + [same]])
+        rc, msg = _commit(layers, 301)
+        assert rc == -1 and "and 300 have the same pages" in msg
+        assert _commit(layers, 300, batch=_batch(n_seq=0))[0] == 0
+
+
+class _Pool:
+    """What PagedLayers looks at of a cache; pages of 2 heads of 16 tokens of 64 values of 2 bytes: 4096 bytes."""
+
+    def __init__(self, k, v, n_pages=8, page_stride=0):
+        self.view = P._Pages(k, v, P.BF16, n_pages, 16, 2, 64, page_stride, None, None)
+        self.k = SimpleNamespace(element_size=lambda: 2)
+
+
+@pytest.mark.parametrize("other,page_stride,shared", [
+    ((A, B), 0, True), ((A + (1 << 20), A), 0, True), ((A + 4096 * 7, B + (1 << 20)), 0, True),
+    ((A + 4096 * 8, B + 4096 * 8), 0, False), ((A + 4096 * 8 - 16, B + 4096 * 8), 0, True), ((A - 4096 * 8, B - 4096 * 8), 0, False),
+    ((A - 4096 * 8 + 16, B - 4096 * 8), 0, True), ((A + 4096, B + 4096), 8192, False), ((A + 2048, B + 4096), 8192, True),
+    ((A + 8192 + 4096, B + 4096), 8192, False), ((A + 8192 + 4112, B + 4096), 8192, True),
+    ((A + 8192 * 7 + 4112, B + (1 << 20)), 8192, True),    # (the first page of the values follows the last of the keys)
+    ((A + 8192 * 7 + 4096, B + (1 << 20)), 8192, False)])
+def test_caches_that_share_pages_are_refused(other, page_stride, shared):
+    """Against the pages one by one."""
+    pools = [_Pool(A, B, page_stride=page_stride // 2), _Pool(*other, page_stride=page_stride // 2)]
+    page, stride = 4096, page_stride or 4096
+    spans = [[range(a + i * stride, a + i * stride + page) for a in (c.view.k, c.view.v) for i in range(8)] for c in pools]
+    assert shared == any(max(x.start, y.start) < min(x.stop, y.stop) for x in spans[0] for y in spans[1])
+    if shared:
+        with pytest.raises(ValueError, match="share"):
+            drafts._check_apart(pools)
+    else:
+        drafts._check_apart(pools)
     assert _commit(batch=_batch(n_seq=0))[0] == 0
 
 
