@@ -106,6 +106,16 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     float *q_shift = reinterpret_cast<float *>(smem + C::SHIFT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    // Tensor memory before all else: the SM's second CTA is let in only when the first has given up the right to
+    // allocate (behind the share, as late as 3 us, the second one's tiles were the last to come).
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    auto free_tmem = [&](uint32_t at) {   // by warp 5
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(256) : "memory");
+    };
     if (threadIdx.x == 128) {
         prefetch_map(&p.tm_k);
         prefetch_map(&p.tm_v);
@@ -116,7 +126,13 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     U u;
     long long total, x0, x1;
     int ctas;
-    if (!find_share<kM, kKeys, 8, 6, true>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) return;
+    if (!find_share<kM, kKeys, 8, 6, true>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) {
+        fence_before();
+        __syncthreads();
+        fence_after();
+        if (warp == 5) free_tmem(*tmem_slot);
+        return;
+    }
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::LOADS; ++i) mbar_init(&full[i], 1);
@@ -133,11 +149,6 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
         mbar_fence_init();
     }
     fence_proxy_async_smem();   // the sums stood where the ring's copies will land
-    if (warp == 5) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     fence_before();
     __syncthreads();
     fence_after();
@@ -765,7 +776,7 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     __syncthreads();
     if (warp == 5) {
         fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+        free_tmem(tmem);
     }
 }
 
