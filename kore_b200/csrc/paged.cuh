@@ -389,13 +389,18 @@ __device__ __forceinline__ long long quick_div(long long a, long long b) {
     return a / b;
 }
 
-// One head's cost of the sequences s0 + lane and their blocks: a lane a sequence;
+// Sequence s0 + lane; none behind the last.
+template <bool TREE>
+__device__ __forceinline__ Seq lane_seq(const PagedAttnParams &p, int s0) {
+    const int s = s0 + (threadIdx.x & 31);
+    return s < p.n_seq ? load_seq<TREE>(p, s, blockIdx.x == 0) : Seq{0, 0, 0};
+}
+
+// One head's cost of the lanes' sequences and their blocks: a lane a sequence;
 // sequences of several blocks by the whole warp, a lane a block.
 template <int ROWS, int KEYS, bool TREE>
-__device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, int s0, Seq &q, int &nb) {
+__device__ __forceinline__ long long lane_costs(const PagedAttnParams &p, const Seq &q, int &nb) {
     const int lane = threadIdx.x & 31;
-    q = Seq{0, 0, 0};
-    if (s0 + lane < p.n_seq) q = load_seq<TREE>(p, s0 + lane, blockIdx.x == 0);
     nb = (q.n * p.rep + ROWS - 1) / ROWS;
     long long cost = nb == 1 ? block_cost<ROWS, KEYS, TREE>(p, q, 0, 1) : 0;
     if constexpr (TREE) {   // every block has the whole sequence's keys
@@ -427,8 +432,9 @@ __device__ __forceinline__ T warp_scan(T v) {
 }
 
 // The CTA's share [x0, x1) of the row of tiles and the unit that x0 lies in.
-// cum: shared memory for n_seq + 2 sums (batches of more than 32 sequences; up
-// to that every warp finds its share by itself); ctas: CTAs that take a share.
+// cum: shared memory for n_seq + 2 sums (batches of more than 64 sequences; up
+// to that every warp finds its share by itself, with two sequences a lane, which took 0.6 us less for
+// 48 of them); ctas: CTAs that take a share.
 // Called by every thread of the CTA; false where there is nothing for it to do.
 // Units of no more than WHOLE tiles on average are not cut for the sake of more
 // CTAs, since joining the parts takes as long as some tiles; others may be, down to
@@ -437,23 +443,34 @@ template <int ROWS, int KEYS, int WHOLE, int MIN, bool TREE>
 __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *cum, Unit<ROWS, KEYS, TREE> &u,
                                            long long &total, int &ctas, long long &x0, long long &x1) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-    const bool few = p.n_seq <= 32 && p.small;
+    const bool few = p.n_seq <= 64 && p.small;
     long long units, cost = 0;
-    int sum = 0;   // few: of the costs up to this lane's sequence and with it
-    Seq q;
+    int sum = 0;                     // few: of the costs up to this lane's sequence and with it
+    int cost2 = 0, sum2 = 0;         // of sequence 32 + lane
+    Seq q, q2{0, 0, 0};
     if (few) {
+        q = lane_seq<TREE>(p, 0);
+        if (p.n_seq > 32) q2 = lane_seq<TREE>(p, 32);
         int nb;
-        cost = lane_costs<ROWS, KEYS, TREE>(p, 0, q, nb);
+        cost = lane_costs<ROWS, KEYS, TREE>(p, q, nb);
         sum = warp_scan((int)cost);
-        total = __shfl_sync(0xffffffffu, sum, 31);
+        int all = __shfl_sync(0xffffffffu, sum, 31);
         units = __reduce_add_sync(0xffffffffu, nb);
+        if (p.n_seq > 32) {
+            cost2 = (int)lane_costs<ROWS, KEYS, TREE>(p, q2, nb);
+            sum2 = all + warp_scan(cost2);
+            all = __shfl_sync(0xffffffffu, sum2, 31);
+            units += __reduce_add_sync(0xffffffffu, nb);
+        }
+        total = all;
     } else {
         long long &shared_units = cum[p.n_seq + 1];   // of one head of every sequence
         if (threadIdx.x == 0) shared_units = 0;
         __syncthreads();
         for (int s0 = warp * 32; s0 < p.n_seq; s0 += warps * 32) {
             int nb;
-            const long long c = lane_costs<ROWS, KEYS, TREE>(p, s0, q, nb);
+            q = lane_seq<TREE>(p, s0);
+            const long long c = lane_costs<ROWS, KEYS, TREE>(p, q, nb);
             if (s0 + lane < p.n_seq) cum[s0 + lane + 1] = c;
             const int n = __reduce_add_sync(0xffffffffu, nb);
             if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long *>(&shared_units), (unsigned long long)n);
@@ -482,10 +499,16 @@ __device__ __forceinline__ bool find_share(const PagedAttnParams &p, long long *
     x1 = quick_div(total * (blockIdx.x + 1), ctas);
     long long before;   // one head's cost of the sequences before u.s
     if (few) {
-        const int a = __ffs(__ballot_sync(0xffffffffu, (long long)sum * p.G > x0)) - 1;
+        const unsigned first = __ballot_sync(0xffffffffu, (long long)sum * p.G > x0);
+        if (!first) {   // among the sequences from the 33rd on
+            q = q2;
+            cost = cost2;
+            sum = sum2;
+        }
+        const int a = __ffs(first ? first : __ballot_sync(0xffffffffu, (long long)sum * p.G > x0)) - 1;
         before = __shfl_sync(0xffffffffu, sum - (int)cost, a);
         cost = __shfl_sync(0xffffffffu, (int)cost, a);
-        u.s = a;
+        u.s = first ? a : 32 + a;
         u.q = Seq{__shfl_sync(0xffffffffu, q.q0, a), __shfl_sync(0xffffffffu, q.n, a), __shfl_sync(0xffffffffu, q.kv, a)};
     } else {
         int a = 0, b = p.n_seq - 1;   // the sequence with cum[a] * G <= x0 < cum[a + 1] * G

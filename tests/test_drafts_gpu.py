@@ -14,6 +14,7 @@ import random
 import pytest
 
 import kore_b200 as K
+from tests.test_paged_gpu import attend as attend_chunks
 from tests.test_paged_gpu import DT, GUARD, HINTS, KINDS, TINY, U32, Cache, dev, gen, ints, rand, starts, strided, turned, u
 
 pytestmark = pytest.mark.gpu
@@ -918,3 +919,22 @@ def test_tree_attention_on_two_streams(kernel):
                 C.cache.attend(batch, q, o, tree=t)
     torch.cuda.synchronize()
     assert all(torch.equal(o, out) for o in outs)   # the same call, the same bits
+
+
+@pytest.mark.parametrize("trees", [False, True])
+@pytest.mark.parametrize("n_seq", [32, 33, 63, 64, 65, 97])
+@KERNELS
+def test_batches_around_the_sequences_of_a_warp(kernel, n_seq, trees):
+    """Up to 32 sequences a lane of each warp has one, up to 64 two, behind that the sums are shared: ragged batches,
+    some of whose sequences have no tokens (the 32nd and 33rd too), over shares that begin in either half."""
+    g, r = gen(n_seq), random.Random(n_seq)
+    for empty in (False, True):
+        ns = [0 if r.random() < 0.2 or (empty and 28 <= s < 40) else r.randrange(1, 9) for s in range(n_seq)]
+        kvs = [n + r.choice([0, 1, 40, 300, 900]) for n in ns]
+        C = Cache(g, "bf16", 2, 64, 16, kvs)
+        for s in range(n_seq):
+            C.fill(g, s)
+        if trees:
+            attend(g, C, 14, ns, [sees(tree(r, n, "random")) if n else None for n in ns], "bf16", kernel)
+        else:
+            attend_chunks(g, C, 14, ns, "bf16", kernel)
