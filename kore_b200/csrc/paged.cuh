@@ -237,7 +237,7 @@ cudaError_t launch_paged_tiles(const PagedAttnParams &p, int d, int q_type, int 
 constexpr int kUnitCost = 1;
 // Of the trees' 64-key tiles: the change from one unit to the next and the joint of its parts take about as
 // long as these (32 sequences of 16 tokens on up to 8192, 28/4 heads of 128: 73.9 us with 1, 71.4 with 8 and 15;
-// 48 of up to 33 on 3000, 14/2 heads of 64: 36.3, 34.6 and 36.8).
+// 48 of up to 33 on 3000, 14/2 heads of 64: 31.3 with 5, 31.6 with 8, 32.3 with 11).
 constexpr int kTreeUnitCost = 8;
 
 constexpr uint32_t FULL_WORD = 0xffffffffu;

@@ -53,14 +53,14 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, bool plai
 // share a unit. Row against tile kernel, 28/4 heads of 128, 16 bits: 8 tokens on 520 positions 11 / 16; 16
 // on 16000 41 / 43; 16 x 8 on 1008 33 / 26; 16 x 24 on 324 42 / 15; 16 x 8 on 8008 161 / 68; 48 x 2 on 1002 31 /
 // 40; 64 x 32 on 1532 415 / 94. 8 bits: 16 x 4 on 4004 41 / 50; 64 x 24 on 124 132 / 41. 14/2 heads of 64:
-// 64 on 1064 11 / 16; 64 on 30064 58 / 41. Over 144 batches of three head layouts the choice takes 0.6 % more than the
-// better kernel of each, 21 % at worst.
+// 64 on 1064 11 / 16; 64 on 30064 58 / 41. Over 144 batches of three head layouts the choice takes 0.7 % more than the
+// better kernel of each, 26 % at worst.
 bool trees_in_tiles(int d, bool e8, int G, int rep, int n_seq, int n_tok, double kv, int sms) {
     struct Cost {
         double unit, pass, start, tile, joint;
     };
     const Cost c = d == 128 ? e8 ? Cost{5.0, 0.72, 11.0, 1.6, 5.0} : Cost{3.5, 1.05, 9.5, 1.3, 5.0}
-                            : e8 ? Cost{3.6, 0.55, 9.5, 1.2, 4.5} : Cost{3.0, 0.5, 8.5, 1.05, 4.5};
+                            : e8 ? Cost{3.6, 0.55, 8.5, 1.14, 4.5} : Cost{3.0, 0.5, 7.5, 1.0, 4.5};
     const double packed = (double)n_tok * rep, half = 0.5 * n_seq;
     const double units16 = G * std::fmax(n_seq, packed / 16 + half), units = G * std::fmax(n_seq, packed / 128 + half);
     const double rows = 7 + std::fmax(4, units16 / sms * (c.unit + kv / 128 * c.pass));

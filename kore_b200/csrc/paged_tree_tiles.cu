@@ -7,7 +7,9 @@
 // * rows flops, so HBM and the tensor cores bound it alike at some 100 rows, and what counts is that
 // neither waits: two CTAs an SM, each with one tile of rows, so that one streams while the other starts
 // a unit, joins its parts or writes its outputs (one CTA an SM with two tiles of rows, as for prompts, left
-// 4 to 7 us between a CTA's units in which no key moved).
+// 4 to 7 us between a CTA's units in which no key moved). Measured: 32 sequences of 16 tokens on up to 8192, 28/4 heads
+// of 128, bf16: 70.6 us (4.05 TB/s, 440 TFLOP/s; the keys stream for 43 of them, a CTA's start takes 5, the joints at the
+// end up to 15); 6 of up to 60 on 32768, 8 bits: 121 us (540 TFLOP/s); 48 of up to 33 on 3001, 14/2 heads of 64, f16: 31.5.
 //   warps 0-3    softmax, a thread a row. Per step of 64 keys: S from tensor memory, mask (a word of bits for
 //                32 keys), online softmax (the reference maximum moves only when a score passes it by 2^8;
 //                O in tensor memory is rescaled then), P in 16 bits over S, sums in fp32.
@@ -106,8 +108,9 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     float *q_shift = reinterpret_cast<float *>(smem + C::SHIFT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // Tensor memory before all else: the SM's second CTA is let in only when the first has given up the right to
-    // allocate (behind the share, as late as 3 us, the second one's tiles were the last to come).
+    // The SM's second CTA is let in only when the first has given up the right to allocate tensor memory: before
+    // all else, since behind the share, as late as 3 us, the second one's tiles were the last to come (48 sequences
+    // of up to 33 tokens at d = 64: 31.5 us instead of 35; 16 of 8 tokens on 1008, 8 bits, d = 128: 26 instead of 29).
     if (warp == 5) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256)
                      : "memory");
@@ -127,10 +130,10 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     long long total, x0, x1;
     int ctas;
     if (!find_share<kM, kKeys, 8, 6, true>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) {
-        fence_before();
-        __syncthreads();
-        fence_after();
-        if (warp == 5) free_tmem(*tmem_slot);
+        if (warp == 5) {
+            __syncwarp();
+            free_tmem(*tmem_slot);
+        }
         return;
     }
 

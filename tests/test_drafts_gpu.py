@@ -938,3 +938,19 @@ def test_batches_around_the_sequences_of_a_warp(kernel, n_seq, trees):
             attend(g, C, 14, ns, [sees(tree(r, n, "random")) if n else None for n in ns], "bf16", kernel)
         else:
             attend_chunks(g, C, 14, ns, "bf16", kernel)
+
+
+@pytest.mark.parametrize("tq,tc", KINDS)
+@pytest.mark.parametrize("n,past", [(8, 1000), (24, 300), (24, 6000)])
+def test_trees_of_many_sequences_with_their_own_bounds(tq, tc, n, past):
+    """The batch's real bounds, by which the tile kernel takes it: few tiles a CTA, or many."""
+    g, r = gen(n), random.Random(n)
+    ns, kvs = [n] * 16, [n + past - 7 * s for s in range(16)]
+    C = Cache(g, tc, 4, 128, 64, kvs)
+    for s in range(16):
+        C.fill(g, s)
+    HINTS["own"] = dict(max_q=n, max_kv=n + past)
+    try:
+        attend(g, C, 28, ns, [sees(tree(r, n, "random")) for n in ns], tq, "own")
+    finally:
+        del HINTS["own"]
