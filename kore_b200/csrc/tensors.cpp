@@ -54,6 +54,10 @@ PyObject *rows(PyObject *, PyObject *const *a, Py_ssize_t n_args) {
     const char *name = PyUnicode_AsUTF8(a[2]);
     const long device = PyLong_AsLong(a[3]);
     if (PyErr_Occurred()) return nullptr;
+    if (!r) {
+        PyErr_SetString(PyExc_ValueError, "rows: the address is null");
+        return nullptr;
+    }
     const at::Tensor *t = tensor_of(a[1], name);
     if (!t) return nullptr;
     try {
