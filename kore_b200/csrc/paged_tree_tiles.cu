@@ -108,14 +108,6 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     float *q_shift = reinterpret_cast<float *>(smem + C::SHIFT);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // The SM's second CTA is let in only when the first has given up the right to allocate tensor memory: before
-    // all else, since behind the share, as late as 3 us, the second one's tiles were the last to come (48 sequences
-    // of up to 33 tokens at d = 64: 31.5 us instead of 35; 16 of 8 tokens on 1008, 8 bits, d = 128: 26 instead of 29).
-    if (warp == 5) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
     auto free_tmem = [&](uint32_t at) {   // by warp 5
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(256) : "memory");
     };
@@ -125,15 +117,22 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     }
     __syncwarp();
     grid_dep_wait();
-    grid_dep_launch();
+    // The SM's second CTA is let in only when the first has given up the right to allocate tensor memory, so that
+    // comes first: behind the share, as late as 3 us, the second one's tiles were the last to come (48 sequences
+    // of up to 33 tokens at d = 64: 31.5 us instead of 35; 16 of 8 tokens on 1008, 8 bits, d = 128: 26 instead of 29).
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
     U u;
     long long total, x0, x1;
     int ctas;
     if (!find_share<kM, kKeys, 8, 6, true>(p, reinterpret_cast<long long *>(smem + C::RING), u, total, ctas, x0, x1)) {
-        if (warp == 5) {
-            __syncwarp();
-            free_tmem(*tmem_slot);
-        }
+        fence_before();
+        __syncthreads();
+        fence_after();
+        if (warp == 5) free_tmem(*tmem_slot);
         return;
     }
 
@@ -156,6 +155,9 @@ __global__ void __launch_bounds__(TreeCfg<D, E8>::THREADS, kCtas) paged_tree_ker
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
+    // Not before: a following kernel's CTA that holds tensor memory and waits for this one to end must not
+    // stand in the way of its allocation (nor this one, which allocates behind its wait, in a preceding one's).
+    grid_dep_launch();
     // bounded, by whole warps, with one answer for the warp
     auto wait = [&](uint64_t *bar, uint32_t parity, bool copy = false) -> bool {
         bool got = (!copy || p.wait_ns >= kWaitNs) && mbar_try_wait(bar, parity);

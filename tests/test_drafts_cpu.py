@@ -2,6 +2,7 @@
 one (every check stands before the first CUDA call, so placeholder addresses do). CPU only."""
 import ctypes
 import math
+from pathlib import Path
 from types import SimpleNamespace
 
 import pytest
@@ -284,3 +285,11 @@ def test_products_and_their_commits_are_one_threads():
             end += 1
         covered.append((g.end(), end))
     assert all(any(a <= c < b for a, b in covered) for c in calls)
+
+
+def test_tensor_memory_is_taken_between_the_wait_and_the_trigger():
+    """A CTA that holds tensor memory and waits for the preceding kernel could stand in the way of its allocation; one
+    that lets the following kernel in before it allocates, in its own."""
+    src = (Path(__file__).parents[1] / "kore_b200" / "csrc" / "paged_tree_tiles.cu").read_text()
+    at = [src.index(x) for x in ("grid_dep_wait();", "tcgen05.alloc", "relinquish_alloc_permit", "find_share<", "grid_dep_launch();")]
+    assert at == sorted(at) and all(src.count(x) == 1 for x in ("grid_dep_wait();", "tcgen05.alloc", "grid_dep_launch();"))
