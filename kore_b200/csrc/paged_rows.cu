@@ -27,6 +27,9 @@
 //     fragment wants (2t, 2t+1, 2t+8, 2t+9), and q the same. bf16 queries over it
 //     are scaled by a power of two a row so that they are exact in f16 down
 //     to 2^-22 of the row's largest value (smaller ones lose digits: what f16 operands cost).
+//   * trees of drafted tokens (TREE): a row sees the context and the tokens of its chunk that its mask
+//     names, 32 keys a word; only tiles that reach into the chunk look at the words, and V's rows
+//     that none of the unit's rows sees are cleared. 8 tokens on 520 positions, 28/4 heads: 10.8 us.
 // Measured: 64 sequences of up to 8192 positions, 16/2 heads of 128, bf16: 55.5 us, 5.46
 // TB/s (83 % of the measured copy rate); 12 of up to 32768, 28/4 heads, 8 bits: 49.3 us, 4.77
 // TB/s (latency: two warps a scheduler use 36 % of the issue slots, half of them widening);
