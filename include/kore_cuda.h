@@ -699,8 +699,8 @@ typedef struct kore_cuda_step {
  * inputs alone; the first sequence that the free pages do not suffice for, and all
  * behind it that want some, are left out: their rows count in q_start, their
  * kv_len is 0, their slots are -1 and their requests stay as they are. So are
- * sequences of a request named twice or outside the pool, and those that pass
- * table_stride pages or n_tok rows (7). Entries of page_table behind a sequence's
+ * sequences of a request named twice or outside the pool, with a negative n_new, and
+ * those that pass table_stride pages or (n_new > 0) n_tok rows (7). Entries of page_table behind a sequence's
  * pages are not written. The others' lengths become kv_len. */
 int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *n_new,
                              const kore_cuda_step *step, int *dev_status, void *stream);
@@ -709,7 +709,7 @@ int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_seq, const i
  * back, so that a plan would take the same ones in the same order; their entries in
  * the pool's table become -1. A keep that is not less than the length changes
  * nothing; 0 ends a request. A request that is negative is padding; one that is
- * named twice or has a negative keep is left out (7). */
+ * named twice, or holds something and has a negative keep, is left out (7). */
 int kore_cuda_paged_trim_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *keep,
                              int *dev_status, void *stream);
 
@@ -765,7 +765,8 @@ typedef struct kore_cuda_accepted {
     int path_stride;          /* 1 .. 1024: tokens accepted at most */
     int *count;               /* [n_seq]: accepted tokens, token 0 among them; 0: a sequence without tokens */
     int *next_token;          /* [n_seq]: the model's choice behind the last of them; -1 without tokens */
-    int *kept;                /* [n_seq]: positions that the sequence holds with them; -1: it is left out */
+    int *kept;                /* [n_seq]: positions that the sequence holds with them; -1: it is left out, here or
+                                 by the plan, or has neither tokens nor positions (a trim to -1 takes nothing) */
 } kore_cuda_accepted;
 
 /* The branch that the model follows: from token 0 of each chunk on, the first child

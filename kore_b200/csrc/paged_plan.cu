@@ -99,17 +99,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
         const bool asked = r >= 0;
         int code = 0;
         if (!asked) a = 0;
-        if (asked && (!known(r) || (twice[r >> 5] >> (r & 31) & 1) || len < 0 || len > cap || a < 0)) code = DEV_BAD_SEQUENCE;
+        if (asked && (!known(r) || (twice[r >> 5] >> (r & 31) & 1) || len < 0 || len > cap)) code = DEV_BAD_SEQUENCE;
+        // (what a trim of a request that holds nothing is asked to keep of it makes no difference)
+        if (asked && a < 0 && (!TRIM || len != 0)) code = DEV_BAD_SEQUENCE;
         if (a < 0) a = 0;
         if constexpr (!TRIM) {
             // Sums of rows and of pages at once: the pages of sequences whose rows do not fit count too, but behind the
-            // first of these no sequence has rows that do.
+            // first of these no sequence has rows that do. (One without rows fits wherever it stands.)
             if (asked && !code && (long long)len + a > cap) code = DEV_BAD_SEQUENCE;
             const int have = code ? 0 : pages_of(p, len);
             const long long mine = asked && !code ? pages_of(p, len + a) - have : 0;
             long long rows = a, need = mine;
             block_scan(rows, need, part, rows_run, pages_run);
-            if (asked && !code && rows > p.n_tok) code = DEV_BAD_SEQUENCE;
+            if (asked && !code && a > 0 && rows > p.n_tok) code = DEV_BAD_SEQUENCE;
             if (!code && mine > 0 && need > n_free) code = DEV_NO_PAGES;
             if (s < p.n_seq) {
                 end[s] = (int)min(rows, 0x7fffffffll);

@@ -121,7 +121,9 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Tre
     if (lane == 0) {
         p.count[s] = count;
         p.next[s] = next;
-        p.kept[s] = q.n < 0 ? -1 : q.kv - q.n + count;   // (a sequence without tokens keeps all it has)
+        // A sequence without tokens keeps all it has; one of no positions either may be one that a plan left out (it
+        // writes 0 then), whose request holds some: 0 would end it.
+        p.kept[s] = q.n < 0 || (q.n == 0 && q.kv == 0) ? -1 : q.kv - q.n + count;
     }
 }
 

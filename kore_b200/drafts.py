@@ -194,7 +194,8 @@ class TokenTree:
 
 class AcceptedPath:
     """The accepted branch of each sequence: path [n_seq][max_path] (indexes in the chunk, -1 behind the last), count
-    [n_seq], next_token [n_seq] (the model's choice behind the last) and kept [n_seq] (positions held with them)."""
+    [n_seq], next_token [n_seq] (the model's choice behind the last) and kept [n_seq] (positions held with them; -1 for a
+    sequence that is left out, here or by the plan, of whose pages a trim then takes none)."""
 
     def __init__(self, n_seq: int, max_path: int, *, device=None):
         torch, self.device = _device(device)

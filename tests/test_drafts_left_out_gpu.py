@@ -1,0 +1,82 @@
+"""What a step with drafted tokens leaves out stays as it is through the whole step: requests that a plan did not serve,
+through acceptance and trim; chunks longer than their masks, through store and acceptance."""
+import pytest
+
+import kore_b200 as K
+from tests.test_paged_gpu import GUARD, dev, ints
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+MOST = 2 ** 31 - 1
+
+
+def state(pool):
+    return pool.free.tolist()[: int(pool.n_free)], pool.table.tolist(), pool.length.tolist()
+
+
+def held(lengths, width=9):
+    """A pool whose first requests hold so many positions."""
+    pool = K.PagePool(64, 16, 8, width)
+    step = pool.new_step(len(lengths), sum(lengths), max(lengths))
+    pool.plan(step, ints(range(len(lengths))), ints(lengths))
+    pool.check()
+    return pool
+
+
+def finished(pool, request, n_new, n_tok=50):
+    """Plan, masks, acceptance of token 0 alone and trim; what the plan and the acceptance wrote."""
+    step, tree, path = pool.new_step(len(request), n_tok, 40), K.TokenTree(n_tok, 64), K.AcceptedPath(len(request), 4)
+    none = ints([-1] * n_tok)
+    pool.plan(step, ints(request), ints(n_new))
+    tree.build(step, none)
+    path.accept(step, none, torch.zeros_like(none), none)
+    pool.trim(ints(request), path.kept)
+    torch.cuda.synchronize()
+    return step, path
+
+
+@pytest.mark.parametrize("request_,n_new,served", [
+    ([3, 0, 1], [60, 0, 0], []),             # two that want nothing, behind one whose rows pass the step's
+    ([2, 3, 0], [8, 60, 0], [0]),
+    ([0, 1], [-1, 5], [1]),                  # a negative number
+    ([3, 0, 1], [MOST, 7, 0], []),           # behind a q_start that stands at the most that 32 bits hold
+    ([3, 4, 0, 1], [MOST, MOST, 7, -2], []),
+    ([0, 0, 1], [0, 0, 3], [2])])            # named twice
+def test_requests_that_a_plan_left_out_keep_what_they_hold(request_, n_new, served):
+    lengths = [30, 20, 10]
+    pool = held(lengths)
+    free, table, _ = state(pool)
+    step, path = finished(pool, request_, n_new)
+    want = (lengths + [0] * 8)[:8]
+    for s in served:
+        want[request_[s]] += 1   # token 0
+    assert state(pool)[2] == want
+    more = [-(-b // 16) - -(-a // 16) for a, b in zip(lengths, want)]
+    assert int(pool.n_free) == len(free) - sum(more)
+    for r, (row, now) in enumerate(zip(table, pool.table.tolist())):
+        assert now[: -(-(lengths + [0] * 5)[r] // 16)] == row[: -(-(lengths + [0] * 5)[r] // 16)]
+    left = [s for s, n in enumerate(n_new) if s not in served and n != 0]
+    assert all(int(path.kept[s]) == -1 and int(path.count[s]) == 0 for s in left)
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        pool.check()
+
+
+def test_requests_that_want_nothing_are_served_whatever_the_rows():
+    """They have no rows that could pass the step's."""
+    pool = held([30, 20, 10])
+    step, path = finished(pool, [3, 0, 4, 1, -1], [60, 0, 70, 0, 3])
+    assert step.kv_len.tolist() == [0, 30, 0, 20, 0] and step.q_start.tolist() == [0, 60, 60, 130, 130, 130]
+    assert path.kept.tolist() == [-1, 30, -1, 20, -1] and path.count.tolist() == [0] * 5
+    assert pool.length.tolist() == [30, 20, 10] + [0] * 5
+
+
+def test_a_request_that_holds_nothing_and_wants_nothing_is_no_failure():
+    pool = held([30, 20, 10])
+    before = state(pool)
+    finished(pool, [5, 0, -1, 7], [0, 0, 0, 0])
+    assert state(pool) == before
+    pool.check()
+    pool.trim(ints([5, 0]), ints([-1, -1]))   # the second holds something: a negative number is reported
+    assert state(pool) == before
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        pool.check()
