@@ -778,7 +778,8 @@ int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int
 
 /* Moves the accepted tokens' keys and values together: row path[s][j] of sequence
  * s's chunk to row j of it, in every one of n_layers caches (of one type and geometry,
- * in memory of their own). batch: as the step ran with it, drafts counted. A path that does
+ * in memory of their own; a layer's keys and values too, or they are one memory, whose
+ * rows are moved once). batch: as the step ran with it, drafts counted. A path that does
  * not ascend, or leaves the chunk, is left out (7). */
 int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_layers, const kore_cuda_batch *batch,
                                const int *path, int path_stride, const int *count, int *dev_status, void *stream);

@@ -122,6 +122,15 @@ inline long long page_stride(const kore_cuda_pages *c) {
     return c->page_stride ? c->page_stride : (long long)c->n_head_kv * c->page_tokens * c->head_dim;
 }
 
+// Whether some page of the keys and some page of the values (which may lie between one another's) share memory.
+inline bool pages_overlap(const kore_cuda_pages *c) {
+    const unsigned long long b = type_bytes(c->type), page = (unsigned long long)c->n_head_kv * c->page_tokens * c->head_dim * b;
+    const unsigned long long stride = page_stride(c) * b, n = c->n_pages;
+    const uintptr_t k = reinterpret_cast<uintptr_t>(c->k), v = reinterpret_cast<uintptr_t>(c->v);
+    const unsigned long long apart = k < v ? v - k : k - v, i = apart / stride, rest = apart % stride;
+    return (i < n && rest < page) || (i + 1 < n && stride - rest < page);
+}
+
 // tables: the page table is used
 inline int check_batch(const kore_cuda_batch *b, int n_tok, bool tables = true) {
     if (!b) return refuse(KORE_CUDA_EINVAL, "the batch is null");

@@ -240,6 +240,9 @@ extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_l
     if (path_stride <= 0 || path_stride > kPagedMaxTree)
         return refuse(KORE_CUDA_EINVAL, "path_stride %d outside [1, %d]", path_stride, kPagedMaxTree);
     if (n_layers == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
+    for (int l = 0; l < n_layers; ++l)
+        if (layers[l].k != layers[l].v && pages_overlap(&layers[l]))
+            return refuse(KORE_CUDA_EINVAL, "layer %d: the keys' pages overlap the values'", l);
     OnDeviceOf on(layers->k);
     if (on.rc) return on.rc;
     CommitParams p;
@@ -259,11 +262,10 @@ extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_l
     p.by_page = FastDiv::of((uint32_t)p.P);
     p.page_pieces = page_stride(layers) * type_bytes(layers->type) / 16;
     p.status = dev_status;
-    for (int l0 = 0; l0 < n_layers; l0 += kPagedMaxLayers) {
-        p.n_layers = n_layers - l0 < kPagedMaxLayers ? n_layers - l0 : kPagedMaxLayers;
-        for (int l = 0; l < p.n_layers; ++l) {
-            p.k[l] = layers[l0 + l].k;
-            p.v[l] = layers[l0 + l].v;
+    for (int l = 0; l < n_layers;) {
+        for (p.n_pools = 0; l < n_layers && p.n_pools + 2 <= kPagedMaxPools; ++l) {
+            p.pool[p.n_pools++] = layers[l].k;
+            if (layers[l].v != layers[l].k) p.pool[p.n_pools++] = layers[l].v;   // (one memory's rows move once)
         }
         if (int rc = launched(launch_commit(p, (cudaStream_t)stream), "paged_commit")) return rc;
     }

@@ -8,7 +8,8 @@
 // accept: from token 0 on, the first child whose token is the model's choice behind its parent.
 // move: the accepted tokens path[0] < path[1] < ... stand at kv - n + path[j] and go to kv - n + j.
 //   path[j] >= j, so a row's old place is written by no token before it in the path: a thread
-//   that takes its 16 bytes of every row in the path's order may read all of them first.
+//   that takes its 16 bytes of every row in the path's order may read all of them first. Nobody else may move
+//   the same rows, so keys and values that are one memory are one pool.
 //
 // Masks and acceptance are chains of dependent looks (some tens of ns each, in shared memory). The move is bound by HBM for large batches and by its chain (path,
 // page table, row) for small ones: 16 bytes of a thread at every accepted row, eight rows on their way
@@ -171,10 +172,10 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
     while (j0 < m && rows[j0].x == rows[j0].y) ++j0;
     if (j0 == m) return;
     const int head = p.P * p.row_pieces, layer = p.G * p.row_pieces;   // pieces from head to head, of a token
-    const int all = p.n_layers * 2 * layer;
+    const int all = p.n_pools * layer;
     for (int x = blockIdx.x * blockDim.x + tid; x < all; x += gridDim.x * blockDim.x) {
         const int l = x / layer, y = x - l * layer, g = y / p.row_pieces;
-        uint4 *base = static_cast<uint4 *>((l & 1) ? p.v[l >> 1] : p.k[l >> 1]) + (long long)g * head + (y - g * p.row_pieces);
+        uint4 *base = static_cast<uint4 *>(p.pool[l]) + (long long)g * head + (y - g * p.row_pieces);
         for (int j = j0; j < m; j += 8) {
             uint4 v[8];
 #pragma unroll
@@ -194,7 +195,7 @@ cudaError_t launch_tree_mask(const TreeParams &p, cudaStream_t s) { return launc
 cudaError_t launch_accept(const TreeParams &p, cudaStream_t s) { return launch(accept_kernel, (p.n_seq + 3) / 4, 128, 0, s, p); }
 
 cudaError_t launch_commit(const CommitParams &p, cudaStream_t s) {
-    const int all = p.n_layers * 2 * p.G * p.row_pieces;
+    const int all = p.n_pools * p.G * p.row_pieces;
     const size_t smem = (size_t)p.path_stride * sizeof(longlong2);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((all + 255) / 256 < 32 ? (all + 255) / 256 : 32, p.n_seq);

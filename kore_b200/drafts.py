@@ -228,22 +228,40 @@ class AcceptedPath:
         P._check_status(self.status)
 
 
-def _check_apart(caches) -> None:
-    """Raises if two caches' pages (which may lie between one another's) share memory."""
-    v = caches[0].view
-    size = caches[0].k.element_size()
+def _overlap(cache):
+    """Whether a page of a pool at a and a page of one at b (which may lie between one another's) share memory; pools of
+    cache's geometry."""
+    v = cache.view
+    size = cache.k.element_size()
     page = v.n_head_kv * v.page_tokens * v.head_dim * size
     stride = v.page_stride * size or page
+
+    def overlap(a, b) -> bool:
+        n, rest = divmod(abs((a or 0) - (b or 0)), stride)
+        return (n < v.n_pages and rest < page) or (n + 1 < v.n_pages and stride - rest < page)
+    return overlap
+
+
+def _check_apart(caches) -> None:
+    """Raises if two caches' pages share memory."""
+    overlap = _overlap(caches[0])
     pools = [(a, i) for i, c in enumerate(caches) for a in (c.view.k, c.view.v)]
     for x, (a, i) in enumerate(pools):
         for b, j in pools[x + 1:]:
-            n, rest = divmod(abs((a or 0) - (b or 0)), stride)
-            if i != j and ((n < v.n_pages and rest < page) or (n + 1 < v.n_pages and stride - rest < page)):
+            if i != j and overlap(a, b):
                 raise ValueError(f"caches {i} and {j} share pages")
 
 
+def _check_own(caches) -> None:
+    """Raises if a cache's keys and values share memory and are not one (whose rows are moved once)."""
+    for i, c in enumerate(caches):
+        if c.view.k != c.view.v and _overlap(c)(c.view.k, c.view.v):
+            raise ValueError(f"cache {i}: the keys' pages overlap the values'")
+
+
 class PagedLayers:
-    """The caches of a model's layers, of one type and geometry, whose page tables are the same."""
+    """The caches of a model's layers, of one type and geometry, whose page tables are the same, each in memory of its own
+    (in which its keys and values may be the same)."""
 
     def __init__(self, caches):
         self.caches = caches = list(caches)
@@ -252,6 +270,7 @@ class PagedLayers:
         if any(c.device != caches[0].device for c in caches):
             raise ValueError("the caches are on different devices")
         _check_apart(caches)
+        _check_own(caches)
         self._L, self.device = P._library(), caches[0].device
         self.views = (P._Pages * len(caches))(*[c.view for c in caches])
         self._views = ctypes.addressof(self.views)

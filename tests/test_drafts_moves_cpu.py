@@ -1,0 +1,40 @@
+"""Moves in a cache whose keys and values share memory, as far as no GPU is needed. CPU only."""
+import pytest
+
+from kore_b200 import drafts
+from kore_b200 import paged as P
+from tests.test_drafts_cpu import _commit, _Pool
+from tests.test_paged_cpu import A, _pages
+
+PAGE = 4096   # 2 heads of 16 tokens of 64 values of 2 bytes
+
+
+@pytest.mark.parametrize("apart,stride,overlap", [(16, 0, True), (PAGE, 0, True), (3 * PAGE, 0, True), (4 * PAGE, 0, False),
+                                                  (4 * PAGE - 16, 0, True), (-4 * PAGE + 16, 0, True), (-4 * PAGE, 0, False),
+                                                  (PAGE, 2 * PAGE, False), (PAGE + 16, 2 * PAGE, True), (-PAGE, 2 * PAGE, False),
+                                                  (6 * PAGE, 2 * PAGE, True), (7 * PAGE + 16, 2 * PAGE, False)])
+def test_keys_that_overlap_the_values_are_refused(apart, stride, overlap):
+    """Two threads would move the shared rows, the second from where the first has written."""
+    k, v = 16 * A, 16 * A + apart
+    spans = [[range(x + i * (stride or PAGE), x + i * (stride or PAGE) + PAGE) for i in range(4)] for x in (k, v)]
+    assert overlap == any(max(a.start, b.start) < min(a.stop, b.stop) for a in spans[0] for b in spans[1])
+    layers = (P._Pages * 2)(_pages(k=A), _pages(k=k, v=v, page_stride=stride // 2))
+    layers[0].page_stride, layers[0].v = stride // 2, A + 64 * PAGE   # (of the same geometry, apart)
+    rc, msg = _commit(layers, 2)
+    assert (rc == -1 and "layer 1: the keys' pages overlap" in msg) == overlap, msg
+    pool = _Pool(k, v, n_pages=4, page_stride=stride // 2)
+    if overlap:
+        with pytest.raises(ValueError, match="cache 0: the keys' pages overlap"):
+            drafts._check_own([pool])
+    else:
+        drafts._check_own([pool])
+
+
+def test_keys_and_values_in_one_memory_are_no_overlap():
+    """Their rows are moved once."""
+    for check in (drafts._check_apart, drafts._check_own):
+        check([_Pool(A, A), _Pool(16 * A, 16 * A)])
+    with pytest.raises(ValueError, match="caches 0 and 1 share pages"):
+        drafts._check_apart([_Pool(A, A), _Pool(A, A)])
+    rc, msg = _commit()
+    assert "overlap" not in msg
