@@ -605,7 +605,8 @@ typedef struct kore_cuda_batch {
  * rows. k, v, q and q_out have one type; the cache has it too, or fewer bits
  * (F32 to F16 or BF16; any to E4M3: x / scale rounded to nearest even, values
  * beyond +-448 to +-448; 0 where the scale is 0). Positions must be distinct: no two sequences may
- * write the same slot of a page. */
+ * write the same slot of a page. A cache whose keys and values share memory is refused, unless they are one
+ * memory and k and v the same rows, stored as they are. */
 int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const kore_cuda_batch *batch, int n_tok,
                                const kore_cuda_rows *k, const kore_cuda_rows *v, const kore_cuda_rows *q,
                                const kore_cuda_rows *q_out, const kore_cuda_rope_view *rope, int *dev_status,

@@ -131,6 +131,16 @@ inline bool pages_overlap(const kore_cuda_pages *c) {
     return (i < n && rest < page) || (i + 1 < n && stride - rest < page);
 }
 
+// Keys and values that go into memory that the cache's share: which of them stayed would be chance, unless it is one
+// memory and they are the same. changed: the keys are normed or rotated on the way.
+inline int check_stored_apart(const kore_cuda_pages *c, const kore_cuda_rows *k, const kore_cuda_rows *v, bool changed) {
+    if (!pages_overlap(c)) return KORE_CUDA_OK;
+    const bool alike = c->k == c->v && k->data == v->data && k->token_stride == v->token_stride &&
+                       k->head_stride == v->head_stride && c->k_scale == c->v_scale && !changed;
+    if (alike) return KORE_CUDA_OK;
+    return refuse(KORE_CUDA_EINVAL, "the cache's keys and values share memory, and k and v are not the same rows");
+}
+
 // tables: the page table is used
 inline int check_batch(const kore_cuda_batch *b, int n_tok, bool tables = true) {
     if (!b) return refuse(KORE_CUDA_EINVAL, "the batch is null");

@@ -168,6 +168,7 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
     if (rope)
         if (int rc = check_rope(rope, d)) return rc;
     if (n_tok == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
+    if (int rc = check_stored_apart(cache, k, v, rope != nullptr)) return rc;
     OnDeviceOf on(cache->k);
     if (on.rc) return on.rc;
     RotateParams p;

@@ -127,6 +127,7 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
                       (uintptr_t)(norm->q_head_stride * b) | (uintptr_t)(norm->k_head_stride * b)) & 15) == 0;
     }
     if (n_tok == 0) return KORE_CUDA_OK;
+    if (int rc = check_stored_apart(cache, k, v, rope || (norm && norm->k_weight))) return rc;
     OnDeviceOf on(cache->k);
     if (on.rc) return on.rc;
     StoreParams p;

@@ -3,8 +3,8 @@ import pytest
 
 from kore_b200 import drafts
 from kore_b200 import paged as P
-from tests.test_drafts_cpu import _commit, _Pool
-from tests.test_paged_cpu import A, _pages
+from tests.test_drafts_cpu import _commit, _norm, _Pool, _store, err
+from tests.test_paged_cpu import A, B, _batch, _pages, _ref, _rows
 
 PAGE = 4096   # 2 heads of 16 tokens of 64 values of 2 bytes
 
@@ -38,3 +38,21 @@ def test_keys_and_values_in_one_memory_are_no_overlap():
         drafts._check_apart([_Pool(A, A), _Pool(A, A)])
     rc, msg = _commit()
     assert "overlap" not in msg
+
+
+@pytest.mark.parametrize("cache,k,v,rope,norm,refused", [
+    (dict(), {}, {}, False, None, False), (dict(), {}, dict(data=B), False, None, True),
+    (dict(), {}, dict(ts=256), False, None, True), (dict(), {}, {}, True, None, True),
+    (dict(), {}, {}, False, dict(k_weight=None), False), (dict(), {}, {}, False, dict(), True),
+    (dict(v=A + PAGE), {}, {}, False, None, True), (dict(v=A + 4 * PAGE), {}, dict(data=B), True, dict(), False),
+    (dict(v=A + PAGE, page_stride=PAGE), {}, dict(data=B), True, None, False)])
+def test_different_rows_into_one_memory_are_refused(cache, k, v, rope, norm, refused):
+    """Which of them stayed would be chance."""
+    pages, k, v = _pages(**cache), _rows(**k), _rows(**v)
+    rope = P._RopeView(A, 8, 64, 0) if rope else None
+    calls = [_store(cache=pages, k=k, v=v, rope=rope, norm=None if norm is None else _norm(**norm))]
+    if norm is None:
+        calls.append(err(P._library().kore_cuda_paged_append_dev(
+            _ref(pages), _ref(_batch()), 1, _ref(k), _ref(v), None, None, _ref(rope), None, None)))
+    for rc, msg in calls:
+        assert (rc == -1 and "share memory" in msg) == refused, msg
