@@ -745,9 +745,9 @@ typedef struct kore_cuda_tree {
 /* Masks and positions from parents: parent[t] is the index in the chunk of token
  * t's parent, less than its own, or -1. mask receives the token's ancestors and
  * itself, pos its sequence's context length and its depth. A token with a parent
- * that is not before it above it is left out (7; mask 0, position -1); so is a sequence
- * whose chunk is longer than its kv_len or than the mask's words (its rows are not
- * written). Rows outside every sequence are not touched. */
+ * that is not before it above it is left out (7; mask 0, position -1); so are all of a
+ * chunk that is longer than the mask's words, and a sequence whose chunk is longer than
+ * its kv_len (its rows are not written). Rows outside every sequence are not touched. */
 int kore_cuda_tree_masks_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, unsigned *mask, int words,
                              int *pos, int *dev_status, void *stream);
 

@@ -37,12 +37,22 @@ __device__ __forceinline__ Seq tree_seq(const TreeParams &p, int s, bool report)
 }
 
 // A CTA a sequence, a thread a token: the way up the parents, which stand in shared memory, goes to ever
-// lower bits.
+// lower bits. The tokens of a chunk longer than the masks see nothing and have no position, so that a store leaves
+// them out: what stood there may be another step's.
 __global__ void __launch_bounds__(128) tree_mask_kernel(const __grid_constant__ TreeParams p) {
     grid_dep_wait();
     grid_dep_launch();
     __shared__ int parent[kPagedMaxTree];
     const Seq q = tree_seq(p, blockIdx.x, threadIdx.x == 0);
+    if (q.n < 0) {
+        const int n = __ldg(p.q_start + blockIdx.x + 1) - q.q0;
+        if (n <= p.most || q.q0 < 0 || q.q0 > p.n_tok - n || q.kv < n) return;   // its rows are no chunk's
+        for (int i = threadIdx.x; i < n; i += blockDim.x) {
+            for (int y = 0; y < p.words; ++y) p.mask[(long long)(q.q0 + i) * p.words + y] = 0;
+            p.pos[q.q0 + i] = -1;
+        }
+        return;
+    }
     for (int i = threadIdx.x; i < q.n; i += blockDim.x) parent[i] = __ldg(p.parent + q.q0 + i);
     __syncthreads();
     for (int i = threadIdx.x; i < q.n; i += blockDim.x) {

@@ -80,3 +80,31 @@ def test_a_request_that_holds_nothing_and_wants_nothing_is_no_failure():
     assert state(pool) == before
     with pytest.raises(K.KoreCudaError, match="bounds"):
         pool.check()
+
+
+@pytest.mark.parametrize("most,n", [(32, 33), (32, 40), (64, 300), (1024, 1025)])
+def test_masks_of_a_chunk_that_is_too_long_are_not_another_steps(most, n):
+    """Its tokens have no position, so that a store leaves out their rows; those of the others are as ever."""
+    n_tok = n + 7
+    tree = K.TokenTree(n_tok, most)
+    chain = ints(range(-1, n_tok - 1))
+    tree.build(K.PagedBatch(ints([0, most]), ints([most + 5]), ints([[0]]), most), chain)
+    tree.check()
+    parent = ints(list(range(-1, n - 1)) + [-1, 0, 0, 1, -1] + [-1, -1])
+    tree.mask[n + 5:], tree.pos[n + 5:] = 77, 77
+    tree.build(K.PagedBatch(ints([0, n, n + 5]), ints([n + 9, 25]), ints([[0], [0]]), n), parent)
+    assert (tree.pos[:n] == -1).all() and (tree.mask[:n] == 0).all()
+    assert tree.pos[n:].tolist() == [20, 21, 21, 22, 20, 77, 77]
+    assert tree.mask[n:, 0].tolist() == [1, 3, 5, 11, 16, 77, 77]
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        tree.check()
+    kp, vp = (torch.full((n // 8 + 8, 1, 16, 64), GUARD, device=dev(), dtype=torch.bfloat16) for _ in range(2))
+    cache, rows = K.PagedCache(kp, vp), torch.ones(n_tok, 1, 64, device=dev(), dtype=torch.bfloat16)
+    q, q_out = rows, torch.full_like(rows, GUARD)
+    slots = torch.arange(n_tok, device=dev())
+    slots[n + 5:] = -1
+    cache.store(slots, tree.pos, rows, rows, rope=K.RopeTable(n + 20, 64), q=q, q_out=q_out)
+    cache.check()
+    written = (vp[:, 0, :, 0] == 1).flatten().nonzero().flatten().tolist()
+    assert written == list(range(n, n + 5))
+    assert (q_out[:n] == GUARD).all() and (q_out[n + 5:] == GUARD).all() and not (q_out[n:n + 5] == GUARD).any(-1).any()
