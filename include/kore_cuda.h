@@ -660,7 +660,7 @@ int kore_cuda_paged_attn_dev(const kore_cuda_pages *cache, const kore_cuda_batch
  *                               of queries and keys for each head and the rotation
  *   kore_cuda_paged_tree_attn_dev  a layer: the tokens' attention over the context
  *                               and their own branches
- *   kore_cuda_tree_accept_dev   the branch that the model's choices follow
+ *   kore_cuda_tree_accept_masked_dev  the branch that the model's choices follow
  *   kore_cuda_paged_commit_dev  its keys and values moved together, in all layers
  *   kore_cuda_paged_trim_dev    the pages of the refused drafts given back
  * Plan, store and trim serve steps without trees as well. Pointers, streams, device
@@ -772,10 +772,18 @@ typedef struct kore_cuda_accepted {
 
 /* The branch that the model follows: from token 0 of each chunk on, the first child
  * (by index) whose token[t] is choice of its parent (the model's token behind it; all
- * device [n_tok]), and so on. A sequence that does not fit (as for the masks, or of more
- * than 1024 tokens) is left out (7): count 0, kept -1. */
+ * device [n_tok]), and so on. A sequence whose rows do not fit, or whose chunk is longer
+ * than its kv_len or than 1024 tokens, is left out (7): count 0, kept -1. */
 int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
                               const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream);
+
+/* The same for a step whose masks have `words` words: a chunk that is longer than 32 * words
+ * tokens, which masks, store and attention leave out (so that its choices mean nothing), is
+ * left out here too. (Its request still has the positions that a plan gave it; a trim to
+ * its context takes them back.) */
+int kore_cuda_tree_accept_masked_dev(const kore_cuda_batch *batch, int n_tok, int words, const int *parent,
+                                     const int *token, const int *choice, const kore_cuda_accepted *out,
+                                     int *dev_status, void *stream);
 
 /* Moves the accepted tokens' keys and values together: row path[s][j] of sequence
  * s's chunk to row j of it, in every one of n_layers caches (of one type and geometry,

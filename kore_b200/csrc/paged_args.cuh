@@ -178,12 +178,16 @@ inline int check_appended(const kore_cuda_pages *cache, const kore_cuda_rows *k,
     return KORE_CUDA_OK;
 }
 
+inline int check_words(int words) {
+    if (words <= 0 || words > kPagedMaxTree / 32)
+        return refuse(KORE_CUDA_EINVAL, "the tree's words %d outside [1, %d]", words, kPagedMaxTree / 32);
+    return KORE_CUDA_OK;
+}
+
 inline int check_tree(const kore_cuda_tree *t) {
     if (!t->mask) return refuse(KORE_CUDA_EINVAL, "the tree's mask is null");
     if (reinterpret_cast<uintptr_t>(t->mask) & 3) return refuse(KORE_CUDA_EINVAL, "the tree's mask is not aligned to its type");
-    if (t->words <= 0 || t->words > kPagedMaxTree / 32)
-        return refuse(KORE_CUDA_EINVAL, "the tree's words %d outside [1, %d]", t->words, kPagedMaxTree / 32);
-    return KORE_CUDA_OK;
+    return check_words(t->words);
 }
 
 inline bool rotates_in_vectors(int d, const kore_cuda_rope_view *r) { return d % 16 == 0 && (!r || r->n_rot % 16 == 0); }

@@ -189,8 +189,9 @@ extern "C" int kore_cuda_tree_masks_dev(const kore_cuda_batch *batch, int n_tok,
     return launched(launch_tree_mask(p, (cudaStream_t)stream), "tree_masks");
 }
 
-extern "C" int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
-                                         const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream) {
+// most: tokens of a chunk at most
+static int accept(const kore_cuda_batch *batch, int n_tok, int most, const int *parent, const int *token, const int *choice,
+                  const kore_cuda_accepted *out, int *dev_status, void *stream) {
     if (int rc = check_batch(batch, n_tok, false)) return rc;
     if (!parent || !token || !choice) return refuse(KORE_CUDA_EINVAL, "parent, token or choice is null");
     if (!out || !out->path || !out->count || !out->next_token || !out->kept)
@@ -203,13 +204,25 @@ extern "C" int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok
     TreeParams p = tree_params(batch, n_tok, parent, dev_status);
     p.token = token;
     p.choice = choice;
-    p.most = kPagedMaxTree;
+    p.most = most;
     p.path = out->path;
     p.path_stride = out->path_stride;
     p.count = out->count;
     p.next = out->next_token;
     p.kept = out->kept;
     return launched(launch_accept(p, (cudaStream_t)stream), "tree_accept");
+}
+
+extern "C" int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
+                                         const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream) {
+    return accept(batch, n_tok, kPagedMaxTree, parent, token, choice, out, dev_status, stream);
+}
+
+extern "C" int kore_cuda_tree_accept_masked_dev(const kore_cuda_batch *batch, int n_tok, int words, const int *parent,
+                                                const int *token, const int *choice, const kore_cuda_accepted *out,
+                                                int *dev_status, void *stream) {
+    if (int rc = check_words(words)) return rc;
+    return accept(batch, n_tok, words * 32, parent, token, choice, out, dev_status, stream);
 }
 
 extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_layers, const kore_cuda_batch *batch,

@@ -12,7 +12,7 @@ A step, on the current stream of the tensors' device::
     for cache in layers:                                   # q, k, v of the layer's product
         cache.store(step.slots, tree.pos, k, v, rope=rope, norm=norm, q=q, q_out=q)
         cache.attend(step, q, out, tree=tree)
-    path.accept(step, parent, token, choice)               # the branch that the model's choices follow
+    path.accept(step, parent, token, choice, tree=tree)    # the branch that the model's choices follow
     PagedLayers(layers).commit(step, path)                 # (made once) its rows moved together
     pool.trim(request, path.kept)                          # the refused drafts' pages
 
@@ -210,16 +210,22 @@ class AcceptedPath:
                                 self.kept.data_ptr())
         self._view = ctypes.addressof(self.view)
 
-    def accept(self, batch: PagedBatch, parent, token, choice) -> None:
+    def accept(self, batch: PagedBatch, parent, token, choice, *, tree: TokenTree | None = None) -> None:
         """From token 0 of each chunk on, the first child whose token is the model's choice behind its parent, and so on
-        (parent as for TokenTree.build, token and choice [n_tok]; all int32)."""
+        (parent as for TokenTree.build, token and choice [n_tok]; all int32). tree: the step's, whose masks a chunk may be
+        too long for: it is left out then, as it was by build, store and attention (without tree: of chunks beyond 1024
+        tokens only)."""
         pp, n = _ints(parent, "parent", self.device, 1), parent.shape[0]
         pt, pc = _ints(token, "token", self.device, 1, n), _ints(choice, "choice", self.device, 1, n)
         if batch.device != self.device or batch.view.n_seq != self.path.shape[0]:
             raise ValueError(f"expected a batch of {self.path.shape[0]} sequences on {self.device}")
+        if tree is not None and (tree.device != self.device or tree.mask.shape[0] != n):
+            raise ValueError(f"tree: expected masks of {n} tokens on {self.device}")
         if batch.view.n_seq == 0:
             return
-        rc = self._L.kore_cuda_tree_accept_dev(batch._view, n, pp, pt, pc, self._view, self._status, _stream(self.device))
+        words = tree.view.words if tree is not None else MAX_TREE // 32
+        rc = self._L.kore_cuda_tree_accept_masked_dev(batch._view, n, words, pp, pt, pc, self._view, self._status,
+                                                      _stream(self.device))
         if rc:
             _ck(self._L, rc)
 

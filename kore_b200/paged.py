@@ -119,6 +119,7 @@ def _library():
         L.kore_cuda_tree_masks_dev.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp]
         L.kore_cuda_paged_tree_attn_dev.argtypes = [_vp, _vp, _i] + [_vp] * 6 + [_ll, _vp, _vp]
         L.kore_cuda_tree_accept_dev.argtypes = [_vp, _i] + [_vp] * 6
+        L.kore_cuda_tree_accept_masked_dev.argtypes = [_vp, _i, _i] + [_vp] * 6
         L.kore_cuda_paged_commit_dev.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp]
         L.kore_cuda_paged_set_wait_limit.argtypes = [ctypes.c_ulonglong]
         L.kore_cuda_capture_id.argtypes = [_vp]

@@ -108,3 +108,25 @@ def test_masks_of_a_chunk_that_is_too_long_are_not_another_steps(most, n):
     written = (vp[:, 0, :, 0] == 1).flatten().nonzero().flatten().tolist()
     assert written == list(range(n, n + 5))
     assert (q_out[:n] == GUARD).all() and (q_out[n + 5:] == GUARD).all() and not (q_out[n:n + 5] == GUARD).any(-1).any()
+
+
+@pytest.mark.parametrize("most,n", [(32, 33), (64, 70), (64, 1000)])
+def test_a_chunk_that_is_too_long_for_its_masks_is_not_accepted(most, n):
+    """What the model chose behind its tokens means nothing: the attention has left them out."""
+    pool = K.PagePool(n // 16 + 20, 16, 8, n // 16 + 9)
+    step, tree, path = pool.new_step(2, n + 6, n), K.TokenTree(n + 6, most), K.AcceptedPath(2, 4)
+    pool.plan(step, ints([0, 1]), ints([n, 6]))
+    parent = ints(list(range(-1, n - 1)) + list(range(-1, 5)))
+    ones = torch.ones_like(parent)
+    tree.build(step, parent)
+    path.accept(step, parent, ones, ones, tree=tree)
+    assert path.count.tolist() == [0, 4] and path.kept.tolist() == [-1, 4] and path.next_token.tolist() == [-1, 1]
+    assert path.path.tolist() == [[-1] * 4, [0, 1, 2, 3]]
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        path.check()
+    path.accept(step, parent[:n], ones[:n], ones[:n])   # (without the masks, and rows for the first chunk alone)
+    assert path.count.tolist() == [4, 0]
+    with pytest.raises(K.KoreCudaError, match="bounds"):
+        path.check()
+    with pytest.raises(ValueError, match="tree"):
+        path.accept(step, parent[:n], ones[:n], ones[:n], tree=tree)

@@ -1,4 +1,5 @@
-"""Moves in a cache whose keys and values share memory, as far as no GPU is needed. CPU only."""
+"""Stores into and moves in a cache whose keys and values share memory, and the acceptance of a step with masks, as far as
+no GPU is needed. CPU only."""
 import pytest
 
 from kore_b200 import drafts
@@ -56,3 +57,13 @@ def test_different_rows_into_one_memory_are_refused(cache, k, v, rope, norm, ref
             _ref(pages), _ref(_batch()), 1, _ref(k), _ref(v), None, None, _ref(rope), None, None)))
     for rc, msg in calls:
         assert (rc == -1 and "share memory" in msg) == refused, msg
+
+
+@pytest.mark.parametrize("words", [-1, 0, 33])
+def test_an_acceptance_with_masks_of_no_size_is_refused(words):
+    out = P._Accepted(A, 4, A, A, A)
+    call = P._library().kore_cuda_tree_accept_masked_dev
+    rc, msg = err(call(_ref(_batch()), 1, words, A, A, A, _ref(out), None, None))
+    assert rc == -1 and "words" in msg
+    assert err(call(_ref(_batch()), 1, 1, None, A, A, _ref(out), None, None))[0] == -1
+    assert call(_ref(_batch(n_seq=0)), 1, 32, A, A, A, _ref(out), None, None) == 0
