@@ -89,7 +89,7 @@ struct StoreParams {
     const void *q_weight, *k_weight;   // null: those heads have no norm
     int weight_type;
     long long q_weight_hs, k_weight_hs;
-    float eps;
+    float eps, most;                   // most: heads whose squares' sum passes it are scaled
     int *status;
 };
 

@@ -161,6 +161,7 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
         p.q_weight_hs = norm->q_head_stride;
         p.k_weight_hs = norm->k_head_stride;
         p.eps = norm->eps;
+        p.most = norm->eps < 0x1p100f ? 3.0e38f : 0.f;   // (mean and eps together stay in 32 bits)
     }
     p.status = dev_status;
     const bool vec = (d == 64 || d == 128 || d == 256) && rotates_in_vectors(d, rope) && weights16 &&

@@ -3,7 +3,8 @@
 //
 // y = x / sqrt(mean(x^2) + eps) * w over a head's d values, then the rotation of
 // paged_rope.cu at the token's position, then one rounding to the output's type. The
-// mean and all else in 32 bits; a head whose squares overflow them is scaled by 2^-96 for its sum.
+// mean and all else in 32 bits; a head whose squares (or, with an eps of such a size, their mean and eps) overflow them
+// is scaled by 2^-96 for its sum, and eps with it.
 //
 // Bound by HBM in bytes (every value is read once and written once), and nearly as much by
 // instructions: some 110 for 16 values of a lane, half of them the rotation's separate products and
@@ -44,17 +45,20 @@ __device__ __forceinline__ float rsqrt_normal(float x) {
     return y;
 }
 
+// eps beside a mean of squares of values times 2^-96
+__device__ __forceinline__ float eps_scaled(float eps) { return __fmul_rn(__fmul_rn(eps, 0x1p-96f), 0x1p-96f); }
+
 // 1 / sqrt(mean + eps) from the head's sum of squares, to be followed by a factor `post`: 1, or 2^-96
-// for heads whose squares pass 32 bits, of which again() gives the sum of (x 2^-96)^2 (eps is
-// nothing beside that). The factor stays apart, since their root is below the normal numbers.
+// for heads whose sum passes `most`, of which again() gives the sum of (x 2^-96)^2.
+// The factor stays apart, since their root is below the normal numbers.
 template <typename F>
-__device__ __forceinline__ float root(float sum, int d, float eps, float &post, F again) {
+__device__ __forceinline__ float root(float sum, int d, float eps, float most, float &post, F again) {
     post = 1.f;
-    if (__any_sync(FULL, sum > 3.0e38f)) {
+    if (__any_sync(FULL, sum > most)) {
         const float small = again();
-        if (sum > 3.0e38f) {
+        if (sum > most) {
             post = 0x1p-96f;
-            return rsqrt_normal(__fdiv_rn(small, (float)d));
+            return rsqrt_normal(__fadd_rn(__fdiv_rn(small, (float)d), eps_scaled(eps)));
         }
     }
     return rsqrt_normal(__fadd_rn(__fdiv_rn(sum, (float)d), eps));
@@ -115,9 +119,9 @@ struct Angles {
 };
 
 // a and b: B heads' 16 values a lane, normed and times their weights; by whole warps, the L lanes of a head
-// side by side. weigh(k, wa, wb) gives head k's weights.
+// side by side. weigh(k, wa, wb) gives head k's weights; most: as for root().
 template <int D, int B, typename F>
-__device__ __forceinline__ void norm_heads(Pair (&a)[B][4], Pair (&b)[B][4], float eps, F weigh) {
+__device__ __forceinline__ void norm_heads(Pair (&a)[B][4], Pair (&b)[B][4], float eps, float most, F weigh) {
     // step by step for all of the heads, so that their chains run side by side
     float f[B], post[B];
     auto squares = [&](float x) {
@@ -144,7 +148,7 @@ __device__ __forceinline__ void norm_heads(Pair (&a)[B][4], Pair (&b)[B][4], flo
     bool over = false;
 #pragma unroll
     for (int k = 0; k < B; ++k) {
-        over |= f[k] > 3.0e38f;
+        over |= f[k] > most;
         post[k] = 1.f;
     }
     const bool any = __any_sync(FULL, over);
@@ -155,13 +159,13 @@ __device__ __forceinline__ void norm_heads(Pair (&a)[B][4], Pair (&b)[B][4], flo
         squares(0x1p-96f);
 #pragma unroll
         for (int k = 0; k < B; ++k) {
-            if (g[k] > 3.0e38f) post[k] = 0x1p-96f;   // (eps is nothing beside it)
+            if (g[k] > most) post[k] = 0x1p-96f;
             else f[k] = g[k];
         }
     }
 #pragma unroll
     for (int k = 0; k < B; ++k) {
-        f[k] = rsqrt_normal(post[k] != 1.f ? f[k] * (1.f / D) : __fadd_rn(f[k] * (1.f / D), eps));
+        f[k] = rsqrt_normal(__fadd_rn(f[k] * (1.f / D), post[k] != 1.f ? eps_scaled(eps) : eps));
         Pair wa[4], wb[4];
         weigh(k, wa, wb);
         const Pair ff = pk2(f[k], f[k]);
@@ -254,7 +258,7 @@ __device__ __forceinline__ void store_heads(const StoreParams &p, int t, int str
         for (int k = 0; k < B; ++k) widen(raw[k], a[k], b[k]);
         load_rows(raw, t + stride);
         if (at.page >= 0 && wt)
-            norm_heads<D, B>(a, b, p.eps, [&](int k, Pair (&x)[4], Pair (&y)[4]) {
+            norm_heads<D, B>(a, b, p.eps, p.most, [&](int k, Pair (&x)[4], Pair (&y)[4]) {
                 if (k > 0 && w_hs) load_weights(k, x, y);
                 else {
 #pragma unroll
@@ -361,7 +365,7 @@ __global__ void __launch_bounds__(256) store_pairs_kernel(const __grid_constant_
                 return sum;
             };
             float post;
-            const float f = root(squares(1.f), p.d, p.eps, post, [&]() { return squares(0x1p-96f); });
+            const float f = root(squares(1.f), p.d, p.eps, p.most, post, [&]() { return squares(0x1p-96f); });
             const long long w0 = (long long)hh * (is_q ? p.q_weight_hs : p.k_weight_hs);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
