@@ -495,7 +495,7 @@ int kore_cuda_attn_decode_noalloc(const kore_cuda_kv_view *kv, int pos, const fl
  *                              and values, and rotates its queries
  *   kore_cuda_paged_attn_dev   attention of the batch's queries over the cache
  *
- * All pointers are device pointers; calls are ordered on `stream` (a
+ * All pointers are device pointers, aligned to their type (refused otherwise); calls are ordered on `stream` (a
  * cudaStream_t of the device that holds the buffers; NULL for the default
  * stream), allocate nothing, return without synchronising and can be captured
  * into a graph. What they read, the batch's arrays among it, must not change

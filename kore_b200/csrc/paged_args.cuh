@@ -79,6 +79,12 @@ inline int check_rows(const kore_cuda_rows *r, const char *name, int head_dim) {
     return KORE_CUDA_OK;
 }
 
+// Arrays of 32-bit values: a kernel's load or store off their alignment would fault.
+template <typename... P>
+bool words_aligned(const P *...p) {
+    return ((... | reinterpret_cast<uintptr_t>(p)) & 3) == 0;
+}
+
 // Rows that are written: several in one place would leave whichever came last.
 inline int check_written(const kore_cuda_rows *r, const char *name, int n_tok) {
     if ((n_tok > 1 && r->token_stride == 0) || (r->n_head > 1 && r->head_stride == 0))
@@ -115,6 +121,7 @@ inline int check_pages(const kore_cuda_pages *c, bool attention) {
                       c->page_stride, page);
     if (c->type != KORE_CUDA_E4M3 && (c->k_scale || c->v_scale))
         return refuse(KORE_CUDA_EINVAL, "scales belong to an E4M3 cache");
+    if (!words_aligned(c->k_scale, c->v_scale)) return refuse(KORE_CUDA_EINVAL, "the scales are not aligned to their type");
     return KORE_CUDA_OK;
 }
 
@@ -149,6 +156,8 @@ inline int check_batch(const kore_cuda_batch *b, int n_tok, bool tables = true) 
         return refuse(KORE_CUDA_ERANGE, "n_seq %d outside [0, %d]", b->n_seq, kPagedMaxSeqs);
     if (b->n_seq > 0 && (!b->q_start || !b->kv_len || (tables && !b->page_table)))
         return refuse(KORE_CUDA_EINVAL, "q_start, kv_len or page_table is null");
+    if (!words_aligned(b->q_start, b->kv_len, b->page_table))
+        return refuse(KORE_CUDA_EINVAL, "q_start, kv_len or page_table is not aligned to its type");
     if (tables && b->n_seq > 0 && b->table_stride <= 0) return refuse(KORE_CUDA_EINVAL, "table_stride %d", b->table_stride);
     if (b->max_q < 0) return refuse(KORE_CUDA_EINVAL, "max_q %d", b->max_q);
     if (b->max_kv < 0) return refuse(KORE_CUDA_EINVAL, "max_kv %d", b->max_kv);
@@ -186,7 +195,7 @@ inline int check_words(int words) {
 
 inline int check_tree(const kore_cuda_tree *t) {
     if (!t->mask) return refuse(KORE_CUDA_EINVAL, "the tree's mask is null");
-    if (reinterpret_cast<uintptr_t>(t->mask) & 3) return refuse(KORE_CUDA_EINVAL, "the tree's mask is not aligned to its type");
+    if (!words_aligned(t->mask)) return refuse(KORE_CUDA_EINVAL, "the tree's mask is not aligned to its type");
     return check_words(t->words);
 }
 

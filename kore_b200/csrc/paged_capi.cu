@@ -130,6 +130,7 @@ extern "C" int kore_cuda_rope_table_dev(const kore_cuda_rope_spec *spec, int n_p
 extern "C" int kore_cuda_rope_dev(const kore_cuda_rows *x, const kore_cuda_rows *out, int n_tok, const int *pos,
                                   const kore_cuda_rope_view *rope, int *dev_status, void *stream) {
     if (!x || !rope || !pos) return refuse(KORE_CUDA_EINVAL, "null argument");
+    if (!words_aligned(pos, dev_status)) return refuse(KORE_CUDA_EINVAL, "pos or dev_status is not aligned to its type");
     const int d = x->head_dim;
     if (d < 2 || (d & 1) || d > 256) return refuse(KORE_CUDA_EINVAL, "head_dim %d must be even, 2 to 256", d);
     if (int rc = check_rows(x, "x", d)) return rc;
@@ -165,6 +166,7 @@ extern "C" int kore_cuda_paged_append_dev(const kore_cuda_pages *cache, const ko
     if (int rc = check_batch(batch, n_tok)) return rc;
     const int d = cache->head_dim;
     if (int rc = check_appended(cache, k, v, q, q_out, n_tok)) return rc;
+    if (!words_aligned(dev_status)) return refuse(KORE_CUDA_EINVAL, "dev_status is not aligned to its type");
     if (rope)
         if (int rc = check_rope(rope, d)) return rc;
     if (n_tok == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
@@ -236,6 +238,7 @@ static int attend(const kore_cuda_pages *cache, const kore_cuda_batch *batch, in
     if ((long long)n_tok * (q->n_head / G) > 0x7fffffffll - kPagedRowsMax)
         return refuse(KORE_CUDA_ERANGE, "%d tokens are too many for one call", n_tok);
     if (!opts) return refuse(KORE_CUDA_EINVAL, "opts is null");
+    if (!words_aligned(lse, dev_status)) return refuse(KORE_CUDA_EINVAL, "lse or dev_status is not aligned to its type");
     if (opts->window < 0) return refuse(KORE_CUDA_EINVAL, "window %d", opts->window);
     if (!std::isfinite(opts->scale)) return refuse(KORE_CUDA_EINVAL, "scale is not finite");
     if (tree) {

@@ -10,7 +10,7 @@
 namespace kore {
 namespace {
 
-int check_pool(const kore_cuda_page_pool *p, int n_seq, const int *request, const int *amount) {
+int check_pool(const kore_cuda_page_pool *p, int n_seq, const int *request, const int *amount, const int *status) {
     if (!p || !p->free_pages || !p->n_free || !p->table || !p->length) return refuse(KORE_CUDA_EINVAL, "the pool is null");
     if (p->n_pages <= 0) return refuse(KORE_CUDA_EINVAL, "n_pages %d must be positive", p->n_pages);
     if (p->page_tokens <= 0 || p->page_tokens % 16)
@@ -20,6 +20,8 @@ int check_pool(const kore_cuda_page_pool *p, int n_seq, const int *request, cons
     if (p->table_stride <= 0) return refuse(KORE_CUDA_EINVAL, "table_stride %d", p->table_stride);
     if (n_seq < 0 || n_seq > kPagedMaxSeqs) return refuse(KORE_CUDA_ERANGE, "n_seq %d outside [0, %d]", n_seq, kPagedMaxSeqs);
     if (n_seq > 0 && (!request || !amount)) return refuse(KORE_CUDA_EINVAL, "request, n_new or keep is null");
+    if (!words_aligned(p->free_pages, p->n_free, p->table, p->length, request, amount, status))
+        return refuse(KORE_CUDA_EINVAL, "an array of the pool, request, n_new, keep or dev_status is not aligned to its type");
     return KORE_CUDA_OK;
 }
 
@@ -68,13 +70,13 @@ using namespace kore;
 
 extern "C" int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *n_new,
                                         const kore_cuda_step *step, int *dev_status, void *stream) {
-    if (int rc = check_pool(pool, n_seq, request, n_new)) return rc;
+    if (int rc = check_pool(pool, n_seq, request, n_new, dev_status)) return rc;
     if (!step || !step->q_start) return refuse(KORE_CUDA_EINVAL, "the step is null");
     if (int rc = check_tokens(step->n_tok)) return rc;
     if (n_seq > 0 && (!step->kv_len || !step->page_table)) return refuse(KORE_CUDA_EINVAL, "kv_len or page_table is null");
     if (step->n_tok > 0 && (!step->slots || !step->pos)) return refuse(KORE_CUDA_EINVAL, "slots or pos is null");
-    if ((reinterpret_cast<uintptr_t>(step->slots) & 7) || (reinterpret_cast<uintptr_t>(step->pos) & 3))
-        return refuse(KORE_CUDA_EINVAL, "slots or pos is not aligned to its type");
+    if ((reinterpret_cast<uintptr_t>(step->slots) & 7) || !words_aligned(step->q_start, step->kv_len, step->page_table, step->pos))
+        return refuse(KORE_CUDA_EINVAL, "an array of the step is not aligned to its type");
     if (step->table_stride < pool->table_stride)
         return refuse(KORE_CUDA_EINVAL, "the step's table_stride %d is less than the pool's %d", step->table_stride, pool->table_stride);
     OnDeviceOf on(pool->table);
@@ -92,7 +94,7 @@ extern "C" int kore_cuda_paged_plan_dev(const kore_cuda_page_pool *pool, int n_s
 
 extern "C" int kore_cuda_paged_trim_dev(const kore_cuda_page_pool *pool, int n_seq, const int *request, const int *keep,
                                         int *dev_status, void *stream) {
-    if (int rc = check_pool(pool, n_seq, request, keep)) return rc;
+    if (int rc = check_pool(pool, n_seq, request, keep, dev_status)) return rc;
     if (n_seq == 0) return KORE_CUDA_OK;
     OnDeviceOf on(pool->table);
     if (on.rc) return on.rc;
@@ -106,8 +108,8 @@ extern "C" int kore_cuda_paged_store_dev(const kore_cuda_pages *cache, int n_tok
     if (int rc = check_pages(cache, false)) return rc;
     if (int rc = check_tokens(n_tok)) return rc;
     if (n_tok > 0 && !slots) return refuse(KORE_CUDA_EINVAL, "slots is null");
-    if ((reinterpret_cast<uintptr_t>(slots) & 7) || (reinterpret_cast<uintptr_t>(pos) & 3))
-        return refuse(KORE_CUDA_EINVAL, "slots or pos is not aligned to its type");
+    if ((reinterpret_cast<uintptr_t>(slots) & 7) || !words_aligned(pos, dev_status))
+        return refuse(KORE_CUDA_EINVAL, "slots, pos or dev_status is not aligned to its type");
     const int d = cache->head_dim;
     if (int rc = check_appended(cache, k, v, q, q_out, n_tok)) return rc;
     if (rope) {
@@ -179,6 +181,7 @@ extern "C" int kore_cuda_tree_masks_dev(const kore_cuda_batch *batch, int n_tok,
     const kore_cuda_tree tree{mask, words};
     if (int rc = check_tree(&tree)) return rc;
     if (!parent || !pos) return refuse(KORE_CUDA_EINVAL, "parent or pos is null");
+    if (!words_aligned(parent, pos, dev_status)) return refuse(KORE_CUDA_EINVAL, "parent, pos or dev_status is not aligned to its type");
     if (n_tok == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
     OnDeviceOf on(mask);
     if (on.rc) return on.rc;
@@ -197,6 +200,8 @@ static int accept(const kore_cuda_batch *batch, int n_tok, int most, const int *
     if (!parent || !token || !choice) return refuse(KORE_CUDA_EINVAL, "parent, token or choice is null");
     if (!out || !out->path || !out->count || !out->next_token || !out->kept)
         return refuse(KORE_CUDA_EINVAL, "path, count, next_token or kept is null");
+    if (!words_aligned(parent, token, choice, out->path, out->count, out->next_token, out->kept, dev_status))
+        return refuse(KORE_CUDA_EINVAL, "parent, token, choice, an array of the acceptance or dev_status is not aligned to its type");
     if (out->path_stride <= 0 || out->path_stride > kPagedMaxTree)
         return refuse(KORE_CUDA_EINVAL, "path_stride %d outside [1, %d]", out->path_stride, kPagedMaxTree);
     if (batch->n_seq == 0) return KORE_CUDA_OK;
@@ -252,6 +257,7 @@ extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_l
     }
     if (int rc = check_batch(batch, 0, true)) return rc;
     if (batch->n_seq > 0 && (!path || !count)) return refuse(KORE_CUDA_EINVAL, "path or count is null");
+    if (!words_aligned(path, count, dev_status)) return refuse(KORE_CUDA_EINVAL, "path, count or dev_status is not aligned to its type");
     if (path_stride <= 0 || path_stride > kPagedMaxTree)
         return refuse(KORE_CUDA_EINVAL, "path_stride %d outside [1, %d]", path_stride, kPagedMaxTree);
     if (n_layers == 0 || batch->n_seq == 0) return KORE_CUDA_OK;
