@@ -1,8 +1,8 @@
 """Builds kore_b200/libkore_cuda.so (the C-ABI library) with nvcc for sm_100a.
 
 Usage: ``python -m kore_b200.build [--force] [--verbose] [--trace]``; also
-kore_b200/_tensors.so, with which the Python operators describe torch tensors. The
-library is built in-tree so that it travels with the repository to the GPU
+kore_b200/_tensors.*.so, with which the Python operators describe torch tensors
+(without it they do so themselves). The library is built in-tree so that it travels with the repository to the GPU
 machine. ``--trace`` builds kore_b200/libkore_cuda_trace.so instead: the same
 library compiled with KORE_TRACE, whose decode and merge CTAs record
 %globaltimer stamps (read by ``python -m kore_b200.trace_decode``).
@@ -21,7 +21,8 @@ ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 INCLUDE = os.path.join(ROOT, "include")
 LIB = os.path.join(PKG, "libkore_cuda.so")
-TENSORS = os.path.join(PKG, "_tensors.so")   # the Python module that describes torch tensors for the library
+# the Python module that describes torch tensors for the library, named for the Python that it is compiled for
+TENSORS = os.path.join(PKG, "_tensors" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 TRACE_LIB = os.path.join(PKG, "libkore_cuda_trace.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -76,23 +77,44 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False, out: 
     return lib
 
 
+def _tensors_stale(deps: list[str], version: str) -> bool:
+    if not os.path.exists(TENSORS) or any(os.path.getmtime(d) > os.path.getmtime(TENSORS) for d in deps):
+        return True
+    # another torch may be older than the module: the module holds the version it was compiled against
+    with open(TENSORS, "rb") as f:
+        return version.encode() + b"\0" not in f.read()
+
+
 def build_tensors(force: bool = False) -> str | None:
-    """Compiles csrc/tensors.cpp against the torch that is installed (none: there are no tensors to describe)."""
+    """Compiles csrc/tensors.cpp against the torch and for the Python that are installed; returns the module's path. None,
+    and no module, where it cannot be: without torch there are no tensors to describe, and without a C++ compiler or
+    Python's headers kore_b200/paged.py describes them itself, in some microseconds more a call."""
     try:
         import torch
-    except ImportError:
+    except (ImportError, OSError):
         return None
+    untagged = os.path.join(PKG, "_tensors.so")   # (every Python would import one of this name)
+    if untagged != TENSORS and os.path.exists(untagged):
+        os.remove(untagged)
     src = os.path.join(CSRC, "tensors.cpp")
-    deps = [src, os.path.join(INCLUDE, "kore_cuda.h"), torch.__file__]
-    if not force and os.path.exists(TENSORS) and all(os.path.getmtime(d) <= os.path.getmtime(TENSORS) for d in deps):
+    version = torch.__version__.split("+")[0]
+    if not force and not _tensors_stale([src, os.path.join(INCLUDE, "kore_cuda.h"), torch.__file__], version):
         return TENSORS
     home = os.path.dirname(torch.__file__)
     cxx = os.environ.get("CXX") or shutil.which("g++") or "c++"
     tmp = TENSORS + ".tmp"
-    subprocess.run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
-                    "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], "-isystem", os.path.join(home, "include"),
-                    "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
-                    src, "-o", tmp, "-L", os.path.join(home, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"], check=True)
+    try:
+        subprocess.run([cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
+                        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+                        "-I", INCLUDE, "-I", sysconfig.get_paths()["include"], "-isystem", os.path.join(home, "include"),
+                        "-isystem", os.path.join(home, "include", "torch", "csrc", "api", "include"),
+                        src, "-o", tmp, "-L", os.path.join(home, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python"], check=True)
+    except (OSError, subprocess.CalledProcessError) as e:
+        for f in (tmp, TENSORS):   # (what is there is not of these sources)
+            if os.path.exists(f):
+                os.remove(f)
+        print(f"{os.path.basename(TENSORS)} is not built, tensors are described in Python: {e}", file=sys.stderr)
+        return None
     os.replace(tmp, TENSORS)
     return TENSORS
 
