@@ -798,6 +798,13 @@ int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_layers, cons
  * that wants to hear of a failure sooner sets less. */
 int kore_cuda_paged_set_wait_limit(unsigned long long nanoseconds);
 
+/* Which kernel the attention of trees that is launched (or captured) from now on takes, in
+ * the whole process: by the batch's sizes (0, the default), the one of 16 rows (1) or the
+ * one of 128 rows on the tensor cores (2). Either gives the same attention, up to rounding:
+ * for tests of both at any size, and for measurements of the choice. */
+enum kore_cuda_tree_kernel { KORE_CUDA_TREE_BY_SIZE = 0, KORE_CUDA_TREE_ROWS = 1, KORE_CUDA_TREE_TILES = 2 };
+int kore_cuda_paged_set_tree_kernel(int kernel);
+
 /* Identity of the graph capture that `stream` is in (0: none), for callers that
  * keep one workspace per capture. */
 unsigned long long kore_cuda_capture_id(void *stream);

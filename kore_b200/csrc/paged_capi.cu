@@ -13,6 +13,7 @@ namespace kore {
 namespace {
 
 std::atomic<unsigned long long> g_wait_ns{kWaitNs};   // of launches from now on
+std::atomic<int> g_tree_kernel{KORE_CUDA_TREE_BY_SIZE};
 
 // The pool as a tensor [page][head][token][d], boxes of `box` tokens x 128 bytes
 // (or the 64 of a short row), swizzled within rows of that width or (plain) as it is.
@@ -210,6 +211,12 @@ extern "C" int kore_cuda_paged_set_wait_limit(unsigned long long nanoseconds) {
     return KORE_CUDA_OK;
 }
 
+extern "C" int kore_cuda_paged_set_tree_kernel(int kernel) {
+    if (kernel < KORE_CUDA_TREE_BY_SIZE || kernel > KORE_CUDA_TREE_TILES) return refuse(KORE_CUDA_EINVAL, "tree kernel %d", kernel);
+    g_tree_kernel = kernel;
+    return KORE_CUDA_OK;
+}
+
 extern "C" long long kore_cuda_paged_attn_workspace(int head_dim) {
     if (head_dim != 64 && head_dim != 128) return refuse(KORE_CUDA_EINVAL, "head_dim %d is not supported here", head_dim);
     return (long long)kPagedZeroed + (long long)kPagedMaxCtas * 2 * kPagedRowsMax * (head_dim + 2) * (long long)sizeof(float);
@@ -316,10 +323,12 @@ static int attend(const kore_cuda_pages *cache, const kore_cuda_batch *batch, in
     // counted: 32 tokens that look back 512 of 30000 positions take the tiles' 19 where the rows take 11.
     const double rows16 = (double)p.G * ((double)n_tok * p.rep / 16 + p.n_seq);
     const double passes = (batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P) / 128 + 3;
-    const bool tiles = (long long)batch->max_q * p.rep > 16 &&
-                       (tree ? trees_in_tiles(d, cache->type == KORE_CUDA_E4M3, G, p.rep, p.n_seq, n_tok,
-                                              batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P, ctas)
-                             : rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0));
+    bool tiles = (long long)batch->max_q * p.rep > 16 &&
+                 (tree ? trees_in_tiles(d, cache->type == KORE_CUDA_E4M3, G, p.rep, p.n_seq, n_tok,
+                                        batch->max_kv > 0 ? batch->max_kv : (double)p.table_stride * p.P, ctas)
+                       : rows16 * passes > (cache->type == KORE_CUDA_E4M3 ? 13500.0 : 6200.0));
+    const int wanted = g_tree_kernel;
+    if (tree && wanted != KORE_CUDA_TREE_BY_SIZE) tiles = wanted == KORE_CUDA_TREE_TILES;
     const bool plain = tiles && cache->type == KORE_CUDA_E4M3;   // widened before it is read as an operand
     // tokens of a box: the largest power of two that divides the page, up to a tile
     const int most = tiles ? (tree ? 64 : 128) : d * type_bytes(cache->type) == 256 ? 16 : 32;

@@ -24,11 +24,12 @@ import struct
 
 from . import KoreCudaError, load_library
 
-__all__ = ["RopeTable", "PagedCache", "PagedBatch", "rope_frequencies", "set_wait_limit"]
+__all__ = ["RopeTable", "PagedCache", "PagedBatch", "rope_frequencies", "set_wait_limit", "set_tree_kernel"]
 
 F32, F16, BF16, E4M3 = 0, 1, 30, 1000
 WORKSPACE_ZEROED = 1024
 SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
+TREE_KERNELS = {"auto": 0, "rows": 1, "tiles": 2}
 DEVICE_FAILURES = {1: "a tile copy or product did not come in time", 3: "page id outside the pool", 6: "position outside the rotation table",
                    7: "a sequence's bounds do not fit the rows, its length or its page table",
                    8: "too few free pages in the pool"}
@@ -122,6 +123,7 @@ def _library():
         L.kore_cuda_tree_accept_masked_dev.argtypes = [_vp, _i, _i] + [_vp] * 6
         L.kore_cuda_paged_commit_dev.argtypes = [_vp, _i, _vp, _vp, _i, _vp, _vp, _vp]
         L.kore_cuda_paged_set_wait_limit.argtypes = [ctypes.c_ulonglong]
+        L.kore_cuda_paged_set_tree_kernel.argtypes = [_i]
         L.kore_cuda_capture_id.argtypes = [_vp]
         L.kore_cuda_capture_id.restype = ctypes.c_ulonglong
         _fns = L
@@ -247,6 +249,15 @@ def set_wait_limit(seconds: float) -> None:
         raise ValueError(f"seconds = {seconds}")
     L = _library()
     _ck(L, L.kore_cuda_paged_set_wait_limit(int(seconds * 1e9)))
+
+
+def set_tree_kernel(kernel: str) -> None:
+    """Which kernel the attention of trees launched from now on takes, in the whole process: "auto" (by the batch's sizes),
+    "rows" or "tiles" (kore_cuda_paged_set_tree_kernel)."""
+    if kernel not in TREE_KERNELS:
+        raise ValueError(f"kernel {kernel!r} is none of {sorted(TREE_KERNELS)}")
+    L = _library()
+    _ck(L, L.kore_cuda_paged_set_tree_kernel(TREE_KERNELS[kernel]))
 
 
 class RopeTable:

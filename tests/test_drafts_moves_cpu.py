@@ -67,3 +67,12 @@ def test_an_acceptance_with_masks_of_no_size_is_refused(words):
     assert rc == -1 and "words" in msg
     assert err(call(_ref(_batch()), 1, 1, None, A, A, _ref(out), None, None))[0] == -1
     assert call(_ref(_batch(n_seq=0)), 1, 32, A, A, A, _ref(out), None, None) == 0
+
+
+def test_only_kernels_that_there_are_can_be_set():
+    L = P._library()
+    for x in (-1, 3, 1 << 30):
+        assert L.kore_cuda_paged_set_tree_kernel(x) == -1
+    with pytest.raises(ValueError, match="kernel"):
+        P.set_tree_kernel("other")
+    P.set_tree_kernel("auto")
