@@ -11,10 +11,10 @@
 //
 // Two running sums and then writes: no arithmetic to speak of, some tens of KB, so a
 // call's time is its chain (requests, lengths, sums, pages). One cluster: every CTA forms the sums
-// of the whole batch for itself (4096 sequences are four a thread), writes its share of tokens
+// of the whole batch for itself (4096 sequences are eight a thread), writes its share of tokens
 // and tables from the state as it was, and only behind the cluster's barrier does the state change;
 // a second launch for the writes, or a pass over counters in memory, would take longer than the sums do.
-// A plan and a trim together: 8.4 us for 32 requests of 63 pages, 15.2 for 500 trees of up to 20 tokens with
+// A plan and a trim together: 8.4 us for 32 requests of 63 pages, 15.2 for 500 trees of up to 24 tokens with
 // their masks, 14.2 for 96 prompts of 100000 tokens (1.2 MB, which HBM would take in 0.2 us: a launch of a
 // cluster of sixteen is some 2 us of each, the chain of loads 2 to 3).
 
@@ -24,14 +24,16 @@ namespace kore {
 namespace {
 
 constexpr unsigned FULL = 0xffffffffu;
+constexpr int kPlanThreads = 512;   // of a CTA at most
+constexpr int kPlanWarps = kPlanThreads / 32;
 
 __device__ __forceinline__ void cluster_barrier() {
     asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 
 // Inclusive sums of a and b over the block, on top of what came before (run_a, run_b: updated).
-__device__ __forceinline__ void block_scan(long long &a, long long &b, longlong2 (&part)[33], long long &run_a, long long &run_b) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;   // (at most 32)
+__device__ __forceinline__ void block_scan(long long &a, long long &b, longlong2 (&part)[kPlanWarps + 1], long long &run_a, long long &run_b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     a = warp_scan(a);
     b = warp_scan(b);
     if (lane == 31) part[warp + 1] = make_longlong2(a, b);
@@ -55,9 +57,9 @@ __device__ __forceinline__ int pages_of(const PlanParams &p, int n) {
 }
 
 template <bool TRIM>
-__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanParams p) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanParams p) {
     extern __shared__ int smem[];
-    __shared__ longlong2 part[33];
+    __shared__ longlong2 part[kPlanWarps + 1];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int words = (p.n_requests + 31) / 32;
     // requests named by the batch, and those named twice
@@ -282,11 +284,13 @@ cudaError_t launch_p(const PlanParams &p, int ctas, int threads, cudaStream_t s)
 }  // namespace
 
 cudaError_t launch_plan(const PlanParams &p, bool trim, cudaStream_t s) {
-    // A portable cluster of small CTAs, or one of sixteen for many tokens, sequences or table entries (plan and
-    // trim of 32 requests of 63 pages: 8.5 us with 8 x 256 threads, 9.1 with 16 x 512; of 500 of up to 251 pages 27.2
-    // and 15.3; of 96 with 100000 tokens 28.7 and 14.1)
+    // A portable cluster of small CTAs, or one of sixteen for many tokens, sequences or table entries. Plan and
+    // trim, 8 x 256 against 16 x 512 threads, us: 32 requests of 63 pages 8.5 / 9.1; 500 of up to 251 pages 27.2 / 15.3;
+    // 96 with 100000 tokens 28.7 / 14.1. Near the borders: a token for 128, 240, 264 requests of 63, 63, 16 pages 9.5 / 9.3,
+    // 11.4 / 9.4, 14.0 / 10.1; 64 requests of 251 pages 10.1 / 9.3; 16 prompts of 120, 136 tokens 7.7 / 7.6, 8.1 / 7.6; one
+    // of 2048, 4096 tokens 7.3 / 7.5, 7.6 / 7.4. (So the smaller ones lose up to 2 us just below the borders.)
     const bool large = p.n_tok > 2048 || p.n_seq > 256 || (long long)p.n_seq * p.stride > 16384;
-    const int ctas = large ? 16 : 8, threads = large ? 512 : 256;
+    const int ctas = large ? 16 : 8, threads = large ? kPlanThreads : 256;
     return trim ? launch_p<true>(p, ctas, threads, s) : launch_p<false>(p, ctas, threads, s);
 }
 
