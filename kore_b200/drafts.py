@@ -234,34 +234,38 @@ class AcceptedPath:
         P._check_status(self.status)
 
 
-def _overlap(cache):
-    """Whether a page of a pool at a and a page of one at b (which may lie between one another's) share memory; pools of
-    cache's geometry."""
-    v = cache.view
-    size = cache.k.element_size()
+def _spans(cache):
+    """Bytes of a page, from one page to the next, and from a pool's first byte to its last, of cache's geometry."""
+    v, size = cache.view, cache.k.element_size()
     page = v.n_head_kv * v.page_tokens * v.head_dim * size
     stride = v.page_stride * size or page
+    return page, stride, (v.n_pages - 1) * stride + page
 
-    def overlap(a, b) -> bool:
-        n, rest = divmod(abs((a or 0) - (b or 0)), stride)
-        return (n < v.n_pages and rest < page) or (n + 1 < v.n_pages and stride - rest < page)
-    return overlap
+
+def _overlap(apart: int, page: int, stride: int, span: int) -> bool:
+    """Whether pools that begin so many bytes apart, whose pages may lie between one another's, share memory."""
+    rest = apart % stride
+    return apart < span and (rest < page or stride - rest < page and apart - rest + stride < span)
 
 
 def _check_apart(caches) -> None:
     """Raises if two caches' pages share memory."""
-    overlap = _overlap(caches[0])
-    pools = [(a, i) for i, c in enumerate(caches) for a in (c.view.k, c.view.v)]
+    page, stride, span = _spans(caches[0])
+    pools = sorted((a or 0, i) for i, c in enumerate(caches) for a in (c.view.k, c.view.v))
     for x, (a, i) in enumerate(pools):
-        for b, j in pools[x + 1:]:
-            if i != j and overlap(a, b):
-                raise ValueError(f"caches {i} and {j} share pages")
+        for y in range(x + 1, len(pools)):
+            b, j = pools[y]
+            if b - a >= span:   # (so are all behind it)
+                break
+            if i != j and _overlap(b - a, page, stride, span):
+                raise ValueError(f"caches {min(i, j)} and {max(i, j)} share pages")
 
 
 def _check_own(caches) -> None:
     """Raises if a cache's keys and values share memory and are not one (whose rows are moved once)."""
     for i, c in enumerate(caches):
-        if c.view.k != c.view.v and _overlap(c)(c.view.k, c.view.v):
+        apart = abs((c.view.k or 0) - (c.view.v or 0))
+        if apart and _overlap(apart, *_spans(c)):
             raise ValueError(f"cache {i}: the keys' pages overlap the values'")
 
 
