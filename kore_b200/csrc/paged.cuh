@@ -20,7 +20,7 @@ constexpr int kPagedMaxSeqs = 4096;      // sequences of one batch
 constexpr int kPagedMaxRequests = 65536; // requests of one pool
 constexpr int kPagedMaxTree = 1024;      // tokens of a tree
 constexpr int kPagedMaxTokens = 1 << 30; // rows of a plan or a store: steps beyond the last stay in 32 bits
-constexpr int kPagedMaxPools = 256;      // pools whose rows one launch moves: keys and values of 128 layers
+constexpr int kPagedMaxLayers = 128;     // layers of one launch
 constexpr int kPagedMaxCtas = 160;       // CTAs (SMs) that an attention launch uses at most
 constexpr int kPagedRowsMax = 256;       // query rows of a work unit at most
 constexpr size_t kPagedZeroed = 1024;    // leading workspace bytes that are zero between calls
@@ -104,11 +104,11 @@ struct TreeParams {
 
 struct CommitParams {
     const int *q_start, *kv_len, *page_table, *path, *count;
-    int n_seq, table_stride, path_stride, n_pages, n_pools, P, G, row_pieces;   // pieces: of 16 bytes
+    int n_seq, table_stride, path_stride, n_pages, n_layers, P, G, row_pieces;   // pieces: of 16 bytes
     FastDiv by_page;
     long long page_pieces;
     int *status;
-    void *pool[kPagedMaxPools];                   // keys and values of the layers
+    void *k[kPagedMaxLayers], *v[kPagedMaxLayers];   // v null: the keys' memory is the values' too
 };
 
 struct PagedAttnParams {

@@ -283,10 +283,11 @@ extern "C" int kore_cuda_paged_commit_dev(const kore_cuda_pages *layers, int n_l
     p.by_page = FastDiv::of((uint32_t)p.P);
     p.page_pieces = page_stride(layers) * type_bytes(layers->type) / 16;
     p.status = dev_status;
-    for (int l = 0; l < n_layers;) {
-        for (p.n_pools = 0; l < n_layers && p.n_pools + 2 <= kPagedMaxPools; ++l) {
-            p.pool[p.n_pools++] = layers[l].k;
-            if (layers[l].v != layers[l].k) p.pool[p.n_pools++] = layers[l].v;   // (one memory's rows move once)
+    for (int l0 = 0; l0 < n_layers; l0 += kPagedMaxLayers) {
+        p.n_layers = n_layers - l0 < kPagedMaxLayers ? n_layers - l0 : kPagedMaxLayers;
+        for (int l = 0; l < p.n_layers; ++l) {
+            p.k[l] = layers[l0 + l].k;
+            p.v[l] = layers[l0 + l].v != p.k[l] ? layers[l0 + l].v : nullptr;   // (one memory's rows move once)
         }
         if (int rc = launched(launch_commit(p, (cudaStream_t)stream), "paged_commit")) return rc;
     }

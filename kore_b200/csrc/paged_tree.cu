@@ -182,10 +182,12 @@ __global__ void __launch_bounds__(256) commit_kernel(const __grid_constant__ Com
     while (j0 < m && rows[j0].x == rows[j0].y) ++j0;
     if (j0 == m) return;
     const int head = p.P * p.row_pieces, layer = p.G * p.row_pieces;   // pieces from head to head, of a token
-    const int all = p.n_pools * layer;
+    const int all = p.n_layers * 2 * layer;
     for (int x = blockIdx.x * blockDim.x + tid; x < all; x += gridDim.x * blockDim.x) {
         const int l = x / layer, y = x - l * layer, g = y / p.row_pieces;
-        uint4 *base = static_cast<uint4 *>(p.pool[l]) + (long long)g * head + (y - g * p.row_pieces);
+        void *pool = (l & 1) ? p.v[l >> 1] : p.k[l >> 1];
+        if (!pool) continue;
+        uint4 *base = static_cast<uint4 *>(pool) + (long long)g * head + (y - g * p.row_pieces);
         for (int j = j0; j < m; j += 8) {
             uint4 v[8];
 #pragma unroll
@@ -205,7 +207,7 @@ cudaError_t launch_tree_mask(const TreeParams &p, cudaStream_t s) { return launc
 cudaError_t launch_accept(const TreeParams &p, cudaStream_t s) { return launch(accept_kernel, (p.n_seq + 3) / 4, 128, 0, s, p); }
 
 cudaError_t launch_commit(const CommitParams &p, cudaStream_t s) {
-    const int all = p.n_pools * p.G * p.row_pieces;
+    const int all = p.n_layers * 2 * p.G * p.row_pieces;
     const size_t smem = (size_t)p.path_stride * sizeof(longlong2);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((all + 255) / 256 < 32 ? (all + 255) / 256 : 32, p.n_seq);

@@ -13,7 +13,7 @@ torch = pytest.importorskip("torch")
 @pytest.mark.parametrize("t,G,d,layers", [("bf16", 4, 128, 28), ("e4m3", 2, 64, 3), ("f16", 1, 64, 200)])
 @pytest.mark.parametrize("every", [1, 2])
 def test_keys_and_values_in_one_memory_move_once(t, G, d, layers, every):
-    """Every layer, or every second one: between 128 and 256 pools a launch."""
+    """Every layer, or every second one; more layers than a launch takes."""
     g, r, P = gen(layers), random.Random(layers), 16
     ns = [6, 64, 1, 40, 9]
     kvs = [n + r.randrange(60) for n in ns]
