@@ -52,10 +52,11 @@ bool encode_pages(const void *base, const kore_cuda_pages *c, int box, bool plai
 // unit of 16 rows an SM works on a time of its own and one for every 128 keys; the tile kernel its start, a
 // time for every 64 keys (and 8 more of them a unit) of a CTA's share, and a joint for each doubling of the CTAs that
 // share a unit. Row against tile kernel, 28/4 heads of 128, 16 bits: 8 tokens on 520 positions 11 / 16; 16
-// on 16000 41 / 43; 16 x 8 on 1008 33 / 26; 16 x 24 on 324 42 / 15; 16 x 8 on 8008 161 / 68; 48 x 2 on 1002 31 /
-// 40; 64 x 32 on 1532 415 / 94. 8 bits: 16 x 4 on 4004 41 / 50; 64 x 24 on 124 132 / 41. 14/2 heads of 64:
-// 64 on 1064 11 / 16; 64 on 30064 58 / 41. Over 144 batches of three head layouts the choice takes 0.7 % more than the
-// better kernel of each, 26 % at worst.
+// on 16016 41 / 43; 16 x 8 on 1008 33 / 24; 16 x 24 on 324 42 / 15; 16 x 8 on 8008 161 / 67; 48 x 2 on 1002 30 /
+// 36; 64 x 32 on 1532 408 / 89. 8 bits: 16 x 4 on 4004 40 / 47; 64 x 24 on 124 131 / 28. 14/2 heads of 64:
+// 64 on 1064 11 / 17; 64 on 30064 58 / 39. Over 144 batches of groups of 7 and 8 query heads the choice takes 0.7 % more than
+// the better kernel of each, 35 % at worst (28/4 of 128, 8 bits, 16 x 8 on 1008: 35 for 26). Groups of other sizes were not
+// fitted: over 100 batches of 1, 4 and 16 heads 2.5 %, at worst 71 % (8/8 of 128, 8 bits, 16 x 24 on 324: 28 for 16).
 bool trees_in_tiles(int d, bool e8, int G, int rep, int n_seq, int n_tok, double kv, int sms) {
     struct Cost {
         double unit, pass, start, tile, joint;

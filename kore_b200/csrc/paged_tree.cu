@@ -11,10 +11,11 @@
 //   that takes its 16 bytes of every row in the path's order may read all of them first. Nobody else may move
 //   the same rows, so keys and values that are one memory are one pool.
 //
-// Masks and acceptance are chains of dependent looks (some tens of ns each, in shared memory). The move is bound by HBM for large batches and by its chain (path,
-// page table, row) for small ones: 16 bytes of a thread at every accepted row, eight rows on their way
-// at once. Acceptance and move together: 4.7 us for a sequence, 28 layers; 10.9 for 32 sequences of 16 tokens, 28
-// layers of 4 heads of 128 in bf16 (17 MB, 2.6 us of HBM; 8.8 out of L2).
+// Masks and acceptance are chains of dependent looks (some tens of ns each, in shared memory). The move is bound by
+// HBM for large batches and by its chain (path, page table, row) for small ones: 16 bytes of a thread at every accepted
+// row, eight rows on their way at once. Acceptance and move together: 4.5 us for a sequence, 24 layers of 2 heads of 64
+// in f16; 11.1 for 64 sequences of up to 24 tokens, 28 layers of 4 heads of 128 in bf16 (17 MB, 2.6 us of HBM; 8.8 out
+// of L2).
 
 #include "paged_values.cuh"
 

@@ -7,9 +7,12 @@
 // * rows flops, so HBM and the tensor cores bound it alike at some 100 rows, and what counts is that
 // neither waits: two CTAs an SM, each with one tile of rows, so that one streams while the other starts
 // a unit, joins its parts or writes its outputs (one CTA an SM with two tiles of rows, as for prompts, left
-// 4 to 7 us between a CTA's units in which no key moved). Measured: 32 sequences of 16 tokens on up to 8192, 28/4 heads
-// of 128, bf16: 70.6 us (4.05 TB/s, 440 TFLOP/s; the keys stream for 43 of them, a CTA's start takes 5, the joints at the
-// end up to 15); 6 of up to 60 on 32768, 8 bits: 121 us (540 TFLOP/s); 48 of up to 33 on 3001, 14/2 heads of 64, f16: 31.5.
+// 4 to 7 us between a CTA's units in which no key moved). Measured, the GPU's time alone (a call among others takes 3 us more at the first
+// two): 32 sequences of 16 tokens on up to 8192, 28/4 heads of 128, bf16: 70.7 us (4.05 TB/s, 440 TFLOP/s; the keys
+// stream for 43 of them, a CTA's start takes 5, the joints at the end up to 15); 6 of up to 60 on 32768, 8 bits: 122 us
+// (535 TFLOP/s); 48 of up to 33 on 3001, 14/2 heads of 64, f16: 31.4; 8 bits and d = 64: 64 tokens on 30064 42, 48 x 16 on
+// 2016 31 (floors 4.2 and 4.2). Every instance spills: at 128 registers a thread (16 bits) 252 bytes of stores and
+// 196 of loads at d = 128, 40 and 132 at d = 64; at 80 (8 bits) 584 to 588 and 744 to 780.
 //   warps 0-3    softmax, a thread a row. Per step of 64 keys: S from tensor memory, mask (a word of bits for
 //                32 keys), online softmax (the reference maximum moves only when a score passes it by 2^8;
 //                O in tensor memory is rescaled then), P in 16 bits over S, sums in fp32.
