@@ -772,8 +772,9 @@ typedef struct kore_cuda_accepted {
 
 /* The branch that the model follows: from token 0 of each chunk on, the first child
  * (by index) whose token[t] is choice of its parent (the model's token behind it; all
- * device [n_tok]), and so on. A sequence whose rows do not fit, or whose chunk is longer
- * than its kv_len or than 1024 tokens, is left out (7): count 0, kept -1. */
+ * device [n_tok]), and so on. A sequence whose rows do not fit, whose chunk is longer
+ * than its kv_len or than 1024 tokens, or whose token 0 has a parent (it is no tree's root,
+ * the masks leave it out), is left out (7): count 0, kept -1. */
 int kore_cuda_tree_accept_dev(const kore_cuda_batch *batch, int n_tok, const int *parent, const int *token,
                               const int *choice, const kore_cuda_accepted *out, int *dev_status, void *stream);
 

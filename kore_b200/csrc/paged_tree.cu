@@ -94,7 +94,7 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Tre
     const int lane = threadIdx.x & 31, s = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     if (s >= p.n_seq) return;
     __shared__ int near[4][3][kNear];
-    const Seq q = tree_seq(p, s, lane == 0);
+    Seq q = tree_seq(p, s, lane == 0);
     int *path = p.path + (long long)s * p.path_stride;
     int count = 0, now = 0, next = -1;
     if (q.n > 0) {
@@ -111,7 +111,11 @@ __global__ void __launch_bounds__(128) accept_kernel(const __grid_constant__ Tre
             token = to[1];
             choice = to[2];
         }
-        for (;;) {
+        if (parent[0] != -1) {   // masks and store have left out token 0, and all behind it
+            if (lane == 0) raise_error(p.status, DEV_BAD_SEQUENCE);
+            q.n = -1;
+        }
+        while (q.n > 0) {
             if (lane == 0) path[count] = now;
             ++count;
             next = choice[now];

@@ -130,3 +130,21 @@ def test_a_chunk_that_is_too_long_for_its_masks_is_not_accepted(most, n):
         path.check()
     with pytest.raises(ValueError, match="tree"):
         path.accept(step, parent[:n], ones[:n], ones[:n], tree=tree)
+
+
+@pytest.mark.parametrize("n", [1, 6, 300])   # (walked in shared memory, and not)
+@pytest.mark.parametrize("root", [0, 3, -2, -2 ** 31])
+def test_a_chunk_whose_first_token_is_no_root_is_not_accepted(n, root):
+    """Masks and store leave that token out, and with it all of its branches."""
+    batch = K.PagedBatch(ints([0, 4, 4 + n, 8 + n]), ints([9, 50 + n, 4]), ints([[0]] * 3), 300)
+    chain = list(range(-1, 3))
+    parent = ints(chain + [root] + list(range(n - 1)) + chain)
+    tree, path, ones = K.TokenTree(8 + n, 320), K.AcceptedPath(3, 3), torch.ones_like(parent)
+    tree.build(batch, parent)
+    assert (tree.pos[4:4 + n] == -1).all() and tree.pos[:4].tolist() == [5, 6, 7, 8]
+    path.accept(batch, parent, ones, ones, tree=tree)
+    assert path.count.tolist() == [3, 0, 3] and path.kept.tolist() == [8, -1, 3] and path.next_token.tolist() == [1, -1, 1]
+    assert path.path.tolist() == [[0, 1, 2], [-1] * 3, [0, 1, 2]]
+    for x in (tree, path):
+        with pytest.raises(K.KoreCudaError, match="bounds"):
+            x.check()
