@@ -132,10 +132,12 @@ inline long long page_stride(const kore_cuda_pages *c) {
 // Whether some page of the keys and some page of the values (which may lie between one another's) share memory.
 inline bool pages_overlap(const kore_cuda_pages *c) {
     const unsigned long long b = type_bytes(c->type), page = (unsigned long long)c->n_head_kv * c->page_tokens * c->head_dim * b;
-    const unsigned long long stride = page_stride(c) * b, n = c->n_pages;
+    const unsigned long long stride = page_stride(c) * b, span = (c->n_pages - 1) * stride + page;
     const uintptr_t k = reinterpret_cast<uintptr_t>(c->k), v = reinterpret_cast<uintptr_t>(c->v);
-    const unsigned long long apart = k < v ? v - k : k - v, i = apart / stride, rest = apart % stride;
-    return (i < n && rest < page) || (i + 1 < n && stride - rest < page);
+    const unsigned long long apart = k < v ? v - k : k - v;
+    if (apart >= span) return false;   // (most: a commit asks of every layer, and a division takes as long as the rest)
+    const unsigned long long rest = apart % stride;
+    return rest < page || (stride - rest < page && apart - rest + stride < span);
 }
 
 // Keys and values that go into memory that the cache's share: which of them stayed would be chance, unless it is one
